@@ -3,7 +3,7 @@ TriangleAttention and the inference prefill/decode op behind the reference's Pyt
 running hand-written sm_100a CUDA through the C ABI in ``include/acct_b200.h``."""
 
 __all__ = ["FlashAttention", "TriangleAttention", "get_flash_attention", "get_flash_attention_grad",
-           "FlashAttentionTik", "flash_attention_tik", "flash_attention_decode"]
+           "FlashAttentionTik", "flash_attention_tik", "flash_attention_decode", "Kv4Cache", "Kv4Workspace"]
 
 
 def __getattr__(name):
@@ -18,5 +18,8 @@ def __getattr__(name):
         return getattr(m, name)
     if name in ("FlashAttentionTik", "flash_attention_tik", "flash_attention_decode"):
         from .infer import flash_attention as m
+        return getattr(m, name)
+    if name in ("Kv4Cache", "Kv4Workspace"):
+        from .infer import kv4_cache as m
         return getattr(m, name)
     raise AttributeError(name)

@@ -33,6 +33,8 @@ EXPORTS = [
     "acct_ms_set_fa_attrs", "acct_ms_fa_fwd", "acct_ms_fa_grad", "acct_ms_infer_fa", "acct_dropout_mask",
     "acct_mask_is_causal", "acct_mask_tiles_bytes", "acct_mask_classify_tiles", "acct_mask_tiles_scratch",
     "acct_selftest_wait_timeout", "acct_ms_fa_attrs_slot", "acct_ms_fa_attrs_slot_ex",
+    "acct_kv4_record_bytes", "acct_kv4_append", "acct_kv4_read", "acct_kv4_decode_workspace_bytes", "acct_kv4_decode",
+    "acct_kv4_evict",
 ] + [f"acct_ms_fa_{kind}_s{k}" for k in range(32) for kind in ("fwd", "grad")]
 
 
@@ -90,6 +92,35 @@ class DecodeArgs(C.Structure):
         ("scale", C.c_float), ("num_splits", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("N_kv", C.c_int32),
         ("block_table", C.c_void_p), ("page_size", C.c_int32), ("max_pages", C.c_int32),
+    ]
+
+
+class Kv4CacheArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("N_kv", C.c_int32), ("D", C.c_int32), ("S_max", C.c_int32),
+        ("records", C.c_void_p), ("block_table", C.c_void_p),
+        ("page_size", C.c_int32), ("max_pages", C.c_int32), ("num_pages", C.c_int32),
+    ]
+
+
+class Kv4Rows(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+        ("T", C.c_int32), ("cu_seqlens", C.c_void_p), ("start", C.c_void_p),
+    ]
+
+
+class Kv4DecodeArgs(C.Structure):
+    _fields_ = [
+        ("N", C.c_int32), ("q", C.c_void_p), ("y", C.c_void_p), ("seq_lens", C.c_void_p), ("weights", C.c_void_p),
+        ("scale", C.c_float), ("num_splits", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class Kv4EvictArgs(C.Structure):
+    _fields_ = [
+        ("weights", C.c_void_p), ("weights_out", C.c_void_p), ("kept", C.c_void_p),
+        ("seq_lens", C.c_void_p), ("seq_lens_out", C.c_void_p), ("keep", C.c_int32), ("recent", C.c_int32),
     ]
 
 
@@ -157,6 +188,18 @@ def load():
     lib.acct_mask_classify_tiles.restype = C.c_int
     lib.acct_selftest_wait_timeout.argtypes = [C.c_void_p]
     lib.acct_selftest_wait_timeout.restype = C.c_int
+    lib.acct_kv4_record_bytes.argtypes = [C.c_int32]
+    lib.acct_kv4_record_bytes.restype = C.c_size_t
+    lib.acct_kv4_append.argtypes = [C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows), C.c_void_p]
+    lib.acct_kv4_append.restype = C.c_int
+    lib.acct_kv4_read.argtypes = [C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows), C.c_void_p]
+    lib.acct_kv4_read.restype = C.c_int
+    lib.acct_kv4_decode_workspace_bytes.argtypes = [C.POINTER(Kv4CacheArgs), C.c_int32, C.c_int32, C.c_int32]
+    lib.acct_kv4_decode_workspace_bytes.restype = C.c_size_t
+    lib.acct_kv4_decode.argtypes = [C.POINTER(Kv4CacheArgs), C.POINTER(Kv4DecodeArgs), C.c_void_p]
+    lib.acct_kv4_decode.restype = C.c_int
+    lib.acct_kv4_evict.argtypes = [C.POINTER(Kv4CacheArgs), C.POINTER(Kv4CacheArgs), C.POINTER(Kv4EvictArgs), C.c_void_p]
+    lib.acct_kv4_evict.restype = C.c_int
     lib.acct_abi_version.argtypes = []
     lib.acct_abi_version.restype = C.c_int
     if lib.acct_abi_version() != ABI_VERSION:

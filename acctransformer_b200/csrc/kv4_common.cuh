@@ -1,0 +1,98 @@
+// The cache in 4 bits: how a record of 16 rows is laid out, and where it is.
+//
+// Every 32 neighbouring values of a row (one token, one head; the last group may be short) share a minimum m and a step s, both
+// in the cache's 16-bit type, and are codes 0..15; code c stands for c * s + m.  A row of head_dim 128 takes 160 bytes for K and
+// V instead of 512.
+//
+// 16 rows of K and of V of one head are one record, 640 bytes per group of 32 columns (2 560 at head_dim 128), laid out for the
+// lanes that multiply it (lane = 4 g + t, as in the operands of mma.m16n8k16), so that one bulk copy brings a record in, a lane
+// finds its words side by side, and no word has to be moved between lanes:
+//   K codes    lane (g, t), word 8-row half * NG + group: row g of the half, columns 32 group + 8 t .. + 7, nibble = column
+//   V codes    lane (g, t), word p * NG + group: rows 8 p + 2 t (low 16 bits) and 8 p + 2 t + 1 (high), columns
+//              32 group + 4 g .. + 3, nibble = column: two rows of one column are where a B operand has them
+//   K steps    [half][t][group][2]: rows 2 t and 2 t + 1 of the half, as the accumulators of Q K^T have them
+//   K minima   [row][group]
+//   V both     [p][t][group][steps of the two rows, minima of the two rows]
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace acct {
+
+constexpr int kKv4Rows = 16;        // rows of a record
+constexpr int kKv4MaxGroups = 4;    // head_dim up to 128
+
+// byte offsets inside a record
+template <int NG>
+struct Kv4Record {
+  static constexpr int kWords = 2 * NG;                 // words of K, and of V, per lane
+  static constexpr int kUnit = NG % 2 == 0 ? 4 : 2;     // of which so many are neighbours: [kWords / kUnit][32 lanes][kUnit]
+  static constexpr int kV = 256 * NG, kKs = 512 * NG, kKm = 544 * NG, kVsm = 576 * NG, kBytes = 640 * NG;
+
+  // byte offset of word w of the unit at `place` (0..31)
+  __host__ __device__ static constexpr int word(int w, int place) { return (((w / kUnit) * 32 + place) * kUnit + w % kUnit) * 4; }
+  // Where lane (g, t) has its V words: the eight lanes that hold a pair of rows side by side (a row is read and written alone,
+  // too), turned by 2 t so that any eight consecutive lanes still cover all banks.
+  __host__ __device__ static constexpr int v_place(int g, int t) { return t * 8 + ((g + 2 * t) & 7); }
+  __host__ __device__ static constexpr int k_step(int row, int grp) { return kKs + ((((row >> 3) * 4 + ((row & 7) >> 1)) * NG + grp) * 2 + (row & 1)) * 2; }
+  __host__ __device__ static constexpr int k_min(int row, int grp) { return kKm + (row * NG + grp) * 2; }
+  __host__ __device__ static constexpr int v_step(int row, int grp) { return kVsm + ((((row >> 3) * 4 + ((row & 7) >> 1)) * NG + grp) * 4 + (row & 1)) * 2; }
+  __host__ __device__ static constexpr int v_min(int row, int grp) { return v_step(row, grp) + 4; }
+};
+
+struct Kv4Cache {
+  uint8_t* records;                 // [B, N_kv, recs][record], or pages [num_pages, N_kv, 1 << page_shift][record]
+  const int* table;                 // [B, max_pages], or null: contiguous
+  int B, N_kv, D, S_max;
+  int recs;                         // records per head of a contiguous cache
+  int page_shift;                   // records per page = 1 << page_shift
+  int max_pages, num_pages;
+};
+
+// Record `rec` of a head.  A page number that is none reads and writes page 0 or the last one, never memory outside.
+__device__ __forceinline__ uint8_t* kv4_record(const Kv4Cache& c, int b, int h, int rec, int bytes) {
+  if (c.table == nullptr) return c.records + ((static_cast<int64_t>(b) * c.N_kv + h) * c.recs + rec) * bytes;
+  const int page = min(max(c.table[static_cast<int64_t>(b) * c.max_pages + (rec >> c.page_shift)], 0), c.num_pages - 1);
+  return c.records + (((static_cast<int64_t>(page) * c.N_kv + h) << c.page_shift) + (rec & ((1 << c.page_shift) - 1))) * bytes;
+}
+
+struct Kv4Rows {                    // rows of tokens outside the cache: [T, N_kv, D]
+  void *k, *v;
+  int64_t k_stride[2], v_stride[2]; // elements, of a token and of a head
+  const int* cu;                    // [B + 1]: sequence b has rows cu[b] .. cu[b + 1] - 1; null: row b, T = B
+  const int* start;                 // [B]: the first of them is slot start[b] of its sequence
+  int T;
+};
+
+struct Kv4DecodeParams {
+  Kv4Cache cache;
+  const void* q;
+  void* y;
+  const int* seq_lens;
+  float* weights;                   // [B, N_kv, S_max] or null: every key's probability is added, over the group's heads
+  float* scores;                    // with weights: [B, N, S_pad] scratch
+  float* part_acc;                  // [B * N, splits, D]
+  float* part_ml;                   // [B * N, splits, 2]
+  unsigned int* status;
+  int B, N, D, kv_group, splits, S_pad;
+  int clustered;
+  float scale_log2;
+};
+
+struct Kv4EvictParams {
+  Kv4Cache src, dst;
+  const float* weights;             // [B, N_kv, src.S_max]
+  float* weights_out;               // [B, N_kv, dst.S_max]
+  int* kept;                        // [B, N_kv, keep]
+  const int* seq_lens;
+  int* seq_lens_out;
+  int keep, recent;
+};
+
+cudaError_t launch_kv4_append(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);
+cudaError_t launch_kv4_read(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);
+cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int* resident = nullptr);
+cudaError_t launch_kv4_evict(const Kv4EvictParams& p, cudaStream_t stream);
+
+}  // namespace acct

@@ -38,6 +38,10 @@ struct Library {
   decltype(&acct_fa_bwd_workspace_bytes) fa_bwd_workspace_bytes;
   decltype(&acct_infer_prefill) infer_prefill;
   decltype(&acct_infer_decode) infer_decode;
+  decltype(&acct_kv4_append) kv4_append;
+  decltype(&acct_kv4_read) kv4_read;
+  decltype(&acct_kv4_decode) kv4_decode;
+  decltype(&acct_kv4_evict) kv4_evict;
 } g_lib;
 
 #define HOST_CHECK TORCH_CHECK_VALUE
@@ -388,6 +392,10 @@ PyObject* py_init(PyObject*, PyObject* path) {
   g_lib.fa_bwd_workspace_bytes = reinterpret_cast<decltype(g_lib.fa_bwd_workspace_bytes)>(sym("acct_fa_bwd_workspace_bytes"));
   g_lib.infer_prefill = reinterpret_cast<decltype(g_lib.infer_prefill)>(sym("acct_infer_prefill"));
   g_lib.infer_decode = reinterpret_cast<decltype(g_lib.infer_decode)>(sym("acct_infer_decode"));
+  g_lib.kv4_append = reinterpret_cast<decltype(g_lib.kv4_append)>(sym("acct_kv4_append"));
+  g_lib.kv4_read = reinterpret_cast<decltype(g_lib.kv4_read)>(sym("acct_kv4_read"));
+  g_lib.kv4_decode = reinterpret_cast<decltype(g_lib.kv4_decode)>(sym("acct_kv4_decode"));
+  g_lib.kv4_evict = reinterpret_cast<decltype(g_lib.kv4_evict)>(sym("acct_kv4_evict"));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -536,6 +544,210 @@ PyObject* py_infer_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the cache in 4 bits.  A cache is a tuple (records, block_table | None, dtype, B, N_kv, S_max, D, page_size) that its Python
+// object keeps; its tensors were checked when it was made, what a call adds is checked here.
+struct Kv4 {
+  Tensor records, table;
+  acct_kv4_cache c;
+  at::ScalarType dtype;
+};
+Kv4 kv4_arg(PyObject* p) {
+  HOST_CHECK(PyTuple_Check(p) && PyTuple_GET_SIZE(p) == 8, "not a cache");
+  Kv4 out;
+  memset(&out.c, 0, sizeof(out.c));
+  out.records = tensor_arg(PyTuple_GET_ITEM(p, 0), "records");
+  out.table = tensor_or_undefined(PyTuple_GET_ITEM(p, 1));
+  out.c.dtype = int_arg(PyTuple_GET_ITEM(p, 2));
+  out.c.B = int_arg(PyTuple_GET_ITEM(p, 3));
+  out.c.N_kv = int_arg(PyTuple_GET_ITEM(p, 4));
+  out.c.S_max = int_arg(PyTuple_GET_ITEM(p, 5));
+  out.c.D = int_arg(PyTuple_GET_ITEM(p, 6));
+  out.c.records = out.records.data_ptr();
+  if (out.table.defined()) {
+    out.c.block_table = static_cast<const int32_t*>(out.table.const_data_ptr());
+    out.c.page_size = int_arg(PyTuple_GET_ITEM(p, 7));
+    out.c.max_pages = out.table.size(1);
+    out.c.num_pages = out.records.size(0);
+  }
+  out.dtype = out.c.dtype == ACCT_BF16 ? at::kBFloat16 : at::kHalf;
+  return out;
+}
+// `n` or more int32 on the cache's device
+Tensor ints_on(const char* name, const Tensor& t, int64_t n, const Tensor& like) {
+  require_cuda(name, t);
+  HOST_CHECK(t.device() == like.device(), name, " must be on the device of the cache, ", like.device(), ", not on ", t.device());
+  HOST_CHECK(t.numel() >= n && !t.is_floating_point(), name, " must hold ", n, " integers, got ", t.numel(), " of ", t.scalar_type());
+  return t.to(at::kInt).contiguous();
+}
+void kv4_rows(const Kv4& cache, const Tensor& start, const Tensor& cu, acct_kv4_rows& r) {
+  memset(&r, 0, sizeof(r));
+  r.start = static_cast<const int32_t*>(start.const_data_ptr());
+  if (cu.defined()) r.cu_seqlens = static_cast<const int32_t*>(cu.const_data_ptr());
+}
+
+// A tensor whose rows a kernel can read as they are, else a packed copy
+Tensor rows_readable(const Tensor& t, int64_t (&strides)[2]) {
+  bool as_is = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  for (int i = 0; i < 2; ++i) {
+    strides[i] = t.stride(i);
+    as_is = as_is && strides[i] >= t.size(2) && strides[i] % 8 == 0;
+  }
+  if (as_is) return t;
+  strides[0] = strides[1] = 0;
+  return t.contiguous();
+}
+
+// kv4_append(cache, k, v, start, cu_seqlens | None)
+PyObject* py_kv4_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 5, "kv4_append takes 5 arguments, got ", n);
+  Kv4 cache = kv4_arg(args[0]);
+  Tensor k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), start = tensor_arg(args[3], "start"), cu = tensor_or_undefined(args[4]);
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    require_on("k", k, cache.records); require_on("v", v, cache.records);
+    HOST_CHECK(k.scalar_type() == cache.dtype && v.scalar_type() == cache.dtype, "k and v must have the cache's dtype, ", cache.dtype);
+    HOST_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == cache.c.N_kv && k.size(2) == cache.c.D, "k and v must be [tokens, ",
+               cache.c.N_kv, ", ", cache.c.D, "], got ", k.sizes(), " and ", v.sizes());
+    HOST_CHECK(cu.defined() || k.size(0) == cache.c.B, "without cu_seqlens k and v hold one token for each of ", cache.c.B, " sequences, got ", k.size(0));
+    start = ints_on("start", start, cache.c.B, cache.records);
+    if (cu.defined()) cu = ints_on("cu_seqlens", cu, cache.c.B + 1, cache.records);
+    c10::cuda::OptionalCUDAGuard guard(cache.records.device());
+    acct_kv4_rows r;
+    kv4_rows(cache, start, cu, r);
+    k = rows_readable(k, r.k_stride); v = rows_readable(v, r.v_stride);
+    r.k = const_cast<void*>(k.const_data_ptr()); r.v = const_cast<void*>(v.const_data_ptr());
+    r.T = k.size(0);
+    check(g_lib.kv4_append(&cache.c, &r, stream_of(cache.records)));
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_read(cache, start, cu_seqlens | None, total) -> (k, v)
+PyObject* py_kv4_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 4, "kv4_read takes 4 arguments, got ", n);
+  Kv4 cache = kv4_arg(args[0]);
+  Tensor start = tensor_arg(args[1], "start"), cu = tensor_or_undefined(args[2]), k, v;
+  const int64_t total = int_arg(args[3]);
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    HOST_CHECK(total >= 0 && total <= INT32_MAX, "total must be the number of rows");
+    HOST_CHECK(cu.defined() || total == cache.c.B, "without cu_seqlens there is one token for each of ", cache.c.B, " sequences, not ", total);
+    start = ints_on("start", start, cache.c.B, cache.records);
+    if (cu.defined()) cu = ints_on("cu_seqlens", cu, cache.c.B + 1, cache.records);
+    c10::cuda::OptionalCUDAGuard guard(cache.records.device());
+    k = empty_like_shape({total, cache.c.N_kv, cache.c.D}, cache.dtype, cache.records);
+    v = empty_like_shape({total, cache.c.N_kv, cache.c.D}, cache.dtype, cache.records);
+    acct_kv4_rows r;
+    kv4_rows(cache, start, cu, r);
+    r.k = k.data_ptr(); r.v = v.data_ptr();
+    r.T = total;
+    check(g_lib.kv4_read(&cache.c, &r, stream_of(cache.records)));
+  }
+  PyObject* out = PyTuple_New(2);
+  PyTuple_SET_ITEM(out, 0, wrap(k));
+  PyTuple_SET_ITEM(out, 1, wrap(v));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_decode(cache, q, seq_lens | None, weights | None, scale, num_splits, workspace, out | None) -> y
+PyObject* py_kv4_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 8, "kv4_decode takes 8 arguments, got ", n);
+  Kv4 cache = kv4_arg(args[0]);
+  Tensor q = tensor_arg(args[1], "q"), lens = tensor_or_undefined(args[2]), weights = tensor_or_undefined(args[3]);
+  const double scale = float_arg(args[4]);
+  const int64_t splits = int_arg(args[5]);
+  const Tensor ws = tensor_arg(args[6], "workspace");
+  Tensor y = tensor_or_undefined(args[7]);
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    require_on("q", q, cache.records); require_on("workspace", ws, cache.records);
+    HOST_CHECK(q.scalar_type() == cache.dtype, "q must have the cache's dtype, ", cache.dtype);
+    HOST_CHECK(q.dim() == 4 && q.size(2) == 1 && q.size(0) == cache.c.B && q.size(3) == cache.c.D, "q must be [", cache.c.B, ", N, 1, ", cache.c.D,
+               "] (decode takes one query token), got ", q.sizes());
+    HOST_CHECK(splits >= INT32_MIN && splits <= INT32_MAX, "num_splits out of range");
+    c10::cuda::OptionalCUDAGuard guard(cache.records.device());
+    q = q.contiguous();
+    if (y.defined()) {
+      require_on("out", y, q);
+      HOST_CHECK(y.scalar_type() == q.scalar_type() && y.is_contiguous() && y.numel() == q.numel(),
+                 "out must be a contiguous tensor with the dtype and the number of elements of q");
+    } else {
+      y = empty_like_shape(q.sizes(), q.scalar_type(), q);
+    }
+    acct_kv4_decode_args a;
+    memset(&a, 0, sizeof(a));
+    a.N = q.size(1);
+    a.q = q.const_data_ptr(); a.y = y.data_ptr();
+    if (lens.defined()) {
+      lens = ints_on("seq_lens", lens, cache.c.B, cache.records);
+      a.seq_lens = static_cast<const int32_t*>(lens.const_data_ptr());
+    }
+    if (weights.defined()) {
+      require_on("weights", weights, q);
+      HOST_CHECK(weights.scalar_type() == at::kFloat && weights.is_contiguous() && weights.dim() == 3 && weights.size(0) == cache.c.B &&
+                     weights.size(1) == cache.c.N_kv && weights.size(2) == cache.c.S_max,
+                 "weights must be a contiguous float32 tensor [", cache.c.B, ", ", cache.c.N_kv, ", ", cache.c.S_max, "], got ", weights.sizes());
+      a.weights = static_cast<float*>(weights.data_ptr());
+    }
+    a.scale = static_cast<float>(scale);
+    a.num_splits = splits;
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = ws.nbytes();
+    check(g_lib.kv4_decode(&cache.c, &a, stream_of(q)));
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// kv4_evict(src, dst, weights, seq_lens, keep, recent) -> (kept, weights_out, seq_lens_out)
+PyObject* py_kv4_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 6, "kv4_evict takes 6 arguments, got ", n);
+  Kv4 src = kv4_arg(args[0]), dst = kv4_arg(args[1]);
+  Tensor weights = tensor_arg(args[2], "weights"), lens = tensor_arg(args[3], "seq_lens"), kept, weights_out, lens_out;
+  const int64_t keep = int_arg(args[4]), recent = int_arg(args[5]);
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    require_on("weights", weights, src.records);
+    HOST_CHECK(dst.records.device() == src.records.device(), "both caches must be on one device");
+    HOST_CHECK(weights.scalar_type() == at::kFloat && weights.dim() == 3 && weights.size(0) == src.c.B && weights.size(1) == src.c.N_kv &&
+                   weights.size(2) == src.c.S_max,
+               "weights must be a float32 tensor [", src.c.B, ", ", src.c.N_kv, ", ", src.c.S_max, "], got ", weights.sizes());
+    HOST_CHECK(keep >= 1 && keep <= dst.c.S_max && recent >= 0 && recent <= keep, "need 0 <= recent <= keep and 1 <= keep <= ", dst.c.S_max,
+               " (the slots of the smaller cache), got keep ", keep, " and recent ", recent);
+    weights = weights.contiguous();
+    lens = ints_on("seq_lens", lens, src.c.B, src.records);
+    c10::cuda::OptionalCUDAGuard guard(src.records.device());
+    kept = empty_like_shape({src.c.B, src.c.N_kv, keep}, at::kInt, weights);
+    weights_out = empty_like_shape({src.c.B, src.c.N_kv, dst.c.S_max}, at::kFloat, weights);
+    lens_out = empty_like_shape({src.c.B}, at::kInt, weights);
+    acct_kv4_evict_args a;
+    memset(&a, 0, sizeof(a));
+    a.weights = static_cast<const float*>(weights.const_data_ptr());
+    a.weights_out = static_cast<float*>(weights_out.data_ptr());
+    a.kept = static_cast<int32_t*>(kept.data_ptr());
+    a.seq_lens = static_cast<const int32_t*>(lens.const_data_ptr());
+    a.seq_lens_out = static_cast<int32_t*>(lens_out.data_ptr());
+    a.keep = keep; a.recent = recent;
+    check(g_lib.kv4_evict(&src.c, &dst.c, &a, stream_of(weights)));
+  }
+  PyObject* out = PyTuple_New(3);
+  PyTuple_SET_ITEM(out, 0, wrap(kept));
+  PyTuple_SET_ITEM(out, 1, wrap(weights_out));
+  PyTuple_SET_ITEM(out, 2, wrap(lens_out));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)); }
 
@@ -544,6 +756,10 @@ PyMethodDef kMethods[] = {
     {"fa_apply", fast<py_fa_apply>(), METH_FASTCALL, "training operator, differentiable"},
     {"infer_prefill", fast<py_infer_prefill>(), METH_FASTCALL, "inference op"},
     {"infer_decode", fast<py_infer_decode>(), METH_FASTCALL, "one decoding step"},
+    {"kv4_append", fast<py_kv4_append>(), METH_FASTCALL, "rows into a cache in 4 bits"},
+    {"kv4_read", fast<py_kv4_read>(), METH_FASTCALL, "rows out of a cache in 4 bits"},
+    {"kv4_decode", fast<py_kv4_decode>(), METH_FASTCALL, "one decoding step over a cache in 4 bits"},
+    {"kv4_evict", fast<py_kv4_evict>(), METH_FASTCALL, "what stays of a cache in 4 bits, into another one"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_host", "native host path of acctransformer_b200", -1, kMethods,

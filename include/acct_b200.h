@@ -322,6 +322,79 @@ ACCT_API int acct_infer_decode(const acct_decode_args* a, void* stream);
 #define ACCT_DECODE_STATIC_SCRATCH_BYTES (8 * 1024 * 1024)
 ACCT_API int acct_infer_decode_static(const acct_decode_args* a, void* stream);
 
+/* ---- A key/value cache held in 4 bits.  No counterpart in the reference (it has no cache).
+ *
+ * Of every row (one token, one head; K and V alike) up to 32 neighbouring values share a minimum m and a step s, both in the
+ * cache's 16-bit type, and each is a code of 4 bits that stands for code * s + m:
+ *   m = min x;  s = (max x - m) / 15, rounded down to 16 bits;  code = round((x - m) / s), half to even, at most 15
+ * ((x - m) times 1 / s, each step rounded to fp32; s = 0 gives codes of 0).  A group with a value that is not finite, or whose
+ * range is not, reads as NaN.  That is 0.625 bytes a value: 160 bytes for a row of K and V at head_dim 128 instead of 512.
+ *
+ * 16 rows of a head are one record of acct_kv4_record_bytes(D) bytes, whose inner layout is the library's own.  Contents need no
+ * initialisation: slots at or past a sequence's length are never looked at, whatever they hold. */
+typedef struct acct_kv4_cache {
+  int32_t dtype;            /* ACCT_F16 or ACCT_BF16: type of the rows that go in and come out */
+  int32_t B, N_kv, D;       /* sequences, heads, head_dim: a multiple of 8 up to 128 */
+  int32_t S_max;            /* slots per sequence (paged: max_pages * page_size) */
+  void* records;            /* device, 16-byte aligned: [B, N_kv, ceil(S_max / 16)] records, or, with a block_table, a pool
+                               [num_pages, N_kv, page_size / 16] of them */
+  const int32_t* block_table; /* device [B, max_pages] or NULL: slot s of sequence b is row s % page_size of page
+                               block_table[b, s / page_size]; a number outside [0, num_pages) stands for the nearest one inside */
+  int32_t page_size;        /* a power of two >= 16 */
+  int32_t max_pages, num_pages;
+} acct_kv4_cache;
+
+ACCT_API size_t acct_kv4_record_bytes(int32_t D);
+
+/* Rows of tokens [T, N_kv, D] into slots of their sequences (append) and out of them (read).  Sequence b has rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1, and the first of them is slot start[b]; a row whose slot is outside [0, S_max) is
+ * neither written nor read.  Lengths are the caller's: nothing of the cache says how much of it is in use. */
+typedef struct acct_kv4_rows {
+  void* k;                  /* device [T, N_kv, D]; append reads them, read writes them */
+  void* v;
+  int64_t k_stride[2];      /* element strides of token and head, multiples of 8; 0 = packed */
+  int64_t v_stride[2];
+  int32_t T;
+  const int32_t* cu_seqlens;/* device [B + 1], ascending from 0 to T; NULL: one row per sequence, T = B */
+  const int32_t* start;     /* device [B] */
+} acct_kv4_rows;
+
+ACCT_API int acct_kv4_append(const acct_kv4_cache* c, const acct_kv4_rows* r, void* stream);
+ACCT_API int acct_kv4_read(const acct_kv4_cache* c, const acct_kv4_rows* r, void* stream);
+
+/* Decode over such a cache: acct_infer_decode's result on the values that it stands for.  A sequence of length 0 gives zeros.
+ * With `weights` the probability that each key received, summed over the query heads of its group, is added to
+ * weights[b, head, slot]; slots past the length are left alone. */
+typedef struct acct_kv4_decode_args {
+  int32_t N;                /* query heads: a multiple of N_kv, up to 16 per cache head */
+  const void* q;            /* device [B, N, 1, D] packed, in the cache's type */
+  void* y;                  /* the same */
+  const int32_t* seq_lens;  /* device [B], each in [0, S_max]; NULL = S_max everywhere */
+  float* weights;           /* device [B, N_kv, S_max] fp32, or NULL */
+  float scale;
+  int32_t num_splits;       /* key ranges per sequence and head, up to 64; 0 = chosen by the library, no more than fit the workspace */
+  void* workspace;          /* device, 16-byte aligned, >= acct_kv4_decode_workspace_bytes() */
+  size_t workspace_bytes;
+} acct_kv4_decode_args;
+
+ACCT_API size_t acct_kv4_decode_workspace_bytes(const acct_kv4_cache* c, int32_t N, int32_t num_splits, int32_t with_weights);
+ACCT_API int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void* stream);
+
+/* Eviction by accumulated weight.  Of every sequence and head min(length, keep) slots stay: the last `recent` ones, and of those
+ * before them the ones with the largest weights (equal ones: the lowest slots; a NaN counts as the largest).  They go to slots
+ * 0, 1, .. of `dst` in their order, their codes as they are.  `dst` is another cache of the same B, N_kv, D and dtype with at
+ * least `keep` slots (one spare cache serves all layers in turn). */
+typedef struct acct_kv4_evict_args {
+  const float* weights;     /* device [B, N_kv, src S_max] fp32 */
+  float* weights_out;       /* device [B, N_kv, dst S_max] fp32: those of what stays, 0 behind it */
+  int32_t* kept;            /* device [B, N_kv, keep]: the slots that stay, ascending, then -1 */
+  const int32_t* seq_lens;  /* device [B] */
+  int32_t* seq_lens_out;    /* device [B]: min(length, keep); may not be seq_lens */
+  int32_t keep, recent;     /* 0 <= recent <= keep, keep >= 1 */
+} acct_kv4_evict_args;
+
+ACCT_API int acct_kv4_evict(const acct_kv4_cache* src, const acct_kv4_cache* dst, const acct_kv4_evict_args* a, void* stream);
+
 /* The same operators behind the calling convention MindSpore uses for ops.Custom(func_type="aot"):
  *   int f(int nparam, void** params, int* ndims, int64_t** shapes, const char** dtypes, void* stream, void* extra)
  * with params = the inputs followed by the outputs (device pointers), dtypes as MindSpore names them ("float16",
