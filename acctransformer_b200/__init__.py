@@ -3,7 +3,8 @@ TriangleAttention and the inference prefill/decode op behind the reference's Pyt
 running hand-written sm_100a CUDA through the C ABI in ``include/acct_b200.h``."""
 
 __all__ = ["FlashAttention", "TriangleAttention", "get_flash_attention", "get_flash_attention_grad",
-           "FlashAttentionTik", "flash_attention_tik", "flash_attention_decode", "Kv4Cache", "Kv4Workspace"]
+           "FlashAttentionTik", "flash_attention_tik", "flash_attention_decode", "flash_attention_packed",
+           "Kv4Cache", "Kv4Workspace"]
 
 
 def __getattr__(name):
@@ -16,7 +17,7 @@ def __getattr__(name):
     if name in ("get_flash_attention", "get_flash_attention_grad"):
         from .flash_attention.ops.flash_attention import flash_attention_impl as m
         return getattr(m, name)
-    if name in ("FlashAttentionTik", "flash_attention_tik", "flash_attention_decode"):
+    if name in ("FlashAttentionTik", "flash_attention_tik", "flash_attention_decode", "flash_attention_packed"):
         from .infer import flash_attention as m
         return getattr(m, name)
     if name in ("Kv4Cache", "Kv4Workspace"):

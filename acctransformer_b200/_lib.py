@@ -33,7 +33,7 @@ EXPORTS = [
     "acct_ms_set_fa_attrs", "acct_ms_fa_fwd", "acct_ms_fa_grad", "acct_ms_infer_fa", "acct_dropout_mask",
     "acct_mask_is_causal", "acct_mask_tiles_bytes", "acct_mask_classify_tiles", "acct_mask_tiles_scratch",
     "acct_selftest_wait_timeout", "acct_ms_fa_attrs_slot", "acct_ms_fa_attrs_slot_ex",
-    "acct_kv4_record_bytes", "acct_kv4_append", "acct_kv4_read", "acct_kv4_decode_workspace_bytes", "acct_kv4_decode",
+    "acct_infer_packed", "acct_kv4_record_bytes", "acct_kv4_append", "acct_kv4_read", "acct_kv4_decode_workspace_bytes", "acct_kv4_decode",
     "acct_kv4_evict",
 ] + [f"acct_ms_fa_{kind}_s{k}" for k in range(32) for kind in ("fwd", "grad")]
 
@@ -92,6 +92,16 @@ class DecodeArgs(C.Structure):
         ("scale", C.c_float), ("num_splits", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("N_kv", C.c_int32),
         ("block_table", C.c_void_p), ("page_size", C.c_int32), ("max_pages", C.c_int32),
+    ]
+
+
+class PackedArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("N_kv", C.c_int32),
+        ("T_q", C.c_int32), ("T_k", C.c_int32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("y", C.c_void_p), ("lse", C.c_void_p),
+        ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2), ("y_stride", C.c_int64 * 2),
+        ("cu_seqlens_q", C.c_void_p), ("cu_seqlens_k", C.c_void_p), ("causal", C.c_int32), ("scale", C.c_float),
     ]
 
 
@@ -188,6 +198,8 @@ def load():
     lib.acct_mask_classify_tiles.restype = C.c_int
     lib.acct_selftest_wait_timeout.argtypes = [C.c_void_p]
     lib.acct_selftest_wait_timeout.restype = C.c_int
+    lib.acct_infer_packed.argtypes = [C.POINTER(PackedArgs), C.c_void_p]
+    lib.acct_infer_packed.restype = C.c_int
     lib.acct_kv4_record_bytes.argtypes = [C.c_int32]
     lib.acct_kv4_record_bytes.restype = C.c_size_t
     lib.acct_kv4_append.argtypes = [C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows), C.c_void_p]

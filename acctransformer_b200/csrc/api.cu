@@ -1,5 +1,6 @@
 // C-ABI entry points of libacct_b200.so: argument validation (the role the reference's Python
 // checks and its C++ InferShape play), tensor-map construction and kernel launches.
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <stdarg.h>
@@ -699,6 +700,79 @@ int acct_infer_prefill(const acct_infer_args* a, void* stream) {
   f.keep_prob = 1.0f;
   f.N_kv = a->N_kv;
   return acct_fa_fwd(&f, stream);
+}
+
+int acct_infer_packed(const acct_packed_args* a, void* stream) {
+  if (a == nullptr) return fail(ACCT_ERR_NULL, "args is NULL");
+  if (a->dtype != ACCT_F16 && a->dtype != ACCT_BF16) return fail(ACCT_ERR_DTYPE, "dtype must be ACCT_F16 or ACCT_BF16");
+  if (a->B <= 0 || a->N <= 0) return fail(ACCT_ERR_SHAPE, "B and N must be positive");
+  if (a->T_q < 0 || a->T_k < 0) return fail(ACCT_ERR_SHAPE, "T_q and T_k must not be negative");
+  if (a->N_kv < 0 || (a->N_kv > 0 && a->N % a->N_kv != 0))
+    return fail(ACCT_ERR_SHAPE, "N_kv = %d must be 0 or a divisor of N = %d", a->N_kv, a->N);
+  const int n_kv = a->N_kv > 0 ? a->N_kv : a->N;
+  int rc = check_head_dim(a->D, kMaxHeadDimFwd, "forward");
+  if (rc) return rc;
+  if (!a->cu_seqlens_q) return fail(ACCT_ERR_NULL, "cu_seqlens_q is NULL");
+  if ((a->T_q > 0 && (!a->q || !a->y)) || (a->T_k > 0 && (!a->k || !a->v))) return fail(ACCT_ERR_NULL, "q, k, v, y must be non-NULL");
+  if (a->cu_seqlens_k == nullptr && a->T_k != a->T_q) return fail(ACCT_ERR_SHAPE, "without cu_seqlens_k, T_k = %d must be T_q = %d", a->T_k, a->T_q);
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->y))
+    return fail(ACCT_ERR_ALIGN, "q, k, v, y must be 16-byte aligned");
+  if (!(a->scale > 0.f) || !(a->scale < 1e30f)) return fail(ACCT_ERR_SHAPE, "scale must be a positive finite number");
+  // as one batch entry: strides of row, head
+  struct Operand {
+    const char* name;
+    const void* ptr;
+    const int64_t* stride;
+    int rows, heads;
+    CUtensorMap* map;
+  };
+  FwdParams p;
+  memset(&p, 0, sizeof(p));
+  const Operand operands[4] = {{"q", a->q, a->q_stride, a->T_q, a->N, &p.map_q},
+                               {"k", a->k, a->k_stride, a->T_k, n_kv, &p.map_k},
+                               {"v", a->v, a->v_stride, a->T_k, n_kv, &p.map_v},
+                               {"y", a->y, a->y_stride, a->T_q, a->N, &p.map_o}};
+  int64_t strides[4][2];
+  for (int i = 0; i < 4; ++i) {
+    const Operand& x = operands[i];
+    strides[i][0] = packed_or(x.stride[0], static_cast<int64_t>(x.heads) * a->D);
+    strides[i][1] = packed_or(x.stride[1], a->D);
+    for (int64_t s : strides[i]) {
+      if (s < a->D) return fail(ACCT_ERR_SHAPE, "%s strides must not be smaller than head_dim", x.name);
+      if (s % 8 != 0) return fail(ACCT_ERR_ALIGN, "%s stride (%lld elements) is not a multiple of 8", x.name, (long long)s);
+    }
+  }
+  PerDevice* dev = nullptr;
+  if ((rc = init_device(&dev))) return rc;
+  if (a->T_q == 0) return ACCT_OK;
+  const int64_t tiles = (static_cast<int64_t>(a->T_q) + 127ll * a->B) / 128 + 1;
+  if (tiles * a->N > INT32_MAX) return fail(ACCT_ERR_SHAPE, "T_q = %d rows of N = %d heads are too many for one call", a->T_q, a->N);
+  for (int i = 0; i < 4; ++i) {
+    TensorDesc4 t;
+    t.dtype = a->dtype;
+    const bool none = operands[i].rows == 0;       // no keys at all: a map of one row that no load asks for
+    t.ptr = none ? a->q : operands[i].ptr;
+    t.dims[0] = a->D; t.dims[1] = none ? 1 : operands[i].rows; t.dims[2] = none ? 1 : operands[i].heads; t.dims[3] = 1;
+    t.strides[0] = strides[i][0]; t.strides[1] = strides[i][1];
+    t.strides[2] = std::max(strides[i][0], strides[i][1]);      // (of a dimension of size 1)
+    if ((rc = make_tmap_4d(operands[i].map, t, kTile))) return rc;
+  }
+  p.o = a->y;
+  p.lse = a->lse;
+  p.o_stride_s = strides[3][0]; p.o_stride_h = strides[3][1];
+  p.B = a->B; p.N = a->N; p.S_q = a->T_q; p.S_k = a->T_k; p.D = a->D;
+  p.T_q = a->T_q; p.T_k = a->T_k;
+  p.cu_q = a->cu_seqlens_q;
+  p.cu_k = a->cu_seqlens_k != nullptr ? a->cu_seqlens_k : a->cu_seqlens_q;
+  p.kv_group = a->N / n_kv;
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * kLog2e;
+  p.mods.causal = a->causal ? 1 : 0;
+  p.mods.prev_block_num = p.mods.next_block_num = ACCT_BAND_UNBOUNDED;
+  p.status = dev->status;
+  const cudaError_t e = launch_fa_fwd_packed(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda(e, "launching the packed forward kernel");
+  return ACCT_OK;
 }
 
 size_t acct_infer_decode_workspace_bytes(const acct_decode_args* a) {

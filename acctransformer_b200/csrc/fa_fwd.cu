@@ -65,6 +65,11 @@ __device__ __forceinline__ TileRange kv_tile_range(int i, int s_q, int kv_len, c
   return r;
 }
 
+// What a thread block of the packed form works on: tile (pair) `pair` of the sequence whose rows begin at q0 and k0.
+struct PackedItem {
+  int pair, q0, len_q, k0, len_k;
+};
+
 struct FwdShared {
   uint64_t q_full;
   uint64_t k_full[kStages], k_empty[kStages];
@@ -77,14 +82,111 @@ struct FwdShared {
   volatile uint32_t abort_flag;
   uint32_t need[2][kPlanWords];           // K/V tiles of each Q tile that the mask plan leaves (all ones without a plan)
   alignas(16) float alibi[2][2][kTile];   // [softmax group][tile parity]: alibi row of the K/V tile, log2 units
+  PackedItem item;
 };
+
+// The `item`-th tile (pair) of all sequences, those with the most K/V tiles first (a late start of a long one is what the SMs
+// would wait for at the end); len_q = 0 where there are not so many.  One warp; a lane has sequences lane, lane + 32, ...  Up to
+// 128 sequences the order comes from a search over the number of K/V tiles, which no plan made beforehand could do much faster
+// (some 500 clk while the block sets itself up); with more, long ones matter less, and they come one after the other.
+template <int NQ>
+__device__ __forceinline__ void find_packed_item(const FwdParams& p, int item, PackedItem* out) {
+  constexpr int kRows = NQ * kTile, kPer = 4;
+  const int lane = threadIdx.x & 31;
+  auto read = [&](int b, PackedItem& s) {      // (whatever cu holds, no row outside [0, T) is touched)
+    s.q0 = min(max(p.cu_q[b], 0), p.T_q);
+    s.len_q = min(max(p.cu_q[b + 1], s.q0), p.T_q) - s.q0;
+    s.k0 = min(max(p.cu_k[b], 0), p.T_k);
+    s.len_k = min(max(p.cu_k[b + 1], s.k0), p.T_k) - s.k0;
+  };
+  // pairs of the sequence with `tiles` or more K/V tiles: from a certain one on, with a causal mask
+  auto pairs_with = [&](const PackedItem& s, int tiles) {
+    const int n = (s.len_q + kRows - 1) / kRows;
+    if (tiles <= 0) return n;
+    const int keys = (tiles - 1) * kTile + 1;                  // a pair that sees this many
+    if (s.len_k < keys) return 0;
+    if (!p.mods.causal) return n;
+    const int rows = keys - (s.len_k - s.len_q);               // ... has its last row here or later
+    return n - min(n, max(0, (rows + kRows - 1) / kRows - 1));
+  };
+  PackedItem found = {0, 0, 0, 0, 0};
+  auto settle = [&](const PackedItem& s, int n, int first, int& left) {      // true where the item is one of this round's
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const unsigned int past = __ballot_sync(0xffffffffu, upto > left);
+    if (past == 0u) {
+      left -= __shfl_sync(0xffffffffu, upto, 31);
+      return false;
+    }
+    const int from = __ffs(past) - 1;
+    found.pair = __shfl_sync(0xffffffffu, first, from) + left - __shfl_sync(0xffffffffu, upto - n, from);
+    found.q0 = __shfl_sync(0xffffffffu, s.q0, from);
+    found.len_q = __shfl_sync(0xffffffffu, s.len_q, from);
+    found.k0 = __shfl_sync(0xffffffffu, s.k0, from);
+    found.len_k = __shfl_sync(0xffffffffu, s.len_k, from);
+    return true;
+  };
+  if (p.B <= 32 * kPer) {
+    PackedItem s[kPer];
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      s[i] = {0, 0, 0, 0, 0};
+      if (lane + 32 * i < p.B) read(lane + 32 * i, s[i]);
+      most = max(most, (s[i].len_k + kTile - 1) / kTile);
+    }
+    auto count = [&](int tiles) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) n += pairs_with(s[i], tiles);
+      return __reduce_add_sync(0xffffffffu, n);
+    };
+    most = __reduce_max_sync(0xffffffffu, most);
+    int lo = 0, hi = most + 1, before = 0;       // count(lo) > item >= count(hi) = before
+    if (count(0) > item) {
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2, n = count(mid);
+        if (n > item) lo = mid;
+        else { hi = mid; before = n; }
+      }
+      int left = item - before;                  // among the pairs with exactly `lo` tiles
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (!done) {
+          const int least = pairs_with(s[i], lo), n = least - pairs_with(s[i], lo + 1);
+          done = settle(s[i], n, (s[i].len_q + kRows - 1) / kRows - least, left);
+        }
+    }
+  } else {
+    int left = item;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      PackedItem s = {0, 0, 0, 0, 0};
+      if (b0 + lane < p.B) read(b0 + lane, s);
+      const int n = pairs_with(s, 0);
+      if (settle(s, n, 0, left)) {
+        found.pair = (found.len_q + kRows - 1) / kRows - 1 - found.pair;
+        break;
+      }
+    }
+  }
+  if (lane == 0) *out = found;
+}
 
 }  // namespace
 
 // MODS: bit 0 = a mask tensor may be present, bit 1 = alibi may be present.  DROP: 0 no dropout, 1 in-kernel
 // generator, 2 dropout mask tensor of any type, 3 uint8 {0,1} mask tensor with 16-byte aligned rows read as byte masks.  Every instantiation carries only the code of what it may meet: code that is
 // compiled in but never run still costs the common path of every tile (register allocation, spills).
-template <int DPAD, bool BF16, int MODS, int DROP>
+// PACKED: sequences of different lengths, one behind the other in [T, N, D] tensors, a causal mask that ends at the last key of
+// the sequence, or none; MODS = DROP = 0.  A tile's TMA loads run on into the next sequence's rows: their scores are left out
+// like those past a valid length, their rows of V are zeroed in shared memory (0 times what they hold might be a NaN), and
+// a cut tile of O leaves by plain stores.
+template <int DPAD, bool BF16, int MODS, int DROP, bool PACKED = false>
 __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_constant__ FwdParams p) {
   constexpr int NB = DPAD / 64;                 // 64-column (128-byte) blocks per row
   constexpr uint32_t kTileBytes = NB * 16384u;  // one 128-row tile
@@ -115,7 +217,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
   const int n_pairs = (p.S_q + NQ * kTile - 1) / (NQ * kTile);
   const int n_units = p.B * p.N;
   int bh, pair;
-  {
+  int len_q = p.S_q, q_base = 0, k_base = 0;     // PACKED: of the sequence
+  if constexpr (PACKED) {
+    const int per_group = p.tile_bound * p.head_group;
+    const int hg = blockIdx.x / per_group, within = blockIdx.x % per_group;
+    const int heads = min(p.head_group, p.N - hg * p.head_group);
+    bh = hg * p.head_group + within % heads;
+    if (warp == 0) find_packed_item<NQ>(p, within / heads, &sh.item);
+    __syncthreads();
+    pair = sh.item.pair; len_q = sh.item.len_q; q_base = sh.item.q0; k_base = sh.item.k0;
+  } else {
     const int kUnitGroup = p.unit_group;
     const int per_group = n_pairs * kUnitGroup;
     const int g = blockIdx.x / per_group;
@@ -124,14 +235,26 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
     pair = n_pairs - 1 - within / g_units;
     bh = g * kUnitGroup + within % g_units;
   }
-  const int b = bh / p.N, h = bh % p.N;
+  const int b = PACKED ? 0 : bh / p.N, h = PACKED ? bh : bh % p.N;
   const int h_kv = h / p.kv_group;   // grouped-query attention: several query heads read one key/value head
 
-  int kv_len = p.S_k;
-  if (mods.seq_lens != nullptr) kv_len = min(p.S_k, max(0, mods.seq_lens[b]));
+  int kv_len = PACKED ? sh.item.len_k : p.S_k;
+  if (!PACKED && mods.seq_lens != nullptr) kv_len = min(p.S_k, max(0, mods.seq_lens[b]));
 
   TileRange r0 = kv_tile_range(NQ * pair, p.S_q, kv_len, mods);
   TileRange r1 = kv_tile_range(NQ * pair + 1, p.S_q, kv_len, mods);
+  const int behind = kv_len - len_q;             // PACKED: keys that the first row sees besides its own
+  if constexpr (PACKED) {
+    auto range = [&](int i) {
+      TileRange r = {0, (kv_len + kTile - 1) / kTile - 1};
+      const int last_key = min(i * kTile + kTile, len_q) - 1 + behind;
+      if (mods.causal) r.hi = last_key < 0 ? -1 : min(r.hi, last_key / kTile);
+      if (i * kTile >= len_q) r.hi = -1;
+      return r;
+    };
+    r0 = range(NQ * pair);
+    r1 = range(NQ * pair + 1);
+  }
   if (NQ == 1) { r1.lo = 0; r1.hi = -1; }
   // Tiles that the mask plan leaves out: every role walks the same bits.  The ranges shrink to the first and last tile
   // needed, and the others are skipped one by one (next_tile, needed).
@@ -209,20 +332,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
       for (int qt = 0; qt < NQ; ++qt)
         for (int nb = 0; nb < blocks; ++nb)
           tma_load_4d(sQ + qt * kTileBytes + nb * 16384, &p.map_q, &sh.q_full, nb * 64,
-                      (NQ * pair + qt) * kTile, h, b);
+                      q_base + (NQ * pair + qt) * kTile, h, b);
       auto load_k = [&](int it, int j) {
         const int st = it % kSt;
         if (it >= kSt) mbar_wait(&sh.k_empty[st], ((it / kSt) - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         mbar_expect_tx(&sh.k_full[st], tile_bytes);
         for (int nb = 0; nb < blocks; ++nb)
-          tma_load_4d(sK + st * kTileBytes + nb * 16384, &p.map_k, &sh.k_full[st], nb * 64, j * kTile, h_kv, b);
+          tma_load_4d(sK + st * kTileBytes + nb * 16384, &p.map_k, &sh.k_full[st], nb * 64, k_base + j * kTile, h_kv, b);
       };
       auto load_v = [&](int it, int j) {
         const int st = it % kSt;
         if (it >= kSt) mbar_wait(&sh.v_empty[st], ((it / kSt) - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         mbar_expect_tx(&sh.v_full[st], tile_bytes);
         for (int nb = 0; nb < blocks; ++nb)
-          tma_load_4d(sV + st * kTileBytes + nb * 16384, &p.map_v, &sh.v_full[st], nb * 64, j * kTile, h_kv, b);
+          tma_load_4d(sV + st * kTileBytes + nb * 16384, &p.map_v, &sh.v_full[st], nb * 64, k_base + j * kTile, h_kv, b);
       };
       if constexpr (NQ == 1) {
         // the scores run a tile ahead of P V: K of the next tile before V of this one
@@ -462,8 +585,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
     // group, causal triangle.  `bound_tile` is the smallest bound of any row of the tile.
     const int tri_end = mods.tri_block > 0 ? (min(q_row, p.S_q - 1) / mods.tri_block + 1) * mods.tri_block : 0x7fffffff;
     const int tri_end_tile = mods.tri_block > 0 ? ((q_tile * kTile) / mods.tri_block + 1) * mods.tri_block : 0x7fffffff;
-    const int bound = min(min(kv_len, tri_end), mods.causal ? q_row + 1 : 0x7fffffff);
-    const int bound_tile = min(min(kv_len, tri_end_tile), mods.causal ? q_tile * kTile + 1 : 0x7fffffff);
+    const int shift = PACKED ? behind : 0;
+    const int bound = min(min(kv_len, tri_end), mods.causal ? q_row + shift + 1 : 0x7fffffff);
+    const int bound_tile = min(min(kv_len, tri_end_tile), mods.causal ? q_tile * kTile + shift + 1 : 0x7fffffff);
 
     // Optional per-tile summary of a full mask tensor: the class of tile (q_tile, j) is fetched one tile ahead,
     // before the wait for S, so that its latency is not on the path.
@@ -750,6 +874,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
         mbar_wait(&sh.o_done[qt], (n - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
         tc_fence_after_sync();
       }
+      if constexpr (PACKED) if (col_base + kTile > kv_len) {
+        // Rows of V that are not this sequence's (either group does it, and neither P V starts before its group has).  The P V
+        // of the tile before has been waited for, or was issued before the scores, and this tile's waits for this group: the
+        // stage's barrier can be in no other phase than this tile's.
+        const int at = j - cta_lo;
+        mbar_wait(&sh.v_full[at % kSt], (at / kSt) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+        if (col_base + row_in_tile >= kv_len)
+          for (int nb = 0; nb < NB; ++nb) {
+            uint4* row = reinterpret_cast<uint4*>(sV + (at % kSt) * kTileBytes + nb * 16384 + row_in_tile * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        fence_proxy_async_smem();
+      }
       if (n > 0 && any_grow) {
         // O of the previous tiles is complete: the S MMA just waited for was issued after their P V, or, where the scores
         // run ahead, that P V has been waited for
@@ -802,7 +940,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
 
     // epilogue: O / l through this group's (now dead) Q tile in shared memory and a TMA store, which
     // clips rows past S_q and columns past D; L = m + ln l straight to global memory
-    if (qt < NQ && q_tile * kTile < p.S_q) {
+    if (qt < NQ && q_tile * kTile < len_q) {
       if (n > 0) {
         mbar_wait(&sh.o_done[qt], NQ == 1 || kAhead ? (n - 1) & 1 : 0, abort_flag, p.status, DEV_TIMEOUT_MMA);
         tc_fence_after_sync();
@@ -816,7 +954,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
       for (int c = 0; c < DPAD / 32 && (NQ > 1 || c * 32 < p.D); ++c) {
         uint32_t r[32];
         if (n > 0) { tmem_ld32(t_o + c * 32, r); tmem_wait_ld(); }
-        else {
+        if (n == 0 || (PACKED && l_run == 0.f)) {      // (a row that sees nothing: 0, also where V is not finite)
 #pragma unroll
           for (int i = 0; i < 32; ++i) r[i] = 0u;
         }
@@ -832,13 +970,25 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
       }
       fence_proxy_async_smem();
       named_barrier(1 + qt, 128);
-      if (row_in_tile == 0) {
+      const bool cut = PACKED && (q_tile + 1) * kTile > len_q;     // the rows behind it are the next sequence's
+      if (cut) {
+        const int rows = len_q - q_tile * kTile, per_row = p.D / 8;
+        uint16_t* at = static_cast<uint16_t*>(p.o) + (static_cast<int64_t>(q_base) + q_tile * kTile) * p.o_stride_s + h * p.o_stride_h;
+        for (int i = row_in_tile; i < rows * per_row; i += 128) {
+          const int row = i / per_row, chunk = i % per_row;
+          *reinterpret_cast<uint4*>(at + row * p.o_stride_s + chunk * 8) =
+              *reinterpret_cast<const uint4*>(stage + (chunk >> 3) * 16384 + swz128(row, chunk & 7));
+        }
+      } else if (row_in_tile == 0) {
         for (int nb = 0; nb < NB; ++nb)
-          if (nb * 64 < p.D) tma_store_4d(&p.map_o, stage + nb * 16384, nb * 64, q_tile * kTile, h, b);
+          if (nb * 64 < p.D) tma_store_4d(&p.map_o, stage + nb * 16384, nb * 64, q_base + q_tile * kTile, h, b);
         tma_store_commit();
         tma_store_wait_read();
       }
-      if (q_row < p.S_q && p.lse != nullptr)
+      if constexpr (PACKED) {
+        if (q_row < len_q && p.lse != nullptr)
+          p.lse[static_cast<int64_t>(h) * p.T_q + q_base + q_row] = n > 0 && l_run != 0.f ? m_run * kLn2 + logf(l_run) : kNegInf;
+      } else if (q_row < p.S_q && p.lse != nullptr)
         p.lse[static_cast<int64_t>(bh) * p.S_q + q_row] =
             (n > 0 && l_run > 0.f) ? m_run * kLn2 + logf(l_run) : kNegInf;
     }
@@ -952,6 +1102,25 @@ cudaError_t launch_mask_classify(const void* mask, int dtype, int batch, int S_q
   const bool vec = (static_cast<int64_t>(S_k) * esize) % 16 == 0 && (reinterpret_cast<uintptr_t>(mask) & 15u) == 0;
   if (vec) mask_classify_kernel<true><<<grid, 256, 0, stream>>>(mask, dtype, S_q, S_k, tiles);
   else mask_classify_kernel<false><<<grid, 256, 0, stream>>>(mask, dtype, S_q, S_k, tiles);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_fa_fwd_packed(const FwdParams& p, bool bf16, cudaStream_t stream) {
+  const int dpad = p.D <= 64 ? 64 : (p.D <= 128 ? 128 : 256);
+  const int nq = dpad > 128 ? 1 : 2, stages = dpad > 128 ? 1 : kStages, rows = nq * kTile;
+  const size_t smem = static_cast<size_t>(nq + 2 * stages) * (dpad / 64) * 16384 + 1024;
+  FwdParams pp = p;
+  pp.tile_bound = static_cast<int>((static_cast<int64_t>(p.T_q) + static_cast<int64_t>(rows - 1) * p.B) / rows);
+  // Heads that run at the same time share L2: as many as have their K and V in 48 MB of it, whole groups of query heads.
+  const int64_t head_bytes = 4ll * p.T_k * p.D;
+  const int64_t fit = (48ll << 20) / (head_bytes > 0 ? head_bytes : 1);
+  pp.head_group = static_cast<int>(fit < 1 ? p.kv_group : fit * p.kv_group < p.N ? fit * p.kv_group : p.N);
+  void (*kern)(const FwdParams) = dpad == 64    ? (bf16 ? fa_fwd_kernel<64, true, 0, 0, true> : fa_fwd_kernel<64, false, 0, 0, true>)
+                                  : dpad == 128 ? (bf16 ? fa_fwd_kernel<128, true, 0, 0, true> : fa_fwd_kernel<128, false, 0, 0, true>)
+                                                : (bf16 ? fa_fwd_kernel<256, true, 0, 0, true> : fa_fwd_kernel<256, false, 0, 0, true>);
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
+  if (e != cudaSuccess) return e;
+  kern<<<static_cast<unsigned>(pp.tile_bound) * static_cast<unsigned>(p.N), kFwdThreads, smem, stream>>>(pp);
   return cudaGetLastError();
 }
 

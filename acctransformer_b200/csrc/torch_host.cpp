@@ -38,6 +38,7 @@ struct Library {
   decltype(&acct_fa_bwd_workspace_bytes) fa_bwd_workspace_bytes;
   decltype(&acct_infer_prefill) infer_prefill;
   decltype(&acct_infer_decode) infer_decode;
+  decltype(&acct_infer_packed) infer_packed;
   decltype(&acct_kv4_append) kv4_append;
   decltype(&acct_kv4_read) kv4_read;
   decltype(&acct_kv4_decode) kv4_decode;
@@ -392,6 +393,7 @@ PyObject* py_init(PyObject*, PyObject* path) {
   g_lib.fa_bwd_workspace_bytes = reinterpret_cast<decltype(g_lib.fa_bwd_workspace_bytes)>(sym("acct_fa_bwd_workspace_bytes"));
   g_lib.infer_prefill = reinterpret_cast<decltype(g_lib.infer_prefill)>(sym("acct_infer_prefill"));
   g_lib.infer_decode = reinterpret_cast<decltype(g_lib.infer_decode)>(sym("acct_infer_decode"));
+  g_lib.infer_packed = reinterpret_cast<decltype(g_lib.infer_packed)>(sym("acct_infer_packed"));
   g_lib.kv4_append = reinterpret_cast<decltype(g_lib.kv4_append)>(sym("acct_kv4_append"));
   g_lib.kv4_read = reinterpret_cast<decltype(g_lib.kv4_read)>(sym("acct_kv4_read"));
   g_lib.kv4_decode = reinterpret_cast<decltype(g_lib.kv4_decode)>(sym("acct_kv4_decode"));
@@ -572,10 +574,10 @@ Kv4 kv4_arg(PyObject* p) {
   out.dtype = out.c.dtype == ACCT_BF16 ? at::kBFloat16 : at::kHalf;
   return out;
 }
-// `n` or more int32 on the cache's device
+// `n` or more integers on the device of `like`, as int32
 Tensor ints_on(const char* name, const Tensor& t, int64_t n, const Tensor& like) {
   require_cuda(name, t);
-  HOST_CHECK(t.device() == like.device(), name, " must be on the device of the cache, ", like.device(), ", not on ", t.device());
+  HOST_CHECK(t.device() == like.device(), name, " must be on the device of the other operands, ", like.device(), ", not on ", t.device());
   HOST_CHECK(t.numel() >= n && !t.is_floating_point(), name, " must hold ", n, " integers, got ", t.numel(), " of ", t.scalar_type());
   return t.to(at::kInt).contiguous();
 }
@@ -595,6 +597,66 @@ Tensor rows_readable(const Tensor& t, int64_t (&strides)[2]) {
   if (as_is) return t;
   strides[0] = strides[1] = 0;
   return t.contiguous();
+}
+
+// infer_packed(q, k, v, cu_seqlens_q, cu_seqlens_k | None, causal, scale, out | None, want_lse) -> y, or (y, lse)
+PyObject* py_infer_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 9, "infer_packed takes 9 arguments, got ", n);
+  Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v");
+  Tensor cu_q = tensor_arg(args[3], "cu_seqlens_q"), cu_k = tensor_or_undefined(args[4]);
+  const bool causal = bool_arg(args[5]);
+  const double scale = float_arg(args[6]);
+  Tensor y = tensor_or_undefined(args[7]), lse;
+  const bool want_lse = bool_arg(args[8]);
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    require_cuda("q", q); require_on("k", k, q); require_on("v", v, q);
+    const auto dt = q.scalar_type();
+    HOST_CHECK((dt == at::kHalf || dt == at::kBFloat16) && k.scalar_type() == dt && v.scalar_type() == dt,
+               "q, k, v must share dtype float16 or bfloat16");
+    HOST_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && q.size(2) == k.size(2) && k.size(1) >= 1 && q.size(1) >= 1 &&
+                   q.size(1) % k.size(1) == 0,
+               "q must be [T_q, N, D] and k, v [T_k, N_kv, D] with N_kv dividing N, got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+    HOST_CHECK(cu_q.dim() == 1 && cu_q.numel() >= 2, "cu_seqlens_q must hold a start for each sequence and the end, got ", cu_q.sizes());
+    HOST_CHECK(q.size(0) <= INT32_MAX && k.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX, "too many rows");
+    cu_q = ints_on("cu_seqlens_q", cu_q, cu_q.numel(), q);
+    if (cu_k.defined()) {
+      HOST_CHECK(cu_k.numel() == cu_q.numel(), "cu_seqlens_k must have as many entries as cu_seqlens_q, ", cu_q.numel(), ", not ", cu_k.numel());
+      cu_k = ints_on("cu_seqlens_k", cu_k, cu_q.numel(), q);
+    } else {
+      HOST_CHECK(k.size(0) == q.size(0), "without cu_seqlens_k, k must have as many rows as q, ", q.size(0), ", not ", k.size(0));
+    }
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    acct_packed_args a;
+    memset(&a, 0, sizeof(a));
+    q = rows_readable(q, a.q_stride); k = rows_readable(k, a.k_stride); v = rows_readable(v, a.v_stride);
+    if (y.defined()) {
+      require_on("out", y, q);
+      HOST_CHECK(y.scalar_type() == dt && y.sizes() == q.sizes() && y.is_contiguous() && reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0,
+                 "out must be a contiguous tensor shaped and typed like q");
+    } else {
+      y = empty_like_shape(q.sizes(), dt, q);
+    }
+    if (want_lse) lse = empty_like_shape({q.size(1), q.size(0)}, at::kFloat, q);
+    a.dtype = dt == at::kBFloat16 ? ACCT_BF16 : ACCT_F16;
+    a.B = cu_q.numel() - 1; a.N = q.size(1); a.D = q.size(2); a.N_kv = k.size(1);
+    a.T_q = q.size(0); a.T_k = k.size(0);
+    a.q = q.const_data_ptr(); a.k = k.const_data_ptr(); a.v = v.const_data_ptr(); a.y = y.data_ptr();
+    if (lse.defined()) a.lse = static_cast<float*>(lse.data_ptr());
+    a.cu_seqlens_q = static_cast<const int32_t*>(cu_q.const_data_ptr());
+    if (cu_k.defined()) a.cu_seqlens_k = static_cast<const int32_t*>(cu_k.const_data_ptr());
+    a.causal = causal ? 1 : 0;
+    a.scale = static_cast<float>(scale);
+    check(g_lib.infer_packed(&a, stream_of(q)));
+  }
+  if (!want_lse) return wrap(y);
+  PyObject* out = PyTuple_New(2);
+  PyTuple_SET_ITEM(out, 0, wrap(y));
+  PyTuple_SET_ITEM(out, 1, wrap(lse));
+  return out;
+  END_HANDLE_TH_ERRORS
 }
 
 // kv4_append(cache, k, v, start, cu_seqlens | None)
@@ -756,6 +818,7 @@ PyMethodDef kMethods[] = {
     {"fa_apply", fast<py_fa_apply>(), METH_FASTCALL, "training operator, differentiable"},
     {"infer_prefill", fast<py_infer_prefill>(), METH_FASTCALL, "inference op"},
     {"infer_decode", fast<py_infer_decode>(), METH_FASTCALL, "one decoding step"},
+    {"infer_packed", fast<py_infer_packed>(), METH_FASTCALL, "inference op over packed sequences"},
     {"kv4_append", fast<py_kv4_append>(), METH_FASTCALL, "rows into a cache in 4 bits"},
     {"kv4_read", fast<py_kv4_read>(), METH_FASTCALL, "rows out of a cache in 4 bits"},
     {"kv4_decode", fast<py_kv4_decode>(), METH_FASTCALL, "one decoding step over a cache in 4 bits"},

@@ -10,6 +10,9 @@ rank-3 ``[B*N, S, D]`` or rank-4 ``[B, N, S, D]`` inputs, y shaped like q, no sc
 
 ``flash_attention_decode`` is the q_len = 1 step over a KV cache with per-sequence valid lengths;
 the reference has no such path.
+
+``flash_attention_packed`` takes prompts of different lengths in one call, one behind the other in ``[T, N, D]`` tensors; the
+reference's op takes one length per call.
 """
 from __future__ import annotations
 
@@ -17,7 +20,7 @@ import torch
 
 from .. import ops as _ops
 
-__all__ = ["FlashAttentionTik", "flash_attention_tik", "flash_attention_decode", "DecodeWorkspace"]
+__all__ = ["FlashAttentionTik", "flash_attention_tik", "flash_attention_decode", "flash_attention_packed", "DecodeWorkspace"]
 
 DecodeWorkspace = _ops.DecodeWorkspace
 
@@ -51,3 +54,16 @@ def flash_attention_decode(q, k_cache, v_cache, seq_lens=None, *, scale=None, nu
     """y[b,n,0,:] = softmax(scale * q[b,n,0,:] K[b,n,:len_b]^T) V[b,n,:len_b]; scale defaults to D^-1/2."""
     return _ops.infer_decode(q, k_cache, v_cache, seq_lens, scale=scale, num_splits=num_splits,
                              workspace=workspace, out=out)
+
+
+def flash_attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, scale=None, out=None, return_lse=False):
+    """Attention of packed sequences: q [T_q, N, D], k and v [T_k, N_kv, D] with N_kv dividing N, and int32 tensors [B + 1] on the
+    device with every sequence's first row and the end (``cu_seqlens_k`` defaults to ``cu_seqlens_q``).
+
+    ``causal``: the last query of a sequence sees its last key, the one before it all keys but that, and so on, so that a
+    sequence with more keys than queries is a chunk of a prompt behind a prefix.  A query that sees no key gives 0.  scale
+    defaults to D^-1/2; ``return_lse`` adds the logarithms of the softmax sums, float32 [N, T_q].  For serving: no gradient."""
+    for t in (q, k, v):
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("flash_attention_packed has no gradient: call it under torch.no_grad() or on detached tensors")
+    return _ops.infer_packed(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, scale=scale, out=out, return_lse=return_lse)

@@ -313,6 +313,13 @@ def infer_prefill(q, k, v, *, causal=False, scale=1.0, seq_lens=None):
     return host().infer_prefill(q, k, v, causal, scale, seq_lens)
 
 
+def infer_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, scale=None, out=None, return_lse=False):
+    """The inference op over packed sequences: q [T_q, N, D], k and v [T_k, N_kv, D], cu_seqlens [B + 1] int32."""
+    if scale is None and isinstance(q, torch.Tensor):
+        scale = 1.0 / math.sqrt(max(1, q.shape[-1]))
+    return host().infer_packed(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, scale, out, return_lse)
+
+
 class DecodeWorkspace:
     """Caller-owned scratch for ``infer_decode`` (partial results of the key splits)."""
 

@@ -273,6 +273,34 @@ typedef struct acct_infer_args {
 
 ACCT_API int acct_infer_prefill(const acct_infer_args* a, void* stream);
 
+/* The same op over packed sequences of different lengths: prompts one behind the other in [T, N, D] tensors, which a serving
+ * batch has anyway.  No counterpart in the reference (its op takes one length per call).  Sequence b has the query rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 and the key rows cu_seqlens_k[b] .. ; with `causal` its last query sees its last key,
+ * the query before it all keys but that one, and so on (a chunk of a prompt whose beginning is in the keys already).  A query
+ * that sees no key gives 0 (lse -inf).  Nothing of another sequence, or of rows past the last one, reaches a result, NaNs
+ * included; inside a sequence what is not finite in V reaches, besides the queries that see it, those of its 128-row tile. */
+typedef struct acct_packed_args {
+  int32_t dtype;            /* ACCT_F16 or ACCT_BF16 */
+  int32_t B, N, D;          /* sequences, query heads, head_dim: a multiple of 8 up to 256 */
+  int32_t N_kv;             /* heads of k and v: 0 or N, or a divisor of N */
+  int32_t T_q, T_k;         /* rows of q and y, of k and v; either may be 0 */
+  const void* q;            /* device [T_q, N, D] */
+  const void* k;            /* device [T_k, N_kv, D] */
+  const void* v;
+  void* y;                  /* device [T_q, N, D] */
+  float* lse;               /* device [N, T_q] fp32 packed, or NULL */
+  int64_t q_stride[2];      /* element strides of row and head, multiples of 8; 0 = packed */
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  int64_t y_stride[2];
+  const int32_t* cu_seqlens_q; /* device [B + 1], ascending from 0 to T_q */
+  const int32_t* cu_seqlens_k; /* device [B + 1], or NULL: those of q */
+  int32_t causal;
+  float scale;
+} acct_packed_args;
+
+ACCT_API int acct_infer_packed(const acct_packed_args* a, void* stream);
+
 /* Decode (one query token per sequence over a KV cache).  The reference has no decode path; this is the
  * q_len = 1 case of the op above with per-sequence valid lengths:
  *   y[b,n,0,:] = softmax(scale * q[b,n,0,:] K[b,n,0:len_b,:]^T) V[b,n,0:len_b,:]
