@@ -1,4 +1,6 @@
 // C-ABI entry points of the cache in 4 bits: argument checks and launches.
+#include <algorithm>
+
 #include "common.cuh"
 #include "fa_kernels.cuh"
 #include "kv4_common.cuh"
@@ -72,7 +74,8 @@ size_t parts_bytes(int B, int N, int D, int splits) {
   return (static_cast<size_t>(B) * N * splits * (static_cast<size_t>(D) + 2) * 4 + 15) / 16 * 16;
 }
 int padded_slots(int S_max) { return static_cast<int>((static_cast<int64_t>(S_max) + kKv4Rows - 1) / kKv4Rows * kKv4Rows); }
-size_t scores_bytes(int B, int N, int S_max) { return static_cast<size_t>(B) * N * padded_slots(S_max) * 4; }
+int padded_group(int N, int N_kv) { return (N / N_kv + 1) / 2 * 2; }
+size_t scores_bytes(int B, int N, int N_kv, int S_max) { return static_cast<size_t>(B) * N_kv * padded_group(N, N_kv) * padded_slots(S_max) * 4; }
 
 constexpr int kMaxSplits = 64;
 
@@ -90,8 +93,8 @@ int acct_kv4_append(const acct_kv4_cache* c, const acct_kv4_rows* r, void* strea
 int acct_kv4_read(const acct_kv4_cache* c, const acct_kv4_rows* r, void* stream) { return rows_call(c, r, false, stream); }
 
 size_t acct_kv4_decode_workspace_bytes(const acct_kv4_cache* c, int32_t N, int32_t num_splits, int32_t with_weights) {
-  if (c == nullptr || c->B <= 0 || c->D <= 0 || c->S_max <= 0 || N <= 0 || num_splits > kMaxSplits) return 0;
-  return parts_bytes(c->B, N, c->D, num_splits > 0 ? num_splits : kMaxSplits) + (with_weights ? scores_bytes(c->B, N, c->S_max) : 0);
+  if (c == nullptr || c->B <= 0 || c->N_kv <= 0 || c->D <= 0 || c->S_max <= 0 || N < c->N_kv || num_splits > kMaxSplits) return 0;
+  return parts_bytes(c->B, N, c->D, num_splits > 0 ? num_splits : kMaxSplits) + (with_weights ? scores_bytes(c->B, N, c->N_kv, c->S_max) : 0);
 }
 
 int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void* stream) {
@@ -106,7 +109,7 @@ int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void
   if (group > 16) return fail(ACCT_ERR_SHAPE, "decode takes up to 16 query heads per cache head, got %d", group);
   if (!(a->scale > 0.f) || !(a->scale < 1e30f)) return fail(ACCT_ERR_SHAPE, "scale must be a positive finite number");
   if (a->num_splits < 0 || a->num_splits > kMaxSplits) return fail(ACCT_ERR_SHAPE, "num_splits must be in [0, %d]", kMaxSplits);
-  const size_t scores = a->weights != nullptr ? scores_bytes(c->B, a->N, c->S_max) : 0;
+  const size_t scores = a->weights != nullptr ? scores_bytes(c->B, a->N, c->N_kv, c->S_max) : 0;
   const size_t given = a->workspace != nullptr ? a->workspace_bytes : 0;
   const size_t least = parts_bytes(c->B, a->N, c->D, a->num_splits > 0 ? a->num_splits : 1) + scores;
   if (given < least) return fail(ACCT_ERR_WORKSPACE, "decode workspace: need %zu bytes, got %zu", least, given);
@@ -115,17 +118,23 @@ int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void
   if ((rc = device_info(&info))) return rc;
   const int64_t units = static_cast<int64_t>(c->B) * c->N_kv;
   int64_t splits = a->num_splits;
+  p.parts = 0;
   if (splits == 0) {
-    splits = (static_cast<int64_t>(info.sm_count) * 12 + units - 1) / units;
-    const int64_t most = (static_cast<int64_t>(c->S_max) + 255) / 256;
-    if (splits > most) splits = most;
-    if (splits > kMaxSplits) splits = kMaxSplits;
+    // Parts for one round of resident thread blocks (a sequence wastes half a part on average), or for two where they stay long:
+    // those of 32 x 8 slices of up to 16 384 keys 95 -> 90 us, of 8 x 8 slices 36 -> 40.
+    const int64_t slots = static_cast<int64_t>(info.sm_count) * kv4_decode_blocks_per_sm(group);
+    const int64_t steps = static_cast<int64_t>(c->B) * ((static_cast<int64_t>(c->S_max) + 31) / 32);
+    auto parts = [&](int64_t rounds) { return std::max<int64_t>(1, slots * rounds / c->N_kv - c->B / 2); };
+    const int64_t rounds = (units + slots - 1) / slots;
+    p.parts = static_cast<int>(parts(steps >= 160 * parts(rounds) ? 2 * rounds : rounds));
+    splits = std::min<int64_t>(kMaxSplits, (static_cast<int64_t>(c->S_max) + 511) / 512);
     while (splits > 1 && parts_bytes(c->B, a->N, c->D, static_cast<int>(splits)) + scores > given) --splits;
   }
   p.q = a->q; p.y = a->y; p.seq_lens = a->seq_lens; p.weights = a->weights;
   p.B = c->B; p.N = a->N; p.D = c->D; p.kv_group = group;
   p.splits = static_cast<int>(splits);
   p.S_pad = padded_slots(c->S_max);
+  p.G_pad = padded_group(a->N, c->N_kv);
   p.part_acc = static_cast<float*>(a->workspace);
   p.part_ml = p.part_acc + static_cast<size_t>(c->B) * a->N * p.splits * c->D;
   p.scores = a->weights != nullptr ? reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + parts_bytes(c->B, a->N, c->D, p.splits)) : nullptr;

@@ -9,9 +9,8 @@
 // finds its words side by side, and no word has to be moved between lanes:
 //   K codes    lane (g, t), word 8-row half * NG + group: row g of the half, columns 32 group + 8 t .. + 7, nibble = column
 //   V codes    lane (g, t), word p * NG + group: rows 8 p + 2 t (low 16 bits) and 8 p + 2 t + 1 (high), columns
-//              32 group + 4 g .. + 3, nibble = column: two rows of one column are where a B operand has them
-//   K steps    [half][t][group][2]: rows 2 t and 2 t + 1 of the half, as the accumulators of Q K^T have them
-//   K minima   [row][group]
+//              32 group + 4 g .. + 3, nibble = column: two rows of one column are where an operand of P V has them
+//   K steps, K minima   [row][group] each
 //   V both     [p][t][group][steps of the two rows, minima of the two rows]
 #pragma once
 #include <cuda_bf16.h>
@@ -35,7 +34,7 @@ struct Kv4Record {
   // Where lane (g, t) has its V words: the eight lanes that hold a pair of rows side by side (a row is read and written alone,
   // too), turned by 2 t so that any eight consecutive lanes still cover all banks.
   __host__ __device__ static constexpr int v_place(int g, int t) { return t * 8 + ((g + 2 * t) & 7); }
-  __host__ __device__ static constexpr int k_step(int row, int grp) { return kKs + ((((row >> 3) * 4 + ((row & 7) >> 1)) * NG + grp) * 2 + (row & 1)) * 2; }
+  __host__ __device__ static constexpr int k_step(int row, int grp) { return kKs + (row * NG + grp) * 2; }
   __host__ __device__ static constexpr int k_min(int row, int grp) { return kKm + (row * NG + grp) * 2; }
   __host__ __device__ static constexpr int v_step(int row, int grp) { return kVsm + ((((row >> 3) * 4 + ((row & 7) >> 1)) * NG + grp) * 4 + (row & 1)) * 2; }
   __host__ __device__ static constexpr int v_min(int row, int grp) { return v_step(row, grp) + 4; }
@@ -71,11 +70,14 @@ struct Kv4DecodeParams {
   void* y;
   const int* seq_lens;
   float* weights;                   // [B, N_kv, S_max] or null: every key's probability is added, over the group's heads
-  float* scores;                    // with weights: [B, N, S_pad] scratch
+  float* scores;                    // with weights: [B, N_kv, S_pad, G_pad] scratch
   float* part_acc;                  // [B * N, splits, D]
   float* part_ml;                   // [B * N, splits, 2]
   unsigned int* status;
-  int B, N, D, kv_group, splits, S_pad;
+  int B, N, D, kv_group;
+  int splits;                       // most parts of a sequence, and room for so many in part_acc and part_ml
+  int parts;                        // 0: every sequence has `splits` parts; else the parts that the whole batch is cut into, about
+  int S_pad, G_pad;                 // slots in whole records, query heads per cache head rounded up to an even number
   int clustered;
   float scale_log2;
 };
@@ -92,6 +94,7 @@ struct Kv4EvictParams {
 
 cudaError_t launch_kv4_append(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);
 cudaError_t launch_kv4_read(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);
+int kv4_decode_blocks_per_sm(int kv_group);      // that are resident at once
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int* resident = nullptr);
 cudaError_t launch_kv4_evict(const Kv4EvictParams& p, cudaStream_t stream);
 

@@ -2,19 +2,24 @@
 //
 // The step is bound by reading the cache once (160 bytes per key and head at head_dim 128), but at 5 bits a value there is little
 // time per value: an SM gets 23 bytes per clock, a 16-row record in 110, in which its four schedulers issue 440 instructions
-// for 4 096 codes.  So a code takes no arithmetic of its own that can be avoided:
-//   S = Q K^T    k = s c + m splits into s (Q c) + m (sum of Q): the codes go to mma.m16n8k16 as they are, one group of 32 columns
-//                at a time, and s and m meet 16 x 16 sums instead of 16 x 128 values.  In fp16 a code in the low bits of a half is
-//                the subnormal number c * 2^-24, exact to multiply (and c * 2^-20 four bits up: those columns of Q are divided by
-//                16), so a mask is all it takes; in bf16 it goes into the low bits of 128 and 128 is subtracted.  m times the sum
-//                of Q is one more product, whose operand holds the sums in three parts so that nothing of them is lost.
-//   O += P V     here the steps belong to the contraction: v = s c + m is formed in 16 bits (one rounding, as if the cache were
-//                in 16 bits), two rows of a column at a time, with the code subtracted out of 1024 + c, 64 + c or 128 + c.
-// Records come in by one bulk copy each through a ring per warp; nothing is shared between the warps of a block before the end.
+// for 4 096 codes.  So rows and columns of the cache are the 16-row operand of mma.m16n8k16 and the query heads the 8 columns of
+// the other (17 products a record for up to 8 heads), and a code takes no arithmetic of its own that can be avoided:
+//   S^T = K Q^T   k = s c + m splits into s (c Q) + m (sum of Q): the codes go into the product as they are, one group of 32 columns
+//                 at a time, and s and m meet 16 x 8 sums instead of 16 x 128 values.  In fp16 a code in the low bits of a half is
+//                 the subnormal number c * 2^-24, exact to multiply (and c * 2^-20 four bits up: those columns of Q are divided by
+//                 16), so a mask is all it takes; in bf16 it goes into the low bits of 128 and 128 is subtracted.  m times the sum
+//                 of Q is one more product, whose operand holds the sums in three parts so that nothing of them is lost.
+//   O^T += V^T P  here the steps belong to the contraction: v = s c + m is formed in 16 bits (one rounding, as if the cache were
+//                 in 16 bits), two rows of a column at a time, with the code subtracted out of 1024 + c, 64 + c or 128 + c.
+// The running maximum is only refreshed where a score exceeds it by more than 8 (in log2 units), so that most records need no
+// exchange between lanes.  Records come in by one bulk copy each through a ring per warp; nothing is shared between the warps of
+// a block before the end.
 //
 // The parts of a slice leave (acc[D], max, sum) per query head; kv4_finish_kernel joins them and, where the probabilities are
 // wanted, takes the scores that were left in scratch (4 bytes per key and query head) to exp2(x - max) / sum, added up over the
-// group.  Where few slices leave room on the GPU, the parts of one are a cluster and join without a second kernel.
+// group.
+#include <algorithm>
+
 #include "fa_common.cuh"
 #include "fa_kernels.cuh"
 #include "kv4_common.cuh"
@@ -24,22 +29,40 @@ namespace acct {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4;
-constexpr int kSlots = 4;             // records in a warp's ring
+constexpr int kStepRecs = 2;          // records that a warp takes at a time: waits, addresses and softmax checks for both at once
+constexpr int kSlots = 3;             // steps in a warp's ring
 
 // D (16x8, fp32) += A (16x16, row) * B (16x8, col); 16-bit operands
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-               "r"(bytes), "r"(smem_u32(bar))
+// the same with nothing to add to
+template <bool BF16>
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// A bulk copy whose lines are the first to leave L2: the cache is read once a step, what should stay are the scores.
+__device__ __forceinline__ uint64_t read_once_policy() {
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
                : "memory");
 }
 
@@ -63,6 +86,13 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
   else return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
+// (w & mask) | bits
+__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(w), "r"(mask), "r"(bits));
+  return d;
+}
+
 // The four pairs of codes of a word (nibble j of either half), for Q K^T: what they multiply to is the code times
 // 2^-24, 2^-20, 2^-24, 2^-20 in fp16, the code itself in bf16.
 constexpr float kCodeScaleF16 = 16777216.0f;
@@ -70,7 +100,7 @@ template <bool BF16>
 __device__ __forceinline__ void key_codes(uint32_t w, uint32_t (&x)[4]) {
   if constexpr (BF16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = sub2<true>(((w >> (4 * j)) & 0x000f000fu) | 0x43004300u, 0x43004300u);
+    for (int j = 0; j < 4; ++j) x[j] = sub2<true>(mask_or(w >> (4 * j), 0x000f000fu, 0x43004300u), 0x43004300u);
   } else {
     const uint32_t u = w >> 8;
     x[0] = w & 0x000f000fu; x[1] = w & 0x00f000f0u; x[2] = u & 0x000f000fu; x[3] = u & 0x00f000f0u;
@@ -81,56 +111,139 @@ template <bool BF16>
 __device__ __forceinline__ void value_pairs(uint32_t w, uint32_t step, uint32_t low, uint32_t (&x)[4]) {
   if constexpr (BF16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = sub2<true>(((w >> (4 * j)) & 0x000f000fu) | 0x43004300u, 0x43004300u);
+    for (int j = 0; j < 4; ++j) x[j] = sub2<true>(mask_or(w >> (4 * j), 0x000f000fu, 0x43004300u), 0x43004300u);
   } else {
     const uint32_t u = w >> 8;
-    x[0] = sub2<false>((w & 0x000f000fu) | 0x64006400u, 0x64006400u);      // 1024 + c
-    x[1] = sub2<false>((w & 0x00f000f0u) | 0x54005400u, 0x54005400u);      // 64 + c
-    x[2] = sub2<false>((u & 0x000f000fu) | 0x64006400u, 0x64006400u);
-    x[3] = sub2<false>((u & 0x00f000f0u) | 0x54005400u, 0x54005400u);
+    x[0] = sub2<false>(mask_or(w, 0x000f000fu, 0x64006400u), 0x64006400u);      // 1024 + c
+    x[1] = sub2<false>(mask_or(w, 0x00f000f0u, 0x54005400u), 0x54005400u);      // 64 + c
+    x[2] = sub2<false>(mask_or(u, 0x000f000fu, 0x64006400u), 0x64006400u);
+    x[3] = sub2<false>(mask_or(u, 0x00f000f0u, 0x54005400u), 0x54005400u);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) x[j] = fma2<BF16>(x[j], step, low);
 }
 
 template <int N>
-__device__ __forceinline__ void shared_words(uint32_t addr, uint32_t* x) {      // N words, in as few loads as their alignment allows
+__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* x) {      // N words, in as few loads as their alignment allows
   if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]) : "r"(addr + 4 * i));
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(at + 4 * i);
+      x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    }
   } else if constexpr (N % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x[i]), "=r"(x[i + 1]) : "r"(addr + 4 * i));
+    for (int i = 0; i < N; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(at + 4 * i);
+      x[i] = v.x; x[i + 1] = v.y;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[i]) : "r"(addr + 4 * i));
+    for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const uint32_t*>(at + 4 * i);
   }
 }
 // the words of a lane's place: units of kUnit words, 32 units apart
 template <int NG>
-__device__ __forceinline__ void lane_words(uint32_t base, int place, uint32_t (&x)[2 * NG]) {
+__device__ __forceinline__ void lane_words(const uint8_t* base, int place, uint32_t (&x)[2 * NG]) {
   using R = Kv4Record<NG>;
 #pragma unroll
-  for (int u = 0; u < R::kWords; u += R::kUnit) shared_words<R::kUnit>(base + R::word(u, place), x + u);
+  for (int u = 0; u < R::kWords; u += R::kUnit) load_words<R::kUnit>(base + R::word(u, place), x + u);
+}
+// NG 16-bit numbers of a row, as floats
+template <int NG, bool BF16>
+__device__ __forceinline__ void row_steps(const uint8_t* at, float (&s)[NG]) {
+  if constexpr (NG % 2 == 0) {
+    uint32_t w[NG / 2];
+    load_words<NG / 2>(at, w);
+#pragma unroll
+    for (int i = 0; i < NG / 2; ++i) {
+      const float2 f = unpack2<BF16>(w[i]);
+      s[2 * i] = f.x; s[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) s[i] = unpack2<BF16>(*reinterpret_cast<const uint16_t*>(at + 2 * i)).x;
+  }
+}
+// the transpose of an 8 x 8 matrix of 16-bit numbers, lane (g, t) having row g, columns 2 t and 2 t + 1
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
-// UPPER: the group has more than 8 query heads, i.e. rows 8..15 of the MMAs carry heads too.
-template <int NG, bool BF16, bool UPPER>
-__global__ void __launch_bounds__(kThreads) kv4_decode_kernel(const Kv4DecodeParams p) {
+// How the batch is cut.  Every sequence into `splits` parts, where the caller says so.  Otherwise into parts of about equal length,
+// `p.parts` for the heads of the batch together, so that thread blocks finish together whatever the lengths are: the length of
+// a part follows from the sum of all lengths, which every block forms for itself (one load and a reduction, at the latency of
+// the length that it needs anyway).  Never shorter than kMinSteps.
+constexpr int kMinSteps = 16;
+__device__ __forceinline__ int steps_of(const Kv4DecodeParams& p, int b) {
+  int len = p.cache.S_max;
+  if (p.seq_lens != nullptr) len = min(len, max(0, p.seq_lens[b]));
+  return (len + kStepRecs * kKv4Rows - 1) / (kStepRecs * kKv4Rows);
+}
+// steps of a part, the same in all lanes
+__device__ __forceinline__ int part_steps(const Kv4DecodeParams& p) {
+  int total = 0;
+  for (int b = threadIdx.x & 31; b < p.B; b += 32) total += steps_of(p, b);
+  total = __reduce_add_sync(0xffffffffu, total);
+  return max(kMinSteps, (total + p.parts - 1) / p.parts);
+}
+__device__ __forceinline__ int parts_of(const Kv4DecodeParams& p, int steps, int part) {
+  return p.parts == 0 ? p.splits : min(p.splits, max(1, (steps + part - 1) / part));
+}
+
+constexpr float kRefresh = 8.0f;      // log2 units by which a score may exceed the running maximum
+
+// Resident thread blocks per SM, which the registers decide (152 and 230 a thread).  With four, at 128 registers, or five, at 96
+// and a record at a time, the step is no faster (32 x 8 slices of up to 16 384 keys 95 and 103 us against 90).
+constexpr int blocks_per_sm(int hi) { return hi == 1 ? 3 : 2; }
+
+// HI: columns of 8 query heads (1 up to a group of 8, else 2).
+template <int NG, bool BF16, int HI>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel(const Kv4DecodeParams p) {
   using R = Kv4Record<NG>;
-  constexpr int kHi = UPPER ? 2 : 1;
-  constexpr int DPAD = 32 * NG;
+  constexpr int DPAD = 32 * NG, kHeads = 8 * HI;
 
   extern __shared__ __align__(128) uint8_t ksm[];
   __shared__ uint64_t full[kWarps][kSlots];
   __shared__ volatile uint32_t abort_flag;
 
   const int G = p.kv_group;
-  const int split = blockIdx.x, unit_kv = blockIdx.y;
-  const int b = unit_kv / p.cache.N_kv, h_kv = unit_kv % p.cache.N_kv;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+
+  // block -> head, and the `item`-th of all parts: sequence b, part `split` of n_parts
+  const int h_kv = blockIdx.x % p.cache.N_kv;
+  int item = blockIdx.x / p.cache.N_kv, b = 0, split = 0, n_parts = p.splits, n_steps = 0;
+  if (p.parts == 0) {
+    b = item / p.splits;
+    split = item % p.splits;
+    n_steps = steps_of(p, b);
+  } else {
+    const int part = part_steps(p);
+    bool found = false;
+    for (int b0 = 0; b0 < p.B && !found; b0 += 32) {
+      const int steps = b0 + lane < p.B ? steps_of(p, b0 + lane) : 0, n = b0 + lane < p.B ? parts_of(p, steps, part) : 0;
+      int upto = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += x;
+      }
+      const unsigned int past = __ballot_sync(0xffffffffu, upto > item);
+      found = past != 0u;
+      const int from = found ? __ffs(past) - 1 : 31;
+      const int before = __shfl_sync(0xffffffffu, found ? upto - n : upto, from);
+      item -= before;
+      b = b0 + from;
+      split = item;
+      n_parts = __shfl_sync(0xffffffffu, n, from);
+      n_steps = __shfl_sync(0xffffffffu, steps, from);
+    }
+    if (!found) return;
+  }
+  const int unit_kv = b * p.cache.N_kv + h_kv;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWarps * kSlots; ++i) mbar_init(&full[0][0] + i, 1);
@@ -142,42 +255,55 @@ __global__ void __launch_bounds__(kThreads) kv4_decode_kernel(const Kv4DecodePar
   int len = p.cache.S_max;
   if (p.seq_lens != nullptr) len = min(len, max(0, p.seq_lens[b]));
   const int n_rec = (len + kKv4Rows - 1) / kKv4Rows;
-  const int per = ((n_rec + p.splits - 1) / p.splits + kWarps - 1) / kWarps * kWarps;
-  const int r0 = split * per, r1 = min(n_rec, r0 + per);
-  const int mine = r1 - r0 > warp ? (r1 - r0 - warp + kWarps - 1) / kWarps : 0;      // records r0 + warp, r0 + warp + 4, ..
+  const int per = ((n_steps + n_parts - 1) / n_parts + kWarps - 1) / kWarps * kWarps;
+  const int s0 = split * per + warp, s1 = min(n_steps, (split + 1) * per);      // this warp: steps s0, s0 + 4, .. before s1
 
-  uint8_t* ring = ksm + warp * (kSlots * R::kBytes);
+  constexpr int kStepBytes = kStepRecs * R::kBytes;
+  uint8_t* ring = ksm + warp * (kSlots * kStepBytes);
   const bool paged = p.cache.table != nullptr;
-  int pages = 0;                       // lane i: the page of this warp's record (i of the last 32 asked for)
-  auto issue = [&](int i) {            // the i-th record of this warp into ring slot i % kSlots; the whole warp calls it
-    const int rec = r0 + warp + i * kWarps;
-    const uint8_t* src;
+  const uint8_t* records = p.cache.records;
+  if (!paged) records += (static_cast<int64_t>(b) * p.cache.N_kv + h_kv) * p.cache.recs * R::kBytes;
+  const uint64_t policy = read_once_policy();
+  int pages = 0;                       // lane i: the page of the i-th of the last 32 records asked for, two for each step
+  auto issue = [&](int step, int slot, int turn) {      // a step's records into a ring slot; the whole warp calls it
+    const int rec = step * kStepRecs;
+    const bool both = rec + 1 < n_rec;
+    const uint8_t *src, *src1;
     if (paged) {
-      if ((i & 31) == 0) {
-        const int r = rec + lane * kWarps;
-        pages = r < r1 ? p.cache.table[static_cast<int64_t>(b) * p.cache.max_pages + (r >> p.cache.page_shift)] : 0;
+      if (turn % 16 == 0) {
+        const int r = (step + (lane >> 1) * kWarps) * kStepRecs + (lane & 1);
+        pages = r < n_rec ? p.cache.table[static_cast<int64_t>(b) * p.cache.max_pages + (r >> p.cache.page_shift)] : 0;
         pages = min(max(pages, 0), p.cache.num_pages - 1);
       }
-      const int64_t page = __shfl_sync(0xffffffffu, pages, i & 31);
-      src = p.cache.records + (((page * p.cache.N_kv + h_kv) << p.cache.page_shift) + (rec & ((1 << p.cache.page_shift) - 1))) * R::kBytes;
+      const int64_t page = __shfl_sync(0xffffffffu, pages, turn % 16 * 2), page1 = __shfl_sync(0xffffffffu, pages, turn % 16 * 2 + 1);
+      const int mask = (1 << p.cache.page_shift) - 1;
+      src = records + (((page * p.cache.N_kv + h_kv) << p.cache.page_shift) + (rec & mask)) * R::kBytes;
+      src1 = records + (((page1 * p.cache.N_kv + h_kv) << p.cache.page_shift) + ((rec + 1) & mask)) * R::kBytes;
     } else {
-      src = p.cache.records + ((static_cast<int64_t>(b) * p.cache.N_kv + h_kv) * p.cache.recs + rec) * R::kBytes;
+      src = records + static_cast<int64_t>(rec) * R::kBytes;
+      src1 = src + R::kBytes;
     }
     if (elect_one()) {
-      uint64_t* bar = &full[warp][i % kSlots];
-      mbar_expect_tx(bar, R::kBytes);
-      bulk_load(ring + (i % kSlots) * R::kBytes, src, R::kBytes, bar);
+      uint64_t* bar = &full[warp][slot];
+      uint8_t* dst = ring + slot * kStepBytes;
+      mbar_expect_tx(bar, both ? kStepBytes : R::kBytes);
+      if (both && src1 == src + R::kBytes) {
+        bulk_load(dst, src, kStepBytes, bar, policy);
+      } else {
+        bulk_load(dst, src, R::kBytes, bar, policy);
+        if (both) bulk_load(dst + R::kBytes, src1, R::kBytes, bar, policy);
+      }
     }
   };
 #pragma unroll
   for (int i = 0; i < kSlots - 1; ++i)
-    if (i < mine) issue(i);
+    if (s0 + i * kWarps < s1) issue(s0 + i * kWarps, i, i);
 
-  // ---- the query heads as A fragments, columns in the order of the codes: of a thread's eight columns 32 grp + 8 t + .. of a
-  // group the pairs (0, 4), (1, 5), (2, 6), (3, 7); in fp16 the second and fourth pair divided by 16
-  uint32_t qa[2 * NG][2 * kHi], qm[2 * kHi];
+  // ---- the query heads as B fragments (column g = head g), columns of Q in the order of the codes: of a thread's eight 32 grp +
+  // 8 t + .. of a group the pairs (0, 4), (1, 5), (2, 6), (3, 7); in fp16 the second and fourth pair divided by 16
+  uint32_t qb[HI][2 * NG][2], qm[HI][2];
 #pragma unroll
-  for (int hi = 0; hi < kHi; ++hi) {
+  for (int hi = 0; hi < HI; ++hi) {
     const int head = g + 8 * hi;
     float mean_t = 0.f;
 #pragma unroll
@@ -194,124 +320,164 @@ __global__ void __launch_bounds__(kThreads) kv4_decode_kernel(const Kv4DecodePar
         sum += f.x + f.y;
         uint32_t w = pairs[j];
         if (!BF16 && (j & 1) != 0) w = pack2<BF16>(f.x * 0.0625f, f.y * 0.0625f);
-        qa[2 * grp + (j >> 1)][(j & 1) * kHi + hi] = w;
+        qb[hi][2 * grp + (j >> 1)][j & 1] = w;
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       if (t == grp) mean_t = sum * 0.03125f;          // of the group's 32 columns: in the range of Q whatever that is
     }
     // the mean as a sum of three 16-bit numbers
-    uint32_t w0 = pack2<BF16>(mean_t, 0.f);
+    const uint32_t w0 = pack2<BF16>(mean_t, 0.f);
     const float rest1 = mean_t - unpack2<BF16>(w0).x;
     const uint32_t w1 = pack2<BF16>(rest1, 0.f);
     const float rest2 = rest1 - unpack2<BF16>(w1).x;
-    qm[hi] = (w0 & 0xffffu) | (w1 << 16);
-    qm[kHi + hi] = pack2<BF16>(rest2, 0.f);
+    qm[hi][0] = (w0 & 0xffffu) | (w1 << 16);
+    qm[hi][1] = pack2<BF16>(rest2, 0.f);
   }
 
-  float o[4 * NG][2 * kHi];
+  // O^T: rows g and g + 8 of tile (grp, j) are columns 32 grp + 4 g + 2 j and the next; columns heads 2 t and 2 t + 1
+  float o[HI][2 * NG][4];
+  float m_run[HI][2], l_run[HI][2];      // heads 2 t and 2 t + 1; l is this thread's share
 #pragma unroll
-  for (int i = 0; i < 4 * NG; ++i)
+  for (int hi = 0; hi < HI; ++hi) {
+    m_run[hi][0] = m_run[hi][1] = -INFINITY;
+    l_run[hi][0] = l_run[hi][1] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2 * kHi; ++e) o[i][e] = 0.f;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};      // rows g and g + 8; l is this thread's share
+    for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[hi][i][e] = 0.f;
+  }
   const float f_code = BF16 ? p.scale_log2 : p.scale_log2 * kCodeScaleF16, f_mean = p.scale_log2 * 32.0f;
 
-  for (int it = 0; it < mine; ++it) {
-    if (it + kSlots - 1 < mine) issue(it + kSlots - 1);
-    mbar_wait(&full[warp][it % kSlots], (it / kSlots) & 1, &abort_flag, p.status, DEV_TIMEOUT_TMA);
-    const uint32_t rec = smem_u32(ring + (it % kSlots) * R::kBytes);
-    const int row0 = (r0 + warp + it * kWarps) * kKv4Rows;
-    const bool partial = row0 + kKv4Rows > len;
+  float* scores = p.scores == nullptr ? nullptr : p.scores + (static_cast<int64_t>(unit_kv) * p.S_pad + g) * p.G_pad + 2 * t;
 
-    // ---- S = Q K^T, in log2 units: x[half][row half of the MMA][column]
-    float x[2][kHi][2];
-    {
-      uint32_t kw[2 * NG];
+  int turn = 0, slot = 0;
+  uint32_t parity = 0;
+  for (int step = s0; step < s1; step += kWarps, ++turn) {
+    if (step + (kSlots - 1) * kWarps < s1) issue(step + (kSlots - 1) * kWarps, slot == 0 ? kSlots - 1 : slot - 1, turn + kSlots - 1);
+    mbar_wait(&full[warp][slot], parity, &abort_flag, p.status, DEV_TIMEOUT_TMA);
+    const uint8_t* rec0 = ring + slot * kStepBytes;
+    const int row0 = step * (kStepRecs * kKv4Rows);
+    const bool partial = row0 + kStepRecs * kKv4Rows > len;      // (then what is there of the second record may be an earlier one)
+
+    // ---- S^T = K Q^T, in log2 units: x[record][hi] = rows g (0, 1) and g + 8 (2, 3), heads 2 t and 2 t + 1
+    float x[kStepRecs][HI][4];
+#pragma unroll
+    for (int r = 0; r < kStepRecs; ++r) {
+      const uint8_t* rec = rec0 + r * R::kBytes;
+      uint32_t kw[2 * NG], low[2] = {0u, 0u};
+      float step_of[2][NG];
       lane_words<NG>(rec, lane, kw);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t low = 0u, steps[NG];
-        if (t < NG) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(low) : "r"(rec + R::kKm + ((half * 8 + g) * NG + t) * 2));
-        low = __byte_perm(low, 0u, 0x1010);
-        shared_words<NG>(rec + R::kKs + (half * 4 + t) * NG * 4, steps);
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816<BF16>(c, qm[0], UPPER ? qm[kHi - 1] : 0u, qm[kHi], UPPER ? qm[2 * kHi - 1] : 0u, low, low);
+        if (t < NG) low[half] = *reinterpret_cast<const uint16_t*>(rec + R::k_min(half * 8, 0) + (g * NG + t) * 2);
+        low[half] = __byte_perm(low[half], 0u, 0x1010);
+        row_steps<NG, BF16>(rec + R::k_step(half * 8, 0) + g * NG * 2, step_of[half]);
+      }
 #pragma unroll
-        for (int hi = 0; hi < kHi; ++hi) x[half][hi][0] = x[half][hi][1] = 0.f;
+      for (int hi = 0; hi < HI; ++hi)
 #pragma unroll
-        for (int grp = 0; grp < NG; ++grp) {
-          uint32_t kb[4];
-          key_codes<BF16>(kw[half * NG + grp], kb);
-          float a[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < 4; ++e) x[r][hi][e] = 0.f;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t(&q)[2 * kHi] = qa[2 * grp + j];
-            mma16816<BF16>(a, q[0], UPPER ? q[kHi - 1] : 0u, q[kHi], UPPER ? q[2 * kHi - 1] : 0u, kb[2 * j], kb[2 * j + 1]);
-          }
-          const float2 s = unpack2<BF16>(steps[grp]);
+      for (int grp = 0; grp < NG; ++grp) {
+        uint32_t ka[2][4];
+        key_codes<BF16>(kw[grp], ka[0]);
+        key_codes<BF16>(kw[NG + grp], ka[1]);
 #pragma unroll
-          for (int hi = 0; hi < kHi; ++hi) {
-            x[half][hi][0] = fmaf(a[2 * hi], s.x, x[half][hi][0]);
-            x[half][hi][1] = fmaf(a[2 * hi + 1], s.y, x[half][hi][1]);
-          }
+        for (int hi = 0; hi < HI; ++hi) {
+          float c[4];
+          mma16816_zero<BF16>(c, ka[0][0], ka[1][0], ka[0][1], ka[1][1], qb[hi][2 * grp][0], qb[hi][2 * grp][1]);
+          mma16816<BF16>(c, ka[0][2], ka[1][2], ka[0][3], ka[1][3], qb[hi][2 * grp + 1][0], qb[hi][2 * grp + 1][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[r][hi][e] = fmaf(c[e], step_of[e >> 1][grp], x[r][hi][e]);
         }
+      }
 #pragma unroll
-        for (int hi = 0; hi < kHi; ++hi)
+      for (int hi = 0; hi < HI; ++hi) {
+        float c[4];
+        mma16816_zero<BF16>(c, low[0], low[1], low[0], low[1], qm[hi][0], qm[hi][1]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) x[half][hi][e] = fmaf(x[half][hi][e], f_code, c[2 * hi + e] * f_mean);
+        for (int e = 0; e < 4; ++e) x[r][hi][e] = fmaf(x[r][hi][e], f_code, c[e] * f_mean);
       }
     }
     if (partial) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int r = 0; r < kStepRecs; ++r)
 #pragma unroll
-        for (int hi = 0; hi < kHi; ++hi)
+        for (int hi = 0; hi < HI; ++hi)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (row0 + half * 8 + 2 * t + e >= len) x[half][hi][e] = -INFINITY;
+          for (int e = 0; e < 4; ++e)
+            if (row0 + r * kKv4Rows + g + 8 * (e >> 1) >= len) x[r][hi][e] = -INFINITY;
     }
-    if (p.scores != nullptr) {
+    if (scores != nullptr) {
+      float* at = scores + static_cast<int64_t>(row0) * p.G_pad;
 #pragma unroll
-      for (int hi = 0; hi < kHi; ++hi)
-        if (g + 8 * hi < G) {
-          float* at = p.scores + (static_cast<int64_t>(b) * p.N + h_kv * G + g + 8 * hi) * p.S_pad + row0 + 2 * t;
-          *reinterpret_cast<float2*>(at) = make_float2(x[0][hi][0], x[0][hi][1]);
-          *reinterpret_cast<float2*>(at + 8) = make_float2(x[1][hi][0], x[1][hi][1]);
-        }
-    }
-    // ---- online softmax; this thread holds, per row, keys 2t, 2t+1 of each half
-    uint32_t pa[4] = {0u, 0u, 0u, 0u};
+      for (int r = 0; r < kStepRecs; ++r) {
+        if (r > 0 && row0 + r * kKv4Rows >= len) break;
 #pragma unroll
-    for (int hi = 0; hi < kHi; ++hi) {
-      float mx = fmaxf(fmaxf(x[0][hi][0], x[0][hi][1]), fmaxf(x[1][hi][0], x[1][hi][1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(m_run[hi], mx);           // row0 < len, so the record's first key exists
-      const float alpha = ex2(m_run[hi] - m_new);         // 0 on the first record (m_run = -inf)
-      const float p0 = ex2(x[0][hi][0] - m_new), p1 = ex2(x[0][hi][1] - m_new), p2 = ex2(x[1][hi][0] - m_new), p3 = ex2(x[1][hi][1] - m_new);
-      l_run[hi] = fmaf(l_run[hi], alpha, (p0 + p1) + (p2 + p3));
-      m_run[hi] = m_new;
-      pa[hi] = pack2<BF16>(p0, p1);                       // P in 16 bits is the operand of P V; the sum is of what it was before
-      pa[2 + hi] = pack2<BF16>(p2, p3);
-      if (__any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll
-        for (int i = 0; i < 4 * NG; ++i) {
-          o[i][2 * hi] *= alpha;
-          o[i][2 * hi + 1] *= alpha;
-        }
+        for (int hi = 0; hi < HI; ++hi)
+          if (8 * hi + 2 * t < G) {
+            *reinterpret_cast<float2*>(at + 8 * hi) = make_float2(x[r][hi][0], x[r][hi][1]);
+            *reinterpret_cast<float2*>(at + 8 * p.G_pad + 8 * hi) = make_float2(x[r][hi][2], x[r][hi][3]);
+          }
+        at += kKv4Rows * p.G_pad;
       }
     }
-    // ---- O += P V
-    {
+    // ---- online softmax
+    bool exceeds = false;
+    float most[HI][2];
+#pragma unroll
+    for (int hi = 0; hi < HI; ++hi)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        most[hi][e] = fmaxf(x[0][hi][e], x[0][hi][e + 2]);
+#pragma unroll
+        for (int r = 1; r < kStepRecs; ++r) most[hi][e] = fmax3(most[hi][e], x[r][hi][e], x[r][hi][e + 2]);
+        exceeds |= most[hi][e] > m_run[hi][e] + kRefresh;
+      }
+    if (__any_sync(0xffffffffu, exceeds)) {          // (always at the first step: row0 < len, so it has a key that exists)
+#pragma unroll
+      for (int hi = 0; hi < HI; ++hi)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = most[hi][e];
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float m_new = fmaxf(m_run[hi][e], mx);
+          const float alpha = m_run[hi][e] == -INFINITY ? 0.f : ex2(m_run[hi][e] - m_new);
+          m_run[hi][e] = m_new;
+          l_run[hi][e] *= alpha;
+#pragma unroll
+          for (int i = 0; i < 2 * NG; ++i) {
+            o[hi][i][e] *= alpha;
+            o[hi][i][e + 2] *= alpha;
+          }
+        }
+    }
+    // ---- P, and O^T += V^T P
+#pragma unroll
+    for (int r = 0; r < kStepRecs; ++r) {
+      uint32_t pb[HI][2];      // P in 16 bits is the operand of P V; the sum is of what it was before
+#pragma unroll
+      for (int hi = 0; hi < HI; ++hi) {
+        float pr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pr[e] = ex2(x[r][hi][e] - m_run[hi][e & 1]);
+        l_run[hi][0] += pr[0] + pr[2];
+        l_run[hi][1] += pr[1] + pr[3];
+        pb[hi][0] = transpose8(pack2<BF16>(pr[0], pr[1]));
+        pb[hi][1] = transpose8(pack2<BF16>(pr[2], pr[3]));
+      }
+      const uint8_t* rec = rec0 + r * R::kBytes;
       uint32_t vw[2 * NG], vsm[2][2 * NG];
       lane_words<NG>(rec + R::kV, R::v_place(g, t), vw);
-      shared_words<2 * NG>(rec + R::kVsm + t * NG * 8, vsm[0]);
-      shared_words<2 * NG>(rec + R::kVsm + (4 + t) * NG * 8, vsm[1]);
+      load_words<2 * NG>(rec + R::kVsm + t * NG * 8, vsm[0]);
+      load_words<2 * NG>(rec + R::kVsm + (4 + t) * NG * 8, vsm[1]);
       if (partial) {      // rows that do not exist: whatever their steps and minima are, 0 times them has to be 0
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int row = row0 + q * 8 + 2 * t;
+          const int row = row0 + r * kKv4Rows + q * 8 + 2 * t;
           const uint32_t there = (row < len ? 0xffffu : 0u) | (row + 1 < len ? 0xffff0000u : 0u);
 #pragma unroll
           for (int i = 0; i < 2 * NG; ++i) vsm[q][i] &= there;
@@ -323,42 +489,40 @@ __global__ void __launch_bounds__(kThreads) kv4_decode_kernel(const Kv4DecodePar
         value_pairs<BF16>(vw[grp], vsm[0][2 * grp], vsm[0][2 * grp + 1], v0);
         value_pairs<BF16>(vw[NG + grp], vsm[1][2 * grp], vsm[1][2 * grp + 1], v1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float(&acc)[2 * kHi] = o[4 * grp + j];
-          float c[4] = {acc[0], acc[1], UPPER ? acc[2 * kHi - 2] : 0.f, UPPER ? acc[2 * kHi - 1] : 0.f};
-          mma16816<BF16>(c, pa[0], pa[1], pa[2], pa[3], v0[j], v1[j]);
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 2 * kHi; ++e) acc[e] = c[e];
-        }
+          for (int hi = 0; hi < HI; ++hi)
+            mma16816<BF16>(o[hi][2 * grp + j], v0[2 * j], v0[2 * j + 1], v1[2 * j], v1[2 * j + 1], pb[hi][0], pb[hi][1]);
       }
     }
+    if (++slot == kSlots) { slot = 0; parity ^= 1u; }
     __syncwarp();      // every lane has read this slot before a later copy may land in it
   }
 
   // ---- merge the four warps per query head, then write the part's result (the rings are dead by now: their memory holds the
   // warps' accumulators)
 #pragma unroll
-  for (int hi = 0; hi < 2; ++hi) {
-    l_run[hi] += __shfl_xor_sync(0xffffffffu, l_run[hi], 1);
-    l_run[hi] += __shfl_xor_sync(0xffffffffu, l_run[hi], 2);
-  }
+  for (int hi = 0; hi < HI; ++hi)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int bit = 4; bit < 32; bit <<= 1) l_run[hi][e] += __shfl_xor_sync(0xffffffffu, l_run[hi][e], bit);
   linger_after_abort(&abort_flag);
   __syncthreads();
-  constexpr int kHeads = 8 * kHi;
   float* s_acc = reinterpret_cast<float*>(ksm);                       // [warp][kHeads][DPAD]
   float* s_m = s_acc + kWarps * kHeads * DPAD;                        // [warp][kHeads]
   float* s_l = s_m + kWarps * kHeads;
 #pragma unroll
-  for (int hi = 0; hi < kHi; ++hi) {
-    const int head = g + 8 * hi;
-    if (t == 0) { s_m[warp * kHeads + head] = m_run[hi]; s_l[warp * kHeads + head] = l_run[hi]; }
+  for (int hi = 0; hi < HI; ++hi)
 #pragma unroll
-    for (int grp = 0; grp < NG; ++grp)
+    for (int e = 0; e < 2; ++e) {
+      const int head = warp * kHeads + 8 * hi + 2 * t + e;
+      if (g == 0) { s_m[head] = m_run[hi][e]; s_l[head] = l_run[hi][e]; }
 #pragma unroll
-      for (int e = 0; e < 2; ++e)      // columns 2t and 2t+1 of the MMA: 4 (2t) + j and 4 (2t+1) + j of the group
-        *reinterpret_cast<float4*>(s_acc + (warp * kHeads + head) * DPAD + 32 * grp + 8 * t + 4 * e) =
-            make_float4(o[4 * grp][2 * hi + e], o[4 * grp + 1][2 * hi + e], o[4 * grp + 2][2 * hi + e], o[4 * grp + 3][2 * hi + e]);
-  }
+      for (int grp = 0; grp < NG; ++grp)
+        *reinterpret_cast<float4*>(s_acc + head * DPAD + 32 * grp + 4 * g) =
+            make_float4(o[hi][2 * grp][e], o[hi][2 * grp][e + 2], o[hi][2 * grp + 1][e], o[hi][2 * grp + 1][e + 2]);
+    }
   __syncthreads();
   for (int head = 0; head < G; ++head) {
     const int64_t slot = (static_cast<int64_t>(b) * p.N + h_kv * G + head) * p.splits + split;
@@ -385,74 +549,119 @@ __global__ void __launch_bounds__(kThreads) kv4_decode_kernel(const Kv4DecodePar
   }
 }
 
-// Joins the parts: block (x, unit) has head x of the group for the output, and keys from x * kFinishKeys on for the weights.
-constexpr int kFinishThreads = 128, kFinishKeys = 1024;
+// Joins the parts.  Block (x, unit) has head x of the group for the output, and the keys from x * kFinishKeys on for the weights,
+// of which a thread takes four.  What bounds it is latency, so nothing waits for a load before all of them are out: those of the
+// parts' maxima and sums, of the first 16 parts of the output, of the weights and of two heads' scores.
+constexpr int kFinishThreads = 128, kFinishKeys = 4 * kFinishThreads, kFinishBatch = 16;
 template <bool BF16>
 __global__ void __launch_bounds__(kFinishThreads) kv4_finish_kernel(const Kv4DecodeParams p) {
+  __shared__ float s_share[16][64];      // what a part counts for: exp2(its maximum - the largest)
   __shared__ float s_m[16], s_inv[16];
   const int unit_kv = blockIdx.y, b = unit_kv / p.cache.N_kv, h_kv = unit_kv % p.cache.N_kv;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.kv_group, n = p.splits;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.kv_group, d = threadIdx.x;
   const int64_t unit0 = static_cast<int64_t>(b) * p.N + h_kv * G;      // the group's first query head
-  auto of_part = [&](int head, int s) {
-    const float2 none = make_float2(-INFINITY, 0.f);
-    return s < n ? reinterpret_cast<const float2*>(p.part_ml)[(unit0 + head) * n + s] : none;
+  int len = p.cache.S_max;
+  if (p.seq_lens != nullptr) len = min(len, max(0, p.seq_lens[b]));
+  const int first = blockIdx.x * kFinishKeys;
+  const bool output = blockIdx.x < G, weigh = p.weights != nullptr && first < len;
+  if (!output && !weigh) return;
+  const int n = parts_of(p, (len + kStepRecs * kKv4Rows - 1) / (kStepRecs * kKv4Rows), p.parts == 0 ? 1 : part_steps(p));
+
+  const float* part = p.part_acc + (unit0 + blockIdx.x) * p.splits * p.D + d;
+  float v[kFinishBatch], old[4];
+  float2 x[4];
+  if (output) {
+#pragma unroll
+    for (int i = 0; i < kFinishBatch; ++i) v[i] = i < n && d < p.D ? part[static_cast<int64_t>(i) * p.D] : 0.f;
+  }
+  float* weights = p.weights + static_cast<int64_t>(unit_kv) * p.cache.S_max;
+  const float* scores = p.scores + static_cast<int64_t>(unit_kv) * p.S_pad * p.G_pad;
+  auto load_scores = [&](int head) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = first + i * kFinishThreads + threadIdx.x;
+      x[i] = key < len ? *reinterpret_cast<const float2*>(scores + static_cast<int64_t>(key) * p.G_pad + head) : make_float2(-INFINITY, -INFINITY);
+    }
   };
-  for (int head = warp; head < G; head += kFinishThreads / 32) {
-    const float2 e0 = of_part(head, lane), e1 = of_part(head, 32 + lane);
+  if (weigh) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = first + i * kFinishThreads + threadIdx.x;
+      old[i] = key < len ? weights[key] : 0.f;
+    }
+    load_scores(0);
+  }
+  for (int head = weigh ? warp : blockIdx.x + warp * 16; head < (weigh ? G : blockIdx.x + 1); head += kFinishThreads / 32) {
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (unit0 + head) * p.splits;
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 e0 = lane < n ? ml[lane] : none, e1 = 32 + lane < n ? ml[32 + lane] : none;
     float big = fmaxf(e0.x, e1.x);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-    float l = (e0.x == -INFINITY ? 0.f : e0.y * ex2(e0.x - big)) + (e1.x == -INFINITY ? 0.f : e1.y * ex2(e1.x - big));
+    const float w0 = e0.x == -INFINITY ? 0.f : ex2(e0.x - big), w1 = e1.x == -INFINITY ? 0.f : ex2(e1.x - big);
+    float l = e0.y * w0 + e1.y * w1;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    if (lane == 0) {
-      s_m[head] = big;
-      s_inv[head] = l != 0.f ? 1.0f / l : 0.f;
-    }
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    s_share[head][lane] = w0;
+    s_share[head][32 + lane] = w1;
+    if (lane == 0) { s_m[head] = big; s_inv[head] = inv; }
   }
   __syncthreads();
-  if (blockIdx.x < G) {
-    const int head = blockIdx.x;
-    for (int d = threadIdx.x; d < p.D; d += kFinishThreads) {
-      const float* part = p.part_acc + (unit0 + head) * n * p.D + d;
-      float a = 0.f;
-#pragma unroll 8
-      for (int s = 0; s < n; ++s) {
-        const float ms = reinterpret_cast<const float2*>(p.part_ml)[(unit0 + head) * n + s].x;
-        a = fmaf(part[static_cast<int64_t>(s) * p.D], ms == -INFINITY ? 0.f : ex2(ms - s_m[head]), a);
+  if (output && d < p.D) {
+    float a = 0.f;
+    for (int i0 = 0; i0 < n; i0 += kFinishBatch) {
+      if (i0 > 0) {
+#pragma unroll
+        for (int i = 0; i < kFinishBatch; ++i) v[i] = i0 + i < n ? part[static_cast<int64_t>(i0 + i) * p.D] : 0.f;
       }
-      a *= s_inv[head];
-      const int64_t at = (unit0 + head) * p.D + d;
-      if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16(a);
-      else reinterpret_cast<__half*>(p.y)[at] = __float2half(a);
+#pragma unroll
+      for (int i = 0; i < kFinishBatch; ++i) a = fmaf(v[i], s_share[blockIdx.x][i0 + i], a);
+    }
+    a *= s_inv[blockIdx.x];
+    const int64_t at = (unit0 + blockIdx.x) * p.D + d;
+    if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16(a);
+    else reinterpret_cast<__half*>(p.y)[at] = __float2half(a);
+  }
+  if (!weigh) return;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int head = 0; head < G; head += 2) {
+    if (head > 0) load_scores(head);
+    const bool two = head + 1 < G;
+    const float m0 = s_m[head], i0 = s_inv[head], m1 = two ? s_m[head + 1] : 0.f, i1 = two ? s_inv[head + 1] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = fmaf(ex2(x[i].x - m0), i0, w[i]);
+      if (two) w[i] = fmaf(ex2(x[i].y - m1), i1, w[i]);
     }
   }
-  if (p.weights == nullptr) return;
-  int len = p.cache.S_max;
-  if (p.seq_lens != nullptr) len = min(len, max(0, p.seq_lens[b]));
-  const int end = min(len, (static_cast<int>(blockIdx.x) + 1) * kFinishKeys);
-  for (int key = blockIdx.x * kFinishKeys + threadIdx.x; key < end; key += kFinishThreads) {
-    float w = 0.f;
-    for (int head = 0; head < G; ++head) w = fmaf(ex2(p.scores[(unit0 + head) * p.S_pad + key] - s_m[head]), s_inv[head], w);
-    p.weights[static_cast<int64_t>(unit_kv) * p.cache.S_max + key] += w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = first + i * kFinishThreads + threadIdx.x;
+    if (key < len) weights[key] = old[i] + w[i];
   }
 }
 
 template <int NG>
 cudaError_t launch_ng(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream) {
   const bool upper = p.kv_group > 8;
-  const size_t ring = static_cast<size_t>(kWarps) * kSlots * Kv4Record<NG>::kBytes;
+  const size_t ring = static_cast<size_t>(kWarps) * kSlots * kStepRecs * Kv4Record<NG>::kBytes;
   const size_t merge = static_cast<size_t>(kWarps) * (upper ? 16 : 8) * (32 * NG + 2) * sizeof(float);
-  const size_t smem = ring > merge ? ring : merge;
-  void (*kern)(const Kv4DecodeParams) = bf16 ? (upper ? kv4_decode_kernel<NG, true, true> : kv4_decode_kernel<NG, true, false>)
-                                             : (upper ? kv4_decode_kernel<NG, false, true> : kv4_decode_kernel<NG, false, false>);
+  // No more blocks to an SM than the grid counts on, also where fewer groups need less: with room for more, some SMs are given more
+  // and others fewer, and everybody waits for the former.
+  const size_t least = (227 << 10) / (blocks_per_sm(upper ? 2 : 1) + 1) + 1;
+  const size_t smem = std::max({ring, merge, least});
+  void (*kern)(const Kv4DecodeParams) = bf16 ? (upper ? kv4_decode_kernel<NG, true, 2> : kv4_decode_kernel<NG, true, 1>)
+                                             : (upper ? kv4_decode_kernel<NG, false, 2> : kv4_decode_kernel<NG, false, 1>);
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(p.splits, p.B * p.cache.N_kv), kThreads, smem, stream>>>(p);
+  kern<<<(p.parts == 0 ? p.B * p.splits : p.parts + p.B) * p.cache.N_kv, kThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace
+
+int kv4_decode_blocks_per_sm(int kv_group) { return blocks_per_sm(kv_group > 8 ? 2 : 1); }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int*) {
   const int groups = (p.D + 31) / 32;
