@@ -160,6 +160,26 @@ cudaError_t allow_smem(const void* kernel, size_t bytes) {
   return cudaSuccess;
 }
 
+cudaError_t resident_clusters(const void* kernel, const cudaLaunchConfig_t& cfg, int splits, int* out) {
+  struct Seen {
+    const void* kernel;
+    int splits, dev, n;
+  };
+  static thread_local Seen seen[32];       // zero-initialised; newest entry overwrites the oldest
+  static thread_local unsigned next = 0;
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  for (const Seen& s : seen)
+    if (s.kernel == kernel && s.splits == splits && s.dev == dev) {
+      *out = s.n;
+      return cudaSuccess;
+    }
+  e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
+  if (e == cudaSuccess) seen[next++ % 32] = {kernel, splits, dev, *out};
+  return e;
+}
+
 unsigned int* device_status_ptr() {
   PerDevice* d = nullptr;
   if (init_device(&d)) return nullptr;

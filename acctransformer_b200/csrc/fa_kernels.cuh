@@ -158,6 +158,10 @@ cudaError_t launch_mask_plan(const void* mask, int mask_dtype, int mask_batch, c
 // Raises a kernel's dynamic shared memory limit, once per thread, kernel and device (the call costs the host about as
 // much as a launch argument block, and every operator call would repeat it).
 cudaError_t allow_smem(const void* kernel, size_t bytes);
+// How many clusters of `splits` blocks of this kernel the device holds at once.  Fewer than its SMs could hold blocks: a
+// cluster stays inside one GPC, and what is left over there is too small for another.  Asked once per thread, kernel, cluster
+// size and device.
+cudaError_t resident_clusters(const void* kernel, const cudaLaunchConfig_t& cfg, int splits, int* out);
 
 // Launchers: return cudaGetLastError() of the launch.
 cudaError_t launch_fa_fwd(const FwdParams& p, bool bf16, int sm_count, cudaStream_t stream);

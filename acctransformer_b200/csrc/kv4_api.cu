@@ -117,6 +117,8 @@ int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
   const int64_t units = static_cast<int64_t>(c->B) * c->N_kv;
+  p.B = c->B; p.N = a->N; p.D = c->D; p.kv_group = group;
+  p.clustered = 0;
   int64_t splits = a->num_splits;
   p.parts = 0;
   if (splits == 0) {
@@ -129,6 +131,29 @@ int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void
     p.parts = static_cast<int>(parts(steps >= 160 * parts(rounds) ? 2 * rounds : rounds));
     splits = std::min<int64_t>(kMaxSplits, (static_cast<int64_t>(c->S_max) + 511) / 512);
     while (splits > 1 && parts_bytes(c->B, a->N, c->D, static_cast<int>(splits)) + scores > given) --splits;
+    // Short contexts of few slices: the parts of a slice are one cluster and finish without a second kernel.  All clusters have to
+    // be resident at once (16 x 8 slices of 1 024 keys in 2 parts, 128 of 222 that fit: 12.5 us against 17.7 of two kernels, in 4,
+    // of 104 that fit: 18.5), and no part may be long, since the longest sequence decides (a group of 4 heads, 8 192 keys in 8
+    // parts, 32 slices 18.8 -> 16.7 us, 8 slices 14.7 -> 14.7; 32 768 keys 22.7 -> 33.0; of 12 heads, 4 096 keys 16.6 -> 14.5, 8 192
+    // 18.8 -> 20.8) or shorter than 128 keys.  One part is no cluster and need not be resident: 64 x 8 slices of 512 keys 18.8 -> 15.7.
+    const int longest = group > 8 ? 512 : 1024;
+    for (int parts : {8, 4, 2, 1}) {
+      if (parts > 1 && parts * 128ll > c->S_max + 127ll) continue;
+      if (static_cast<int64_t>(parts) * longest < c->S_max) break;
+      Kv4DecodeParams q = p;
+      q.clustered = 1;
+      q.splits = parts;
+      q.parts = 0;
+      int resident = 0;
+      if (parts > 1 && launch_kv4_decode(q, c->dtype == ACCT_BF16, nullptr, &resident) != cudaSuccess) {
+        cudaGetLastError();      // a device that will not say gets no clusters
+        resident = 0;
+      }
+      if (parts > 1 && units > resident) continue;
+      p = q;
+      splits = parts;
+      break;
+    }
   }
   p.q = a->q; p.y = a->y; p.seq_lens = a->seq_lens; p.weights = a->weights;
   p.B = c->B; p.N = a->N; p.D = c->D; p.kv_group = group;
@@ -137,9 +162,10 @@ int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void
   p.G_pad = padded_group(a->N, c->N_kv);
   p.part_acc = static_cast<float*>(a->workspace);
   p.part_ml = p.part_acc + static_cast<size_t>(c->B) * a->N * p.splits * c->D;
-  p.scores = a->weights != nullptr ? reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + parts_bytes(c->B, a->N, c->D, p.splits)) : nullptr;
+  p.scores = a->weights == nullptr ? nullptr
+             : p.clustered         ? p.part_acc      // (no results of parts then)
+                                   : reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + parts_bytes(c->B, a->N, c->D, p.splits));
   p.status = device_status_ptr();
-  p.clustered = 0;
   p.scale_log2 = a->scale * kLog2e;
   const cudaError_t e = launch_kv4_decode(p, c->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "launching the 4-bit decode kernels");

@@ -95,6 +95,7 @@ struct Kv4EvictParams {
 cudaError_t launch_kv4_append(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);
 cudaError_t launch_kv4_read(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);
 int kv4_decode_blocks_per_sm(int kv_group);      // that are resident at once
+// (with `resident` nothing is launched: it receives how many clusters of p.splits blocks the device holds at once)
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int* resident = nullptr);
 cudaError_t launch_kv4_evict(const Kv4EvictParams& p, cudaStream_t stream);
 

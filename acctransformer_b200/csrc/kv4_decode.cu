@@ -199,8 +199,17 @@ constexpr float kRefresh = 8.0f;      // log2 units by which a score may exceed 
 // and a record at a time, the step is no faster (32 x 8 slices of up to 16 384 keys 95 and 103 us against 90).
 constexpr int blocks_per_sm(int hi) { return hi == 1 ? 3 : 2; }
 
-// HI: columns of 8 query heads (1 up to a group of 8, else 2).
-template <int NG, bool BF16, int HI>
+// the float at `p` of this block's shared memory, in that of block `rank` of the cluster
+__device__ __forceinline__ float cluster_read(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_map(p, rank)) : "memory");
+  return v;
+}
+
+constexpr int kMaxCluster = 8;
+
+// HI: columns of 8 query heads (1 up to a group of 8, else 2).  CL: the parts of a slice are one cluster, and finish together.
+template <int NG, bool BF16, int HI, bool CL>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel(const Kv4DecodeParams p) {
   using R = Kv4Record<NG>;
   constexpr int DPAD = 32 * NG, kHeads = 8 * HI;
@@ -214,9 +223,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
   const int g = lane >> 2, t = lane & 3;
 
   // block -> head, and the `item`-th of all parts: sequence b, part `split` of n_parts
-  const int h_kv = blockIdx.x % p.cache.N_kv;
+  int h_kv = blockIdx.x % p.cache.N_kv;
   int item = blockIdx.x / p.cache.N_kv, b = 0, split = 0, n_parts = p.splits, n_steps = 0;
-  if (p.parts == 0) {
+  if constexpr (CL) {
+    split = blockIdx.x % p.splits;
+    item = blockIdx.x / p.splits;
+    b = item / p.cache.N_kv;
+    h_kv = item % p.cache.N_kv;
+    n_steps = steps_of(p, b);
+  } else if (p.parts == 0) {
     b = item / p.splits;
     split = item % p.splits;
     n_steps = steps_of(p, b);
@@ -524,28 +539,113 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
             make_float4(o[hi][2 * grp][e], o[hi][2 * grp][e + 2], o[hi][2 * grp + 1][e], o[hi][2 * grp + 1][e + 2]);
     }
   __syncthreads();
-  for (int head = 0; head < G; ++head) {
-    const int64_t slot = (static_cast<int64_t>(b) * p.N + h_kv * G + head) * p.splits + split;
-    float big = -INFINITY;
+  // the block's result of a head: acc[d], maximum, sum
+  auto of_head = [&](int head, float& big, float& lsum, float (&weight)[kWarps]) {
+    big = -INFINITY;
+    lsum = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) big = fmaxf(big, s_m[w * kHeads + head]);
-    float weight[kWarps], lsum = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float mw = s_m[w * kHeads + head];
       weight[w] = mw == -INFINITY ? 0.f : ex2(mw - big);
       lsum = fmaf(s_l[w * kHeads + head], weight[w], lsum);
     }
-    for (int d = threadIdx.x; d < p.D; d += kThreads) {
-      float a = 0.f;
+  };
+  if constexpr (!CL) {
+    for (int head = 0; head < G; ++head) {
+      const int64_t slot = (static_cast<int64_t>(b) * p.N + h_kv * G + head) * p.splits + split;
+      float big, lsum, weight[kWarps];
+      of_head(head, big, lsum, weight);
+      for (int d = threadIdx.x; d < p.D; d += kThreads) {
+        float a = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) a = fmaf(s_acc[(w * kHeads + head) * DPAD + d], weight[w], a);
-      p.part_acc[slot * p.D + d] = a;
+        for (int w = 0; w < kWarps; ++w) a = fmaf(s_acc[(w * kHeads + head) * DPAD + d], weight[w], a);
+        p.part_acc[slot * p.D + d] = a;
+      }
+      if (threadIdx.x == 0) {
+        p.part_ml[slot * 2] = big;
+        p.part_ml[slot * 2 + 1] = lsum;
+      }
     }
-    if (threadIdx.x == 0) {
-      p.part_ml[slot * 2] = big;
-      p.part_ml[slot * 2 + 1] = lsum;
+  } else {
+    __shared__ float s_part[kHeads][DPAD], s_pm[kHeads], s_pl[kHeads];      // this block's, which the others of the cluster read
+    __shared__ float s_max[kHeads], s_inv[kHeads], s_share[kMaxCluster][kHeads];
+    for (int head = 0; head < G; ++head) {
+      float big, lsum, weight[kWarps];
+      of_head(head, big, lsum, weight);
+      for (int d = threadIdx.x; d < p.D; d += kThreads) {
+        float a = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) a = fmaf(s_acc[(w * kHeads + head) * DPAD + d], weight[w], a);
+        s_part[head][d] = a;
+      }
+      if (threadIdx.x == 0) { s_pm[head] = big; s_pl[head] = lsum; }
     }
+    cluster_sync();
+    if (threadIdx.x < G) {
+      const int head = threadIdx.x;
+      float m[kMaxCluster], l[kMaxCluster], big = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) {
+        m[s] = s < p.splits ? cluster_read(&s_pm[head], s) : -INFINITY;
+        l[s] = s < p.splits ? cluster_read(&s_pl[head], s) : 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) big = fmaxf(big, m[s]);
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) {
+        const float w = m[s] == -INFINITY ? 0.f : ex2(m[s] - big);
+        s_share[s][head] = w;
+        sum = fmaf(l[s], w, sum);
+      }
+      s_max[head] = big;
+      s_inv[head] = sum != 0.f ? 1.0f / sum : 0.f;
+    }
+    __syncthreads();
+    // every splits-th 128 of the group's G x D results
+    for (int i = split * kThreads + threadIdx.x; i < G * p.D; i += kThreads * p.splits) {
+      const int head = i / p.D, d = i % p.D;
+      float v[kMaxCluster], a = 0.f;
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) v[s] = s < p.splits ? cluster_read(&s_part[head][d], s) : 0.f;
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) a = fmaf(v[s], s_share[s][head], a);
+      a *= s_inv[head];
+      const int64_t at = (static_cast<int64_t>(b) * p.N + h_kv * G + head) * p.D + d;
+      if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16(a);
+      else reinterpret_cast<__half*>(p.y)[at] = __float2half(a);
+    }
+    if (p.weights != nullptr) {
+      // the keys of this block, whose scores it has written itself; four at a time, whose loads do not wait for one another
+      const int first = split * per * kStepRecs * kKv4Rows, end = min(len, first + per * kStepRecs * kKv4Rows);
+      const float* row = p.scores + static_cast<int64_t>(unit_kv) * p.S_pad * p.G_pad;
+      float* weights = p.weights + static_cast<int64_t>(unit_kv) * p.cache.S_max;
+      for (int key0 = first + threadIdx.x; key0 < end; key0 += 4 * kThreads) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = key0 + i * kThreads < end ? weights[key0 + i * kThreads] : 0.f;
+        for (int head = 0; head < G; head += 2) {
+          const bool two = head + 1 < G;
+          const float m0 = s_max[head], i0 = s_inv[head], m1 = two ? s_max[head + 1] : 0.f, i1 = two ? s_inv[head + 1] : 0.f;
+          float2 sc[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sc[i] = key0 + i * kThreads < end ? *reinterpret_cast<const float2*>(row + static_cast<int64_t>(key0 + i * kThreads) * p.G_pad + head)
+                                              : make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float sum = ex2(sc[i].x - m0) * i0;
+            if (two) sum = fmaf(ex2(sc[i].y - m1), i1, sum);
+            w[i] += sum;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key0 + i * kThreads < end) weights[key0 + i * kThreads] = w[i];
+      }
+    }
+    cluster_sync();      // nobody's shared memory goes away while another block still reads it
   }
 }
 
@@ -643,7 +743,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_finish_kernel(const Kv4Dec
 }
 
 template <int NG>
-cudaError_t launch_ng(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream) {
+cudaError_t launch_ng(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int* resident) {
   const bool upper = p.kv_group > 8;
   const size_t ring = static_cast<size_t>(kWarps) * kSlots * kStepRecs * Kv4Record<NG>::kBytes;
   const size_t merge = static_cast<size_t>(kWarps) * (upper ? 16 : 8) * (32 * NG + 2) * sizeof(float);
@@ -651,23 +751,37 @@ cudaError_t launch_ng(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream) 
   // and others fewer, and everybody waits for the former.
   const size_t least = (227 << 10) / (blocks_per_sm(upper ? 2 : 1) + 1) + 1;
   const size_t smem = std::max({ring, merge, least});
-  void (*kern)(const Kv4DecodeParams) = bf16 ? (upper ? kv4_decode_kernel<NG, true, 2> : kv4_decode_kernel<NG, true, 1>)
-                                             : (upper ? kv4_decode_kernel<NG, false, 2> : kv4_decode_kernel<NG, false, 1>);
+#define KV4_DECODE(BF, HI) (p.clustered ? kv4_decode_kernel<NG, BF, HI, true> : kv4_decode_kernel<NG, BF, HI, false>)
+  void (*kern)(const Kv4DecodeParams) = bf16 ? (upper ? KV4_DECODE(true, 2) : KV4_DECODE(true, 1)) : (upper ? KV4_DECODE(false, 2) : KV4_DECODE(false, 1));
+#undef KV4_DECODE
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  kern<<<(p.parts == 0 ? p.B * p.splits : p.parts + p.B) * p.cache.N_kv, kThreads, smem, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.parts == 0 ? p.B * p.splits : p.parts + p.B) * p.cache.N_kv);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.clustered ? 1 : 0;
+  if (resident != nullptr) return resident_clusters(reinterpret_cast<const void*>(kern), cfg, p.splits, resident);
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 }  // namespace
 
 int kv4_decode_blocks_per_sm(int kv_group) { return blocks_per_sm(kv_group > 8 ? 2 : 1); }
 
-cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int*) {
+cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int* resident) {
   const int groups = (p.D + 31) / 32;
-  cudaError_t e = groups == 1 ? launch_ng<1>(p, bf16, stream) : groups == 2 ? launch_ng<2>(p, bf16, stream)
-                  : groups == 3 ? launch_ng<3>(p, bf16, stream) : launch_ng<4>(p, bf16, stream);
-  if (e != cudaSuccess) return e;
+  const cudaError_t e = groups == 1   ? launch_ng<1>(p, bf16, stream, resident)
+                        : groups == 2 ? launch_ng<2>(p, bf16, stream, resident)
+                        : groups == 3 ? launch_ng<3>(p, bf16, stream, resident)
+                                      : launch_ng<4>(p, bf16, stream, resident);
+  if (e != cudaSuccess || p.clustered) return e;
   const int chunks = p.weights != nullptr ? (p.cache.S_max + kFinishKeys - 1) / kFinishKeys : 1;
   const dim3 grid(chunks > p.kv_group ? chunks : p.kv_group, p.B * p.cache.N_kv);
   if (bf16) kv4_finish_kernel<true><<<grid, kFinishThreads, 0, stream>>>(p);
