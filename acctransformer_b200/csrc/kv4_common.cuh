@@ -56,6 +56,71 @@ __device__ __forceinline__ uint8_t* kv4_record(const Kv4Cache& c, int b, int h, 
   return c.records + (((static_cast<int64_t>(page) * c.N_kv + h) << c.page_shift) + (rec & ((1 << c.page_shift) - 1))) * bytes;
 }
 
+template <bool BF16>
+__device__ __forceinline__ uint32_t kv4_sub2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t kv4_fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// (w & mask) | bits
+__device__ __forceinline__ uint32_t kv4_mask_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(w), "r"(mask), "r"(bits));
+  return d;
+}
+
+// The values of the four pairs of codes of a word (nibble j of either half): code * step + minimum, rounded once.  The code is
+// subtracted out of 1024 + c, 64 + c or 128 + c.
+template <bool BF16>
+__device__ __forceinline__ void kv4_value_pairs(uint32_t w, uint32_t step, uint32_t low, uint32_t (&x)[4]) {
+  if constexpr (BF16) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = kv4_sub2<true>(kv4_mask_or(w >> (4 * j), 0x000f000fu, 0x43004300u), 0x43004300u);
+  } else {
+    const uint32_t u = w >> 8;
+    x[0] = kv4_sub2<false>(kv4_mask_or(w, 0x000f000fu, 0x64006400u), 0x64006400u);      // 1024 + c
+    x[1] = kv4_sub2<false>(kv4_mask_or(w, 0x00f000f0u, 0x54005400u), 0x54005400u);      // 64 + c
+    x[2] = kv4_sub2<false>(kv4_mask_or(u, 0x000f000fu, 0x64006400u), 0x64006400u);
+    x[3] = kv4_sub2<false>(kv4_mask_or(u, 0x00f000f0u, 0x54005400u), 0x54005400u);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = kv4_fma2<BF16>(x[j], step, low);
+}
+
+// the NG neighbouring words from word w of the unit at `place` on
+template <int NG>
+__device__ __forceinline__ void kv4_store_words(uint8_t* rec, int w, int place, const uint32_t (&x)[NG]) {
+  using R = Kv4Record<NG>;
+  if constexpr (NG == 4) *reinterpret_cast<uint4*>(rec + R::word(w, place)) = make_uint4(x[0], x[1], x[2], x[3]);
+  else if constexpr (NG == 2) *reinterpret_cast<uint2*>(rec + R::word(w, place)) = make_uint2(x[0], x[1]);
+  else {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) *reinterpret_cast<uint32_t*>(rec + R::word(w + i, place)) = x[i];
+  }
+}
+template <int NG>
+__device__ __forceinline__ void kv4_load_words(const uint8_t* rec, int w, int place, uint32_t (&x)[NG]) {
+  using R = Kv4Record<NG>;
+  if constexpr (NG == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(rec + R::word(w, place));
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else if constexpr (NG == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(rec + R::word(w, place));
+    x[0] = v.x; x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) x[i] = *reinterpret_cast<const uint32_t*>(rec + R::word(w + i, place));
+  }
+}
+
 struct Kv4Rows {                    // rows of tokens outside the cache: [T, N_kv, D]
   void *k, *v;
   int64_t k_stride[2], v_stride[2]; // elements, of a token and of a head
@@ -91,6 +156,25 @@ struct Kv4EvictParams {
   int* seq_lens_out;
   int keep, recent;
 };
+
+// A kernel that is launched behind another one of the same call starts while that one still runs (programmatic dependent launch):
+// its launch and its prologue are off the path.  The first says when (every block, or by ending), the second waits, before it
+// touches anything that the first has written, until the whole of the first is done and its writes are visible.
+__device__ __forceinline__ void release_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class P>
+cudaError_t launch_behind(void (*kern)(const P), const P& p, dim3 grid, int threads, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
 
 cudaError_t launch_kv4_append(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);
 cudaError_t launch_kv4_read(const Kv4Cache& c, const Kv4Rows& r, bool bf16, cudaStream_t stream);

@@ -67,30 +67,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 template <bool BF16>
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t x) {
   if constexpr (BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
   else return __half22float2(*reinterpret_cast<const __half2*>(&x));
-}
-
-// (w & mask) | bits
-__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask, uint32_t bits) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(w), "r"(mask), "r"(bits));
-  return d;
 }
 
 // The four pairs of codes of a word (nibble j of either half), for Q K^T: what they multiply to is the code times
@@ -100,29 +79,12 @@ template <bool BF16>
 __device__ __forceinline__ void key_codes(uint32_t w, uint32_t (&x)[4]) {
   if constexpr (BF16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = sub2<true>(mask_or(w >> (4 * j), 0x000f000fu, 0x43004300u), 0x43004300u);
+    for (int j = 0; j < 4; ++j) x[j] = kv4_sub2<true>(kv4_mask_or(w >> (4 * j), 0x000f000fu, 0x43004300u), 0x43004300u);
   } else {
     const uint32_t u = w >> 8;
     x[0] = w & 0x000f000fu; x[1] = w & 0x00f000f0u; x[2] = u & 0x000f000fu; x[3] = u & 0x00f000f0u;
   }
 }
-// The same for P V: the values, code * step + minimum, of two rows.
-template <bool BF16>
-__device__ __forceinline__ void value_pairs(uint32_t w, uint32_t step, uint32_t low, uint32_t (&x)[4]) {
-  if constexpr (BF16) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = sub2<true>(mask_or(w >> (4 * j), 0x000f000fu, 0x43004300u), 0x43004300u);
-  } else {
-    const uint32_t u = w >> 8;
-    x[0] = sub2<false>(mask_or(w, 0x000f000fu, 0x64006400u), 0x64006400u);      // 1024 + c
-    x[1] = sub2<false>(mask_or(w, 0x00f000f0u, 0x54005400u), 0x54005400u);      // 64 + c
-    x[2] = sub2<false>(mask_or(u, 0x000f000fu, 0x64006400u), 0x64006400u);
-    x[3] = sub2<false>(mask_or(u, 0x00f000f0u, 0x54005400u), 0x54005400u);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = fma2<BF16>(x[j], step, low);
-}
-
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* x) {      // N words, in as few loads as their alignment allows
   if constexpr (N % 4 == 0) {
@@ -218,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
   __shared__ uint64_t full[kWarps][kSlots];
   __shared__ volatile uint32_t abort_flag;
 
+  if constexpr (!CL) release_dependents();
   const int G = p.kv_group;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -501,8 +464,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
 #pragma unroll
       for (int grp = 0; grp < NG; ++grp) {
         uint32_t v0[4], v1[4];
-        value_pairs<BF16>(vw[grp], vsm[0][2 * grp], vsm[0][2 * grp + 1], v0);
-        value_pairs<BF16>(vw[NG + grp], vsm[1][2 * grp], vsm[1][2 * grp + 1], v1);
+        kv4_value_pairs<BF16>(vw[grp], vsm[0][2 * grp], vsm[0][2 * grp + 1], v0);
+        kv4_value_pairs<BF16>(vw[NG + grp], vsm[1][2 * grp], vsm[1][2 * grp + 1], v1);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -660,6 +623,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_finish_kernel(const Kv4Dec
   const int unit_kv = blockIdx.y, b = unit_kv / p.cache.N_kv, h_kv = unit_kv % p.cache.N_kv;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.kv_group, d = threadIdx.x;
   const int64_t unit0 = static_cast<int64_t>(b) * p.N + h_kv * G;      // the group's first query head
+  wait_for_primary();
   int len = p.cache.S_max;
   if (p.seq_lens != nullptr) len = min(len, max(0, p.seq_lens[b]));
   const int first = blockIdx.x * kFinishKeys;
@@ -784,9 +748,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t 
   if (e != cudaSuccess || p.clustered) return e;
   const int chunks = p.weights != nullptr ? (p.cache.S_max + kFinishKeys - 1) / kFinishKeys : 1;
   const dim3 grid(chunks > p.kv_group ? chunks : p.kv_group, p.B * p.cache.N_kv);
-  if (bf16) kv4_finish_kernel<true><<<grid, kFinishThreads, 0, stream>>>(p);
-  else kv4_finish_kernel<false><<<grid, kFinishThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_behind(bf16 ? kv4_finish_kernel<true> : kv4_finish_kernel<false>, p, grid, kFinishThreads, stream);
 }
 
 }  // namespace acct
