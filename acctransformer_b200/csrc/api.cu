@@ -186,12 +186,12 @@ unsigned int* device_status_ptr() {
   return d->status;
 }
 
-int make_tmap_4d(CUtensorMap* out, const TensorDesc4& t, int box_rows) {
+int make_tmap_4d(CUtensorMap* out, const TensorDesc4& t, int box_rows, int box_outer) {
   cuuint64_t dims[4] = {(cuuint64_t)t.dims[0], (cuuint64_t)t.dims[1], (cuuint64_t)t.dims[2], (cuuint64_t)t.dims[3]};
   // rows of the box are 128 bytes: 64 sixteen-bit elements, or 32 fp32 elements (the dQ accumulator)
   const cuuint64_t esz = t.dtype == ACCT_F32 ? 4 : 2;
   cuuint64_t strides[3] = {(cuuint64_t)t.strides[0] * esz, (cuuint64_t)t.strides[1] * esz, (cuuint64_t)t.strides[2] * esz};
-  cuuint32_t box[4] = {(cuuint32_t)(128 / esz), (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t box[4] = {(cuuint32_t)(128 / esz), (cuuint32_t)box_rows, (cuuint32_t)box_outer, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUtensorMapDataType dt = t.dtype == ACCT_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : t.dtype == ACCT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -624,7 +624,7 @@ int acct_fa_bwd_planned(const acct_fa_args* a, const acct_fa_bwd_io* g, const in
   float* delta = static_cast<float*>(g->workspace);
   const int kernel = bwd_kernel(a);
   const bool mid = kernel == ACCT_BWD_MID, pair = kernel == ACCT_BWD_PAIR;
-  const bool wide = a->D > 128;      // the split-width kernel: 64-row Q / dO boxes, 64-row dQ box, 2 counters per tile
+  const bool wide = a->D > 128 || (getenv("PKL") && atoi(getenv("PKL")));      // the split-width kernel: 64-row Q / dO boxes, 64-row dQ box, 2 counters per tile
   const size_t q_tiles = static_cast<size_t>(a->B) * a->N * ((a->S_q + kTile - 1) / kTile) * (wide ? 2 : 1) + 1;   // + work counter
   const size_t order_bytes = ((q_tiles * 4 + 255) / 256) * 256;
   unsigned int* dq_order = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(g->workspace) + ((rows * 4 + 255) / 256) * 256);
@@ -765,17 +765,40 @@ int acct_infer_packed(const acct_packed_args* a, void* stream) {
   PerDevice* dev = nullptr;
   if ((rc = init_device(&dev))) return rc;
   if (a->T_q == 0) return ACCT_OK;
-  const int64_t tiles = (static_cast<int64_t>(a->T_q) + 127ll * a->B) / 128 + 1;
-  if (tiles * a->N > INT32_MAX) return fail(ACCT_ERR_SHAPE, "T_q = %d rows of N = %d heads are too many for one call", a->T_q, a->N);
+  // Two kernels.  fa_fwd.cu has two tiles of a head in a block, which share each load of K and V; fa_fwd_packed.cu has one tile of
+  // several heads in a block and two blocks on an SM, which hide each other's beginnings and ends.  The time of the first over that
+  // of the second (10 .. 40 heads of 64 and 128, on as many or on a quarter): 1.5-1.9 at 256 tokens per sequence, 1.2-1.35 at
+  // 1 024, 1.0-1.2 at 2 048, 0.8-1.06 at 4 096, 0.85-0.95 at 16 384; with 256 queries on 8 192 keys 0.58-1.05.  Fewer queries
+  // than that would leave the second tile of a pair empty.
+  const bool pairs = a->D > 128 || (a->T_k >= static_cast<int64_t>(4096) * a->B && a->T_q >= static_cast<int64_t>(256) * a->B);
+  // Rows of a tile in the second: query heads that share a head of K and V, as many as fill 120 of 128 with whole tokens (all of a
+  // group up to 8, of 10, 12, 16, ..), else those that fill the most.
+  const int group = a->N / n_kv;
+  p.tile_heads = 1;
+  p.tile_tokens = kTile;
+  for (int heads = group < kTile ? group : kTile, most = 0; !pairs && heads >= 1; --heads) {
+    const int rows = kTile / heads * heads;
+    if (group % heads != 0 || rows <= most) continue;
+    most = rows;
+    p.tile_heads = heads;
+    p.tile_tokens = kTile / heads;
+    if (rows >= 120) break;
+  }
+  const int64_t tiles = (static_cast<int64_t>(a->T_q) + static_cast<int64_t>(p.tile_tokens) * a->B) / p.tile_tokens + 1;
+  if (tiles * (a->N / p.tile_heads) > INT32_MAX) return fail(ACCT_ERR_SHAPE, "T_q = %d rows of N = %d heads are too many for one call", a->T_q, a->N);
   for (int i = 0; i < 4; ++i) {
     TensorDesc4 t;
     t.dtype = a->dtype;
     const bool none = operands[i].rows == 0;       // no keys at all: a map of one row that no load asks for
+    const bool by_head = !pairs && (i == 0 || i == 3);      // (column, head, row) instead of (column, row, head)
     t.ptr = none ? a->q : operands[i].ptr;
-    t.dims[0] = a->D; t.dims[1] = none ? 1 : operands[i].rows; t.dims[2] = none ? 1 : operands[i].heads; t.dims[3] = 1;
-    t.strides[0] = strides[i][0]; t.strides[1] = strides[i][1];
+    t.dims[0] = a->D; t.dims[3] = 1;
+    t.dims[by_head ? 2 : 1] = none ? 1 : operands[i].rows;
+    t.dims[by_head ? 1 : 2] = none ? 1 : operands[i].heads;
+    t.strides[by_head ? 1 : 0] = strides[i][0];
+    t.strides[by_head ? 0 : 1] = strides[i][1];
     t.strides[2] = std::max(strides[i][0], strides[i][1]);      // (of a dimension of size 1)
-    if ((rc = make_tmap_4d(operands[i].map, t, kTile))) return rc;
+    if ((rc = make_tmap_4d(operands[i].map, t, by_head ? p.tile_heads : kTile, by_head ? p.tile_tokens : 1))) return rc;
   }
   p.o = a->y;
   p.lse = a->lse;
@@ -790,7 +813,9 @@ int acct_infer_packed(const acct_packed_args* a, void* stream) {
   p.mods.causal = a->causal ? 1 : 0;
   p.mods.prev_block_num = p.mods.next_block_num = ACCT_BAND_UNBOUNDED;
   p.status = dev->status;
-  const cudaError_t e = launch_fa_fwd_packed(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  const bool bf16 = a->dtype == ACCT_BF16;
+  const cudaError_t e = pairs ? launch_fa_fwd_packed_long(p, bf16, static_cast<cudaStream_t>(stream))
+                              : launch_fa_fwd_packed(p, bf16, dev->info.sm_count, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "launching the packed forward kernel");
   return ACCT_OK;
 }

@@ -27,7 +27,8 @@ struct TensorDesc4 {
   int64_t strides[3];     // element strides of S, N, B
 };
 // Tiled map with a {64, box_rows, 1, 1} box and 128-byte swizzle (64 two-byte elements per row).
-int make_tmap_4d(CUtensorMap* out, const TensorDesc4& t, int box_rows);
+// (box_outer: entries of the third dimension, side by side behind the rows of the second)
+int make_tmap_4d(CUtensorMap* out, const TensorDesc4& t, int box_rows, int box_outer = 1);
 
 inline int64_t packed_or(int64_t given, int64_t packed) { return given == 0 ? packed : given; }
 

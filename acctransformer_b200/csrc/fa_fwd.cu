@@ -31,6 +31,7 @@
 
 #include "fa_common.cuh"
 #include "fa_kernels.cuh"
+#include "fa_packed.cuh"
 #include "ptx.cuh"
 
 namespace acct {
@@ -65,11 +66,6 @@ __device__ __forceinline__ TileRange kv_tile_range(int i, int s_q, int kv_len, c
   return r;
 }
 
-// What a thread block of the packed form works on: tile (pair) `pair` of the sequence whose rows begin at q0 and k0.
-struct PackedItem {
-  int pair, q0, len_q, k0, len_k;
-};
-
 struct FwdShared {
   uint64_t q_full;
   uint64_t k_full[kStages], k_empty[kStages];
@@ -84,98 +80,6 @@ struct FwdShared {
   alignas(16) float alibi[2][2][kTile];   // [softmax group][tile parity]: alibi row of the K/V tile, log2 units
   PackedItem item;
 };
-
-// The `item`-th tile (pair) of all sequences, those with the most K/V tiles first (a late start of a long one is what the SMs
-// would wait for at the end); len_q = 0 where there are not so many.  One warp; a lane has sequences lane, lane + 32, ...  Up to
-// 128 sequences the order comes from a search over the number of K/V tiles, which no plan made beforehand could do much faster
-// (some 500 clk while the block sets itself up); with more, long ones matter less, and they come one after the other.
-template <int NQ>
-__device__ __forceinline__ void find_packed_item(const FwdParams& p, int item, PackedItem* out) {
-  constexpr int kRows = NQ * kTile, kPer = 4;
-  const int lane = threadIdx.x & 31;
-  auto read = [&](int b, PackedItem& s) {      // (whatever cu holds, no row outside [0, T) is touched)
-    s.q0 = min(max(p.cu_q[b], 0), p.T_q);
-    s.len_q = min(max(p.cu_q[b + 1], s.q0), p.T_q) - s.q0;
-    s.k0 = min(max(p.cu_k[b], 0), p.T_k);
-    s.len_k = min(max(p.cu_k[b + 1], s.k0), p.T_k) - s.k0;
-  };
-  // pairs of the sequence with `tiles` or more K/V tiles: from a certain one on, with a causal mask
-  auto pairs_with = [&](const PackedItem& s, int tiles) {
-    const int n = (s.len_q + kRows - 1) / kRows;
-    if (tiles <= 0) return n;
-    const int keys = (tiles - 1) * kTile + 1;                  // a pair that sees this many
-    if (s.len_k < keys) return 0;
-    if (!p.mods.causal) return n;
-    const int rows = keys - (s.len_k - s.len_q);               // ... has its last row here or later
-    return n - min(n, max(0, (rows + kRows - 1) / kRows - 1));
-  };
-  PackedItem found = {0, 0, 0, 0, 0};
-  auto settle = [&](const PackedItem& s, int n, int first, int& left) {      // true where the item is one of this round's
-    int upto = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += x;
-    }
-    const unsigned int past = __ballot_sync(0xffffffffu, upto > left);
-    if (past == 0u) {
-      left -= __shfl_sync(0xffffffffu, upto, 31);
-      return false;
-    }
-    const int from = __ffs(past) - 1;
-    found.pair = __shfl_sync(0xffffffffu, first, from) + left - __shfl_sync(0xffffffffu, upto - n, from);
-    found.q0 = __shfl_sync(0xffffffffu, s.q0, from);
-    found.len_q = __shfl_sync(0xffffffffu, s.len_q, from);
-    found.k0 = __shfl_sync(0xffffffffu, s.k0, from);
-    found.len_k = __shfl_sync(0xffffffffu, s.len_k, from);
-    return true;
-  };
-  if (p.B <= 32 * kPer) {
-    PackedItem s[kPer];
-    int most = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      s[i] = {0, 0, 0, 0, 0};
-      if (lane + 32 * i < p.B) read(lane + 32 * i, s[i]);
-      most = max(most, (s[i].len_k + kTile - 1) / kTile);
-    }
-    auto count = [&](int tiles) {
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) n += pairs_with(s[i], tiles);
-      return __reduce_add_sync(0xffffffffu, n);
-    };
-    most = __reduce_max_sync(0xffffffffu, most);
-    int lo = 0, hi = most + 1, before = 0;       // count(lo) > item >= count(hi) = before
-    if (count(0) > item) {
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2, n = count(mid);
-        if (n > item) lo = mid;
-        else { hi = mid; before = n; }
-      }
-      int left = item - before;                  // among the pairs with exactly `lo` tiles
-      bool done = false;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (!done) {
-          const int least = pairs_with(s[i], lo), n = least - pairs_with(s[i], lo + 1);
-          done = settle(s[i], n, (s[i].len_q + kRows - 1) / kRows - least, left);
-        }
-    }
-  } else {
-    int left = item;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      PackedItem s = {0, 0, 0, 0, 0};
-      if (b0 + lane < p.B) read(b0 + lane, s);
-      const int n = pairs_with(s, 0);
-      if (settle(s, n, 0, left)) {
-        found.pair = (found.len_q + kRows - 1) / kRows - 1 - found.pair;
-        break;
-      }
-    }
-  }
-  if (lane == 0) *out = found;
-}
 
 }  // namespace
 
@@ -223,9 +127,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
     const int hg = blockIdx.x / per_group, within = blockIdx.x % per_group;
     const int heads = min(p.head_group, p.N - hg * p.head_group);
     bh = hg * p.head_group + within % heads;
-    if (warp == 0) find_packed_item<NQ>(p, within / heads, &sh.item);
+    if (warp == 0) {
+      const PackedItem found = PackedFinder(p, NQ * kTile).find(within / heads);
+      if (lane == 0) sh.item = found;
+    }
     __syncthreads();
-    pair = sh.item.pair; len_q = sh.item.len_q; q_base = sh.item.q0; k_base = sh.item.k0;
+    pair = sh.item.tile; len_q = sh.item.len_q; q_base = sh.item.q0; k_base = sh.item.k0;
   } else {
     const int kUnitGroup = p.unit_group;
     const int per_group = n_pairs * kUnitGroup;
@@ -1105,15 +1012,14 @@ cudaError_t launch_mask_classify(const void* mask, int dtype, int batch, int S_q
   return cudaGetLastError();
 }
 
-cudaError_t launch_fa_fwd_packed(const FwdParams& p, bool bf16, cudaStream_t stream) {
+cudaError_t launch_fa_fwd_packed_long(const FwdParams& p, bool bf16, cudaStream_t stream) {
   const int dpad = p.D <= 64 ? 64 : (p.D <= 128 ? 128 : 256);
   const int nq = dpad > 128 ? 1 : 2, stages = dpad > 128 ? 1 : kStages, rows = nq * kTile;
   const size_t smem = static_cast<size_t>(nq + 2 * stages) * (dpad / 64) * 16384 + 1024;
   FwdParams pp = p;
   pp.tile_bound = static_cast<int>((static_cast<int64_t>(p.T_q) + static_cast<int64_t>(rows - 1) * p.B) / rows);
   // Heads that run at the same time share L2: as many as have their K and V in 48 MB of it, whole groups of query heads.
-  const int64_t head_bytes = 4ll * p.T_k * p.D;
-  const int64_t fit = (48ll << 20) / (head_bytes > 0 ? head_bytes : 1);
+  const int64_t fit = (48ll << 20) / (4ll * p.T_k * p.D + 1);
   pp.head_group = static_cast<int>(fit < 1 ? p.kv_group : fit * p.kv_group < p.N ? fit * p.kv_group : p.N);
   void (*kern)(const FwdParams) = dpad == 64    ? (bf16 ? fa_fwd_kernel<64, true, 0, 0, true> : fa_fwd_kernel<64, false, 0, 0, true>)
                                   : dpad == 128 ? (bf16 ? fa_fwd_kernel<128, true, 0, 0, true> : fa_fwd_kernel<128, false, 0, 0, true>)

@@ -87,11 +87,12 @@ struct alignas(64) FwdParams {
   float scale, scale_log2;          // scale_log2 = scale * log2(e)
   ScoreMods mods;
   unsigned int* status;
-  // packed sequences (launch_fa_fwd_packed): q, o are [T_q, N, D], k, v [T_k, N_kv, D], lse [N, T_q]
+  // packed sequences (launch_fa_fwd_packed, launch_fa_fwd_packed_long): q, o are [T_q, N, D], k, v [T_k, N_kv, D], lse [N, T_q]
   const int *cu_q, *cu_k;           // [B + 1]: sequence b has rows cu[b] .. cu[b + 1] - 1
   int T_q, T_k;
-  int tile_bound;                   // tiles (pairs of them up to head_dim 128) that T_q rows of B sequences can make
-  int head_group;                   // heads whose thread blocks are interleaved
+  int tile_heads, tile_tokens;      // a tile is so many query heads (a divisor of kv_group) of so many tokens, 128 rows at most
+  int tile_bound;                   // tiles that T_q rows of B sequences can make
+  int head_group;                   // heads, or groups of tile_heads, whose thread blocks are interleaved
 };
 
 struct alignas(64) BwdParams {
@@ -165,8 +166,10 @@ cudaError_t resident_clusters(const void* kernel, const cudaLaunchConfig_t& cfg,
 
 // Launchers: return cudaGetLastError() of the launch.
 cudaError_t launch_fa_fwd(const FwdParams& p, bool bf16, int sm_count, cudaStream_t stream);
-// packed sequences: maps of one batch entry with T_q, T_k rows; mods.causal and no other limit
-cudaError_t launch_fa_fwd_packed(const FwdParams& p, bool bf16, cudaStream_t stream);
+// packed sequences: maps of one batch entry with T_q, T_k rows, mods.causal and no other limit.  The first: head_dim up to 128, maps
+// of q and o with dimensions (column, head, row) and boxes of tile_heads x tile_tokens; the second: any head_dim, launch_fa_fwd's maps.
+cudaError_t launch_fa_fwd_packed(const FwdParams& p, bool bf16, int sm_count, cudaStream_t stream);
+cudaError_t launch_fa_fwd_packed_long(const FwdParams& p, bool bf16, cudaStream_t stream);
 cudaError_t launch_fa_bwd(const BwdParams& p, bool bf16, int sm_count, cudaStream_t stream);
 // head_dim in (64, 128], dQ in any order, no mask tensor, alibi, band, valid lengths or dropout, row groups of whole tiles:
 // like launch_fa_bwd with 64-row boxes of the Q, dO and dQ maps

@@ -578,7 +578,9 @@ Kv4 kv4_arg(PyObject* p) {
 Tensor ints_on(const char* name, const Tensor& t, int64_t n, const Tensor& like) {
   require_cuda(name, t);
   HOST_CHECK(t.device() == like.device(), name, " must be on the device of the other operands, ", like.device(), ", not on ", t.device());
-  HOST_CHECK(t.numel() >= n && !t.is_floating_point(), name, " must hold ", n, " integers, got ", t.numel(), " of ", t.scalar_type());
+  HOST_CHECK(t.numel() >= n && at::isIntegralType(t.scalar_type(), /*includeBool=*/false), name, " must hold ", n, " integers, got ", t.numel(),
+             " of ", t.scalar_type());
+  if (t.scalar_type() == at::kInt && t.is_contiguous()) return t;      // (the usual case, without two trips through the dispatcher)
   return t.to(at::kInt).contiguous();
 }
 void kv4_rows(const Kv4& cache, const Tensor& start, const Tensor& cu, acct_kv4_rows& r) {
