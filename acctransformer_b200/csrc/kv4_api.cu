@@ -86,7 +86,7 @@ using namespace acct;
 
 extern "C" {
 
-size_t acct_kv4_record_bytes(int32_t D) { return D > 0 && D <= 32 * kKv4MaxGroups ? static_cast<size_t>(640) * ((D + 31) / 32) : 0; }
+size_t acct_kv4_record_bytes(int32_t D) { return D > 0 && D % 8 == 0 && D <= 32 * kKv4MaxGroups ? static_cast<size_t>(640) * ((D + 31) / 32) : 0; }
 
 int acct_kv4_append(const acct_kv4_cache* c, const acct_kv4_rows* r, void* stream) { return rows_call(c, r, true, stream); }
 

@@ -3,7 +3,7 @@
 // The step is bound by reading the cache once (160 bytes per key and head at head_dim 128), but at 5 bits a value there is little
 // time per value: an SM gets 23 bytes per clock, a 16-row record in 110, in which its four schedulers issue 440 instructions
 // for 4 096 codes.  So rows and columns of the cache are the 16-row operand of mma.m16n8k16 and the query heads the 8 columns of
-// the other (17 products a record for up to 8 heads), and a code takes no arithmetic of its own that can be avoided:
+// the other (17 products a record for up to 4 heads), and a code takes no arithmetic of its own that can be avoided:
 //   S^T = K Q^T   k = s c + m splits into s (c Q) + m (sum of Q): the codes go into the product as they are, one group of 32 columns
 //                 at a time, and s and m meet 16 x 8 sums instead of 16 x 128 values.  In fp16 a code in the low bits of a half is
 //                 the subnormal number c * 2^-24, exact to multiply (and c * 2^-20 four bits up: those columns of Q are divided by
@@ -11,6 +11,11 @@
 //                 of Q is one more product, whose operand holds the sums in three parts so that nothing of them is lost.
 //   O^T += V^T P  here the steps belong to the contraction: v = s c + m is formed in 16 bits (one rounding, as if the cache were
 //                 in 16 bits), two rows of a column at a time, with the code subtracted out of 1024 + c, 64 + c or 128 + c.
+//                 P is rounded to 16 bits too, which would cost as much again (in fp16, over 2 048 keys, 3.4e-4 of the result from
+//                 the exact one; its own last rounding makes 2.1e-4).  What the rounding leaves is an operand as well: with up to 4
+//                 heads in the 4 columns that they leave free, where it costs 12 instructions a record (105 -> 108 us at 32 x 8
+//                 slices of up to 16 384 keys), up to 8 in products of its own (124 -> 129): 2.8e-4.  With more it is left out: 212
+//                 us would be 237, and the 4 bits are coarser by two orders.
 // The running maximum is only refreshed where a score exceeds it by more than 8 (in log2 units), so that most records need no
 // exchange between lanes.  Records come in by one bulk copy each through a ring per warp; nothing is shared between the warps of
 // a block before the end.
@@ -159,7 +164,7 @@ constexpr float kRefresh = 8.0f;      // log2 units by which a score may exceed 
 
 // Resident thread blocks per SM, which the registers decide (152 and 230 a thread).  With four, at 128 registers, or five, at 96
 // and a record at a time, the step is no faster (32 x 8 slices of up to 16 384 keys 95 and 103 us against 90).
-constexpr int blocks_per_sm(int hi) { return hi == 1 ? 3 : 2; }
+constexpr int blocks_per_sm(int heads) { return heads <= 8 ? 3 : 2; }
 
 // the float at `p` of this block's shared memory, in that of block `rank` of the cluster
 __device__ __forceinline__ float cluster_read(const float* p, uint32_t rank) {
@@ -170,11 +175,13 @@ __device__ __forceinline__ float cluster_read(const float* p, uint32_t rank) {
 
 constexpr int kMaxCluster = 8;
 
-// HI: columns of 8 query heads (1 up to a group of 8, else 2).  CL: the parts of a slice are one cluster, and finish together.
-template <int NG, bool BF16, int HI, bool CL>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel(const Kv4DecodeParams p) {
+// HEADS: 4, 8 or 16, query heads per cache head at most.  CL: the parts of a slice are one cluster, and finish together.
+template <int NG, bool BF16, int HEADS, bool CL>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(HEADS)) kv4_decode_kernel(const Kv4DecodeParams p) {
   using R = Kv4Record<NG>;
-  constexpr int DPAD = 32 * NG, kHeads = 8 * HI;
+  constexpr int DPAD = 32 * NG, HI = HEADS > 8 ? 2 : 1, kHeads = 8 * HI;      // HI: times 8 columns
+  constexpr bool kSpare = HEADS == 4;      // columns 4..7 are heads 0..3 once more, with what is left of P
+  constexpr bool kRest = HEADS == 8;       // a product of its own for what is left
 
   extern __shared__ __align__(128) uint8_t ksm[];
   __shared__ uint64_t full[kWarps][kSlots];
@@ -282,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
   uint32_t qb[HI][2 * NG][2], qm[HI][2];
 #pragma unroll
   for (int hi = 0; hi < HI; ++hi) {
-    const int head = g + 8 * hi;
+    const int head = kSpare ? g & 3 : g + 8 * hi;
     float mean_t = 0.f;
 #pragma unroll
     for (int grp = 0; grp < NG; ++grp) {
@@ -436,7 +443,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
     // ---- P, and O^T += V^T P
 #pragma unroll
     for (int r = 0; r < kStepRecs; ++r) {
-      uint32_t pb[HI][2];      // P in 16 bits is the operand of P V; the sum is of what it was before
+      // P in 16 bits is the operand of P V, and what that leaves of it another one; the sum of P is of what it was before
+      uint32_t pb[HI][2], rest[HI][2];
 #pragma unroll
       for (int hi = 0; hi < HI; ++hi) {
         float pr[4];
@@ -444,8 +452,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
         for (int e = 0; e < 4; ++e) pr[e] = ex2(x[r][hi][e] - m_run[hi][e & 1]);
         l_run[hi][0] += pr[0] + pr[2];
         l_run[hi][1] += pr[1] + pr[3];
-        pb[hi][0] = transpose8(pack2<BF16>(pr[0], pr[1]));
-        pb[hi][1] = transpose8(pack2<BF16>(pr[2], pr[3]));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t w = pack2<BF16>(pr[2 * e], pr[2 * e + 1]);
+          const float2 f = unpack2<BF16>(w);
+          const uint32_t left = pack2<BF16>(pr[2 * e] - f.x, pr[2 * e + 1] - f.y);
+          if (kSpare && t >= 2) w = left;
+          pb[hi][e] = transpose8(w);
+          if (kRest) rest[hi][e] = transpose8(left);
+        }
       }
       const uint8_t* rec = rec0 + r * R::kBytes;
       uint32_t vw[2 * NG], vsm[2][2 * NG];
@@ -469,8 +484,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int hi = 0; hi < HI; ++hi)
+          for (int hi = 0; hi < HI; ++hi) {
             mma16816<BF16>(o[hi][2 * grp + j], v0[2 * j], v0[2 * j + 1], v1[2 * j], v1[2 * j + 1], pb[hi][0], pb[hi][1]);
+            if (kRest) mma16816<BF16>(o[hi][2 * grp + j], v0[2 * j], v0[2 * j + 1], v1[2 * j], v1[2 * j + 1], rest[hi][0], rest[hi][1]);
+          }
       }
     }
     if (++slot == kSlots) { slot = 0; parity ^= 1u; }
@@ -485,6 +502,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HI)) kv4_decode_kernel
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int bit = 4; bit < 32; bit <<= 1) l_run[hi][e] += __shfl_xor_sync(0xffffffffu, l_run[hi][e], bit);
+  if (kSpare) {      // (their maxima are those of the heads, of which they are copies)
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[0][i][e] += __shfl_xor_sync(0xffffffffu, o[0][i][e], 2);
+  }
   linger_after_abort(&abort_flag);
   __syncthreads();
   float* s_acc = reinterpret_cast<float*>(ksm);                       // [warp][kHeads][DPAD]
@@ -708,15 +731,17 @@ __global__ void __launch_bounds__(kFinishThreads) kv4_finish_kernel(const Kv4Dec
 
 template <int NG>
 cudaError_t launch_ng(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int* resident) {
-  const bool upper = p.kv_group > 8;
+  const int heads = p.kv_group > 8 ? 16 : p.kv_group > 4 ? 8 : 4;
   const size_t ring = static_cast<size_t>(kWarps) * kSlots * kStepRecs * Kv4Record<NG>::kBytes;
-  const size_t merge = static_cast<size_t>(kWarps) * (upper ? 16 : 8) * (32 * NG + 2) * sizeof(float);
+  const size_t merge = static_cast<size_t>(kWarps) * (heads > 8 ? 16 : 8) * (32 * NG + 2) * sizeof(float);
   // No more blocks to an SM than the grid counts on, also where fewer groups need less: with room for more, some SMs are given more
   // and others fewer, and everybody waits for the former.
-  const size_t least = (227 << 10) / (blocks_per_sm(upper ? 2 : 1) + 1) + 1;
+  const size_t least = (227 << 10) / (blocks_per_sm(heads) + 1) + 1;
   const size_t smem = std::max({ring, merge, least});
-#define KV4_DECODE(BF, HI) (p.clustered ? kv4_decode_kernel<NG, BF, HI, true> : kv4_decode_kernel<NG, BF, HI, false>)
-  void (*kern)(const Kv4DecodeParams) = bf16 ? (upper ? KV4_DECODE(true, 2) : KV4_DECODE(true, 1)) : (upper ? KV4_DECODE(false, 2) : KV4_DECODE(false, 1));
+#define KV4_DECODE(BF, HEADS) (p.clustered ? kv4_decode_kernel<NG, BF, HEADS, true> : kv4_decode_kernel<NG, BF, HEADS, false>)
+#define KV4_DECODE_HEADS(BF) (heads == 4 ? KV4_DECODE(BF, 4) : heads == 8 ? KV4_DECODE(BF, 8) : KV4_DECODE(BF, 16))
+  void (*kern)(const Kv4DecodeParams) = bf16 ? KV4_DECODE_HEADS(true) : KV4_DECODE_HEADS(false);
+#undef KV4_DECODE_HEADS
 #undef KV4_DECODE
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
@@ -737,7 +762,7 @@ cudaError_t launch_ng(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, 
 
 }  // namespace
 
-int kv4_decode_blocks_per_sm(int kv_group) { return blocks_per_sm(kv_group > 8 ? 2 : 1); }
+int kv4_decode_blocks_per_sm(int kv_group) { return blocks_per_sm(kv_group); }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, bool bf16, cudaStream_t stream, int* resident) {
   const int groups = (p.D + 31) / 32;

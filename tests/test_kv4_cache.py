@@ -67,6 +67,23 @@ def _stood_for(x):
     return torch.from_numpy(out).to(x.dtype)
 
 
+def _stood_for_exactly(x):
+    """The same before the last rounding to 16 bits: what the codes, steps and minima of x say, in float64."""
+    a, u = x.float(), []
+    for at in range(0, a.shape[-1], 32):
+        y = a[..., at:at + 32]
+        lo, hi = y.amin(-1, keepdim=True), y.amax(-1, keepdim=True)
+        want = (hi - lo) / 15
+        if x.dtype == torch.bfloat16:
+            s = (want.view(torch.int32) & -65536).view(torch.float32)
+        else:
+            h = want.half()
+            s = torch.where(h.float() > want, torch.nextafter(h.cpu(), torch.zeros((), dtype=torch.half)).to(h.device), h).float()
+        code = torch.round(torch.clamp((y - lo) * torch.where(s > 0, 1 / s, 0.0), max=15.0))
+        u.append(code.double() * s.double() + lo.double())
+    return torch.cat(u, -1)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # rows in and out
 # ---------------------------------------------------------------------------------------------------------------------
@@ -281,6 +298,85 @@ def test_what_lies_past_the_length_does_not_matter():
     # a NaN inside the length does reach the result
     y = cache.decode(q, _ints([6, 20]))
     assert y[0].isnan().all() and y[1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 8])
+def test_probabilities_keep_more_than_16_bits(group, dtype):
+    """V in 0..15 with both in every group of 32, step 1 and minimum 0: its values are exact.  P is a sum of two 16-bit numbers up to a
+    group of 8 (a relative u^2; in float16 a half unit of its smallest number, 2^-25, for each), so little but the last
+    rounding is left."""
+    lens, N_kv, S, D, u = [5, 40, 300], 2, 300, 128, UNIT[dtype]
+    T = sum(lens)
+    cache = _cache(3, N_kv, S, D, dtype, seed=21)
+    g = torch.Generator(device="cuda").manual_seed(group)
+    k, v = _rows(T, N_kv, D, dtype, 21)[0], torch.randint(0, 16, (T, N_kv, D), device="cuda", generator=g).to(dtype)
+    v[..., 0::32], v[..., 1::32] = 0, 15
+    zero, cu = _ints([0] * 3), _ints([0, 5, 45, 345])
+    cache.append(k, v, zero, cu)
+    _, v_read = cache.read(zero, cu, total=T)
+    assert torch.equal(v_read, v)
+    q = (0.5 * torch.randn(3, N_kv * group, 1, D, device="cuda", generator=g)).to(dtype)
+    w = torch.zeros(3, N_kv, S, device="cuda")
+    y = cache.decode(q, _ints(lens), weights=w)
+    for b, n in enumerate(lens):
+        at = sum(lens[:b])
+        for h in range(N_kv):
+            qq, kk, vv = (x.double() for x in (q[b, h * group:(h + 1) * group, 0], _stood_for_exactly(k[at:at + n, h]).cuda(), v[at:at + n, h]))
+            p = torch.softmax(qq @ kk.T * D ** -0.5, -1)
+            e = 2.0 ** -20 * float((qq.abs() @ kk.abs().T * D ** -0.5).max()) + 2.0 ** -18
+            want = p @ vv
+            room = want * (u * u + math.expm1(2 * e)) + n * 15 * 2.0 ** -25
+            got = y[b, h * group:(h + 1) * group, 0].double()
+            assert ((got - want).abs() <= u * (want + room) + room).all(), float(((got - want).abs() / (u * want)).max())
+
+
+def test_steps_in_a_graph():
+    """Writing, decoding and eviction captured once and replayed on new contents: as the calls themselves give it."""
+    B, N_kv, D, S, dtype = 3, 2, 64, 200, torch.float16
+    lens = [200, 90, 1]
+    zero, cu = _ints([0] * B), _ints([0, 200, 290, 291])
+    k, v = _rows(291, N_kv, D, dtype, 31)
+    q = torch.randn(B, 8, 1, D, device="cuda").to(dtype)
+    w = torch.zeros(B, N_kv, S, device="cuda")
+    seq = _ints(lens)
+    cache, spare = _cache(B, N_kv, S, D, dtype, seed=1), _cache(B, N_kv, 64, D, dtype, seed=2)
+
+    def steps():
+        w.zero_()
+        cache.append(k, v, zero, cu)
+        y = cache.decode(q, seq, weights=w)
+        return (y, w.clone(), *cache.evict(w, seq, 64, 5, spare), *spare.read(zero, cu[:4].clamp(max=64), total=64))
+
+    steps()      # (what a first call sets up)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = steps()
+    for seed in (32, 33):
+        for x, y in zip((k, v), _rows(291, N_kv, D, dtype, seed)):
+            x.copy_(y)
+        q.copy_(torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)))
+        want = [x.clone() for x in steps()]
+        for x in out:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (x, y) in enumerate(zip(out, want)):
+            assert torch.equal(x, y), i
+
+
+def test_the_example(tmp_path):
+    """The example's loop, small enough to fill and evict twice; decoding there agrees with attention over the same rows to what 16-bit
+    values of K and V, P and the result differ by: 4 roundings of 2^-9 rms, and as much again for the scores."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve_kv4.py")
+    spec = importlib.util.spec_from_file_location("serve_kv4", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    r = module.serve(layers=2, batch=3, slots=96, tokens=120, hidden=128)
+    assert r["evictions"] >= 2 and max(r["lens"]) <= 96 and r["difference"] < 8 * 2.0 ** -9 and r["out"].isfinite().all()
+    assert r["cache_bytes"] < 0.33 * r["bytes_in_16_bits"]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
