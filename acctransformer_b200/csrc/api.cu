@@ -767,10 +767,12 @@ int acct_infer_packed(const acct_packed_args* a, void* stream) {
   if (a->T_q == 0) return ACCT_OK;
   // Two kernels.  fa_fwd.cu has two tiles of a head in a block, which share each load of K and V; fa_fwd_packed.cu has one tile of
   // several heads in a block and two blocks on an SM, which hide each other's beginnings and ends.  The time of the first over that
-  // of the second (10 .. 40 heads of 64 and 128, on as many or on a quarter): 1.5-1.9 at 256 tokens per sequence, 1.2-1.35 at
-  // 1 024, 1.0-1.2 at 2 048, 0.8-1.06 at 4 096, 0.85-0.95 at 16 384; with 256 queries on 8 192 keys 0.58-1.05.  Fewer queries
-  // than that would leave the second tile of a pair empty.
-  const bool pairs = a->D > 128 || (a->T_k >= static_cast<int64_t>(4096) * a->B && a->T_q >= static_cast<int64_t>(256) * a->B);
+  // of the second (10 .. 40 heads, on as many or on a quarter), as tokens per sequence: 1.6-2.0 at 256, 1.25-1.4 at 1 024, 1.0-1.25
+  // at 2 048; head_dim 128 0.96-1.0 at 4 096, 0.9 at 8 192, 0.85 at 16 384, 0.86-1.0 with 1 024 queries on 8 192 keys; head_dim 64
+  // 0.98-1.1 at 4 096, 0.92-1.02 at 8 192, 0.88-0.97 at 16 384, 0.96-0.98 with 1 024 queries.  Fewer than 256 queries would leave
+  // the second tile of a pair empty (with 256 0.54-1.04).
+  const int64_t long_enough = a->D > 64 ? 4096 : 8192;
+  const bool pairs = a->D > 128 || (a->T_k >= long_enough * a->B && a->T_q >= static_cast<int64_t>(256) * a->B);
   // Rows of a tile in the second: query heads that share a head of K and V, as many as fill 120 of 128 with whole tokens (all of a
   // group up to 8, of 10, 12, 16, ..), else those that fill the most.
   const int group = a->N / n_kv;

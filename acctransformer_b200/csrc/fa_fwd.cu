@@ -128,7 +128,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fa_fwd_kernel(const __grid_con
     const int heads = min(p.head_group, p.N - hg * p.head_group);
     bh = hg * p.head_group + within % heads;
     if (warp == 0) {
-      const PackedItem found = PackedFinder(p, NQ * kTile).find(within / heads);
+      PackedFinder finder(p);
+      finder.load();
+      const PackedItem found = finder.find(within / heads);
       if (lane == 0) sh.item = found;
     }
     __syncthreads();
@@ -1017,7 +1019,7 @@ cudaError_t launch_fa_fwd_packed_long(const FwdParams& p, bool bf16, cudaStream_
   const int nq = dpad > 128 ? 1 : 2, stages = dpad > 128 ? 1 : kStages, rows = nq * kTile;
   const size_t smem = static_cast<size_t>(nq + 2 * stages) * (dpad / 64) * 16384 + 1024;
   FwdParams pp = p;
-  pp.tile_bound = static_cast<int>((static_cast<int64_t>(p.T_q) + static_cast<int64_t>(rows - 1) * p.B) / rows);
+  set_tile_tokens(pp, rows);
   // Heads that run at the same time share L2: as many as have their K and V in 48 MB of it, whole groups of query heads.
   const int64_t fit = (48ll << 20) / (4ll * p.T_k * p.D + 1);
   pp.head_group = static_cast<int>(fit < 1 ? p.kv_group : fit * p.kv_group < p.N ? fit * p.kv_group : p.N);

@@ -4,22 +4,23 @@
 // each), every block with a list of tiles, whose next one is looked up while one is worked on.  What a tile needs before its first
 // scores and after its last product, a third of its time where a sequence has five tiles of keys, falls under the other block's
 // work; the two tiles per block of fa_fwd.cu are at the same point of theirs at the same time.  24 chunks of up to 1 500 tokens, 16
-// heads of 64: 229 us, 266 there, and 253 with a block for each tile.  8 prompts of up to 4 096 tokens, 32 heads of 128 on 8: 550
-// us, 558 there.  Long sequences go there (the rule is at acct_infer_packed): two tiles share each load of K and V, and one
-// tensor pipe that knows both loses less than two blocks that do not know of one another.
+// heads of 64: 218 us, 266 there.  8 prompts of up to 4 096 tokens, 32 heads of 128 on 8: 544 us, 558 there.  (A block for each
+// tile instead of lists: 253 and 580; one block with both tiles as independent streams: 262 and 588.)  Long sequences go there
+// (the rule is at acct_infer_packed): two tiles share each load of K and V.
 //
 // The rows of a tile are `tile_heads` query heads that read one head of K and V, times 128 / tile_heads tokens (row = token *
 // heads + head: a box of the tensor map as it is).  K and V are then read once per group instead of once per head, and a tile's
 // causal edge is 128 / heads tokens wide, so fewer scores are computed only to be left out.
 //
-// Warps: 0-3 softmax (thread = score row), 4 TMA, 5 MMA, 6 looks up tiles, 7 completes the second warpgroup for the register
-// split.  Per K/V tile: S = Q K^T -> scores in registers, running maximum refreshed only where it grows by more than 2^8, P over S
-// in tensor memory in two halves -> O += P V.  P is rounded to the 16 bits that the product takes, its sum is of the values before
-// that, in 32 bits.  K and V have one buffer each: K of the next tile arrives under this tile's softmax and P V, V under the next
-// scores.
+// Warps: 0-3 softmax (thread = score row), 4 loads, 5 MMA, 6 looks up tiles, 7 stores.  Per K/V tile: S = Q K^T -> scores in
+// registers, running maximum refreshed only where it grows by more than 2^8, P to tensor memory in two halves -> O += P V.  P is
+// rounded to the 16 bits that the product takes, its sum is of the values before that, in 32 bits.  At head_dim up to 64 the next
+// scores are formed under this tile's softmax (chunks 220 -> 210 us in a row of calls); above, there is no room for them.
 //
-// What bounds it: 128 x 128 exponentials take the SM 1 024 clk, and are 2 / 3 of what a tile's softmax issues; two blocks make it
-// 1 830 clk per tile and SM at 8 192 keys and head_dim 64.
+// What bounds it: 128 x 128 exponentials take the SM 1 024 clk, and with maxima, sums and 16-bit packing a tile takes it 1 780 clk at
+// 8 192 keys of 64 and 1 960 of 128; at 1 024 keys 2 380 and 2 960, as half of every diagonal tile is masked and the tile lists end
+// unevenly.  4 prompts of up to 200 tokens, 12.3 us, are latency: 1 200 clk until the block is set up, 2 500 to the first tile's
+// number, 2 000 to its scores, 2 000 to 3 500 per K/V tile, 1 500 to 2 500 for the way out.
 #include "fa_common.cuh"
 #include "fa_kernels.cuh"
 #include "fa_packed.cuh"
@@ -41,37 +42,45 @@ struct Work {
 };
 
 struct Shared {
-  uint64_t q_full, k_full, k_empty, v_full, v_empty;
-  uint64_t s_full, p_half, p_ready, o_done, o_free;
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full, s_free, p_half, p_ready, o_done, o_free, o_staged;
   uint64_t work_full[2], work_empty[2];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
-  Work work[2], softmax_work;
+  Work work[2], softmax_work[2];
 };
 
 template <int DPAD, bool BF16>
 __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid_constant__ FwdParams p) {
   constexpr int NB = DPAD / 64;                 // 64-column (128-byte) blocks per row
   constexpr uint32_t kTileBytes = NB * 16384u;  // one 128-row tile
-  constexpr uint32_t kColO = 128;
+  // At head_dim up to 64 there is room for P beside the scores, and for a second K and V: the next scores are formed under this
+  // tile's softmax.  Above, P lies over the scores and they follow P V.
+  constexpr bool kAhead = DPAD == 64;
+  constexpr int kSt = kAhead ? 2 : 1;           // K and V buffers
+  constexpr uint32_t kColP = kAhead ? 128 : 0, kColO = kAhead ? 192 : 128;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sK = sQ + kTileBytes;
-  uint8_t* sV = sK + kTileBytes;                // and the way out for O, between the last P V of an item and the next item's V
+  uint8_t* sK = sQ + kTileBytes;                // tile n is in buffer n % kSt
+  uint8_t* sV = sK + kSt * kTileBytes;          // the last one of an item is also the way out for O, between its P V and the next V
   __shared__ Shared sh;
 
   const int tid = threadIdx.x;
   const int warp = static_cast<int>(warp_uniform(tid >> 5));
   const bool causal = p.mods.causal != 0;
 
+  PackedFinder finder(p);
+  if (warp == 6) finder.load();
   if (tid == 32) {
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.k_full, 1); mbar_init(&sh.k_empty, 1);
-    mbar_init(&sh.v_full, 1); mbar_init(&sh.v_empty, 1);
-    mbar_init(&sh.s_full, 1); mbar_init(&sh.p_half, 128); mbar_init(&sh.p_ready, 128);
-    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128);
-    for (int i = 0; i < 2; ++i) { mbar_init(&sh.work_full[i], 1); mbar_init(&sh.work_empty[i], 3); }
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(&sh.k_full[i], 1); mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 1); mbar_init(&sh.v_empty[i], 1);
+    }
+    mbar_init(&sh.s_full, 1); mbar_init(&sh.s_free, 128); mbar_init(&sh.p_half, 128); mbar_init(&sh.p_ready, 128);
+    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128); mbar_init(&sh.o_staged, 128);
+    for (int i = 0; i < 2; ++i) { mbar_init(&sh.work_full[i], 1); mbar_init(&sh.work_empty[i], 4); }
     sh.abort_flag = 0;
     mbar_fence_init();
   }
@@ -102,18 +111,22 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
       const Work w = next_work(i);
       if (w.tokens == 0) break;
       if (elect_one()) {
+        if (w.tiles > 0) {      // the scores before were the last to read Q
+          if (n > 0) mbar_wait(&sh.k_empty[(n - 1) % kSt], ((n - 1) / kSt) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+          mbar_expect_tx(&sh.q_full, NB * static_cast<uint32_t>(p.tile_heads * p.tile_tokens) * 128u);
+          for (int nb = 0; nb < NB; ++nb) tma_load_4d(sQ + nb * 16384, &p.map_q, &sh.q_full, nb * 64, w.head0, w.q_row, 0);
+        }
         for (int it = 0; it < w.tiles; ++it) {
-          const uint32_t before = (n + it - 1) & 1;
-          if (n + it > 0) mbar_wait(&sh.k_empty, before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-          if (it == 0) {      // (the scores before, which k_empty stands for, were the last to read Q)
-            mbar_expect_tx(&sh.q_full, NB * static_cast<uint32_t>(p.tile_heads * p.tile_tokens) * 128u);
-            for (int nb = 0; nb < NB; ++nb) tma_load_4d(sQ + nb * 16384, &p.map_q, &sh.q_full, nb * 64, w.head0, w.q_row, 0);
-          }
-          mbar_expect_tx(&sh.k_full, kTileBytes);
-          for (int nb = 0; nb < NB; ++nb) tma_load_4d(sK + nb * 16384, &p.map_k, &sh.k_full, nb * 64, w.k_row + it * kTile, w.h_kv, 0);
-          if (n + it > 0) mbar_wait(&sh.v_empty, before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-          mbar_expect_tx(&sh.v_full, kTileBytes);
-          for (int nb = 0; nb < NB; ++nb) tma_load_4d(sV + nb * 16384, &p.map_v, &sh.v_full, nb * 64, w.k_row + it * kTile, w.h_kv, 0);
+          const uint32_t s = (n + it) % kSt, before = ((n + it) / kSt - 1) & 1;
+          const bool used = n + it >= kSt;
+          if (used) mbar_wait(&sh.k_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+          mbar_expect_tx(&sh.k_full[s], kTileBytes);
+          for (int nb = 0; nb < NB; ++nb)
+            tma_load_4d(sK + s * kTileBytes + nb * 16384, &p.map_k, &sh.k_full[s], nb * 64, w.k_row + it * kTile, w.h_kv, 0);
+          if (used) mbar_wait(&sh.v_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+          mbar_expect_tx(&sh.v_full[s], kTileBytes);
+          for (int nb = 0; nb < NB; ++nb)
+            tma_load_4d(sV + s * kTileBytes + nb * 16384, &p.map_v, &sh.v_full[s], nb * 64, w.k_row + it * kTile, w.h_kv, 0);
         }
       }
       __syncwarp();
@@ -137,52 +150,65 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
       } while (w.tokens != 0 && w.tiles == 0);
       return w.tokens == 0 ? 0 : w.tiles;
     };
-    auto issue_s = [&]() {
+    // scores of tile m, the first of its item or not: what they wait for, and the products
+    auto wait_s = [&](uint32_t m, bool first) {
+      if (first) mbar_wait(&sh.q_full, (items + (m > 0)) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      mbar_wait(&sh.k_full[m % kSt], (m / kSt) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      if (kAhead && m > 0) {
+        mbar_wait(&sh.s_free, (m - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        tc_fence_after_sync();
+      }
+    };
+    auto issue_s = [&](uint32_t m) {
+      const uint32_t s = m % kSt;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DPAD / 16; ++kk) {
           const uint32_t off = (kk >> 2) * 1024u + (kk & 3) * 2u;   // 16-byte units
-          umma_ss_lohi(tmem, q_lo + off, k_hi, kt_lo + off, k_hi, idesc_s, kk > 0);
+          umma_ss_lohi(tmem, q_lo + off, k_hi, kt_lo + s * (kTileBytes >> 4) + off, k_hi, idesc_s, kk > 0);
         }
         umma_commit(&sh.s_full);
-        umma_commit(&sh.k_empty);
+        umma_commit(&sh.k_empty[s]);
       }
     };
     int tiles = next_item();
     if (tiles > 0) {
-      mbar_wait(&sh.q_full, 0, abort_flag, p.status, DEV_TIMEOUT_TMA);
-      mbar_wait(&sh.k_full, 0, abort_flag, p.status, DEV_TIMEOUT_TMA);
-      issue_s();
+      wait_s(0, true);
+      issue_s(0);
     }
     while (tiles > 0) {
       int next = 0;
       for (int it = 0; it < tiles; ++it, ++n) {
         const bool last = it + 1 == tiles;
-        mbar_wait(&sh.v_full, n & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+        const uint32_t s = n % kSt, v_lo = vt_lo + s * (kTileBytes >> 4);
+        if (kAhead && !last) {
+          wait_s(n + 1, false);
+          issue_s(n + 1);
+        }
+        mbar_wait(&sh.v_full[s], (n / kSt) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
         mbar_wait(&sh.p_half, n & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         if (it == 0 && items > 0) mbar_wait(&sh.o_free, (items - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);      // O of the item before
         tc_fence_after_sync();
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kTile / 32; ++kk) umma_ts_lohi(t_o, tmem + kk * 8, vt_lo + kk * 128u, mn_hi, idesc_o, it > 0 || kk > 0);
+          for (int kk = 0; kk < kTile / 32; ++kk) umma_ts_lohi(t_o, tmem + kColP + kk * 8, v_lo + kk * 128u, mn_hi, idesc_o, it > 0 || kk > 0);
         }
-        if (!last) mbar_wait(&sh.k_full, (n + 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+        if (!kAhead && !last) wait_s(n + 1, false);
         mbar_wait(&sh.p_ready, n & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         tc_fence_after_sync();
         if (elect_one()) {
 #pragma unroll
-          for (int kk = kTile / 32; kk < kTile / 16; ++kk) umma_ts_lohi(t_o, tmem + kk * 8, vt_lo + kk * 128u, mn_hi, idesc_o, true);
+          for (int kk = kTile / 32; kk < kTile / 16; ++kk) umma_ts_lohi(t_o, tmem + kColP + kk * 8, v_lo + kk * 128u, mn_hi, idesc_o, true);
           // (of the last tile V is free when O has left through its buffer, which the softmax warps say)
-          umma_commit(last ? &sh.o_done : &sh.v_empty);
+          if (kAhead || last) umma_commit(&sh.o_done);
+          if (!last) umma_commit(&sh.v_empty[s]);
         }
         if (last) {      // (not before this item's last product: with items without tiles between, the next one may wait for its end)
           next = next_item();
-          if (next > 0) {
-            mbar_wait(&sh.q_full, (items + 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-            mbar_wait(&sh.k_full, (n + 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-          }
+          if (next > 0) wait_s(n + 1, true);
         }
-        if (!last || next > 0) issue_s();      // (the tensor pipe runs in order: P is consumed before scores are written over it)
+        // the tensor pipe runs in order: where P lies over the scores it is consumed before they are written over it
+        if (last ? next > 0 : !kAhead) issue_s(n + 1);
       }
       tiles = next;
       ++items;
@@ -190,7 +216,6 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
   } else if (warp == 6) {
     // ------------------------------------------------------------------ scheduler: an item ahead of the others
     reg_dealloc<kRegsControl>();
-    const PackedFinder finder(p, p.tile_tokens);
     const int n_groups = p.N / p.tile_heads, per = p.tile_bound * p.head_group;
     const int64_t total = static_cast<int64_t>(p.tile_bound) * n_groups;
     uint32_t n = 0;
@@ -232,13 +257,31 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
       ++n;
     }
   } else if (warp == 7) {
+    // ------------------------------------------------------------------ stores of whole tiles
     reg_dealloc<kRegsControl>();
+    uint32_t n = 0, whole = 0;      // K/V tiles, and whole tiles of O, so far
+    for (uint32_t i = 0;; ++i) {
+      const Work w = next_work(i);
+      if (w.tokens == 0) break;
+      n += w.tiles;
+      if (w.tiles == 0 || w.tokens < p.tile_tokens) continue;
+      mbar_wait(&sh.o_staged, whole++ & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+      if (elect_one()) {
+        const uint32_t s = (n - 1) % kSt;
+        for (int nb = 0; nb < NB; ++nb)
+          if (nb * 64 < p.D) tma_store_4d(&p.map_o, sV + s * kTileBytes + nb * 16384, nb * 64, w.head0, w.q_row, 0);
+        tma_store_commit();
+        tma_store_wait_read();
+        mbar_arrive(&sh.v_empty[s]);
+      }
+      __syncwarp();
+    }
   } else {
     // ------------------------------------------------------------------ softmax
     reg_alloc<kRegsSoftmax>();
     const int token = tid / p.tile_heads, head = tid - token * p.tile_heads;      // of this thread's row
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t t_s = tmem + lanes, t_o = tmem + lanes + kColO;
+    const uint32_t t_s = tmem + lanes, t_p = t_s + kColP, t_o = t_s + kColO;
     const float mult = p.scale_log2;
     const uint64_t mult2 = f2_pack(mult, mult);
     uint32_t n = 0, items = 0;      // tiles, and items that had any, so far
@@ -247,13 +290,12 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
       // one warp takes the item for all four, so that they agree on it whatever happens
       if (warp == 0) {
         const Work mine = next_work(i);
-        if (elect_one()) sh.softmax_work = mine;
+        if (elect_one()) sh.softmax_work[i & 1] = mine;
       }
       named_barrier(1, 128);
-      const int tokens = sh.softmax_work.tokens, tiles = sh.softmax_work.tiles, kv_len = sh.softmax_work.kv_len;
-      const int sees = sh.softmax_work.sees, q_row = sh.softmax_work.q_row, head0 = sh.softmax_work.head0;
-      named_barrier(1, 128);
-      if (tokens == 0) break;
+      const Work& w = sh.softmax_work[i & 1];
+      const int tiles = w.tiles, kv_len = w.kv_len, sees = w.sees;
+      if (w.tokens == 0) break;
       // keys at or past `bound` do not exist for this row; `bound_tile` is the smallest bound of any row
       const int bound = causal ? min(kv_len, sees + token) : kv_len, bound_tile = min(kv_len, sees);
 
@@ -267,17 +309,9 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, s[c]);
         tmem_wait_ld();
-        if (col_base + kTile > kv_len) {
-          // Rows of V that are not this sequence's: 0 times what they hold might be a NaN.  (The P V before has been issued before
-          // these scores, and this tile's waits for this group: the barrier can be in no other phase.)
-          mbar_wait(&sh.v_full, n & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-          if (col_base + tid >= kv_len)
-            for (int nb = 0; nb < NB; ++nb) {
-              uint4* row = reinterpret_cast<uint4*>(sV + nb * 16384 + tid * 128);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) row[j] = make_uint4(0u, 0u, 0u, 0u);
-            }
-          fence_proxy_async_smem();
+        if constexpr (kAhead) {
+          tc_fence_before_sync();
+          mbar_arrive(&sh.s_free);
         }
         if (col_base + kTile > bound_tile) {      // positions that do not exist: a bit of a word decides, no compare per element
 #pragma unroll
@@ -324,7 +358,13 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
           m_run = m_new;
           l_run *= alpha;
         }
-        if (it > 0 && any_grow) {      // O of the tiles before is complete: these scores were issued after their P V
+        if constexpr (kAhead) {      // the tile before has left O, and its P is not needed any more
+          if (it > 0) {
+            mbar_wait(&sh.o_done, (n - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+            tc_fence_after_sync();
+          }
+        }
+        if (it > 0 && any_grow) {      // (otherwise O is complete because these scores were issued after the P V before)
 #pragma unroll 1
           for (int c = 0; c < DPAD / 32; ++c) {
             uint32_t r[32];
@@ -342,12 +382,25 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
           for (int j = 0; j < 4; ++j) l_part[j] = 0ull;
           exp_chunk(0, negm2, l_part, pk0);
         }
-        // 16-bit P goes back over the scores; the first half is handed on as soon as it is stored
-        tmem_st16(t_s, pk0);
+        // 16-bit P goes back; the first half is handed on as soon as it is stored
+        tmem_st16(t_p, pk0);
         {
           uint32_t pk[16];
           exp_chunk(1, negm2, l_part, pk);
-          tmem_st16(t_s + 16, pk);
+          tmem_st16(t_p + 16, pk);
+          if (col_base + kTile > kv_len) {
+            // Rows of V that are not this sequence's: 0 times what they hold might be a NaN.  (The last use of the buffer is over, as
+            // the P V there has been waited for, here or before these scores were issued, and this tile's P V waits for this group: the
+            // barrier can be in no other phase.)
+            mbar_wait(&sh.v_full[n % kSt], (n / kSt) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+            if (col_base + tid >= kv_len)
+              for (int nb = 0; nb < NB; ++nb) {
+                uint4* row = reinterpret_cast<uint4*>(sV + (n % kSt) * kTileBytes + nb * 16384 + tid * 128);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) row[j] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            fence_proxy_async_smem();
+          }
           tmem_wait_st();
           tc_fence_before_sync();
           mbar_arrive(&sh.p_half);
@@ -358,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
           exp_chunk(3, negm2, l_part, pk3);
 #pragma unroll
           for (int j = 0; j < 16; ++j) { pk[j] = pk2[j]; pk[16 + j] = pk3[j]; }
-          tmem_st32(t_s + 32, pk);
+          tmem_st32(t_p + 32, pk);
         }
         float a0, a1;
         f2_unpack(f2_add(f2_add(l_part[0], l_part[1]), f2_add(l_part[2], l_part[3])), a0, a1);
@@ -368,28 +421,32 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
         mbar_arrive(&sh.p_ready);
       }
 
-      // O / l leaves through the V buffer: by a TMA store, or row by row where the tile is cut (the rows behind it are the next
-      // sequence's); L = m + ln l straight to global memory
-      const bool none = tiles == 0 || l_run == 0.f;      // a row that sees nothing: 0, also where V is not finite
-      if (p.lse != nullptr && token < tokens)
+      // L = m + ln l straight to global memory, and O / l: of a whole tile through the V buffer and a TMA store, else by every thread
+      // its row (the rows behind are the next sequence's)
+      const int tokens = w.tokens, q_row = w.q_row, head0 = w.head0;
+      const bool none = tiles == 0 || l_run == 0.f, there = token < tokens;      // a row that sees nothing: 0, also where V is not finite
+      if (p.lse != nullptr && there)
         p.lse[static_cast<int64_t>(head0 + head) * p.T_q + q_row + token] = none ? kNegInf : m_run * kLn2 + logf(l_run);
-      const int per_row = p.D / 8;
-      uint16_t* out = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(q_row) * p.o_stride_s + static_cast<int64_t>(head0) * p.o_stride_h;
-      if (tiles == 0) {      // (no key at all: nothing has been loaded, and the buffer may be on its way to the next item)
-        for (int j = tid; j < tokens * p.tile_heads * per_row; j += 128) {
-          const int row = j / per_row, tok = row / p.tile_heads;
-          *reinterpret_cast<uint4*>(out + tok * p.o_stride_s + static_cast<int64_t>(row - tok * p.tile_heads) * p.o_stride_h + (j - row * per_row) * 8) =
-              make_uint4(0u, 0u, 0u, 0u);
-        }
+      auto row_of_o = [&]() {
+        int row = q_row + token, col = head0 + head;
+        asm volatile("" : "+r"(row), "+r"(col));      // (nothing of the address is kept in registers over the tiles)
+        return static_cast<uint16_t*>(p.o) + row * p.o_stride_s + col * p.o_stride_h;
+      };
+      if (tiles == 0) {      // no key at all: nothing has been loaded or multiplied
+        uint16_t* out = row_of_o();
+        for (int d = 0; there && d < p.D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0u, 0u, 0u, 0u);
         continue;
       }
-      mbar_wait(&sh.o_done, items & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      mbar_wait(&sh.o_done, (kAhead ? n - 1 : items) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
       tc_fence_after_sync();
       ++items;
+      const bool whole = tokens == p.tile_tokens;
+      uint8_t* exit = sV + (n - 1) % kSt * kTileBytes;
+      if (!whole && tid == 0) mbar_arrive(&sh.v_empty[(n - 1) % kSt]);
       const float inv_l = l_run > 0.f ? 1.0f / l_run : 0.f;
       const int n_chunks = (p.D + 31) / 32;
-#pragma unroll 1
-      for (int c = 0; c < n_chunks; ++c) {
+      // 32 columns of this thread's row, as 16-bit numbers
+      auto row_chunk = [&](int c, uint4 (&u)[4]) {
         uint32_t r[32];
         tmem_ld32(t_o + c * 32, r);
         tmem_wait_ld();
@@ -404,30 +461,29 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
         uint32_t pk[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) pk[j] = pack2<BF16>(__uint_as_float(r[2 * j]) * inv_l, __uint_as_float(r[2 * j + 1]) * inv_l);
-        uint8_t* blk = sV + (c >> 1) * 16384u;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint4*>(blk + swz128(tid, (c & 1) * 4 + g)) = make_uint4(pk[4 * g], pk[4 * g + 1], pk[4 * g + 2], pk[4 * g + 3]);
-      }
-      fence_proxy_async_smem();
-      named_barrier(1, 128);
-      if (tokens == p.tile_tokens) {
-        if (tid == 0) {
-          for (int nb = 0; nb < NB; ++nb)
-            if (nb * 64 < p.D) tma_store_4d(&p.map_o, sV + nb * 16384, nb * 64, head0, q_row, 0);
-          tma_store_commit();
-          tma_store_wait_read();
-          mbar_arrive(&sh.v_empty);
-        }
-      } else {
-        for (int j = tid; j < tokens * p.tile_heads * per_row; j += 128) {
-          const int row = j / per_row, chunk = j - row * per_row, tok = row / p.tile_heads;
-          *reinterpret_cast<uint4*>(out + tok * p.o_stride_s + static_cast<int64_t>(row - tok * p.tile_heads) * p.o_stride_h + chunk * 8) =
-              *reinterpret_cast<const uint4*>(sV + (chunk >> 3) * 16384 + swz128(row, chunk & 7));
+        for (int g = 0; g < 4; ++g) u[g] = make_uint4(pk[4 * g], pk[4 * g + 1], pk[4 * g + 2], pk[4 * g + 3]);
+      };
+      if (whole) {
+#pragma unroll 1
+        for (int c = 0; c < n_chunks; ++c) {
+          uint4 u[4];
+          row_chunk(c, u);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4*>(exit + (c >> 1) * 16384u + swz128(tid, (c & 1) * 4 + g)) = u[g];
         }
         fence_proxy_async_smem();
-        named_barrier(1, 128);
-        if (tid == 0) mbar_arrive(&sh.v_empty);
+        mbar_arrive(&sh.o_staged);
+      } else {
+        uint16_t* out = row_of_o();
+#pragma unroll 1
+        for (int c = 0; c < n_chunks; ++c) {
+          uint4 u[4];
+          row_chunk(c, u);
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (there && c * 32 + g * 8 < p.D) *reinterpret_cast<uint4*>(out + c * 32 + g * 8) = u[g];
+        }
       }
     }
     tc_fence_before_sync();
@@ -445,9 +501,9 @@ __global__ void __launch_bounds__(kThreads, 2) fa_fwd_packed_kernel(const __grid
 
 cudaError_t launch_fa_fwd_packed(const FwdParams& p, bool bf16, int sm_count, cudaStream_t stream) {
   const int dpad = p.D <= 64 ? 64 : 128;
-  const size_t smem = static_cast<size_t>(3) * (dpad / 64) * 16384 + 1024;
+  const size_t smem = static_cast<size_t>(dpad == 64 ? 5 : 6) * 16384 + 1024;      // Q and two K and V of 64 columns, or one of 128
   FwdParams pp = p;
-  pp.tile_bound = static_cast<int>((static_cast<int64_t>(p.T_q) + static_cast<int64_t>(p.tile_tokens - 1) * p.B) / p.tile_tokens);
+  set_tile_tokens(pp, p.tile_tokens);
   // Heads that run at the same time share L2: as many as have their K and V in 48 MB of it.
   const int64_t fit = (48ll << 20) / (4ll * p.T_k * p.D + 1), per_kv = p.kv_group / p.tile_heads, groups = p.N / p.tile_heads;
   pp.head_group = static_cast<int>(fit < 1 ? per_kv : fit * per_kv < groups ? fit * per_kv : groups);

@@ -90,7 +90,9 @@ struct alignas(64) FwdParams {
   // packed sequences (launch_fa_fwd_packed, launch_fa_fwd_packed_long): q, o are [T_q, N, D], k, v [T_k, N_kv, D], lse [N, T_q]
   const int *cu_q, *cu_k;           // [B + 1]: sequence b has rows cu[b] .. cu[b + 1] - 1
   int T_q, T_k;
-  int tile_heads, tile_tokens;      // a tile is so many query heads (a divisor of kv_group) of so many tokens, 128 rows at most
+  int tile_heads, tile_tokens;      // a tile is so many query heads (a divisor of kv_group) of so many tokens: up to 128 rows, or 256
+  unsigned int tile_magic;          // n / tile_tokens = n * tile_magic >> tile_shift, see set_tile_tokens
+  int tile_shift;
   int tile_bound;                   // tiles that T_q rows of B sequences can make
   int head_group;                   // heads, or groups of tile_heads, whose thread blocks are interleaved
 };

@@ -90,10 +90,11 @@ def test_prefixes_and_queries_that_see_nothing(D, N, N_kv, dtype):
         _check(q, k, v, lens_q, lens_k, y, lse, causal, 0.3)
 
 
-# on average: just long enough for two tiles per block, keys just too few, queries just too few, one long prefix among short ones
+# on average: just long enough for two tiles per block (4 096 keys, or 8 192 of 64), keys just too few, queries just too few, ...
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("lens_q, lens_k", [([256], [4096]), ([256], [4095]), ([255], [4096]), ([1, 511], [4096, 4096]), ([700, 0, 69], [5000, 1, 7300]),
-                                            ([513, 300, 1], [9001, 299, 4000]), ([4229], [4229])], ids=str)
+                                            ([513, 300, 1], [9001, 299, 4000]), ([4229], [4229]), ([256], [8192]), ([300, 212], [10000, 6384])],
+                         ids=str)
 @pytest.mark.parametrize("D, N, N_kv", [(128, 4, 1), (64, 3, 3), (72, 2, 1)])
 def test_long_sequences(D, N, N_kv, lens_q, lens_k, dtype):
     from acctransformer_b200 import flash_attention_packed
