@@ -19,8 +19,8 @@
 //
 // What bounds it: 128 x 128 exponentials take the SM 1 024 clk, and with maxima, sums and 16-bit packing a tile takes it 1 780 clk at
 // 8 192 keys of 64 and 1 960 of 128; at 1 024 keys 2 380 and 2 960, as half of every diagonal tile is masked and the tile lists end
-// unevenly.  4 prompts of up to 200 tokens, 12.3 us, are latency: 1 200 clk until the block is set up, 2 500 to the first tile's
-// number, 2 000 to its scores, 2 000 to 3 500 per K/V tile, 1 500 to 2 500 for the way out.
+// unevenly.  4 prompts of up to 200 tokens, 12.3 us, are latency: 1 000 to 1 500 clk until the block is set up, 2 000 to 2 900 to the
+// first tile's number, 2 100 to its scores, 2 000 to 3 500 per K/V tile, 500 to 2 000 for the last P V and 1 100 for the way out.
 #include "fa_common.cuh"
 #include "fa_kernels.cuh"
 #include "fa_packed.cuh"
