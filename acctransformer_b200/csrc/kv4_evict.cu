@@ -7,8 +7,8 @@
 // cache) takes codes as they are: nothing is decoded and rounded again.
 //
 // 32 sequences of up to 8 192 slots, 8 heads of 128, half of them stay: 195 us with the read that follows, 145 at the rate of a copy.  The
-// copy is bound by its reads: rows that stay are 16 bytes here and there, and of a 32-byte sector the neighbour is read with
-// them (16 x 8 heads of 8 192 slots: 135 MB for 84 that stay, at 55 % of the DRAM rate).  Selection there is latency, 17 us.
+// copy is bound by its reads: two rows of V share their words, and four rows of K a sector of steps, so neighbours that go are read
+// with those that stay (16 x 8 heads of 8 192 slots: 135 MB for 84 that stay, at 55 % of the DRAM rate).  Selection there is latency, 17 us.
 #include "fa_kernels.cuh"
 #include "kv4_common.cuh"
 
