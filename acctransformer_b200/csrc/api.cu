@@ -365,6 +365,25 @@ int bwd_kernel(const acct_fa_args* a) {
   return bwd_on_pairs(a) ? ACCT_BWD_PAIR : ACCT_BWD_ONE_BLOCK;
 }
 
+// Two CTAs share a K/V tile by halves of head_dim (or one holds it whole, with the same 64-row tiles): decided by head_dim alone.
+bool bwd_by_halves(const acct_fa_args* a) { return a->D > 128; }
+
+// The backward's workspace: delta [B*N*S_q] fp32 | turn counters of the ordered dQ reduction, one per Q tile (two where it is shared
+// by halves), and the work counter of the persistent thread blocks, u32 | dQ accumulator [B*N*S_q, D] fp32; the first two padded
+// to 256 bytes.  With fp32 gradients dq itself is the accumulator.
+struct BwdWorkspace {
+  size_t counters, order, acc, bytes;      // number of counters; byte offsets of the counters and the accumulator; the whole
+};
+BwdWorkspace bwd_workspace(const acct_fa_args* a) {
+  BwdWorkspace w;
+  const size_t units = static_cast<size_t>(a->B) * a->N, rows = units * a->S_q;
+  w.counters = units * ((a->S_q + kTile - 1) / kTile) * (bwd_by_halves(a) ? 2 : 1) + 1;
+  w.order = (rows * 4 + 255) / 256 * 256;
+  w.acc = w.order + (w.counters * 4 + 255) / 256 * 256;
+  w.bytes = w.acc + ((a->flags & ACCT_FLAG_GRAD_F32) ? 0 : rows * static_cast<size_t>(a->D) * 4);
+  return w;
+}
+
 ScoreMods make_mods(const acct_fa_args* a, const void* plan = nullptr) {
   ScoreMods m;
   memset(&m.plan, 0, sizeof(m.plan));
@@ -577,14 +596,7 @@ int acct_fa_fwd_planned(const acct_fa_args* a, const void* plan, void* stream) {
 
 size_t acct_fa_bwd_workspace_bytes(const acct_fa_args* a) {
   if (a == nullptr || a->B <= 0 || a->N <= 0 || a->S_q <= 0 || a->D <= 0) return 0;
-  const size_t rows = static_cast<size_t>(a->B) * a->N * a->S_q;
-  // (two counters per Q tile above head_dim 128, where two CTAs share a K/V tile by halves of head_dim)
-  const size_t q_tiles = static_cast<size_t>(a->B) * a->N * ((a->S_q + kTile - 1) / kTile) * (a->D > 128 ? 2 : 1) + 1;
-  // (+ 1: the work counter of the persistent thread blocks)
-  // delta [rows] fp32 | turn counters of the ordered dQ reduction [B*N*ceil(S_q/128)] u32 | dQ accumulator
-  // [rows, D] fp32; the first two padded to 256 bytes.  With fp32 gradients dq itself is the accumulator.
-  const size_t acc = (a->flags & ACCT_FLAG_GRAD_F32) ? 0 : rows * static_cast<size_t>(a->D) * 4;
-  return ((rows * 4 + 255) / 256) * 256 + ((q_tiles * 4 + 255) / 256) * 256 + acc;
+  return bwd_workspace(a).bytes;
 }
 
 int acct_fa_bwd_kernel(const acct_fa_args* a) { return a != nullptr ? bwd_kernel(a) : -1; }
@@ -612,9 +624,9 @@ int acct_fa_bwd_planned(const acct_fa_args* a, const acct_fa_bwd_io* g, const in
   if (!g->d_o || !g->dq || !g->dk || !g->dv || !a->lse) return fail(ACCT_ERR_NULL, "d_o, dq, dk, dv and lse must be non-NULL");
   if (!aligned16(g->d_o) || !aligned16(g->dq) || !aligned16(g->dk) || !aligned16(g->dv))
     return fail(ACCT_ERR_ALIGN, "d_o, dq, dk, dv must be 16-byte aligned");
-  const size_t need = acct_fa_bwd_workspace_bytes(a);
-  if (g->workspace == nullptr || g->workspace_bytes < need)
-    return fail(ACCT_ERR_WORKSPACE, "backward workspace: need %zu bytes, got %zu", need, g->workspace ? g->workspace_bytes : (size_t)0);
+  const BwdWorkspace ws = bwd_workspace(a);
+  if (g->workspace == nullptr || g->workspace_bytes < ws.bytes)
+    return fail(ACCT_ERR_WORKSPACE, "backward workspace: need %zu bytes, got %zu", ws.bytes, g->workspace ? g->workspace_bytes : (size_t)0);
   if ((reinterpret_cast<uintptr_t>(g->workspace) & 255u) != 0) return fail(ACCT_ERR_ALIGN, "workspace must be 256-byte aligned");
   PerDevice* dev = nullptr;
   if ((rc = init_device(&dev))) return rc;
@@ -624,14 +636,12 @@ int acct_fa_bwd_planned(const acct_fa_args* a, const acct_fa_bwd_io* g, const in
   float* delta = static_cast<float*>(g->workspace);
   const int kernel = bwd_kernel(a);
   const bool mid = kernel == ACCT_BWD_MID, pair = kernel == ACCT_BWD_PAIR;
-  const bool wide = a->D > 128 || (getenv("PKL") && atoi(getenv("PKL")));      // the split-width kernel: 64-row Q / dO boxes, 64-row dQ box, 2 counters per tile
-  const size_t q_tiles = static_cast<size_t>(a->B) * a->N * ((a->S_q + kTile - 1) / kTile) * (wide ? 2 : 1) + 1;   // + work counter
-  const size_t order_bytes = ((q_tiles * 4 + 255) / 256) * 256;
-  unsigned int* dq_order = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(g->workspace) + ((rows * 4 + 255) / 256) * 256);
+  const bool wide = bwd_by_halves(a);      // the split-width kernel: 64-row Q / dO boxes, 64-row dQ box
+  unsigned int* dq_order = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(g->workspace) + ws.order);
   // fp32 gradients: the kernel's reduce-add lands in the caller's dq directly, no copy afterwards
   const bool dq_in_place = (a->flags & ACCT_FLAG_GRAD_F32) != 0;
   float* dq_acc = dq_in_place ? static_cast<float*>(g->dq)
-                              : reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(dq_order) + order_bytes);
+                              : reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + ws.acc);
 
   BwdParams p;
   memset(&p, 0, sizeof(p));
@@ -668,12 +678,12 @@ int acct_fa_bwd_planned(const acct_fa_args* a, const acct_fa_bwd_io* g, const in
   }
   // one helper pass before the main kernel: row sums, and the zero-fill of the accumulator and the turn counters
   cudaError_t e = launch_bwd_delta(a->o, g->d_o, delta, static_cast<int64_t>(rows), a->D, st.o, st_do, a->N, a->S_q, bf16,
-                                   s, dq_acc, dq_order, static_cast<int64_t>(q_tiles), const_cast<unsigned int*>(p.plan_stats));
+                                   s, dq_acc, dq_order, static_cast<int64_t>(ws.counters), const_cast<unsigned int*>(p.plan_stats));
   if (e != cudaSuccess) return fail_cuda(e, "launching the row-sum kernel");
   p.lse = a->lse; p.delta = delta; p.dq_acc = dq_acc;
   p.dq_order = (a->flags & ACCT_FLAG_DETERMINISTIC) ? dq_order : nullptr;
   p.dk = g->dk; p.dv = g->dv;
-  p.work_counter = dq_order + (q_tiles - 1);
+  p.work_counter = dq_order + (ws.counters - 1);
   p.grads_f32 = (a->flags & ACCT_FLAG_GRAD_F32) ? 1 : 0;
   p.B = a->B; p.N = a->N; p.S_q = a->S_q; p.S_k = a->S_k; p.D = a->D;
   p.kv_group = a->N / kv_heads(a);
