@@ -8,7 +8,9 @@
 //                 at a time, and s and m meet 16 x 8 sums instead of 16 x 128 values.  In fp16 a code in the low bits of a half is
 //                 the subnormal number c * 2^-24, exact to multiply (and c * 2^-20 four bits up: those columns of Q are divided by
 //                 16), so a mask is all it takes; in bf16 it goes into the low bits of 128 and 128 is subtracted.  m times the sum
-//                 of Q is one more product, whose operand holds the sums in three parts so that nothing of them is lost.
+//                 of Q is one more product, whose operand holds the sums in three parts so that nothing of them is lost.  In fp16
+//                 a head of Q whose largest value is below 2^10 is multiplied by a power of two that brings it there, and its
+//                 scores are divided by it: a sixteenth of Q, and the parts of its sums, then lose 2^-34 of that value at most.
 //   O^T += V^T P  here the steps belong to the contraction: v = s c + m is formed in 16 bits (one rounding, as if the cache were
 //                 in 16 bits), two rows of a column at a time, with the code subtracted out of 1024 + c, 64 + c or 128 + c.
 //                 P is rounded to 16 bits too, which would cost as much again (in fp16, over 2 048 keys, 3.4e-4 of the result from
@@ -286,30 +288,53 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HEADS)) kv4_decode_ker
 
   // ---- the query heads as B fragments (column g = head g), columns of Q in the order of the codes: of a thread's eight 32 grp +
   // 8 t + .. of a group the pairs (0, 4), (1, 5), (2, 6), (3, 7); in fp16 the second and fourth pair divided by 16
+  // f_head: what takes the products of heads 2 t and 2 t + 1 to scores in log2 units
   uint32_t qb[HI][2 * NG][2], qm[HI][2];
+  float f_head[HI][2];
 #pragma unroll
   for (int hi = 0; hi < HI; ++hi) {
     const int head = kSpare ? g & 3 : g + 8 * hi;
-    float mean_t = 0.f;
+    uint4 u[NG];
 #pragma unroll
     for (int grp = 0; grp < NG; ++grp) {
       const int d = 32 * grp + 8 * t;
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      u[grp] = make_uint4(0u, 0u, 0u, 0u);
       if (head < G && d < p.D)
-        u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(b) * p.N + h_kv * G + head) * p.D + d);
-      const uint32_t pairs[4] = {__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410), __byte_perm(u.y, u.w, 0x7632)};
+        u[grp] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(b) * p.N + h_kv * G + head) * p.D + d);
+    }
+    float lift = 1.0f;
+    f_head[hi][0] = f_head[hi][1] = p.scale_log2;
+    if constexpr (!BF16) {      // the largest value of the head to 2^10 or more; an infinity or a NaN is larger than that
+      constexpr uint32_t kAbs = 0x7fff7fffu;
+      uint32_t most = 0u;
+#pragma unroll
+      for (int grp = 0; grp < NG; ++grp)
+        most = __vmaxu2(most, __vmaxu2(__vmaxu2(u[grp].x & kAbs, u[grp].y & kAbs), __vmaxu2(u[grp].z & kAbs, u[grp].w & kAbs)));
+      most = max(most & 0xffffu, most >> 16);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int up = max(0, 25 - max(1, static_cast<int>(most >> 10)));      // (2^10 has 25 in its exponent's bits)
+      lift = __int_as_float((127 + up) << 23);
+      const float back = __int_as_float((127 - up) << 23);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) f_head[hi][e] *= kCodeScaleF16 * __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
+    }
+    float mean_t = 0.f;
+#pragma unroll
+    for (int grp = 0; grp < NG; ++grp) {
+      const uint32_t pairs[4] = {__byte_perm(u[grp].x, u[grp].z, 0x5410), __byte_perm(u[grp].x, u[grp].z, 0x7632),
+                                 __byte_perm(u[grp].y, u[grp].w, 0x5410), __byte_perm(u[grp].y, u[grp].w, 0x7632)};
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = unpack2<BF16>(pairs[j]);
         sum += f.x + f.y;
-        uint32_t w = pairs[j];
-        if (!BF16 && (j & 1) != 0) w = pack2<BF16>(f.x * 0.0625f, f.y * 0.0625f);
-        qb[hi][2 * grp + (j >> 1)][j & 1] = w;
+        const float times = (j & 1) != 0 ? 0.0625f * lift : lift;
+        qb[hi][2 * grp + (j >> 1)][j & 1] = BF16 ? pairs[j] : pack2<BF16>(f.x * times, f.y * times);
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == grp) mean_t = sum * 0.03125f;          // of the group's 32 columns: in the range of Q whatever that is
+      if (t == grp) mean_t = sum * (lift * 0.03125f);          // of the group's 32 columns: in the range of Q whatever that is
     }
     // the mean as a sum of three 16-bit numbers
     const uint32_t w0 = pack2<BF16>(mean_t, 0.f);
@@ -332,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HEADS)) kv4_decode_ker
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[hi][i][e] = 0.f;
   }
-  const float f_code = BF16 ? p.scale_log2 : p.scale_log2 * kCodeScaleF16, f_mean = p.scale_log2 * 32.0f;
+  constexpr float kMean = BF16 ? 32.0f : 32.0f / kCodeScaleF16;      // a mean's product in the units of the codes' products
 
   float* scores = p.scores == nullptr ? nullptr : p.scores + (static_cast<int64_t>(unit_kv) * p.S_pad + g) * p.G_pad + 2 * t;
 
@@ -382,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HEADS)) kv4_decode_ker
         float c[4];
         mma16816_zero<BF16>(c, low[0], low[1], low[0], low[1], qm[hi][0], qm[hi][1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[r][hi][e] = fmaf(x[r][hi][e], f_code, c[e] * f_mean);
+        for (int e = 0; e < 4; ++e) x[r][hi][e] = fmaf(c[e], kMean, x[r][hi][e]) * f_head[hi][e & 1];
       }
     }
     if (partial) {
