@@ -163,6 +163,10 @@ __device__ __forceinline__ int parts_of(const Kv4DecodeParams& p, int steps, int
 }
 
 constexpr float kRefresh = 8.0f;      // log2 units by which a score may exceed the running maximum
+// The running maximum before there is one.  A finite number: a key that does not exist, or whose score is below fp32's range, then
+// counts for exp2(-inf - kLowest) = 0 also where a warp has met no other key yet; and as the lowest of fp32 it is no higher than
+// any score that is in range.
+constexpr float kLowest = -3.402823466e38f;
 
 // Resident thread blocks per SM, which the registers decide (152 and 230 a thread).  With four, at 128 registers, or five, at 96
 // and a record at a time, the step is no faster (32 x 8 slices of up to 16 384 keys 95 and 103 us against 90).
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HEADS)) kv4_decode_ker
   float m_run[HI][2], l_run[HI][2];      // heads 2 t and 2 t + 1; l is this thread's share
 #pragma unroll
   for (int hi = 0; hi < HI; ++hi) {
-    m_run[hi][0] = m_run[hi][1] = -INFINITY;
+    m_run[hi][0] = m_run[hi][1] = kLowest;
     l_run[hi][0] = l_run[hi][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * NG; ++i)
@@ -445,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HEADS)) kv4_decode_ker
         for (int r = 1; r < kStepRecs; ++r) most[hi][e] = fmax3(most[hi][e], x[r][hi][e], x[r][hi][e + 2]);
         exceeds |= most[hi][e] > m_run[hi][e] + kRefresh;
       }
-    if (__any_sync(0xffffffffu, exceeds)) {          // (always at the first step: row0 < len, so it has a key that exists)
+    if (__any_sync(0xffffffffu, exceeds)) {
 #pragma unroll
       for (int hi = 0; hi < HI; ++hi)
 #pragma unroll
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HEADS)) kv4_decode_ker
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           const float m_new = fmaxf(m_run[hi][e], mx);
-          const float alpha = m_run[hi][e] == -INFINITY ? 0.f : ex2(m_run[hi][e] - m_new);
+          const float alpha = ex2(m_run[hi][e] - m_new);
           m_run[hi][e] = m_new;
           l_run[hi][e] *= alpha;
 #pragma unroll

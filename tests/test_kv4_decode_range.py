@@ -61,3 +61,51 @@ def test_queries_of_any_size(size, group, D):
             got = y[b, h * group:(h + 1) * group, 0].double()
             assert ((got - want).abs() <= u * (want + room) + room).all(), float(((got - want).abs() / (u * want)).max())
             assert ((w[b, h, :n].double() - p.sum(0)).abs() <= p.sum(0) * (math.expm1(2 * e) + group * 2.0 ** -22) + 1e-9).all()
+
+
+@pytest.mark.parametrize("page", [None, 32])
+@pytest.mark.parametrize("group", [1, 4, 8, 16])
+@pytest.mark.parametrize("splits", [0, 1, 5])
+def test_scores_below_the_range_of_fp32(splits, group, page):
+    """Keys at the lowest value of bfloat16, whose scores are -inf in fp32: weight 0, however many of them come together (whole
+    warps' shares, whole parts), and everywhere but in one sequence: only the others count.  Of the last sequence no key is left."""
+    from acctransformer_b200 import Kv4Cache
+    dtype, N_kv, S, D = torch.bfloat16, 2, 704, 64
+    lens = [700, 100, 33, 640]
+    B, T = len(lens), sum(lens)
+    table = {} if page is None else {"page_size": page, "block_table": torch.randperm(B * S // page).int().view(B, -1).cuda()}
+    cache = Kv4Cache(B, N_kv, S, D, dtype=dtype, **table)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(T, N_kv, D, device="cuda", generator=g).to(dtype) for _ in range(2))
+    there = [range(300, 411), [99], [0], []]                 # keys with a score in range
+    at = 0
+    for n, some in zip(lens, there):
+        hidden = torch.ones(n, dtype=torch.bool, device="cuda")
+        hidden[list(some)] = False
+        k[at:at + n][hidden] = torch.finfo(dtype).min
+        at += n
+    zero, cu = _ints([0] * B), torch.tensor([0] + lens).cumsum(0).int().cuda()
+    cache.append(k, v, zero, cu)
+    k, v = cache.read(zero, cu, total=T)
+    q = (1.0 + torch.rand(B, N_kv * group, 1, D, device="cuda", generator=g)).to(dtype)
+    w = torch.zeros(B, N_kv, cache.S_max, device="cuda")
+    y = cache.decode(q, _ints(lens), weights=w, num_splits=splits)
+    at = 0
+    for b, (n, some) in enumerate(zip(lens, there)):
+        some = list(some)
+        for h in range(N_kv):
+            got, p_got = y[b, h * group:(h + 1) * group, 0].double(), w[b, h].double()
+            if not some:
+                assert (got == 0).all() and (p_got == 0).all()
+                continue
+            qq, kk, vv = (x.double() for x in (q[b, h * group:(h + 1) * group, 0], k[at:at + n, h][some], v[at:at + n, h][some]))
+            x = qq @ kk.T * D ** -0.5
+            p = torch.softmax(x, -1)
+            # u = 2^-8: V and the result rounded (and P, above 8 heads); K came back rounded, a relative u of every product
+            u, A = 2.0 ** -8, float((qq.abs() @ kk.abs().T).max()) * D ** -0.5
+            change = math.expm1(2 * (2.0 ** -20 * A + 2.0 ** -18 + 2 * u * A))
+            assert ((got - p @ vv).abs() <= (p @ vv.abs()) * (4 * u + change) + 1e-6).all()
+            assert ((p_got[some] - p.sum(0)).abs() <= p.sum(0) * change + 1e-9).all()
+            p_got[some] = 0
+            assert (p_got == 0).all()
+        at += n
