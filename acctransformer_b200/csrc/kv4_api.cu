@@ -38,6 +38,17 @@ int check_cache(const char* name, const acct_kv4_cache* c, Kv4Cache* out) {
   return 0;
 }
 
+// bytes of a cache's records (of its whole pool, where it is paged)
+size_t cache_bytes(const Kv4Cache& c) {
+  const size_t recs = c.table != nullptr ? static_cast<size_t>(c.num_pages) << c.page_shift : static_cast<size_t>(c.B) * c.recs;
+  return recs * c.N_kv * acct_kv4_record_bytes(c.D);
+}
+
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y ? y - x < a_bytes : x - y < b_bytes;
+}
+
 int check_rows(const acct_kv4_cache* c, const acct_kv4_rows* r, Kv4Rows* out) {
   if (r == nullptr) return fail(ACCT_ERR_NULL, "rows is NULL");
   if (r->T < 0) return fail(ACCT_ERR_SHAPE, "T must not be negative");
@@ -183,9 +194,14 @@ int acct_kv4_evict(const acct_kv4_cache* src, const acct_kv4_cache* dst, const a
     return fail(ACCT_ERR_NULL, "weights, weights_out, kept, seq_lens and seq_lens_out must be non-NULL");
   if (a->keep < 1 || a->recent < 0 || a->recent > a->keep) return fail(ACCT_ERR_SHAPE, "need 0 <= recent <= keep and keep >= 1, got recent = %d, keep = %d", a->recent, a->keep);
   if (a->keep > dst->S_max) return fail(ACCT_ERR_SHAPE, "keep = %d does not fit dst with S_max = %d", a->keep, dst->S_max);
-  if (a->weights == a->weights_out || a->seq_lens == a->seq_lens_out) return fail(ACCT_ERR_SHAPE, "eviction does not work in place");
-  if (src->records == dst->records && (src->block_table == nullptr || src->block_table == dst->block_table))
-    return fail(ACCT_ERR_SHAPE, "eviction does not work in place: dst must be another cache than src (or other pages of its pool)");
+  // The copy of one record reads where others are written, so nothing may be in both.  Of two tables over one pool only the caller
+  // knows that they share no page.
+  const size_t lens = static_cast<size_t>(src->B) * sizeof(int32_t), heads = static_cast<size_t>(src->B) * src->N_kv * sizeof(float);
+  if (overlap(a->weights, heads * src->S_max, a->weights_out, heads * dst->S_max)) return fail(ACCT_ERR_SHAPE, "eviction does not work in place: weights and weights_out overlap");
+  if (overlap(a->seq_lens, lens, a->seq_lens_out, lens)) return fail(ACCT_ERR_SHAPE, "eviction does not work in place: seq_lens and seq_lens_out overlap");
+  const bool one_pool = src->block_table != nullptr && dst->block_table != nullptr && src->records == dst->records && src->block_table != dst->block_table;
+  if (!one_pool && overlap(src->records, cache_bytes(p.src), dst->records, cache_bytes(p.dst)))
+    return fail(ACCT_ERR_SHAPE, "eviction does not work in place: dst must be other memory than src, or other pages of its pool");
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
   p.weights = a->weights; p.weights_out = a->weights_out; p.kept = a->kept;

@@ -411,13 +411,14 @@ ACCT_API int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args
 /* Eviction by accumulated weight.  Of every sequence and head min(length, keep) slots stay: the last `recent` ones, and of those
  * before them the ones with the largest weights (equal ones: the lowest slots; a NaN counts as the largest).  They go to slots
  * 0, 1, .. of `dst` in their order, their codes as they are.  `dst` is another cache of the same B, N_kv, D and dtype with at
- * least `keep` slots (one spare cache serves all layers in turn). */
+ * least `keep` slots (one spare cache serves all layers in turn).  What is written may be no part of what is read, which is refused;
+ * two caches may be pages of one pool, and then the caller sees to it that their tables share no page. */
 typedef struct acct_kv4_evict_args {
   const float* weights;     /* device [B, N_kv, src S_max] fp32 */
-  float* weights_out;       /* device [B, N_kv, dst S_max] fp32: those of what stays, 0 behind it */
+  float* weights_out;       /* device [B, N_kv, dst S_max] fp32: those of what stays, 0 behind it; no part of weights */
   int32_t* kept;            /* device [B, N_kv, keep]: the slots that stay, ascending, then -1 */
   const int32_t* seq_lens;  /* device [B] */
-  int32_t* seq_lens_out;    /* device [B]: min(length, keep); may not be seq_lens */
+  int32_t* seq_lens_out;    /* device [B]: min(length, keep); no part of seq_lens */
   int32_t keep, recent;     /* 0 <= recent <= keep, keep >= 1 */
 } acct_kv4_evict_args;
 
