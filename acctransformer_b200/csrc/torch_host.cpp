@@ -91,6 +91,15 @@ Tensor lengths(const Tensor& lens, int64_t B, const Tensor& q) {
   return lens.to(at::kInt).contiguous();
 }
 
+// What a serving operator is given needs no gradient and carries no tangent: either would end there without a word.
+void no_gradient(const char* op, std::initializer_list<const Tensor*> operands) {
+  for (const Tensor* t : operands) {
+    if (!t->defined()) continue;
+    HOST_CHECK(!t->requires_grad() || !at::GradMode::is_enabled(), op, " has no gradient: call it under torch.no_grad() or on detached tensors");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), op, " does not support forward mode AD");
+  }
+}
+
 void strides3(const Tensor& t, int64_t (&out)[3]) {
   HOST_CHECK(t.stride(-1) == 1, "head_dim must be contiguous");
   for (int i = 0; i < 3; ++i) out[i] = t.stride(i);
@@ -611,6 +620,7 @@ PyObject* py_infer_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const double scale = float_arg(args[6]);
   Tensor y = tensor_or_undefined(args[7]), lse;
   const bool want_lse = bool_arg(args[8]);
+  no_gradient("flash_attention_packed", {&q, &k, &v});
   {
     pybind11::gil_scoped_release no_gil;
     at::AutoDispatchBelowADInplaceOrView below;
@@ -667,6 +677,7 @@ PyObject* py_kv4_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HOST_CHECK(n == 5, "kv4_append takes 5 arguments, got ", n);
   Kv4 cache = kv4_arg(args[0]);
   Tensor k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), start = tensor_arg(args[3], "start"), cu = tensor_or_undefined(args[4]);
+  no_gradient("Kv4Cache.append", {&k, &v});
   {
     pybind11::gil_scoped_release no_gil;
     at::AutoDispatchBelowADInplaceOrView below;
@@ -729,6 +740,7 @@ PyObject* py_kv4_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t splits = int_arg(args[5]);
   const Tensor ws = tensor_arg(args[6], "workspace");
   Tensor y = tensor_or_undefined(args[7]);
+  no_gradient("Kv4Cache.decode", {&q, &weights});
   {
     pybind11::gil_scoped_release no_gil;
     at::AutoDispatchBelowADInplaceOrView below;
@@ -778,6 +790,7 @@ PyObject* py_kv4_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Kv4 src = kv4_arg(args[0]), dst = kv4_arg(args[1]);
   Tensor weights = tensor_arg(args[2], "weights"), lens = tensor_arg(args[3], "seq_lens"), kept, weights_out, lens_out;
   const int64_t keep = int_arg(args[4]), recent = int_arg(args[5]);
+  no_gradient("Kv4Cache.evict", {&weights});
   {
     pybind11::gil_scoped_release no_gil;
     at::AutoDispatchBelowADInplaceOrView below;

@@ -63,7 +63,4 @@ def flash_attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=T
     ``causal``: the last query of a sequence sees its last key, the one before it all keys but that, and so on, so that a
     sequence with more keys than queries is a chunk of a prompt behind a prefix.  A query that sees no key gives 0.  scale
     defaults to D^-1/2; ``return_lse`` adds the logarithms of the softmax sums, float32 [N, T_q].  For serving: no gradient."""
-    for t in (q, k, v):
-        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("flash_attention_packed has no gradient: call it under torch.no_grad() or on detached tensors")
     return _ops.infer_packed(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, scale=scale, out=out, return_lse=return_lse)

@@ -2,8 +2,9 @@
 decoding step reads.
 
 Up to 32 neighbouring values of a token's row share a minimum and a step in the cache's 16-bit type; every value is a code of 4
-bits (``include/acct_b200.h`` has the formulas).  The cache is storage: how many slots of a sequence are in use is the caller's to
-know, one ``seq_lens`` tensor for all layers:
+bits (``include/acct_b200.h`` has the formulas).  For serving: rows, queries and weights that need a gradient are refused (call
+under ``torch.no_grad()``).  The cache is storage: how many slots of a sequence are in use is the caller's to know, one
+``seq_lens`` tensor for all layers:
 
     cache = Kv4Cache(B, N_kv, S_max, D, dtype=torch.bfloat16)              # per layer, once
     out = flash_attention_packed(q, k, v, cu_seqlens)                      # the prompts ...
