@@ -598,16 +598,24 @@ void kv4_rows(const Kv4& cache, const Tensor& start, const Tensor& cu, acct_kv4_
   if (cu.defined()) r.cu_seqlens = static_cast<const int32_t*>(cu.const_data_ptr());
 }
 
+bool at_16_bytes(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
+// The tensor if it is packed and begins at a multiple of 16 bytes, else a copy that does
+Tensor packed_at_16_bytes(const Tensor& t) {
+  const Tensor x = t.contiguous();
+  return at_16_bytes(x) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
 // A tensor whose rows a kernel can read as they are, else a packed copy
 Tensor rows_readable(const Tensor& t, int64_t (&strides)[2]) {
-  bool as_is = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  bool as_is = t.stride(2) == 1 && at_16_bytes(t);
   for (int i = 0; i < 2; ++i) {
     strides[i] = t.stride(i);
     as_is = as_is && strides[i] >= t.size(2) && strides[i] % 8 == 0;
   }
   if (as_is) return t;
   strides[0] = strides[1] = 0;
-  return t.contiguous();
+  return packed_at_16_bytes(t);
 }
 
 // infer_packed(q, k, v, cu_seqlens_q, cu_seqlens_k | None, causal, scale, out | None, want_lse) -> y, or (y, lse)
@@ -750,7 +758,7 @@ PyObject* py_kv4_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
                "] (decode takes one query token), got ", q.sizes());
     HOST_CHECK(splits >= INT32_MIN && splits <= INT32_MAX, "num_splits out of range");
     c10::cuda::OptionalCUDAGuard guard(cache.records.device());
-    q = q.contiguous();
+    q = packed_at_16_bytes(q);
     if (y.defined()) {
       require_on("out", y, q);
       HOST_CHECK(y.scalar_type() == q.scalar_type() && y.is_contiguous() && y.numel() == q.numel(),
