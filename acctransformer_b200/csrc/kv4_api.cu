@@ -89,6 +89,8 @@ int padded_group(int N, int N_kv) { return (N / N_kv + 1) / 2 * 2; }
 size_t scores_bytes(int B, int N, int N_kv, int S_max) { return static_cast<size_t>(B) * N_kv * padded_group(N, N_kv) * padded_slots(S_max) * 4; }
 
 constexpr int kMaxSplits = 64;
+// the most parts that a sequence is cut into where the library chooses: of 512 slots or more
+int most_splits(int S_max) { return static_cast<int>(std::min<int64_t>(kMaxSplits, (static_cast<int64_t>(S_max) + 511) / 512)); }
 
 }  // namespace
 }  // namespace acct
@@ -105,7 +107,8 @@ int acct_kv4_read(const acct_kv4_cache* c, const acct_kv4_rows* r, void* stream)
 
 size_t acct_kv4_decode_workspace_bytes(const acct_kv4_cache* c, int32_t N, int32_t num_splits, int32_t with_weights) {
   if (c == nullptr || c->B <= 0 || c->N_kv <= 0 || c->D <= 0 || c->S_max <= 0 || N < c->N_kv || num_splits > kMaxSplits) return 0;
-  return parts_bytes(c->B, N, c->D, num_splits > 0 ? num_splits : kMaxSplits) + (with_weights ? scores_bytes(c->B, N, c->N_kv, c->S_max) : 0);
+  const int splits = num_splits > 0 ? num_splits : num_splits == 0 ? kMaxSplits : most_splits(c->S_max);
+  return parts_bytes(c->B, N, c->D, splits) + (with_weights ? scores_bytes(c->B, N, c->N_kv, c->S_max) : 0);
 }
 
 int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void* stream) {
@@ -140,7 +143,7 @@ int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void
     auto parts = [&](int64_t rounds) { return std::max<int64_t>(1, slots * rounds / c->N_kv - c->B / 2); };
     const int64_t rounds = (units + slots - 1) / slots;
     p.parts = static_cast<int>(parts(steps >= 160 * parts(rounds) ? 2 * rounds : rounds));
-    splits = std::min<int64_t>(kMaxSplits, (static_cast<int64_t>(c->S_max) + 511) / 512);
+    splits = most_splits(c->S_max);
     while (splits > 1 && parts_bytes(c->B, a->N, c->D, static_cast<int>(splits)) + scores > given) --splits;
     // Short contexts of few slices: the parts of a slice are one cluster and finish without a second kernel.  All clusters have to
     // be resident at once (16 x 8 slices of 1 024 keys in 2 parts, 128 of 222 that fit: 12.5 us against 17.7 of two kernels, in 4,

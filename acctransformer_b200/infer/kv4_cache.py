@@ -31,7 +31,7 @@ MAX_HEAD_DIM = 128
 
 class Kv4Workspace:
     """Caller-owned scratch for ``Kv4Cache.decode``: partial results, and the scores where probabilities are added up.  One serves
-    all layers of a step."""
+    all layers of a step.  ``num_splits``: that of the calls; 0 has room for any, -1 for calls that leave it to the library."""
 
     def __init__(self, B, N, N_kv, S_max, D, device, *, weights=False, num_splits=0):
         a = _lib.Kv4CacheArgs()
@@ -112,7 +112,7 @@ class Kv4Cache:
             if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 4:
                 raise ValueError("q must be a CUDA tensor [B, N, 1, D] (this library has no CPU path)")
             workspace = Kv4Workspace(self.B, q.shape[1], self.N_kv, self.S_max, self.D, self.records.device, weights=weights is not None,
-                                     num_splits=num_splits)
+                                     num_splits=num_splits or -1)
         return _lib.host().kv4_decode(self._args, q, seq_lens, weights, 1.0 / math.sqrt(self.D) if scale is None else scale, num_splits,
                                       workspace.buf, out)
 

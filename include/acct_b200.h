@@ -405,6 +405,7 @@ typedef struct acct_kv4_decode_args {
   size_t workspace_bytes;
 } acct_kv4_decode_args;
 
+/* num_splits > 0: for calls with so many; 0: for calls with any number; below 0: for calls that leave it to the library (with 0). */
 ACCT_API size_t acct_kv4_decode_workspace_bytes(const acct_kv4_cache* c, int32_t N, int32_t num_splits, int32_t with_weights);
 ACCT_API int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void* stream);
 
