@@ -4,9 +4,9 @@
 // each), every block with a list of tiles, whose next one is looked up while one is worked on.  What a tile needs before its first
 // scores and after its last product, a third of its time where a sequence has five tiles of keys, falls under the other block's
 // work; the two tiles per block of fa_fwd.cu are at the same point of theirs at the same time.  24 chunks of up to 1 500 tokens, 16
-// heads of 64: 218 us, 266 there.  8 prompts of up to 4 096 tokens, 32 heads of 128 on 8: 544 us, 558 there.  (A block for each
-// tile instead of lists: 253 and 580; one block with both tiles as independent streams: 262 and 588.)  Long sequences go there
-// (the rule is at acct_infer_packed): two tiles share each load of K and V.
+// heads of 64: 226 us, 266 there.  8 prompts of up to 4 096 tokens, 32 heads of 128 on 8: 555 us, 569 there.  (A block for each
+// tile instead of lists: 253 and 580, when this took 229 and 550; one block with both tiles as independent streams: 262 and
+// 588.)  Long sequences go there (the rule is at acct_infer_packed): two tiles share each load of K and V.
 //
 // The rows of a tile are `tile_heads` query heads that read one head of K and V, times 128 / tile_heads tokens (row = token *
 // heads + head: a box of the tensor map as it is).  K and V are then read once per group instead of once per head, and a tile's

@@ -136,8 +136,11 @@ int acct_kv4_decode(const acct_kv4_cache* c, const acct_kv4_decode_args* a, void
   int64_t splits = a->num_splits;
   p.parts = 0;
   if (splits == 0) {
-    // Parts for one round of resident thread blocks (a sequence wastes half a part on average), or for two where they stay long:
-    // those of 32 x 8 slices of up to 16 384 keys 95 -> 90 us, of 8 x 8 slices 36 -> 40.
+    // Parts for one round of resident thread blocks (a sequence wastes half a part on average), or for two where a part of one round
+    // has 160 steps (5 120 keys) or more of the slots.  One round and two, us, by steps: groups of 4 heads 80 34.9 / 37.5, 120 43.6 /
+    // 47.1, 161 53.3 / 55.3, 174 60.4 / 60.8, 210 59.0 / 53.3, 261 82.9 / 81.1, 321 107.8 / 93.0, 420 101.5 / 99.0.  Groups of 16,
+    // whose rounds are of fewer blocks, scatter with how the parts divide the lengths: 141 65.7 / 53.2, 186 59.4 / 65.1, 248 98.3 /
+    // 73.8, 282 81.1 / 84.1, 390 100.4 / 82.2, 496 120.5 / 144.8, 780 176.2 / 144.8.
     const int64_t slots = static_cast<int64_t>(info.sm_count) * kv4_decode_blocks_per_sm(group);
     const int64_t steps = static_cast<int64_t>(c->B) * ((static_cast<int64_t>(c->S_max) + 31) / 32);
     auto parts = [&](int64_t rounds) { return std::max<int64_t>(1, slots * rounds / c->N_kv - c->B / 2); };

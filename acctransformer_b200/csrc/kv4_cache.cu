@@ -5,8 +5,9 @@
 // enough warps are resident to keep loads in flight.  Where only some of a record's rows are meant (a single token, the ends of a
 // prompt) it loads and stores those and leaves the others alone.
 //
-// 16 prompts of up to 4 096 tokens, 8 heads of 128, in and out again: 109 us for 497 MB in all, 76 at the rate of a copy.
-// Reading issues in 55 % of the clocks; writing, with extremes, steps and rounding for each value, in 69 %, and that is its bound.
+// 16 prompts of up to 4 096 tokens, 8 heads of 128, in and out again: 110 us for 497 MB in all, 76 at the rate of a copy.
+// Reading issues in 55 % of the clocks; writing, with extremes, steps and rounding for each value, in 69 %: nothing is at its limit,
+// the arithmetic is what comes closest.
 // A single token per sequence is latency: 6.6 us on the device for one write and one read.
 #include "fa_common.cuh"
 #include "fa_kernels.cuh"

@@ -15,9 +15,10 @@
 //                 in 16 bits), two rows of a column at a time, with the code subtracted out of 1024 + c, 64 + c or 128 + c.
 //                 P is rounded to 16 bits too, which would cost as much again (in fp16, over 2 048 keys, 3.4e-4 of the result from
 //                 the exact one; its own last rounding makes 2.1e-4).  What the rounding leaves is an operand as well: with up to 4
-//                 heads in the 4 columns that they leave free, where it costs 12 instructions a record (105 -> 108 us at 32 x 8
-//                 slices of up to 16 384 keys), up to 8 in products of its own (124 -> 129): 2.8e-4.  With more it is left out: 212
-//                 us would be 237, and the 4 bits are coarser by two orders.
+//                 heads in the 4 columns that they leave free, where it costs 12 instructions a record (32 x 8 slices of up to
+//                 16 384 keys, fp16: 97 -> 101 us, 115 -> 119 with probabilities), up to 8 in products of its own (102 -> 111,
+//                 134 -> 143): 2.8e-4.  With more it is left out: 145 us would be 170, 220 be 242, and the 4 bits are coarser
+//                 by two orders.
 // The running maximum is only refreshed where a score exceeds it by more than 8 (in log2 units), so that most records need no
 // exchange between lanes.  Records come in by one bulk copy each through a ring per warp; nothing is shared between the warps of
 // a block before the end.
@@ -168,8 +169,9 @@ constexpr float kRefresh = 8.0f;      // log2 units by which a score may exceed 
 // any score that is in range.
 constexpr float kLowest = -3.402823466e38f;
 
-// Resident thread blocks per SM, which the registers decide (152 and 230 a thread).  With four, at 128 registers, or five, at 96
-// and a record at a time, the step is no faster (32 x 8 slices of up to 16 384 keys 95 and 103 us against 90).
+// Resident thread blocks per SM, which the registers decide (152 to 168 and 228 to 234 a thread at head_dim 128).  With four, at 128
+// registers, or five, at 96 and a record at a time, the step is no faster (32 x 8 slices of up to 16 384 keys 95 and 103 us against
+// 90, all before what P's rounding leaves was multiplied).
 constexpr int blocks_per_sm(int heads) { return heads <= 8 ? 3 : 2; }
 
 // the float at `p` of this block's shared memory, in that of block `rank` of the cluster

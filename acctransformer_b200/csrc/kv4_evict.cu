@@ -6,7 +6,7 @@
 // equal to it, placed by one prefix sum.  The result depends on no order of execution.  The copy (a warp for two records of the smaller
 // cache) takes codes as they are: nothing is decoded and rounded again.
 //
-// 32 sequences of up to 8 192 slots, 8 heads of 128, half of them stay: 195 us with the read that follows, 145 at the rate of a copy.  The
+// 32 sequences of up to 8 192 slots, 8 heads of 128, half of them stay: 197 us with the read that follows, 145 at the rate of a copy.  The
 // copy is bound by its reads: two rows of V share their words, and four rows of K a sector of steps, so neighbours that go are read
 // with those that stay (16 x 8 heads of 8 192 slots: 135 MB for 84 that stay, at 55 % of the DRAM rate).  Selection there is latency, 17 us.
 #include "fa_kernels.cuh"

@@ -61,6 +61,7 @@ def flash_attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=T
     device with every sequence's first row and the end (``cu_seqlens_k`` defaults to ``cu_seqlens_q``).
 
     ``causal``: the last query of a sequence sees its last key, the one before it all keys but that, and so on, so that a
-    sequence with more keys than queries is a chunk of a prompt behind a prefix.  A query that sees no key gives 0.  scale
-    defaults to D^-1/2; ``return_lse`` adds the logarithms of the softmax sums, float32 [N, T_q].  For serving: no gradient."""
+    sequence with more keys than queries is a chunk of a prompt behind a prefix.  A query that sees no key gives 0; rows
+    that belong to no sequence are not written.  scale defaults to D^-1/2; ``return_lse`` adds the logarithms of the softmax
+    sums, float32 [N, T_q].  For serving: no gradient."""
     return _ops.infer_packed(q, k, v, cu_seqlens_q, cu_seqlens_k, causal=causal, scale=scale, out=out, return_lse=return_lse)

@@ -277,8 +277,9 @@ ACCT_API int acct_infer_prefill(const acct_infer_args* a, void* stream);
  * batch has anyway.  No counterpart in the reference (its op takes one length per call).  Sequence b has the query rows
  * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 and the key rows cu_seqlens_k[b] .. ; with `causal` its last query sees its last key,
  * the query before it all keys but that one, and so on (a chunk of a prompt whose beginning is in the keys already).  A query
- * that sees no key gives 0 (lse -inf).  Nothing of another sequence, or of rows past the last one, reaches a result, NaNs
- * included; inside a sequence what is not finite in V reaches, besides the queries that see it, those of its 128-row tile. */
+ * that sees no key gives 0 (lse -inf); rows of y that no sequence has are not written.  Nothing of another sequence, or of rows past
+ * the last one, reaches a result, NaNs included; inside a sequence what is not finite in V reaches, besides the queries that see
+ * it, some of the up to 254 before them, as tiles of 128 keys are multiplied whole (0 times a NaN being one). */
 typedef struct acct_packed_args {
   int32_t dtype;            /* ACCT_F16 or ACCT_BF16 */
   int32_t B, N, D;          /* sequences, query heads, head_dim: a multiple of 8 up to 256 */
