@@ -4,7 +4,8 @@ running hand-written sm_100a CUDA through the C ABI in ``include/acct_b200.h``."
 
 __all__ = ["FlashAttention", "TriangleAttention", "get_flash_attention", "get_flash_attention_grad",
            "FlashAttentionTik", "flash_attention_tik", "flash_attention_decode", "flash_attention_packed",
-           "Kv4Cache", "Kv4Workspace"]
+           "Kv4Cache", "Kv4Workspace", "LinearAttention", "linear_attention", "linear_attention_packed", "linear_attention_step", "Rotary"]
+
 
 
 def __getattr__(name):
@@ -23,4 +24,10 @@ def __getattr__(name):
     if name in ("Kv4Cache", "Kv4Workspace"):
         from .infer import kv4_cache as m
         return getattr(m, name)
+    if name in ("LinearAttention", "linear_attention", "linear_attention_packed", "linear_attention_step"):
+        from . import linear as m
+        return getattr(m, name)
+    if name == "Rotary":
+        from .rotary import Rotary
+        return Rotary
     raise AttributeError(name)

@@ -35,6 +35,7 @@ EXPORTS = [
     "acct_selftest_wait_timeout", "acct_ms_fa_attrs_slot", "acct_ms_fa_attrs_slot_ex",
     "acct_infer_packed", "acct_kv4_record_bytes", "acct_kv4_append", "acct_kv4_read", "acct_kv4_decode_workspace_bytes", "acct_kv4_decode",
     "acct_kv4_evict",
+    "acct_linear_fwd_workspace_bytes", "acct_linear_fwd", "acct_linear_bwd_workspace_bytes", "acct_linear_bwd", "acct_linear_step", "acct_rotary",
 ] + [f"acct_ms_fa_{kind}_s{k}" for k in range(32) for kind in ("fwd", "grad")]
 
 
@@ -134,6 +135,43 @@ class Kv4EvictArgs(C.Structure):
     ]
 
 
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("N", C.c_int32), ("S", C.c_int32), ("D", C.c_int32), ("N_kv", C.c_int32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("y", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("y_stride", C.c_int64 * 3),
+        ("log_decay", C.c_void_p), ("cu_seqlens", C.c_void_p), ("seq_lens", C.c_void_p),
+        ("state_in", C.c_void_p), ("state_out", C.c_void_p), ("scale", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LinearBwdIO(C.Structure):
+    _fields_ = [
+        ("d_y", C.c_void_p), ("d_y_stride", C.c_int64 * 3), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LinearStepArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("N_kv", C.c_int32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("y", C.c_void_p),
+        ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+        ("state", C.c_void_p), ("log_decay", C.c_void_p), ("scale", C.c_float),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("S", C.c_int32), ("D", C.c_int32), ("N", C.c_int32), ("N_kv", C.c_int32),
+        ("rotated", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("q_out_stride", C.c_int64 * 3), ("k_out_stride", C.c_int64 * 3),
+        ("positions", C.c_void_p), ("pos_stride", C.c_int64 * 3), ("turns", C.c_void_p), ("axis", C.c_void_p),
+        ("adjacent", C.c_int32), ("inverse", C.c_int32),
+    ]
+
+
 _lib = None
 _host = None
 
@@ -212,6 +250,18 @@ def load():
     lib.acct_kv4_decode.restype = C.c_int
     lib.acct_kv4_evict.argtypes = [C.POINTER(Kv4CacheArgs), C.POINTER(Kv4CacheArgs), C.POINTER(Kv4EvictArgs), C.c_void_p]
     lib.acct_kv4_evict.restype = C.c_int
+    lib.acct_linear_fwd_workspace_bytes.argtypes = [C.POINTER(LinearArgs)]
+    lib.acct_linear_fwd_workspace_bytes.restype = C.c_size_t
+    lib.acct_linear_fwd.argtypes = [C.POINTER(LinearArgs), C.c_void_p]
+    lib.acct_linear_fwd.restype = C.c_int
+    lib.acct_linear_bwd_workspace_bytes.argtypes = [C.POINTER(LinearArgs)]
+    lib.acct_linear_bwd_workspace_bytes.restype = C.c_size_t
+    lib.acct_linear_bwd.argtypes = [C.POINTER(LinearArgs), C.POINTER(LinearBwdIO), C.c_void_p]
+    lib.acct_linear_bwd.restype = C.c_int
+    lib.acct_linear_step.argtypes = [C.POINTER(LinearStepArgs), C.c_void_p]
+    lib.acct_linear_step.restype = C.c_int
+    lib.acct_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
+    lib.acct_rotary.restype = C.c_int
     lib.acct_abi_version.argtypes = []
     lib.acct_abi_version.restype = C.c_int
     if lib.acct_abi_version() != ABI_VERSION:

@@ -1,0 +1,227 @@
+// C-ABI entry points of linear attention and of rotary positions: argument checks and launches.
+#include <algorithm>
+
+#include "common.cuh"
+#include "fa_kernels.cuh"
+#include "linear.cuh"
+
+namespace acct {
+namespace {
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+int check_width(int D) {
+  if (D <= 0 || D % 8 != 0 || D > kLinMaxHeadDim) return fail(ACCT_ERR_UNSUPPORTED_D, "head_dim %d must be a multiple of 8 in (0, %d]", D, kLinMaxHeadDim);
+  return 0;
+}
+
+// Strides of batch entry, head and row; 0 = packed: [rows, heads, D] where sequences are packed, else [B, heads, rows, D].
+int strides_of(const char* name, const int64_t (&given)[3], const acct_linear_args* a, int heads, int64_t (&out)[3]) {
+  const int64_t D = a->D, S = a->S;
+  const bool packed = a->cu_seqlens != nullptr;
+  const int64_t dense[3] = {D * S * heads, packed ? D : D * S, packed ? D * heads : D};
+  for (int i = 0; i < 3; ++i) {
+    out[i] = packed_or(given[i], dense[i]);
+    if (out[i] < D) return fail(ACCT_ERR_SHAPE, "%s strides must not be smaller than head_dim", name);
+    if (out[i] % 8 != 0) return fail(ACCT_ERR_ALIGN, "%s stride (%lld elements) is not a multiple of 8", name, (long long)out[i]);
+  }
+  return 0;
+}
+
+int check_linear(const acct_linear_args* a, LinParams* p, LinOperand* q, LinOperand* k, LinOperand* v) {
+  if (a == nullptr) return fail(ACCT_ERR_NULL, "args is NULL");
+  if (a->dtype != ACCT_F16 && a->dtype != ACCT_BF16) return fail(ACCT_ERR_DTYPE, "dtype must be ACCT_F16 or ACCT_BF16");
+  if (a->B <= 0 || a->N <= 0) return fail(ACCT_ERR_SHAPE, "B, N must be positive");
+  if (a->S < 0 || (a->S == 0 && a->cu_seqlens == nullptr)) return fail(ACCT_ERR_SHAPE, "S must be positive (0 only for packed sequences)");
+  if (a->N_kv < 0 || (a->N_kv > 0 && a->N % a->N_kv != 0)) return fail(ACCT_ERR_SHAPE, "N_kv = %d must be 0 or a divisor of N = %d", a->N_kv, a->N);
+  if (static_cast<int64_t>(a->B) * a->N > (1 << 24)) return fail(ACCT_ERR_SHAPE, "B*N = %lld is too large", (long long)a->B * a->N);
+  int rc = check_width(a->D);
+  if (rc) return rc;
+  if (!a->log_decay) return fail(ACCT_ERR_NULL, "log_decay is NULL");
+  if (a->cu_seqlens != nullptr && a->seq_lens != nullptr) return fail(ACCT_ERR_SHAPE, "seq_lens does not go with packed sequences");
+  if (a->S > 0 && (!a->q || !a->k || !a->v)) return fail(ACCT_ERR_NULL, "q, k, v must be non-NULL");
+  if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v)) return fail(ACCT_ERR_ALIGN, "q, k, v must be 16-byte aligned");
+  if (!(a->scale > -1e30f) || !(a->scale < 1e30f)) return fail(ACCT_ERR_SHAPE, "scale must be a finite number");
+  const int n_kv = a->N_kv > 0 ? a->N_kv : a->N, group = a->N / n_kv;
+  *q = {a->q, {0, 0, 0}, 1};
+  *k = {a->k, {0, 0, 0}, group};
+  *v = {a->v, {0, 0, 0}, group};
+  if ((rc = strides_of("q", a->q_stride, a, a->N, q->stride)) || (rc = strides_of("k", a->k_stride, a, n_kv, k->stride)) ||
+      (rc = strides_of("v", a->v_stride, a, n_kv, v->stride)))
+    return rc;
+  memset(p, 0, sizeof(*p));
+  p->B = a->B; p->N = a->N; p->S = a->S; p->D = a->D;
+  p->log_decay = a->log_decay;
+  p->cu = a->cu_seqlens;
+  p->lens = a->seq_lens;
+  p->scale = a->scale;
+  return 0;
+}
+
+size_t partial_bytes(const acct_linear_args* a) { return static_cast<size_t>(a->B) * a->N * a->S * a->D * 4; }
+
+}  // namespace
+}  // namespace acct
+
+using namespace acct;
+
+extern "C" {
+
+size_t acct_linear_fwd_workspace_bytes(const acct_linear_args*) { return 0; }
+
+int acct_linear_fwd(const acct_linear_args* a, void* stream) {
+  LinParams p;
+  LinOperand q, k, v;
+  int rc = check_linear(a, &p, &q, &k, &v);
+  if (rc) return rc;
+  if (a->S > 0 && !a->y) return fail(ACCT_ERR_NULL, "y must be non-NULL");
+  if (misaligned(a->y) || misaligned(a->state_in) || misaligned(a->state_out)) return fail(ACCT_ERR_ALIGN, "y and the states must be 16-byte aligned");
+  LinPass& pass = p.pass[0];
+  pass.a = q; pass.b = k; pass.c = v;
+  pass.y = a->y;
+  if ((rc = strides_of("y", a->y_stride, a, a->N, pass.y_stride))) return rc;
+  p.passes = 1;
+  p.state_in = a->state_in;
+  p.state_out = a->state_out;
+  DeviceInfo info;
+  if ((rc = device_info(&info))) return rc;
+  p.status = device_status_ptr();
+  const cudaError_t e = launch_linear(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention kernel");
+  return ACCT_OK;
+}
+
+size_t acct_linear_bwd_workspace_bytes(const acct_linear_args* a) {
+  if (a == nullptr || a->B <= 0 || a->N <= 0 || a->S <= 0 || a->D <= 0) return 0;
+  return a->N_kv > 0 && a->N_kv != a->N ? 2 * partial_bytes(a) : 0;
+}
+
+int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void* stream) {
+  LinParams p;
+  LinOperand q, k, v, d;
+  int rc = check_linear(a, &p, &q, &k, &v);
+  if (rc) return rc;
+  if (a->cu_seqlens != nullptr) return fail(ACCT_ERR_SHAPE, "packed sequences have no backward");
+  if (a->state_in != nullptr || a->state_out != nullptr) return fail(ACCT_ERR_SHAPE, "states have no backward");
+  if (g == nullptr || !g->d_y || !g->dq || !g->dk || !g->dv) return fail(ACCT_ERR_NULL, "d_y, dq, dk, dv must be non-NULL");
+  if (misaligned(g->d_y) || misaligned(g->dq) || misaligned(g->dk) || misaligned(g->dv)) return fail(ACCT_ERR_ALIGN, "d_y, dq, dk, dv must be 16-byte aligned");
+  const size_t need = acct_linear_bwd_workspace_bytes(a);
+  if (need > 0 && (g->workspace == nullptr || g->workspace_bytes < need))
+    return fail(ACCT_ERR_WORKSPACE, "workspace of %zu bytes is too small: %zu are needed", g->workspace_bytes, need);
+  if (need > 0 && misaligned(g->workspace)) return fail(ACCT_ERR_ALIGN, "workspace must be 16-byte aligned");
+  d = {g->d_y, {0, 0, 0}, 1};
+  if ((rc = strides_of("d_y", g->d_y_stride, a, a->N, d.stride))) return rc;
+  const int group = k.group, n_kv = a->N / group;
+  const int64_t zero[3] = {0, 0, 0};
+  LinPass &dq = p.pass[0], &dk = p.pass[1], &dv = p.pass[2];
+  dq.a = d; dq.b = v; dq.c = k; dq.y = g->dq;
+  dk.a = v; dk.b = d; dk.c = q; dk.y = g->dk;
+  dv.a = k; dv.b = q; dv.c = d; dv.y = g->dv;
+  dk.reverse = dv.reverse = 1;
+  p.passes = 3;
+  LinReduce r;
+  memset(&r, 0, sizeof(r));
+  if ((rc = strides_of("dq", zero, a, a->N, dq.y_stride)) || (rc = strides_of("dk", zero, a, a->N, dk.y_stride)) ||
+      (rc = strides_of("dv", zero, a, a->N, dv.y_stride)))
+    return rc;
+  if (group > 1) {
+    float* parts = static_cast<float*>(g->workspace);
+    dk.y = parts;
+    dv.y = parts + static_cast<size_t>(a->B) * a->N * a->S * a->D;
+    dk.y_f32 = dv.y_f32 = 1;
+    r.parts[0] = static_cast<const float*>(dk.y); r.parts[1] = static_cast<const float*>(dv.y);
+    r.out[0] = g->dk; r.out[1] = g->dv;
+    if ((rc = strides_of("dk", zero, a, n_kv, r.out_stride[0])) || (rc = strides_of("dv", zero, a, n_kv, r.out_stride[1]))) return rc;
+    r.lens = a->seq_lens;
+    r.B = a->B; r.N_kv = n_kv; r.group = group; r.S = a->S; r.D = a->D;
+  }
+  DeviceInfo info;
+  if ((rc = device_info(&info))) return rc;
+  p.status = device_status_ptr();
+  cudaError_t e = launch_linear(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess && group > 1) e = launch_linear_reduce(r, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention backward");
+  return ACCT_OK;
+}
+
+int acct_linear_step(const acct_linear_step_args* a, void* stream) {
+  if (a == nullptr) return fail(ACCT_ERR_NULL, "args is NULL");
+  if (a->dtype != ACCT_F16 && a->dtype != ACCT_BF16) return fail(ACCT_ERR_DTYPE, "dtype must be ACCT_F16 or ACCT_BF16");
+  if (a->B <= 0 || a->N <= 0) return fail(ACCT_ERR_SHAPE, "B, N must be positive");
+  if (a->N_kv < 0 || (a->N_kv > 0 && a->N % a->N_kv != 0)) return fail(ACCT_ERR_SHAPE, "N_kv = %d must be 0 or a divisor of N = %d", a->N_kv, a->N);
+  if (static_cast<int64_t>(a->B) * a->N > (1 << 24)) return fail(ACCT_ERR_SHAPE, "B*N = %lld is too large", (long long)a->B * a->N);
+  int rc = check_width(a->D);
+  if (rc) return rc;
+  if (!a->q || !a->k || !a->v || !a->y || !a->state || !a->log_decay) return fail(ACCT_ERR_NULL, "q, k, v, y, state, log_decay must be non-NULL");
+  if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v) || misaligned(a->y) || misaligned(a->state))
+    return fail(ACCT_ERR_ALIGN, "q, k, v, y, state must be 16-byte aligned");
+  if (!(a->scale > -1e30f) || !(a->scale < 1e30f)) return fail(ACCT_ERR_SHAPE, "scale must be a finite number");
+  const int n_kv = a->N_kv > 0 ? a->N_kv : a->N;
+  LinStepParams p;
+  memset(&p, 0, sizeof(p));
+  const struct { const char* name; const int64_t* given; int heads; int64_t* out; } rows[3] = {
+      {"q", a->q_stride, a->N, p.q_stride}, {"k", a->k_stride, n_kv, p.k_stride}, {"v", a->v_stride, n_kv, p.v_stride}};
+  for (const auto& x : rows)
+    for (int i = 0; i < 2; ++i) {
+      x.out[i] = packed_or(x.given[i], i == 0 ? static_cast<int64_t>(x.heads) * a->D : a->D);
+      if (x.out[i] < a->D) return fail(ACCT_ERR_SHAPE, "%s strides must not be smaller than head_dim", x.name);
+      if (x.out[i] % 8 != 0) return fail(ACCT_ERR_ALIGN, "%s stride (%lld elements) is not a multiple of 8", x.name, (long long)x.out[i]);
+    }
+  p.q = a->q; p.k = a->k; p.v = a->v; p.y = a->y;
+  p.state = a->state;
+  p.log_decay = a->log_decay;
+  p.B = a->B; p.N = a->N; p.D = a->D; p.group = a->N / n_kv;
+  p.scale = a->scale;
+  DeviceInfo info;
+  if ((rc = device_info(&info))) return rc;
+  const cudaError_t e = launch_linear_step(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention step");
+  return ACCT_OK;
+}
+
+int acct_rotary(const acct_rotary_args* a, void* stream) {
+  if (a == nullptr) return fail(ACCT_ERR_NULL, "args is NULL");
+  if (a->dtype != ACCT_F16 && a->dtype != ACCT_BF16) return fail(ACCT_ERR_DTYPE, "dtype must be ACCT_F16 or ACCT_BF16");
+  if (a->B < 0 || a->S < 0 || a->N < 0 || a->N_kv < 0) return fail(ACCT_ERR_SHAPE, "sizes must not be negative");
+  if (a->D <= 0 || a->D % 8 != 0 || a->D > 256) return fail(ACCT_ERR_UNSUPPORTED_D, "head_dim %d must be a multiple of 8 in (0, 256]", a->D);
+  if (a->rotated <= 0 || a->rotated % 2 != 0 || a->rotated > a->D) return fail(ACCT_ERR_SHAPE, "rotated = %d must be even, in (0, head_dim = %d]", a->rotated, a->D);
+  if (!a->positions || !a->turns || !a->axis) return fail(ACCT_ERR_NULL, "positions, turns, axis must be non-NULL");
+  RotaryParams p;
+  memset(&p, 0, sizeof(p));
+  const int64_t rows = static_cast<int64_t>(a->B) * a->S;
+  const struct { const char* name; const void* x; void* y; const int64_t *xs, *ys; int heads; } t[2] = {
+      {"q", a->q, a->q_out, a->q_stride, a->q_out_stride, a->N}, {"k", a->k, a->k_out, a->k_stride, a->k_out_stride, a->N_kv}};
+  for (int w = 0; w < 2; ++w) {
+    if (t[w].heads == 0 || rows == 0) continue;
+    if (!t[w].x || !t[w].y) return fail(ACCT_ERR_NULL, "%s and its output must be non-NULL", t[w].name);
+    if (misaligned(t[w].x) || misaligned(t[w].y)) return fail(ACCT_ERR_ALIGN, "%s and its output must be 16-byte aligned", t[w].name);
+    const int64_t dense[3] = {static_cast<int64_t>(a->D) * a->S * t[w].heads, static_cast<int64_t>(a->D) * a->S, a->D};
+    for (int i = 0; i < 3; ++i) {
+      p.t[w].x_stride[i] = packed_or(t[w].xs[i], dense[i]);
+      p.t[w].y_stride[i] = packed_or(t[w].ys[i], dense[i]);
+      for (int64_t s : {p.t[w].x_stride[i], p.t[w].y_stride[i]}) {
+        if (s < a->D) return fail(ACCT_ERR_SHAPE, "%s strides must not be smaller than head_dim", t[w].name);
+        if (s % 8 != 0) return fail(ACCT_ERR_ALIGN, "%s stride (%lld elements) is not a multiple of 8", t[w].name, (long long)s);
+      }
+    }
+    p.t[w].x = t[w].x; p.t[w].y = t[w].y;
+    p.t[w].heads = t[w].heads;
+  }
+  if (rows > INT32_MAX || rows * (static_cast<int64_t>(a->N) + a->N_kv) * (a->D / 2) / 256 > INT32_MAX)
+    return fail(ACCT_ERR_SHAPE, "B*S = %lld rows are too many for one call", (long long)rows);
+  p.positions = a->positions;
+  for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->pos_stride[i];
+  p.turns = reinterpret_cast<const unsigned long long*>(a->turns);
+  p.axis = a->axis;
+  p.B = a->B; p.S = a->S; p.D = a->D; p.rotated = a->rotated;
+  p.adjacent = a->adjacent; p.inverse = a->inverse;
+  DeviceInfo info;
+  int rc = device_info(&info);
+  if (rc) return rc;
+  if (rows == 0 || a->N + a->N_kv == 0) return ACCT_OK;
+  const cudaError_t e = launch_rotary(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda(e, "launching the rotary kernel");
+  return ACCT_OK;
+}
+
+}  // extern "C"

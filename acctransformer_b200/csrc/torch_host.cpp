@@ -43,6 +43,12 @@ struct Library {
   decltype(&acct_kv4_read) kv4_read;
   decltype(&acct_kv4_decode) kv4_decode;
   decltype(&acct_kv4_evict) kv4_evict;
+  decltype(&acct_linear_fwd_workspace_bytes) linear_fwd_workspace_bytes;
+  decltype(&acct_linear_fwd) linear_fwd;
+  decltype(&acct_linear_bwd_workspace_bytes) linear_bwd_workspace_bytes;
+  decltype(&acct_linear_bwd) linear_bwd;
+  decltype(&acct_linear_step) linear_step;
+  decltype(&acct_rotary) rotary;
 } g_lib;
 
 #define HOST_CHECK TORCH_CHECK_VALUE
@@ -407,6 +413,12 @@ PyObject* py_init(PyObject*, PyObject* path) {
   g_lib.kv4_read = reinterpret_cast<decltype(g_lib.kv4_read)>(sym("acct_kv4_read"));
   g_lib.kv4_decode = reinterpret_cast<decltype(g_lib.kv4_decode)>(sym("acct_kv4_decode"));
   g_lib.kv4_evict = reinterpret_cast<decltype(g_lib.kv4_evict)>(sym("acct_kv4_evict"));
+  g_lib.linear_fwd_workspace_bytes = reinterpret_cast<decltype(g_lib.linear_fwd_workspace_bytes)>(sym("acct_linear_fwd_workspace_bytes"));
+  g_lib.linear_fwd = reinterpret_cast<decltype(g_lib.linear_fwd)>(sym("acct_linear_fwd"));
+  g_lib.linear_bwd_workspace_bytes = reinterpret_cast<decltype(g_lib.linear_bwd_workspace_bytes)>(sym("acct_linear_bwd_workspace_bytes"));
+  g_lib.linear_bwd = reinterpret_cast<decltype(g_lib.linear_bwd)>(sym("acct_linear_bwd"));
+  g_lib.linear_step = reinterpret_cast<decltype(g_lib.linear_step)>(sym("acct_linear_step"));
+  g_lib.rotary = reinterpret_cast<decltype(g_lib.rotary)>(sym("acct_rotary"));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -833,6 +845,406 @@ PyObject* py_kv4_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- linear attention and rotary positions
+struct LinearCall {
+  Tensor lens;
+  double scale;
+};
+
+// the decays as the kernels read them
+Tensor decays(const Tensor& g, int64_t N, const Tensor& q) {
+  require_on("log_decay", g, q);
+  HOST_CHECK(g.dim() == 1 && g.size(0) == N && at::isFloatingType(g.scalar_type()), "log_decay must hold a number for each of ", N, " heads, got ",
+             g.scalar_type(), " ", g.sizes());
+  HOST_CHECK(!g.requires_grad() || !at::GradMode::is_enabled(), "log_decay has no gradient: give a detached tensor");
+  TORCH_CHECK_NOT_IMPLEMENTED(!g._fw_grad(/*level=*/0).defined(), "linear attention does not support forward mode AD");
+  return g.to(at::kFloat).contiguous();
+}
+
+void check_linear_inputs(const Tensor& q, const Tensor& k, const Tensor& v) {
+  const Tensor* qkv[3] = {&q, &k, &v};
+  const char* names[3] = {"q", "k", "v"};
+  for (int i = 0; i < 3; ++i) {
+    require_on(names[i], *qkv[i], q);
+    HOST_CHECK(qkv[i]->dim() == 4, names[i], " must be [B, N, S, D]");
+  }
+  const auto dt = q.scalar_type();
+  HOST_CHECK((dt == at::kHalf || dt == at::kBFloat16) && k.scalar_type() == dt && v.scalar_type() == dt,
+             "q, k, v must share dtype float16 or bfloat16");
+  HOST_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3) && v.sizes() == k.sizes() && k.size(1) >= 1 &&
+                 q.size(1) % k.size(1) == 0,
+             "shape mismatch: q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), " (k and v may have fewer heads than q if their head count divides q's)");
+  for (int i = 0; i < 4; ++i) HOST_CHECK(q.size(i) >= 1 && q.size(i) <= INT32_MAX, "q must not be empty, got ", q.sizes());
+}
+
+// The operands' part of the argument block; `q`, `k`, `v` become what the pointers point into.
+void fill_linear(acct_linear_args& a, Tensor& q, Tensor& k, Tensor& v, const Tensor& g, const LinearCall& call) {
+  memset(&a, 0, sizeof(a));
+  a.dtype = q.scalar_type() == at::kBFloat16 ? ACCT_BF16 : ACCT_F16;
+  a.B = q.size(0); a.N = q.size(1); a.S = q.size(2); a.D = q.size(3); a.N_kv = k.size(1);
+  q = readable(q, a.q_stride); k = readable(k, a.k_stride); v = readable(v, a.v_stride);
+  a.q = q.const_data_ptr(); a.k = k.const_data_ptr(); a.v = v.const_data_ptr();
+  a.log_decay = static_cast<const float*>(g.const_data_ptr());
+  if (call.lens.defined()) a.seq_lens = static_cast<const int32_t*>(call.lens.const_data_ptr());
+  a.scale = static_cast<float>(call.scale);
+}
+
+// rows behind a sequence's last one are zeros in what a padded batch gives
+Tensor linear_result(const Tensor& like, const LinearCall& call) {
+  return call.lens.defined() ? at::zeros(like.sizes(), like.options().memory_format(at::MemoryFormat::Contiguous).requires_grad(false))
+                             : empty_like_shape(like.sizes(), like.scalar_type(), like);
+}
+
+struct LinearFunction : public torch::autograd::Function<LinearFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& g, const LinearCall& call) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::OptionalCUDAGuard guard(q_in.device());
+    Tensor q = q_in, k = k_in, v = v_in, ws;
+    acct_linear_args a;
+    fill_linear(a, q, k, v, g, call);
+    Tensor y = linear_result(q_in, call);
+    a.y = y.data_ptr();
+    if ((a.workspace_bytes = g_lib.linear_fwd_workspace_bytes(&a)) > 0) {
+      ws = empty_like_shape({static_cast<int64_t>(a.workspace_bytes)}, at::kByte, q);
+      a.workspace = ws.data_ptr();
+    }
+    check(g_lib.linear_fwd(&a, stream_of(q)));
+    ctx->save_for_backward({q_in, k_in, v_in, g, call.lens});
+    ctx->saved_data["scale"] = call.scale;
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    Tensor q = saved[0], k = saved[1], v = saved[2], d_y = grads[0];
+    at::AutoDispatchBelowADInplaceOrView below;
+    check_linear_inputs(q, k, v);      // (saved-tensor hooks may have handed back others)
+    const Tensor log_decay = decays(saved[3], q.size(1), q);
+    LinearCall call{saved[4], ctx->saved_data.at("scale").toDouble()};
+    if (call.lens.defined()) call.lens = ints_on("seq_lens", call.lens, q.size(0), q);
+    if (!d_y.defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    require_on("the gradient of y", d_y, q);
+    HOST_CHECK(d_y.sizes() == q.sizes() && d_y.scalar_type() == q.scalar_type(), "the gradient of y must have the shape and dtype of q");
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    Tensor dq = linear_result(q, call), dk = linear_result(k, call), dv = linear_result(v, call), ws;
+    acct_linear_args a;
+    fill_linear(a, q, k, v, log_decay, call);
+    acct_linear_bwd_io io;
+    memset(&io, 0, sizeof(io));
+    d_y = readable(d_y, io.d_y_stride);
+    io.d_y = d_y.const_data_ptr();
+    io.dq = dq.data_ptr(); io.dk = dk.data_ptr(); io.dv = dv.data_ptr();
+    if ((io.workspace_bytes = g_lib.linear_bwd_workspace_bytes(&a)) > 0) {
+      ws = empty_like_shape({static_cast<int64_t>(io.workspace_bytes)}, at::kByte, q);
+      io.workspace = ws.data_ptr();
+    }
+    check(g_lib.linear_bwd(&a, &io, stream_of(q)));
+    return {dq, dk, dv, Tensor(), Tensor()};
+  }
+};
+
+// linear_apply(q, k, v, log_decay, seq_lens | None, scale) -> y, differentiable in q, k, v
+PyObject* py_linear_apply(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 6, "linear_apply takes 6 arguments, got ", n);
+  const Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v");
+  Tensor g = tensor_arg(args[3], "log_decay"), y;
+  LinearCall call{tensor_or_undefined(args[4]), float_arg(args[5])};
+  for (const Tensor* t : {&q, &k, &v})
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), "linear attention does not support forward mode AD");
+  {
+    pybind11::gil_scoped_release no_gil;
+    check_linear_inputs(q, k, v);
+    {
+      c10::cuda::OptionalCUDAGuard guard(q.device());
+      at::AutoDispatchBelowADInplaceOrView below;
+      g = decays(g, q.size(1), q);
+      if (call.lens.defined()) call.lens = ints_on("seq_lens", call.lens, q.size(0), q);
+    }
+    y = LinearFunction::apply(q, k, v, g, call);
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// a state that a call moves on in place
+void check_state(const Tensor& state, int64_t B, int64_t N, int64_t D, const Tensor& q) {
+  require_on("state", state, q);
+  HOST_CHECK(state.scalar_type() == at::kFloat && state.dim() == 4 && state.size(0) == B && state.size(1) == N && state.size(2) == D &&
+                 state.size(3) == D && state.is_contiguous() && at_16_bytes(state),
+             "state must be a contiguous float32 tensor [", B, ", ", N, ", ", D, ", ", D, "], got ", state.scalar_type(), " ", state.sizes());
+}
+// (what autograd has saved of a tensor that is written in place is noticed there)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// linear_packed(q, k, v, log_decay, cu_seqlens, state | None, scale, out | None) -> (y, state)
+PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 8, "linear_packed takes 8 arguments, got ", n);
+  Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), g = tensor_arg(args[3], "log_decay");
+  Tensor cu = tensor_arg(args[4], "cu_seqlens"), state = tensor_or_undefined(args[5]), y = tensor_or_undefined(args[7]);
+  const double scale = float_arg(args[6]);
+  no_gradient("linear_attention_packed", {&q, &k, &v, &state});
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    require_cuda("q", q); require_on("k", k, q); require_on("v", v, q);
+    const auto dt = q.scalar_type();
+    HOST_CHECK((dt == at::kHalf || dt == at::kBFloat16) && k.scalar_type() == dt && v.scalar_type() == dt,
+               "q, k, v must share dtype float16 or bfloat16");
+    HOST_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && q.size(0) == k.size(0) && q.size(2) == k.size(2) && k.size(1) >= 1 &&
+                   q.size(1) >= 1 && q.size(1) % k.size(1) == 0,
+               "q must be [T, N, D] and k, v [T, N_kv, D] with N_kv dividing N, got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+    HOST_CHECK(cu.dim() == 1 && cu.numel() >= 2, "cu_seqlens must hold a start for each sequence and the end, got ", cu.sizes());
+    HOST_CHECK(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX, "too many rows");
+    const int64_t B = cu.numel() - 1, N = q.size(1), D = q.size(2);
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    cu = ints_on("cu_seqlens", cu, cu.numel(), q);
+    g = decays(g, N, q);
+    acct_linear_args a;
+    memset(&a, 0, sizeof(a));
+    if (state.defined()) {
+      check_state(state, B, N, D, q);
+      a.state_in = static_cast<const float*>(state.const_data_ptr());
+    } else {
+      state = empty_like_shape({B, N, D, D}, at::kFloat, q);
+    }
+    a.state_out = static_cast<float*>(state.data_ptr());
+    Tensor ws;
+    int64_t strides[2];
+    auto operand = [&](Tensor& t, const void*& ptr, int64_t (&out)[3]) {
+      t = rows_readable(t, strides);
+      ptr = t.const_data_ptr();
+      out[1] = strides[1]; out[2] = strides[0];
+    };
+    operand(q, a.q, a.q_stride); operand(k, a.k, a.k_stride); operand(v, a.v, a.v_stride);
+    if (y.defined()) {
+      require_on("out", y, q);
+      HOST_CHECK(y.scalar_type() == dt && y.sizes() == q.sizes() && y.is_contiguous() && at_16_bytes(y), "out must be a contiguous tensor shaped and typed like q");
+    } else {
+      y = empty_like_shape(q.sizes(), dt, q);
+    }
+    a.dtype = dt == at::kBFloat16 ? ACCT_BF16 : ACCT_F16;
+    a.B = B; a.N = N; a.S = q.size(0); a.D = D; a.N_kv = k.size(1);
+    a.y = y.data_ptr();
+    a.log_decay = static_cast<const float*>(g.const_data_ptr());
+    a.cu_seqlens = static_cast<const int32_t*>(cu.const_data_ptr());
+    a.scale = static_cast<float>(scale);
+    if ((a.workspace_bytes = g_lib.linear_fwd_workspace_bytes(&a)) > 0) {
+      ws = empty_like_shape({static_cast<int64_t>(a.workspace_bytes)}, at::kByte, q);
+      a.workspace = ws.data_ptr();
+    }
+    check(g_lib.linear_fwd(&a, stream_of(q)));
+    written(state);
+  }
+  PyObject* out = PyTuple_New(2);
+  PyTuple_SET_ITEM(out, 0, wrap(y));
+  PyTuple_SET_ITEM(out, 1, wrap(state));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_step(q, k, v, log_decay, state, scale, out | None) -> y
+PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 7, "linear_step takes 7 arguments, got ", n);
+  Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), g = tensor_arg(args[3], "log_decay");
+  Tensor state = tensor_arg(args[4], "state"), y = tensor_or_undefined(args[6]);
+  const double scale = float_arg(args[5]);
+  no_gradient("linear_attention_step", {&q, &k, &v, &state});
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    check_linear_inputs(q, k, v);
+    HOST_CHECK(q.size(2) == 1, "a step takes one token per sequence: q must be [B, N, 1, D], got ", q.sizes());
+    const int64_t B = q.size(0), N = q.size(1), D = q.size(3);
+    check_state(state, B, N, D, q);
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    g = decays(g, N, q);
+    acct_linear_step_args a;
+    memset(&a, 0, sizeof(a));
+    // (the stride of the one token may be anything)
+    auto operand = [&](Tensor& t, const void*& ptr, int64_t (&out)[2]) {
+      t = rows_readable(t.squeeze(2), out);
+      ptr = t.const_data_ptr();
+    };
+    operand(q, a.q, a.q_stride); operand(k, a.k, a.k_stride); operand(v, a.v, a.v_stride);
+    if (y.defined()) {
+      require_on("out", y, q);
+      HOST_CHECK(y.scalar_type() == q.scalar_type() && y.is_contiguous() && y.numel() == q.numel() && at_16_bytes(y),
+                 "out must be a contiguous tensor with the dtype and the number of elements of q");
+    } else {
+      y = empty_like_shape({B, N, 1, D}, q.scalar_type(), q);
+    }
+    a.dtype = q.scalar_type() == at::kBFloat16 ? ACCT_BF16 : ACCT_F16;
+    a.B = B; a.N = N; a.D = D; a.N_kv = k.size(1);
+    a.y = y.data_ptr();
+    a.state = static_cast<float*>(state.data_ptr());
+    a.log_decay = static_cast<const float*>(g.const_data_ptr());
+    a.scale = static_cast<float>(scale);
+    check(g_lib.linear_step(&a, stream_of(q)));
+    written(state);
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// What a rotary call carries besides queries and keys; the table is its object's own.
+struct RotaryCall {
+  Tensor positions, turns, axis;
+  int64_t head_dim, rotated, axes, adjacent;
+};
+
+// q or k as [B, heads, rows, D]
+Tensor rotary_rows(const Tensor& t) { return t.dim() == 3 ? t.transpose(0, 1).unsqueeze(0) : t; }
+
+// Turns `x` (undefined ones are left out) into `y`.
+void rotary_launch(const RotaryCall& call, const Tensor (&x)[2], const Tensor (&y)[2], bool inverse) {
+  acct_rotary_args a;
+  memset(&a, 0, sizeof(a));
+  const Tensor& first = x[0].defined() ? x[0] : x[1];
+  c10::cuda::OptionalCUDAGuard guard(first.device());
+  const Tensor shape = rotary_rows(first);
+  a.dtype = first.scalar_type() == at::kBFloat16 ? ACCT_BF16 : ACCT_F16;
+  a.B = shape.size(0); a.S = shape.size(2); a.D = call.head_dim;
+  a.rotated = call.rotated;
+  Tensor from[2];
+  for (int i = 0; i < 2; ++i) {
+    if (!x[i].defined()) continue;
+    int64_t(&xs)[3] = i == 0 ? a.q_stride : a.k_stride;
+    int64_t(&ys)[3] = i == 0 ? a.q_out_stride : a.k_out_stride;
+    from[i] = readable(rotary_rows(x[i]), xs);
+    const Tensor to = rotary_rows(y[i]);
+    for (int j = 0; j < 3; ++j) ys[j] = y[i].is_same(x[i]) ? xs[j] : to.stride(j);
+    (i == 0 ? a.q : a.k) = from[i].const_data_ptr();
+    (i == 0 ? a.q_out : a.k_out) = y[i].data_ptr();
+    (i == 0 ? a.N : a.N_kv) = from[i].size(1);
+  }
+  const Tensor& pos = call.positions;
+  a.positions = static_cast<const int32_t*>(pos.const_data_ptr());
+  for (int i = 0; i < 3; ++i) a.pos_stride[i] = pos.size(i) == 1 ? 0 : pos.stride(i);
+  a.turns = static_cast<const uint64_t*>(call.turns.const_data_ptr());
+  a.axis = static_cast<const int32_t*>(call.axis.const_data_ptr());
+  a.adjacent = call.adjacent;
+  a.inverse = inverse;
+  check(g_lib.rotary(&a, stream_of(first)));
+}
+
+// a new packed tensor of the shape of `t` whose strides are multiples of 8 whatever the sizes of its dimensions
+Tensor rotary_result(const Tensor& t) { return t.defined() ? empty_like_shape(t.sizes(), t.scalar_type(), t) : Tensor(); }
+
+struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+  static variable_list forward(AutogradContext* ctx, const std::optional<Tensor>& q, const std::optional<Tensor>& k, const RotaryCall& call) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x[2] = {q.value_or(Tensor()), k.value_or(Tensor())}, y[2] = {rotary_result(x[0]), rotary_result(x[1])};
+    rotary_launch(call, x, y, false);
+    ctx->save_for_backward({call.positions, call.turns, call.axis});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{call.head_dim, call.rotated, call.axes, call.adjacent, x[0].defined()};
+    variable_list out;
+    for (const Tensor& t : y)
+      if (t.defined()) out.push_back(t);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const std::vector<int64_t> sizes = ctx->saved_data.at("sizes").toIntVector();
+    const variable_list saved = ctx->get_saved_variables();
+    const RotaryCall call{saved[0], saved[1], saved[2], sizes[0], sizes[1], sizes[2], sizes[3]};
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor x[2];
+    size_t at = 0;
+    if (sizes[4]) x[0] = grads[at++];
+    if (at < grads.size()) x[1] = grads[at];
+    const Tensor y[2] = {rotary_result(x[0]), rotary_result(x[1])};
+    if (x[0].defined() || x[1].defined()) rotary_launch(call, x, y, true);
+    return {y[0], y[1], Tensor()};
+  }
+};
+
+// rotary(q | None, k | None, positions, turns, axis, (head_dim, rotated, axes, adjacent), in_place) -> (q | None, k | None)
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  HOST_CHECK(n == 7, "rotary takes 7 arguments, got ", n);
+  const Tensor q = tensor_or_undefined(args[0]), k = tensor_or_undefined(args[1]);
+  RotaryCall call{tensor_arg(args[2], "positions"), tensor_arg(args[3], "turns"), tensor_arg(args[4], "axis"), 0, 0, 0, 0};
+  HOST_CHECK(PyTuple_Check(args[5]) && PyTuple_GET_SIZE(args[5]) == 4, "not a rotary plan");
+  call.head_dim = int_arg(PyTuple_GET_ITEM(args[5], 0));
+  call.rotated = int_arg(PyTuple_GET_ITEM(args[5], 1));
+  call.axes = int_arg(PyTuple_GET_ITEM(args[5], 2));
+  call.adjacent = int_arg(PyTuple_GET_ITEM(args[5], 3));
+  const bool in_place = bool_arg(args[6]);
+  if (in_place) no_gradient("Rotary.apply_", {&q, &k});
+  variable_list out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    HOST_CHECK(q.defined() || k.defined(), "give q, k or both");
+    const Tensor& first = q.defined() ? q : k;
+    const Tensor* both[2] = {&q, &k};
+    for (int i = 0; i < 2; ++i) {
+      const Tensor& t = *both[i];
+      const char* name = i == 0 ? "q" : "k";
+      if (!t.defined()) continue;
+      require_on(name, t, first);
+      HOST_CHECK((t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) && t.scalar_type() == first.scalar_type(),
+                 "q and k must share dtype float16 or bfloat16");
+      HOST_CHECK((t.dim() == 3 || t.dim() == 4) && t.dim() == first.dim() && t.size(1) >= 1 && t.size(-1) == call.head_dim && t.size(0) == first.size(0) &&
+                     (t.dim() == 3 || t.size(2) == first.size(2)),
+                 name, " must be [T, heads, ", call.head_dim, "] or [B, heads, S, ", call.head_dim, "], with as many rows as the other, got ", t.sizes());
+      for (int64_t size : t.sizes()) HOST_CHECK(size <= INT32_MAX, "too many rows");
+      TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), "rotary positions do not support forward mode AD");
+    }
+    HOST_CHECK(call.turns.device() == first.device(), "q and k must be on the device of the plan, ", call.turns.device(), ", not on ", first.device());
+    const int64_t B = first.dim() == 4 ? first.size(0) : 1, S = first.dim() == 4 ? first.size(2) : first.size(0);
+    c10::cuda::OptionalCUDAGuard guard(first.device());
+    Tensor pos = call.positions;      // (as a view that shares its version counter: a change before the backward is noticed)
+    require_on("positions", pos, first);
+    HOST_CHECK(at::isIntegralType(pos.scalar_type(), /*includeBool=*/false), "positions must be integers, got ", pos.scalar_type());
+    // to [axes, batch entries or 1, rows]
+    const auto is = [&](at::IntArrayRef want) { return pos.sizes() == want; };
+    if (call.axes == 1 && is({S})) pos = pos.unsqueeze(0).unsqueeze(0);
+    else if (call.axes == 1 && is({B, S})) pos = pos.unsqueeze(0);
+    else if (is({call.axes, S})) pos = pos.unsqueeze(1);
+    else
+      HOST_CHECK(first.dim() == 4 && is({call.axes, B, S}), "positions must be [", call.axes, " axes, ", first.dim() == 4 ? "batch entries, " : "", S,
+                 " rows]", call.axes == 1 ? " or [rows]" : "", ", got ", pos.sizes());
+    call.positions = pos.scalar_type() == at::kInt ? pos : pos.to(at::kInt);
+    if (in_place || B * S == 0) {
+      at::AutoDispatchBelowADInplaceOrView below;
+      if (B * S > 0) {
+        int64_t strides[3];
+        for (const Tensor* t : both)
+          HOST_CHECK(!t->defined() || readable(rotary_rows(*t), strides).const_data_ptr() == t->const_data_ptr(),
+                     "in place, rows must be contiguous, and addresses and strides whole 16 bytes");
+        rotary_launch(call, {q, k}, {q, k}, false);
+      }
+      for (const Tensor* t : both)
+        if (t->defined()) {
+          if (in_place) written(*t);
+          out.push_back(*t);
+        }
+    }
+    if (out.empty()) {
+      const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+      out = RotaryFunction::apply(given(q), given(k), call);
+    }
+  }
+  PyObject* r = PyTuple_New(2);
+  size_t at = 0;
+  const Tensor* both[2] = {&q, &k};
+  for (int i = 0; i < 2; ++i) {
+    if (both[i]->defined()) {
+      PyTuple_SET_ITEM(r, i, wrap(out[at++]));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(r, i, Py_None);
+    }
+  }
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)); }
 
@@ -846,6 +1258,10 @@ PyMethodDef kMethods[] = {
     {"kv4_read", fast<py_kv4_read>(), METH_FASTCALL, "rows out of a cache in 4 bits"},
     {"kv4_decode", fast<py_kv4_decode>(), METH_FASTCALL, "one decoding step over a cache in 4 bits"},
     {"kv4_evict", fast<py_kv4_evict>(), METH_FASTCALL, "what stays of a cache in 4 bits, into another one"},
+    {"linear_apply", fast<py_linear_apply>(), METH_FASTCALL, "linear attention, differentiable"},
+    {"linear_packed", fast<py_linear_packed>(), METH_FASTCALL, "linear attention over packed sequences, with states"},
+    {"linear_step", fast<py_linear_step>(), METH_FASTCALL, "one step of linear attention"},
+    {"rotary", fast<py_rotary>(), METH_FASTCALL, "rotary positions, differentiable or in place"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_host", "native host path of acctransformer_b200", -1, kMethods,

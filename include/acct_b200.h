@@ -426,6 +426,96 @@ typedef struct acct_kv4_evict_args {
 
 ACCT_API int acct_kv4_evict(const acct_kv4_cache* src, const acct_kv4_cache* dst, const acct_kv4_evict_args* a, void* stream);
 
+/* Linear attention with a decay for each head; the reference has no counterpart.
+ *   S_t = exp(log_decay[n]) S_(t-1) + k_t v_t^T,   y_t = scale S_t^T q_t      (a state S is [D, D], row d = k's element d)
+ * over the rows of every sequence: rows 0 .. seq_lens[b] - 1 of batch entry b (seq_lens NULL: all S), or, with cu_seqlens, rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of packed operands.  Rows that belong to no sequence are neither used nor written; a value that
+ * is not finite reaches the other rows of its sequence only.  States, decays and sums are fp32.  log_decay is meant to be <= 0. */
+typedef struct acct_linear_args {
+  int32_t dtype;               /* ACCT_F16 or ACCT_BF16: q, k, v, y */
+  int32_t B, N, S, D;          /* sequences, query heads, rows (packed: of all sequences together), head_dim: a multiple of 8 up to 128 */
+  int32_t N_kv;                /* heads of k and v: 0 or N, or a divisor of N */
+  const void* q;               /* device [B, N, S, D]; packed: [S, N, D] */
+  const void* k;               /* device [B, N_kv, S, D]; packed: [S, N_kv, D] */
+  const void* v;
+  void* y;                     /* like q */
+  int64_t q_stride[3];         /* element strides of batch entry, head and row, multiples of 8; 0 = packed */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t y_stride[3];
+  const float* log_decay;      /* device [N] */
+  const int32_t* cu_seqlens;   /* device [B + 1], ascending from 0 to S, or NULL */
+  const int32_t* seq_lens;     /* device [B], or NULL; not with cu_seqlens */
+  const float* state_in;       /* device [B, N, D, D], the states before the first rows, or NULL: zeros */
+  float* state_out;            /* device [B, N, D, D], the states behind the last rows, or NULL; may be state_in */
+  float scale;
+  void* workspace;             /* device, acct_linear_fwd_workspace_bytes() */
+  size_t workspace_bytes;
+} acct_linear_args;
+
+ACCT_API size_t acct_linear_fwd_workspace_bytes(const acct_linear_args* a);
+ACCT_API int acct_linear_fwd(const acct_linear_args* a, void* stream);
+
+/* Gradients of q, k and v from that of y; not for packed sequences, and no states.  Rows past seq_lens are not written. */
+typedef struct acct_linear_bwd_io {
+  const void* d_y;             /* device, like q */
+  int64_t d_y_stride[3];
+  void* dq;                    /* device [B, N, S, D] packed, in dtype */
+  void* dk;                    /* device [B, N_kv, S, D] packed */
+  void* dv;
+  void* workspace;             /* device, acct_linear_bwd_workspace_bytes() */
+  size_t workspace_bytes;
+} acct_linear_bwd_io;
+
+ACCT_API size_t acct_linear_bwd_workspace_bytes(const acct_linear_args* a);
+ACCT_API int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void* stream);
+
+/* One row per sequence: the state moves on in place, and is read. */
+typedef struct acct_linear_step_args {
+  int32_t dtype;
+  int32_t B, N, D;
+  int32_t N_kv;                /* 0 or N, or a divisor of N */
+  const void* q;               /* device [B, N, D] */
+  const void* k;               /* device [B, N_kv, D] */
+  const void* v;
+  void* y;                     /* device [B, N, D] packed */
+  int64_t q_stride[2];         /* element strides of sequence and head, multiples of 8; 0 = packed */
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  float* state;                /* device [B, N, D, D] packed, read and written */
+  const float* log_decay;      /* device [N] */
+  float scale;
+} acct_linear_step_args;
+
+ACCT_API int acct_linear_step(const acct_linear_step_args* a, void* stream);
+
+/* Rotary positions with several axes; the reference has no counterpart.  Of every row's first `rotated` values each pair (x1, x2) becomes
+ *   y1 = x1 cos(w) - x2 sin(w),   y2 = x2 cos(w) + x1 sin(w),   w = 2 pi turns[i] / 2^64 * position on axis[i]
+ * for pair i: values i and i + rotated / 2, or with `adjacent` 2 i and 2 i + 1.  The values behind them are copied.  Sums are fp32,
+ * angles exact for any position.  An output is its input (in place) or other memory. */
+typedef struct acct_rotary_args {
+  int32_t dtype;               /* ACCT_F16 or ACCT_BF16 */
+  int32_t B, S, D;             /* batch entries, rows, head_dim: a multiple of 8 up to 256 */
+  int32_t N, N_kv;             /* heads of q and k; either may be 0 */
+  int32_t rotated;             /* even, up to D */
+  const void* q;               /* device [B, N, S, D] */
+  const void* k;               /* device [B, N_kv, S, D] */
+  void* q_out;
+  void* k_out;
+  int64_t q_stride[3];         /* element strides of batch entry, head and row, multiples of 8; 0 = packed */
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  const int32_t* positions;    /* device, of every axis, batch entry and row */
+  int64_t pos_stride[3];       /* their element strides, as they are (0: the same for all) */
+  const uint64_t* turns;       /* device [rotated / 2]: turns per position, in units of 2^-64 */
+  const int32_t* axis;         /* device [rotated / 2]: 0 .. axes - 1 */
+  int32_t adjacent;
+  int32_t inverse;             /* turn by -w: the gradient of a turn by w */
+} acct_rotary_args;
+
+ACCT_API int acct_rotary(const acct_rotary_args* a, void* stream);
+
 /* The same operators behind the calling convention MindSpore uses for ops.Custom(func_type="aot"):
  *   int f(int nparam, void** params, int* ndims, int64_t** shapes, const char** dtypes, void* stream, void* extra)
  * with params = the inputs followed by the outputs (device pointers), dtypes as MindSpore names them ("float16",
