@@ -1,69 +1,648 @@
 // Linear attention with a decay for each head, over whole sequences.
 //
-//   S_t = exp(g) S_(t-1) + b_t c_t^T,   y_t = scale S_t^T a_t
+//   S_t = l S_(t-1) + b_t c_t^T,   y_t = scale S_t^T a_t,   l = exp(g)
 //
-// A thread block has 32 columns of one head's state in registers and walks the sequence's tokens: a warp has 4 columns, a lane 1/8 of
-// a column.  16 tokens at a time are staged in shared memory in fp32.
+// in chunks of 128 rows, r and i in a chunk of L rows, S the state before it:
+//
+//   P  = (A B^T) . l^(r - i) for i <= r     tensor cores, weighted in registers, back to tensor memory in 16 bits
+//   y  = scale (P C + l^(r + 1) A S)        two products; their sum, weighted, in fp32
+//   S' = l^L S + B^T (l^(L - 1 - i) C)      the product on tensor cores, the state itself in registers in fp32
+//
+// (reversed: i >= r, l^(i - r), l^(L - r), l^i, chunks from the last to the first).  A thread block has one head of a sequence and 64 columns
+// of C: of two blocks per head at head_dim above 64 each loads A and B and forms P for itself; they run at the same time, so that
+// the second load comes from L2, and P, half of the products at most, costs less than what the blocks would have to wait for each other.
+//
+// Roundings.  P and S are rounded once to the 16 bits that a product takes, like the probabilities of softmax attention; y is rounded
+// once.  The weighted C goes into the state as a sum of 16-bit numbers, so the state keeps fp32: three for bfloat16 (24 bits), two for
+// float16 (22), two for bfloat16 (16) where no state leaves the call and only 16-bit outputs follow from it.  float16 has no range to
+// spare: the rows of P, the weighted C of a chunk and the state are scaled by powers of two that put their largest value near 2^15,
+// and what follows is scaled back in fp32.
+//
+// Warps: 0-3 weight P (thread = row), 4-7 have the state (thread = row of S), 8-11 split the weighted C and write y (thread = row), 12 loads,
+// 13 issues products, 14 stores.  The products of a chunk are issued as B^T C, the next chunk's A B^T, A S, P C: what each needs of the
+// other warps is made while the ones before it run.
 #include "fa_common.cuh"
+#include "fa_kernels.cuh"
 #include "linear.cuh"
+#include "ptx.cuh"
 
 namespace acct {
 namespace {
 
-constexpr int kCols = 32, kStage = 16, kParts = 8, kPer = kLinMaxHeadDim / kParts;
+constexpr int kThreads = 512;
+constexpr int kRegsWork = 152, kRegsControl = 56;      // of 128 a thread at launch: 3 x 128 x 152 + 128 x 56 = 512 x 128
+constexpr int kCols = 64;                              // columns of C, and of S, in a block
+constexpr uint32_t kTileBytes = kLinChunk * 128;       // 128 rows of 64 16-bit values
+constexpr uint32_t kColP = 0, kColIn = 256, kColOut = 320, kColState = 384;      // tensor memory: P (2 x 128), P C, A S, B^T C (2 x 64)
+
+struct Item {
+  int b, h, c0, pass;
+  int row0, rows;           // of the sequence
+  int chunk0, chunks;       // of the segment
+  int slot;                 // of the segment's state; -1: whole sequences
+  int last;                 // nothing behind this segment (in the order of the pass)
+};
 
 template <bool BF16>
-__global__ void __launch_bounds__(kCols * kParts) linear_kernel(const LinParams p) {
-  __shared__ float sa[kStage][kLinMaxHeadDim], sb[kStage][kLinMaxHeadDim], sc[kStage][kCols];
-  const int slices = (p.D + kCols - 1) / kCols, tid = threadIdx.x;
-  int item = blockIdx.x;
-  const LinPass& pass = p.pass[item % p.passes];
-  item /= p.passes;
-  const int e0 = item % slices * kCols, h = item / slices % p.N, b = item / slices / p.N;
-  int row0, n;
-  lin_rows(p, b, row0, n);
-  const int col = tid / kParts, part = tid % kParts, e = e0 + col;
-  const float lambda = static_cast<float>(exp(static_cast<double>(p.log_decay[h])));
-  float s[kPer];
-  for (int i = 0; i < kPer; ++i) {
-    const int d = part + kParts * i;
-    s[i] = p.state_in != nullptr && d < p.D && e < p.D ? p.state_in[((static_cast<int64_t>(b) * p.N + h) * p.D + d) * p.D + e] : 0.f;
-  }
-  const int64_t batch = p.cu != nullptr ? 0 : b;
-  auto at = [&](const LinOperand& o, int row, int d) {
-    return load16<BF16>(o.ptr, batch * o.stride[0] + (h / o.group) * o.stride[1] + row * o.stride[2] + d);
-  };
-  for (int t0 = 0; t0 < n; t0 += kStage) {
-    __syncthreads();
-    for (int i = tid; i < kStage * kLinMaxHeadDim; i += blockDim.x) {
-      const int t = i / kLinMaxHeadDim, d = i % kLinMaxHeadDim, row = row0 + (pass.reverse ? n - 1 - (t0 + t) : t0 + t);
-      const bool there = t0 + t < n && d < p.D;
-      sa[t][d] = there ? at(pass.a, row, d) : 0.f;
-      sb[t][d] = there ? at(pass.b, row, d) : 0.f;
-      if (d < kCols) sc[t][d] = there && e0 + d < p.D ? at(pass.c, row, e0 + d) : 0.f;
-    }
-    __syncthreads();
-    for (int t = 0; t < kStage && t0 + t < n; ++t) {
-      float y = 0.f;
-      for (int i = 0; i < kPer; ++i) {
-        s[i] = fmaf(lambda, s[i], sb[t][part + kParts * i] * sc[t][col]);
-        y = fmaf(sa[t][part + kParts * i], s[i], y);
+struct Shared {
+  uint64_t a_full[2], a_empty[2], b_full[2], b_empty[2], c_full[2], c_empty[2];
+  uint64_t p_full[2], p_ready[2], split_ready, inc_done[2], s_ready, s_read, o_done, o_free, o_staged[2];
+  uint32_t tmem_base;
+  volatile uint32_t abort_flag;
+  Item item;
+  float power[kLinChunk + 1];                                   // l^j
+  float p_back[BF16 ? 1 : 4][BF16 ? 1 : kLinChunk], c_back[4], s_back[4];      // float16: 1 / the scales of a chunk
+  uint32_t most[2][2][4];
+};
+
+// The power of two that brings `most` (>= 0) to [2^14, 2^15), and its inverse; 1 for 0 and what is not finite.
+__device__ __forceinline__ void near_top(float most, float& scale, float& back) {
+  const int e = static_cast<int>(__float_as_uint(most) >> 23);      // 127 + its exponent
+  const bool usable = e > 0 && e < 255;
+  const int up = usable ? min(max(141 - e, -126), 126) : 0;
+  scale = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+  back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint64_t widen(uint32_t w) {      // two 16-bit values
+  if constexpr (BF16) return f2_pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2_pack(f.x, f.y);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t narrow(uint64_t x) {
+  float a, b;
+  f2_unpack(x, a, b);
+  return pack2<BF16>(a, b);
+}
+
+// What the block works on; by one warp.
+__device__ __forceinline__ Item find_item(const LinParams& p) {
+  const int lane = threadIdx.x & 31, slices = (p.D + kCols - 1) / kCols;
+  int at = blockIdx.x;
+  Item x;
+  x.c0 = at % slices * kCols; at /= slices;
+  x.pass = at % p.passes; at /= p.passes;
+  x.h = at % p.N; at /= p.N;
+  x.chunks = 0; x.chunk0 = 0; x.slot = -1; x.last = 1;
+  const bool reverse = p.pass[x.pass].reverse != 0;
+  if (p.seg_chunks == 0) {
+    x.b = at;
+    if (p.cu != nullptr && p.B > 1 && p.B <= 64) {      // the at-th longest: a late start of a long one is what the SMs would wait for
+      int n[2], rank[2] = {0, 0}, row;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        n[i] = -1;
+        if (lane + 32 * i < p.B) lin_rows(p, lane + 32 * i, row, n[i]);
       }
-      for (int d = 1; d < kParts; d <<= 1) y += __shfl_xor_sync(0xffffffffu, y, d);
-      if (part == 0 && e < p.D) {
-        const int row = row0 + (pass.reverse ? n - 1 - (t0 + t) : t0 + t);
-        const int64_t to = batch * pass.y_stride[0] + h * pass.y_stride[1] + row * pass.y_stride[2] + e;
-        if (pass.y_f32) static_cast<float*>(pass.y)[to] = y * p.scale;
-        else if (BF16) static_cast<__nv_bfloat16*>(pass.y)[to] = __float2bfloat16(y * p.scale);
-        else static_cast<__half*>(pass.y)[to] = __float2half(y * p.scale);
+      for (int j = 0; j < p.B; ++j) {
+        const int other = __shfl_sync(0xffffffffu, n[j >> 5], j & 31);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) rank[i] += other > n[i] || (other == n[i] && j < lane + 32 * i);
       }
+      const unsigned int first = __ballot_sync(0xffffffffu, n[0] >= 0 && rank[0] == at), second = __ballot_sync(0xffffffffu, n[1] >= 0 && rank[1] == at);
+      x.b = first != 0u ? __ffs(first) - 1 : 31 + __ffs(second);
+    }
+    lin_rows(p, x.b, x.row0, x.rows);
+    x.chunks = (x.rows + kLinChunk - 1) / kLinChunk;
+    return x;
+  }
+  x.slot = at;
+  x.b = -1;
+  x.row0 = x.rows = 0;
+  int left = at;
+  for (int b0 = 0; b0 < p.B && x.b < 0; b0 += 32) {      // the sequence that has the at-th segment
+    int row = 0, n = 0;
+    if (b0 + lane < p.B) lin_rows(p, b0 + lane, row, n);
+    const int segs = (n + kLinChunk * p.seg_chunks - 1) / (kLinChunk * p.seg_chunks);
+    int upto = segs;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    const unsigned int past = __ballot_sync(0xffffffffu, upto > left);
+    if (past != 0u) {
+      const int from = __ffs(past) - 1;
+      x.b = b0 + from;
+      const int seg = left - __shfl_sync(0xffffffffu, upto - segs, from);
+      x.row0 = __shfl_sync(0xffffffffu, row, from);
+      x.rows = __shfl_sync(0xffffffffu, n, from);
+      const int all = (x.rows + kLinChunk - 1) / kLinChunk;
+      x.chunk0 = seg * p.seg_chunks;
+      x.chunks = min(p.seg_chunks, all - x.chunk0);
+      x.last = reverse ? seg == 0 : x.chunk0 + x.chunks == all;
+    } else {
+      left -= __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  if (p.state_out != nullptr)
-    for (int i = 0; i < kPer; ++i) {
-      const int d = part + kParts * i;
-      if (d < p.D && e < p.D) p.state_out[((static_cast<int64_t>(b) * p.N + h) * p.D + d) * p.D + e] = s[i];
+  return x;
+}
+
+// STATES: only what each segment alone leaves behind.  SPLIT: 16-bit numbers that stand for a weighted value of C.
+template <int DPAD, bool BF16, int SPLIT, bool STATES>
+__global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_constant__ LinParams p) {
+  constexpr int NB = DPAD / 64;                    // 64-column blocks of A and B
+  constexpr uint32_t kStage = (2 * NB + 1) * kTileBytes;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));      // 2 x (A, B, C)
+  uint8_t* sSplit = stages + 2 * kStage;
+  uint8_t* sS = sSplit + SPLIT * kTileBytes;       // DPAD rows of 64 values
+  __shared__ Shared<BF16> sh;
+
+  const int tid = threadIdx.x;
+  const int warp = static_cast<int>(warp_uniform(tid >> 5));
+  if (warp == 0) {
+    const Item x = find_item(p);
+    if (elect_one()) sh.item = x;
+  }
+  if (tid == 12 * 32) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.a_full[i], 1); mbar_init(&sh.a_empty[i], 1);
+      mbar_init(&sh.b_full[i], 1); mbar_init(&sh.b_empty[i], 1);
+      mbar_init(&sh.c_full[i], 1); mbar_init(&sh.c_empty[i], 1);
+      mbar_init(&sh.p_full[i], 1); mbar_init(&sh.p_ready[i], 128);
+      mbar_init(&sh.inc_done[i], 1); mbar_init(&sh.o_staged[i], 128);
     }
+    mbar_init(&sh.split_ready, 128); mbar_init(&sh.s_ready, 128); mbar_init(&sh.s_read, 1);
+    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128);
+    sh.abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 13) { tmem_alloc(&sh.tmem_base, 512); tmem_relinquish(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = warp_uniform(sh.tmem_base);
+  volatile uint32_t* abort_flag = &sh.abort_flag;
+  const Item x = sh.item;
+  const LinPass& pass = p.pass[x.pass];
+  const bool reverse = pass.reverse != 0;
+  // what leaves no trace: a block past the last segment; with STATES the last segment of a sequence whose state nobody asks for
+  const bool idle = x.b < 0 || (STATES && x.last && p.state_out == nullptr);
+  const int n = idle ? 0 : x.chunks;
+  const int batch = p.cu != nullptr ? 0 : x.b;
+  // the c-th chunk in the order of the pass: its first row, and how many
+  auto first_row = [&](int c) { return (x.chunk0 + (reverse ? n - 1 - c : c)) * kLinChunk; };
+  auto rows_of = [&](int c) { return min(kLinChunk, x.rows - first_row(c)); };
+  if (tid < kLinChunk + 1 && !idle) {
+    const LinPower w = lin_power(p.log_decay[x.h], tid);
+    sh.power[tid] = w.hi + w.lo;
+  }
+  __syncthreads();
+
+  if (warp == 12) {
+    // ------------------------------------------------------------------ loads
+    reg_dealloc<kRegsControl>();
+    if (elect_one()) {
+      const int ha = x.h / pass.a.group, hb = x.h / pass.b.group, hc = x.h / pass.c.group;
+      for (int c = 0; c < n; ++c) {
+        const int s = c & 1, before = ((c >> 1) - 1) & 1, row = x.row0 + first_row(c);
+        uint8_t *sA = stages + s * kStage, *sB = sA + NB * kTileBytes, *sC = sB + NB * kTileBytes;
+        if (c >= 2) mbar_wait(&sh.b_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        mbar_expect_tx(&sh.b_full[s], NB * kTileBytes);
+        for (int nb = 0; nb < NB; ++nb) tma_load_4d(sB + nb * kTileBytes, &pass.b.map, &sh.b_full[s], nb * 64, row, hb, batch);
+        if (c >= 2) mbar_wait(&sh.c_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        mbar_expect_tx(&sh.c_full[s], kTileBytes);
+        tma_load_4d(sC, &pass.c.map, &sh.c_full[s], x.c0, row, hc, batch);
+        if constexpr (!STATES) {
+          if (c >= 2) mbar_wait(&sh.a_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+          mbar_expect_tx(&sh.a_full[s], NB * kTileBytes);
+          for (int nb = 0; nb < NB; ++nb) tma_load_4d(sA + nb * kTileBytes, &pass.a.map, &sh.a_full[s], nb * 64, row, ha, batch);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 13) {
+    // ------------------------------------------------------------------ products
+    reg_dealloc<kRegsControl>();
+    const uint32_t idesc_p = make_idesc(BF16, 128, 128, false, false), idesc_in = make_idesc(BF16, 128, kCols, false, true);
+    const uint32_t idesc_s = make_idesc(BF16, 128, kCols, true, true);
+    const uint64_t kmajor = make_sdesc_base(16, 1024), mnmajor = make_sdesc_base(kTileBytes, 1024);
+    const uint32_t k_hi = static_cast<uint32_t>(kmajor >> 32), mn_hi = static_cast<uint32_t>(mnmajor >> 32);
+    auto at = [](uint64_t base, const uint8_t* t) { return static_cast<uint32_t>(base) | ((smem_u32(t) >> 4) & 0x3fffu); };
+    const uint32_t a_lo = at(kmajor, stages), b_lo = at(kmajor, stages + NB * kTileBytes);
+    const uint32_t bt_lo = at(mnmajor, stages + NB * kTileBytes), c_lo = at(mnmajor, stages + 2 * NB * kTileBytes);
+    const uint32_t split_lo = at(mnmajor, sSplit), s_lo = at(mnmajor, sS);
+    const int k_steps = (p.D + 15) / 16;
+    auto issue_p = [&](int c) {
+      const uint32_t off = (c & 1) * (kStage >> 4);
+      mbar_wait(&sh.a_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      mbar_wait(&sh.b_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      if (elect_one()) {
+        for (int kk = 0; kk < k_steps; ++kk) {
+          const uint32_t o = off + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u;
+          umma_ss_lohi(tmem + kColP + (c & 1) * 128, a_lo + o, k_hi, b_lo + o, k_hi, idesc_p, kk > 0);
+        }
+        umma_commit(&sh.p_full[c & 1]);
+      }
+      __syncwarp();
+    };
+    if (!STATES && n > 0) issue_p(0);
+    for (int c = 0; c < n; ++c) {
+      const uint32_t off = (c & 1) * (kStage >> 4);
+      if constexpr (STATES) {      // the warps of the state have read the product before
+        mbar_wait(&sh.s_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        mbar_wait(&sh.b_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      }
+      mbar_wait(&sh.split_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+      tc_fence_after_sync();
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < SPLIT; ++i)
+#pragma unroll
+          for (int kk = 0; kk < kLinChunk / 16; ++kk)
+            umma_ss_lohi(tmem + kColState + (c & 1) * kCols, bt_lo + off + kk * 128u, mn_hi, split_lo + i * (kTileBytes >> 4) + kk * 128u, mn_hi,
+                         idesc_s, i > 0 || kk > 0);
+        umma_commit(&sh.inc_done[c & 1]);
+        umma_commit(&sh.b_empty[c & 1]);
+        if constexpr (STATES) umma_commit(&sh.c_empty[c & 1]);
+      }
+      __syncwarp();
+      if constexpr (!STATES) {
+        if (c + 1 < n) issue_p(c + 1);      // (the P that it goes over has been consumed: products run in the order of their issue)
+        mbar_wait(&sh.s_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        if (c > 0) mbar_wait(&sh.o_free, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        tc_fence_after_sync();
+        if (elect_one()) {
+          for (int kk = 0; kk < k_steps; ++kk)
+            umma_ss_lohi(tmem + kColOut, a_lo + off + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u, k_hi, s_lo + kk * 128u, mn_hi, idesc_in, kk > 0);
+          umma_commit(&sh.s_read);
+        }
+        __syncwarp();
+        mbar_wait(&sh.p_ready[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kLinChunk / 16; ++kk)
+            umma_ts_lohi(tmem + kColIn, tmem + kColP + (c & 1) * 128 + kk * 8, c_lo + off + kk * 128u, mn_hi, idesc_in, kk > 0);
+          umma_commit(&sh.o_done);
+          umma_commit(&sh.c_empty[c & 1]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 14) {
+    // ------------------------------------------------------------------ stores of whole chunks
+    reg_dealloc<kRegsControl>();
+    if constexpr (!STATES) {
+      for (int c = 0; c < n; ++c) {
+        mbar_wait(&sh.o_staged[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        if (elect_one()) {
+          if (rows_of(c) == kLinChunk && !pass.y_f32) {
+            tma_store_4d(&pass.map_y, stages + (c & 1) * kStage, x.c0, x.row0 + first_row(c), x.h, batch);
+            tma_store_commit();
+            tma_store_wait_read();
+          }
+          mbar_arrive(&sh.a_empty[c & 1]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ weights of P
+    reg_alloc<kRegsWork>();
+    if constexpr (!STATES) {
+      const int lane = tid & 31;
+      const uint32_t t_p = tmem + kColP + (static_cast<uint32_t>(warp * 32) << 16);
+      // A column block of 32 is 32 (warp - block) + lane - j before the row: on the diagonal its weights are the same for all warps;
+      // elsewhere the power is one of the row and the block times one of the column, both <= 1.
+      uint64_t diagonal[16], column[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float d[2], w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int apart = reverse ? 2 * j + u - lane : lane - 2 * j - u;
+          d[u] = apart >= 0 ? sh.power[max(apart, 0)] : 0.f;
+          w[u] = sh.power[reverse ? 2 * j + u : 31 - 2 * j - u];
+        }
+        diagonal[j] = f2_pack(d[0], d[1]);
+        column[j] = f2_pack(w[0], w[1]);
+      }
+      for (int c = 0; c < n; ++c) {
+        const int rows = rows_of(c);
+        const uint32_t t = t_p + (c & 1) * 128;
+        mbar_wait(&sh.p_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+        tc_fence_after_sync();
+        // one block of 32 columns, weighted
+        auto weighted = [&](int block, uint64_t (&v)[16]) {
+          uint32_t r[32];
+          tmem_ld32(t + block * 32, r);
+          tmem_wait_ld();
+          if (block == warp) {      // (by a choice, not by a weight of 0: what is not finite stays out)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const bool in0 = reverse ? 2 * j >= lane : 2 * j <= lane, in1 = reverse ? 2 * j + 1 >= lane : 2 * j + 1 <= lane;
+              v[j] = f2_mul(f2_pack(in0 ? __uint_as_float(r[2 * j]) : 0.f, in1 ? __uint_as_float(r[2 * j + 1]) : 0.f), diagonal[j]);
+            }
+          } else {
+            const float w = sh.power[reverse ? 32 * (block - warp) - lane : 32 * (warp - block) + lane - 31];
+            const uint64_t w2 = f2_pack(w, w);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = f2_mul(f2_mul(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), column[j]), w2);
+          }
+          const int left = rows - block * 32;
+          if (left < 32) {      // columns behind the last row
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float a, b;
+              f2_unpack(v[j], a, b);
+              v[j] = f2_pack(2 * j < left ? a : 0.f, 2 * j + 1 < left ? b : 0.f);
+            }
+          }
+        };
+        uint64_t scale2 = 0;
+        if constexpr (!BF16) {
+          float most = 0.f;
+#pragma unroll 1
+          for (int block = reverse ? warp : 0; block <= (reverse ? 3 : warp); ++block) {
+            uint64_t v[16];
+            weighted(block, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float a, b;
+              f2_unpack(v[j], a, b);
+              most = fmax3(most, fabsf(a), fabsf(b));
+            }
+          }
+          float scale, back;
+          near_top(most, scale, back);
+          scale2 = f2_pack(scale, scale);
+          sh.p_back[c & 3][tid] = back;
+        }
+#pragma unroll 1
+        for (int block = 0; block < 4; ++block) {
+          uint32_t pk[16];
+          if (reverse ? block >= warp : block <= warp) {
+            uint64_t v[16];
+            weighted(block, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) pk[j] = narrow<BF16>(BF16 ? v[j] : f2_mul(v[j], scale2));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) pk[j] = 0u;
+          }
+          tmem_st16(t + block * 16, pk);      // (over scores that have been read, or that nobody needs)
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive(&sh.p_ready[c & 1]);
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ the state
+    reg_alloc<kRegsWork>();
+    const int d = tid - 128, lane = tid & 31;
+    const uint32_t t_s = tmem + kColState + (static_cast<uint32_t>((warp - 4) * 32) << 16);
+    const LinPower step = idle ? LinPower{1.f, 0.f} : lin_power(p.log_decay[x.h], kLinChunk);
+    const int width = min(kCols, p.D - x.c0);      // columns that exist
+    const int64_t one = (static_cast<int64_t>(x.b) * p.N + x.h) * p.D * p.D, row = static_cast<int64_t>(d) * p.D + x.c0;
+    const int64_t slot = ((static_cast<int64_t>(x.slot) * p.passes + x.pass) * p.N + x.h) * p.D * p.D;
+    const float* from = STATES || idle ? nullptr : x.slot >= 0 ? p.seg_states + slot : p.state_in != nullptr ? p.state_in + one : nullptr;
+    float* to = idle ? nullptr : STATES ? p.seg_states + slot : x.slot < 0 && p.state_out != nullptr ? p.state_out + one : nullptr;
+    uint64_t s[kCols / 2];
+#pragma unroll
+    for (int j = 0; j < kCols / 4; ++j) {
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (from != nullptr && d < p.D && 4 * j < width) f = *reinterpret_cast<const float4*>(from + row + 4 * j);
+      s[2 * j] = f2_pack(f.x, f.y);
+      s[2 * j + 1] = f2_pack(f.z, f.w);
+    }
+    // the state before chunk c, to shared memory in 16 bits
+    auto publish = [&](int c) {
+      if constexpr (!STATES) {
+        uint64_t scale2 = 0;
+        if constexpr (!BF16) {
+          float most = 0.f;
+#pragma unroll
+          for (int j = 0; j < kCols / 2; ++j) {
+            float a, b;
+            f2_unpack(s[j], a, b);
+            most = fmax3(most, fabsf(a), fabsf(b));
+          }
+          const uint32_t of_warp = __reduce_max_sync(0xffffffffu, DPAD == 128 || warp < 6 ? __float_as_uint(most) : 0u);
+          if (lane == 0) sh.most[0][c & 1][warp - 4] = of_warp;
+          named_barrier(1, 128);
+          const float of_all = __uint_as_float(max(max(sh.most[0][c & 1][0], sh.most[0][c & 1][1]), max(sh.most[0][c & 1][2], sh.most[0][c & 1][3])));
+          float scale, back;
+          near_top(of_all, scale, back);
+          scale2 = f2_pack(scale, scale);
+          if (d == 0) sh.s_back[c & 3] = back;
+        }
+        if (c > 0) mbar_wait(&sh.s_read, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+        if (d < DPAD) {
+#pragma unroll
+          for (int j = 0; j < kCols / 8; ++j) {
+            uint32_t pk[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) pk[u] = narrow<BF16>(BF16 ? s[4 * j + u] : f2_mul(s[4 * j + u], scale2));
+            *reinterpret_cast<uint4*>(sS + swz128(d, j)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      mbar_arrive(&sh.s_ready);
+    };
+    if (n > 0) publish(0);
+    for (int c = 0; c < n; ++c) {
+      const int rows = rows_of(c);
+      const LinPower w = rows == kLinChunk ? step : lin_power(p.log_decay[x.h], rows);
+      const uint64_t hi2 = f2_pack(w.hi, w.hi), lo2 = f2_pack(w.lo, w.lo);
+      mbar_wait(&sh.inc_done[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      tc_fence_after_sync();
+      uint64_t back2 = 0;
+      if constexpr (!BF16) back2 = f2_pack(sh.c_back[c & 3], sh.c_back[c & 3]);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t r[32];
+        tmem_ld32(t_s + (c & 1) * kCols + half * 32, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          uint64_t inc = f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+          if constexpr (!BF16) inc = f2_mul(inc, back2);
+          uint64_t& v = s[half * 16 + j];
+          v = f2_fma(v, hi2, f2_fma(v, lo2, inc));
+        }
+      }
+      tc_fence_before_sync();
+      if (c + 1 < n) publish(c + 1);
+    }
+    if (to != nullptr && d < p.D) {
+#pragma unroll
+      for (int j = 0; j < kCols / 4; ++j) {
+        float4 f;
+        f2_unpack(s[2 * j], f.x, f.y);
+        f2_unpack(s[2 * j + 1], f.z, f.w);
+        if (4 * j < width) *reinterpret_cast<float4*>(to + row + 4 * j) = f;
+      }
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ weighted C, and y
+    reg_alloc<kRegsWork>();
+    const int row = tid - 256;
+    const uint32_t lanes = static_cast<uint32_t>((warp - 8) * 32) << 16;
+    auto split = [&](int c) {
+      const int rows = rows_of(c), st = c & 1;
+      uint8_t *sB = stages + st * kStage + NB * kTileBytes, *sC = sB + NB * kTileBytes;
+      mbar_wait(&sh.c_full[st], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      const bool there = row < rows;
+      uint4 raw[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) raw[j] = there ? *reinterpret_cast<const uint4*>(sC + swz128(row, j)) : make_uint4(0u, 0u, 0u, 0u);
+      float w = there ? sh.power[reverse ? row : rows - 1 - row] : 0.f;
+      if constexpr (!BF16) {
+        uint32_t most = 0;      // of the absolute values, as 16-bit patterns, which have their order
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t v[4] = {raw[j].x & 0x7fff7fffu, raw[j].y & 0x7fff7fffu, raw[j].z & 0x7fff7fffu, raw[j].w & 0x7fff7fffu};
+          most = __vmaxu2(most, __vmaxu2(__vmaxu2(v[0], v[1]), __vmaxu2(v[2], v[3])));
+        }
+        // times this row's weight
+        const float of_row = __half2float(__ushort_as_half(static_cast<unsigned short>(max(most >> 16, most & 0xffffu)))) * w;
+        const uint32_t of_warp = __reduce_max_sync(0xffffffffu, __float_as_uint(of_row));
+        if ((tid & 31) == 0) sh.most[1][c & 1][warp - 8] = of_warp;
+        named_barrier(2, 128);
+        const float of_all = __uint_as_float(max(max(sh.most[1][c & 1][0], sh.most[1][c & 1][1]), max(sh.most[1][c & 1][2], sh.most[1][c & 1][3])));
+        float scale, back;
+        near_top(of_all, scale, back);
+        w *= scale;
+        if (row == 0) sh.c_back[c & 3] = back;
+      }
+      const uint64_t w2 = f2_pack(w, w);
+      if (c > 0) mbar_wait(&sh.inc_done[(c - 1) & 1], ((c - 1) >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t in[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+        uint32_t out[SPLIT][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint64_t v = f2_mul(widen<BF16>(in[u]), w2);
+#pragma unroll
+          for (int i = 0; i < SPLIT; ++i) {
+            out[i][u] = narrow<BF16>(v);
+            if (i + 1 < SPLIT) {
+              const uint64_t part = widen<BF16>(out[i][u] ^ 0x80008000u);      // minus
+              v = f2_add(v, part);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < SPLIT; ++i)
+          *reinterpret_cast<uint4*>(sSplit + i * kTileBytes + swz128(row, j)) = make_uint4(out[i][0], out[i][1], out[i][2], out[i][3]);
+      }
+      if (rows < kLinChunk) {      // rows that are not this sequence's: 0 times what they hold might be a NaN
+        mbar_wait(&sh.b_full[st], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+        if (!there) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            for (int nb = 0; nb < NB; ++nb) *reinterpret_cast<uint4*>(sB + nb * kTileBytes + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(sC + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sh.split_ready);
+    };
+    auto write_y = [&](int c) {
+      const int rows = rows_of(c);
+      float w = p.scale * sh.power[reverse ? max(rows - row, 0) : row + 1], in = p.scale;
+      mbar_wait(&sh.o_done, c & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      tc_fence_after_sync();
+      if constexpr (!BF16) {
+        w *= sh.s_back[c & 3];
+        in *= sh.p_back[c & 3][row];
+      }
+      const uint64_t w2 = f2_pack(w, w), in2 = f2_pack(in, in);
+      const bool direct = rows < kLinChunk || pass.y_f32;
+      const int64_t at = batch * pass.y_stride[0] + x.h * pass.y_stride[1] + (x.row0 + first_row(c) + row) * pass.y_stride[2] + x.c0;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t r[32], q[32];
+        tmem_ld32(tmem + lanes + kColIn + half * 32, r);
+        tmem_ld32(tmem + lanes + kColOut + half * 32, q);
+        tmem_wait_ld();
+        if (half == 1) {
+          tc_fence_before_sync();
+          mbar_arrive(&sh.o_free);
+        }
+        uint64_t v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          v[j] = f2_fma(f2_pack(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), w2,
+                        f2_mul(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), in2));
+        if (pass.y_f32) {
+          float* out = static_cast<float*>(pass.y) + at + half * 32;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float4 f;
+            f2_unpack(v[2 * j], f.x, f.y);
+            f2_unpack(v[2 * j + 1], f.z, f.w);
+            if (row < rows && x.c0 + half * 32 + 4 * j < p.D) *reinterpret_cast<float4*>(out + 4 * j) = f;
+          }
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 u = make_uint4(narrow<BF16>(v[4 * j]), narrow<BF16>(v[4 * j + 1]), narrow<BF16>(v[4 * j + 2]), narrow<BF16>(v[4 * j + 3]));
+          if (!direct) *reinterpret_cast<uint4*>(stages + (c & 1) * kStage + swz128(row, half * 4 + j)) = u;      // (A is not needed any more)
+          else if (row < rows && x.c0 + half * 32 + 8 * j < p.D) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(pass.y) + at + half * 32 + 8 * j) = u;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sh.o_staged[c & 1]);
+    };
+    for (int c = 0; c <= n; ++c) {
+      if (c < n) split(c);
+      if (!STATES && c > 0) write_y(c - 1);
+    }
+  } else {
+    reg_dealloc<kRegsControl>();
+  }
+
+  tc_fence_before_sync();
+  linger_after_abort(abort_flag);
+  __syncthreads();
+  if (warp == 13) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// What the segments leave, one by one, to the states before them, and the state behind the last; a thread has 4 neighbouring elements.
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinParams p) {
+  const int quads = p.D * p.D / 4, i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y % p.N, pass = blockIdx.y / p.N % p.passes, b = blockIdx.y / p.N / p.passes;
+  int slot0 = 0, row0, rows;
+  const int per = kLinChunk * p.seg_chunks;
+  for (int j = threadIdx.x & 31; j < b; j += 32) {
+    lin_rows(p, j, row0, rows);
+    slot0 += (rows + per - 1) / per;
+  }
+  slot0 = __reduce_add_sync(0xffffffffu, slot0);
+  if (i >= quads) return;
+  lin_rows(p, b, row0, rows);
+  const int segs = (rows + per - 1) / per;
+  const bool reverse = p.pass[pass].reverse != 0;
+  const float g = p.log_decay[h];
+  const int64_t one = (static_cast<int64_t>(b) * p.N + h) * quads + i, stride = static_cast<int64_t>(p.passes) * p.N * quads;
+  float4* slots = reinterpret_cast<float4*>(p.seg_states) + slot0 * stride + (static_cast<int64_t>(pass) * p.N + h) * quads + i;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.state_in != nullptr) s = reinterpret_cast<const float4*>(p.state_in)[one];
+  const LinPower whole = lin_power(g, per);
+  for (int at = 0; at < segs; ++at) {
+    const int seg = reverse ? segs - 1 - at : at;
+    const LinPower w = seg + 1 < segs ? whole : lin_power(g, rows - seg * per);
+    const bool last = at + 1 == segs;
+    float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!last || p.state_out != nullptr) add = slots[seg * stride];      // (the last one's is not there otherwise)
+    slots[seg * stride] = s;
+    s.x = fmaf(s.x, w.hi, fmaf(s.x, w.lo, add.x)); s.y = fmaf(s.y, w.hi, fmaf(s.y, w.lo, add.y));
+    s.z = fmaf(s.z, w.hi, fmaf(s.z, w.lo, add.z)); s.w = fmaf(s.w, w.hi, fmaf(s.w, w.lo, add.w));
+  }
+  if (p.state_out != nullptr) reinterpret_cast<float4*>(p.state_out)[one] = s;
 }
 
 // a thread: 4 neighbouring values
@@ -75,22 +654,47 @@ __global__ void __launch_bounds__(256) linear_reduce_kernel(const LinReduce p) {
   const int d = static_cast<int>(i % quads) * 4, s = static_cast<int>(i / quads % p.S);
   const int h = static_cast<int>(i / quads / p.S % p.N_kv), b = static_cast<int>(i / quads / p.S / p.N_kv);
   if (p.lens != nullptr && s >= p.lens[b]) return;
-  const float* from = p.parts[which] + ((static_cast<int64_t>(b) * p.N_kv + h) * p.group * p.S + s) * p.D + d;
+  const float* from = (which ? p.parts[1] : p.parts[0]) + ((static_cast<int64_t>(b) * p.N_kv + h) * p.group * p.S + s) * p.D + d;
   float4 sum = *reinterpret_cast<const float4*>(from);
   for (int g = 1; g < p.group; ++g) {
     const float4 x = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(g) * p.S * p.D);
     sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
   }
-  uint16_t* to = static_cast<uint16_t*>(p.out[which]) + b * p.out_stride[which][0] + h * p.out_stride[which][1] + s * p.out_stride[which][2] + d;
+  uint16_t* to = static_cast<uint16_t*>(which ? p.out[1] : p.out[0]) + b * p.out_stride[0] + h * p.out_stride[1] + s * p.out_stride[2] + d;
   *reinterpret_cast<uint2*>(to) = make_uint2(pack2<BF16>(sum.x, sum.y), pack2<BF16>(sum.z, sum.w));
+}
+
+template <int DPAD, bool BF16, int SPLIT, bool STATES>
+cudaError_t launch(const LinParams& p, unsigned int blocks, cudaStream_t stream) {
+  const size_t smem = (2 * (2 * DPAD / 64 + 1) + SPLIT) * static_cast<size_t>(kTileBytes) + DPAD * 128 + 1024;
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(linear_kernel<DPAD, BF16, SPLIT, STATES>), smem);
+  if (e != cudaSuccess) return e;
+  linear_kernel<DPAD, BF16, SPLIT, STATES><<<blocks, kThreads, smem, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <int DPAD, bool BF16, int SPLIT>
+cudaError_t launch_all(const LinParams& p, cudaStream_t stream) {
+  const int slices = (p.D + kCols - 1) / kCols;
+  const unsigned int per = static_cast<unsigned int>(p.passes) * slices * p.N;
+  if (p.seg_chunks == 0) return launch<DPAD, BF16, SPLIT, false>(p, per * p.B, stream);
+  cudaError_t e = launch<DPAD, BF16, SPLIT, true>(p, per * p.seg_slots, stream);
+  if (e != cudaSuccess) return e;
+  linear_join_kernel<<<dim3((p.D * p.D / 4 + 255) / 256, p.N * p.passes * p.B), 256, 0, stream>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return launch<DPAD, BF16, SPLIT, false>(p, per * p.seg_slots, stream);
 }
 
 }  // namespace
 
+void linear_segments(LinParams& p, int sm_count) {
+  p.seg_chunks = p.seg_slots = 0;
+}
+
 cudaError_t launch_linear(const LinParams& p, bool bf16, cudaStream_t stream) {
-  const unsigned int blocks = static_cast<unsigned int>(p.passes) * ((p.D + kCols - 1) / kCols) * p.N * p.B;
-  (bf16 ? linear_kernel<true> : linear_kernel<false>)<<<blocks, kCols * kParts, 0, stream>>>(p);
-  return cudaGetLastError();
+  const bool exact = p.state_out != nullptr;
+  if (p.D <= 64) return !bf16 ? launch_all<64, false, 2>(p, stream) : exact ? launch_all<64, true, 3>(p, stream) : launch_all<64, true, 2>(p, stream);
+  return !bf16 ? launch_all<128, false, 2>(p, stream) : exact ? launch_all<128, true, 3>(p, stream) : launch_all<128, true, 2>(p, stream);
 }
 
 cudaError_t launch_linear_reduce(const LinReduce& p, bool bf16, cudaStream_t stream) {

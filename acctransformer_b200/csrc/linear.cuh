@@ -9,10 +9,10 @@ namespace acct {
 constexpr int kLinMaxHeadDim = 128;
 constexpr int kLinChunk = 128;      // rows that the products of one chunk take
 
-// One operand of a pass: element strides of batch entry, head and row; head h of the pass reads head h / group.
+// One operand of a pass: its map (column, row, head, batch entry), boxes of 64 columns and kLinChunk rows; head h of the pass reads head
+// h / group.
 struct LinOperand {
-  const void* ptr;
-  int64_t stride[3];
+  CUtensorMap map;
   int group;
 };
 
@@ -20,13 +20,14 @@ struct LinOperand {
 // (dy, v, k), dk (v, dy, q) reversed and dv (k, q, dy) reversed: one computation serves all four.
 struct LinPass {
   LinOperand a, b, c;
+  CUtensorMap map_y;                // (unused where y is fp32)
   void* y;
-  int64_t y_stride[3];
+  int64_t y_stride[3];              // of batch entry, head and row
   int y_f32;                        // y is fp32 (partial gradients of shared heads)
   int reverse;
 };
 
-struct LinParams {
+struct alignas(64) LinParams {
   LinPass pass[3];
   int passes;
   int B, N, S, D;                   // S: rows of an operand (all sequences' together, where they are packed)
@@ -37,7 +38,28 @@ struct LinParams {
   float* state_out;                 // may be state_in
   float scale;
   unsigned int* status;
+  // Sequences cut into segments of so many chunks; 0: whole.  The slots hold a state for each pass, segment and head, [slots, passes, N, D, D]:
+  // first what a segment alone leaves, then what is before it.
+  int seg_chunks, seg_slots;
+  float* seg_states;
 };
+
+// exp(g n) as the sum of two numbers.  Where it is near 1 it multiplies the same state over and over, and an error of a rounding each time
+// would add up: there expm1 has the distance to 1, of which the leading number takes what it can.
+struct LinPower {
+  float hi, lo;
+};
+__device__ __forceinline__ LinPower lin_power(float g, int n) {
+  if (n == 0) return {1.f, 0.f};
+  const float m = static_cast<float>(n), x = g * m;
+  const float rest = x == -INFINITY ? 0.f : fmaf(g, m, -x);
+  if (x < -0.5f) {
+    const float e = expf(x);
+    return {fmaf(e, rest, e), 0.f};
+  }
+  const float e = expm1f(x), d = fmaf(1.f + e, rest, e), hi = 1.f + d;
+  return {hi, d - (hi - 1.f)};
+}
 
 // rows of sequence b: the first, and how many; whatever cu and lens hold, no row outside [0, S) is touched
 __device__ __forceinline__ void lin_rows(const LinParams& p, int b, int& row0, int& n) {
@@ -50,13 +72,18 @@ __device__ __forceinline__ void lin_rows(const LinParams& p, int b, int& row0, i
   }
 }
 
+// How long sequences are cut (LinParams::seg_chunks and seg_slots; 0: not at all) where there are too few heads for the SMs.
+void linear_segments(LinParams& p, int sm_count);
+inline size_t linear_segment_bytes(const LinParams& p) {
+  return static_cast<size_t>(p.seg_slots) * p.passes * p.N * p.D * p.D * 4;
+}
 cudaError_t launch_linear(const LinParams& p, bool bf16, cudaStream_t stream);
 
 // out[b, h, s, :] = the sum over the `group` heads of parts[b, h * group + i, s, :] in their order, rounded once
 struct LinReduce {
   const float* parts[2];            // fp32 [B, N_kv * group, S, D] packed
   void* out[2];
-  int64_t out_stride[2][3];
+  int64_t out_stride[3];
   const int* lens;
   int B, N_kv, group, S, D;
 };

@@ -28,7 +28,15 @@ int strides_of(const char* name, const int64_t (&given)[3], const acct_linear_ar
   return 0;
 }
 
-int check_linear(const acct_linear_args* a, LinParams* p, LinOperand* q, LinOperand* k, LinOperand* v) {
+// One [B, heads, S, D] operand, for the tensor maps and for plain addresses.
+struct Rows {
+  const char* name;
+  const void* ptr;
+  int heads;
+  int64_t stride[3];
+};
+
+int check_linear(const acct_linear_args* a, LinParams* p, Rows* q, Rows* k, Rows* v) {
   if (a == nullptr) return fail(ACCT_ERR_NULL, "args is NULL");
   if (a->dtype != ACCT_F16 && a->dtype != ACCT_BF16) return fail(ACCT_ERR_DTYPE, "dtype must be ACCT_F16 or ACCT_BF16");
   if (a->B <= 0 || a->N <= 0) return fail(ACCT_ERR_SHAPE, "B, N must be positive");
@@ -42,10 +50,10 @@ int check_linear(const acct_linear_args* a, LinParams* p, LinOperand* q, LinOper
   if (a->S > 0 && (!a->q || !a->k || !a->v)) return fail(ACCT_ERR_NULL, "q, k, v must be non-NULL");
   if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v)) return fail(ACCT_ERR_ALIGN, "q, k, v must be 16-byte aligned");
   if (!(a->scale > -1e30f) || !(a->scale < 1e30f)) return fail(ACCT_ERR_SHAPE, "scale must be a finite number");
-  const int n_kv = a->N_kv > 0 ? a->N_kv : a->N, group = a->N / n_kv;
-  *q = {a->q, {0, 0, 0}, 1};
-  *k = {a->k, {0, 0, 0}, group};
-  *v = {a->v, {0, 0, 0}, group};
+  const int n_kv = a->N_kv > 0 ? a->N_kv : a->N;
+  *q = {"q", a->q, a->N, {0, 0, 0}};
+  *k = {"k", a->k, n_kv, {0, 0, 0}};
+  *v = {"v", a->v, n_kv, {0, 0, 0}};
   if ((rc = strides_of("q", a->q_stride, a, a->N, q->stride)) || (rc = strides_of("k", a->k_stride, a, n_kv, k->stride)) ||
       (rc = strides_of("v", a->v_stride, a, n_kv, v->stride)))
     return rc;
@@ -58,7 +66,64 @@ int check_linear(const acct_linear_args* a, LinParams* p, LinOperand* q, LinOper
   return 0;
 }
 
-size_t partial_bytes(const acct_linear_args* a) { return static_cast<size_t>(a->B) * a->N * a->S * a->D * 4; }
+int make_map(const acct_linear_args* a, const Rows& x, CUtensorMap* map) {
+  TensorDesc4 t;
+  t.ptr = x.ptr;
+  t.dtype = a->dtype;
+  t.dims[0] = a->D; t.dims[1] = a->S; t.dims[2] = x.heads; t.dims[3] = a->cu_seqlens != nullptr ? 1 : a->B;
+  t.strides[0] = x.stride[2]; t.strides[1] = x.stride[1]; t.strides[2] = x.stride[0];
+  return make_tmap_4d(map, t, kLinChunk);
+}
+
+int make_pass(const acct_linear_args* a, const Rows& x, const Rows& y, const Rows& z, LinPass* pass) {
+  const Rows* from[3] = {&x, &y, &z};
+  LinOperand* to[3] = {&pass->a, &pass->b, &pass->c};
+  for (int i = 0; i < 3; ++i) {
+    to[i]->group = a->N / from[i]->heads;
+    if (const int rc = make_map(a, *from[i], &to[i]->map)) return rc;
+  }
+  return 0;
+}
+int make_output(const acct_linear_args* a, const Rows& y, LinPass* pass) {
+  pass->y = const_cast<void*>(y.ptr);
+  for (int i = 0; i < 3; ++i) pass->y_stride[i] = y.stride[i];
+  return make_map(a, y, &pass->map_y);
+}
+
+// fp32 parts of dk and dv by query head, where heads share their keys and values
+size_t partial_bytes(const acct_linear_args* a) {
+  return a->N_kv > 0 && a->N_kv != a->N ? static_cast<size_t>(2) * a->B * a->N * a->S * a->D * 4 : 0;
+}
+
+// Bytes of the segments' states of a call, and (in `p`, unless it is null) how its sequences are cut.  (By the arguments alone: what a
+// workspace was sized for is what a call does.)
+constexpr int kSms = 148;
+size_t segments_of(const acct_linear_args* a, int passes, LinParams* p) {
+  if (a == nullptr || a->B <= 0 || a->N <= 0 || a->S <= 0 || a->D <= 0) return 0;
+  LinParams own;
+  if (p == nullptr) p = &own;
+  p->B = a->B; p->N = a->N; p->S = a->S; p->D = a->D;
+  p->cu = a->cu_seqlens;
+  p->passes = passes;
+  linear_segments(*p, kSms);
+  return (linear_segment_bytes(*p) + 15) / 16 * 16;
+}
+
+int check_workspace(size_t need, const void* workspace, size_t bytes) {
+  if (need > 0 && (workspace == nullptr || bytes < need)) return fail(ACCT_ERR_WORKSPACE, "workspace of %zu bytes is too small: %zu are needed", bytes, need);
+  if (need > 0 && misaligned(workspace)) return fail(ACCT_ERR_ALIGN, "workspace must be 16-byte aligned");
+  return 0;
+}
+
+// no rows at all: the states stay as they are
+int copy_states(const acct_linear_args* a, void* stream) {
+  if (a->state_out == nullptr || a->state_out == a->state_in) return ACCT_OK;
+  const size_t bytes = static_cast<size_t>(a->B) * a->N * a->D * a->D * 4;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = a->state_in != nullptr ? cudaMemcpyAsync(a->state_out, a->state_in, bytes, cudaMemcpyDeviceToDevice, s)
+                                               : cudaMemsetAsync(a->state_out, 0, bytes, s);
+  return e == cudaSuccess ? ACCT_OK : fail_cuda(e, "copying the states");
+}
 
 }  // namespace
 }  // namespace acct
@@ -67,25 +132,26 @@ using namespace acct;
 
 extern "C" {
 
-size_t acct_linear_fwd_workspace_bytes(const acct_linear_args*) { return 0; }
+size_t acct_linear_fwd_workspace_bytes(const acct_linear_args* a) { return segments_of(a, 1, nullptr); }
 
 int acct_linear_fwd(const acct_linear_args* a, void* stream) {
   LinParams p;
-  LinOperand q, k, v;
+  Rows q, k, v, y;
   int rc = check_linear(a, &p, &q, &k, &v);
   if (rc) return rc;
   if (a->S > 0 && !a->y) return fail(ACCT_ERR_NULL, "y must be non-NULL");
   if (misaligned(a->y) || misaligned(a->state_in) || misaligned(a->state_out)) return fail(ACCT_ERR_ALIGN, "y and the states must be 16-byte aligned");
-  LinPass& pass = p.pass[0];
-  pass.a = q; pass.b = k; pass.c = v;
-  pass.y = a->y;
-  if ((rc = strides_of("y", a->y_stride, a, a->N, pass.y_stride))) return rc;
-  p.passes = 1;
+  y = {"y", a->y, a->N, {0, 0, 0}};
+  if ((rc = strides_of("y", a->y_stride, a, a->N, y.stride))) return rc;
+  if ((rc = check_workspace(segments_of(a, 1, &p), a->workspace, a->workspace_bytes))) return rc;
+  p.seg_states = static_cast<float*>(a->workspace);
   p.state_in = a->state_in;
   p.state_out = a->state_out;
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
+  if (a->S == 0) return copy_states(a, stream);
+  if ((rc = make_pass(a, q, k, v, &p.pass[0])) || (rc = make_output(a, y, &p.pass[0]))) return rc;
   const cudaError_t e = launch_linear(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention kernel");
   return ACCT_OK;
@@ -93,51 +159,52 @@ int acct_linear_fwd(const acct_linear_args* a, void* stream) {
 
 size_t acct_linear_bwd_workspace_bytes(const acct_linear_args* a) {
   if (a == nullptr || a->B <= 0 || a->N <= 0 || a->S <= 0 || a->D <= 0) return 0;
-  return a->N_kv > 0 && a->N_kv != a->N ? 2 * partial_bytes(a) : 0;
+  return segments_of(a, 3, nullptr) + partial_bytes(a);
 }
 
 int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void* stream) {
   LinParams p;
-  LinOperand q, k, v, d;
+  Rows q, k, v;
   int rc = check_linear(a, &p, &q, &k, &v);
   if (rc) return rc;
   if (a->cu_seqlens != nullptr) return fail(ACCT_ERR_SHAPE, "packed sequences have no backward");
   if (a->state_in != nullptr || a->state_out != nullptr) return fail(ACCT_ERR_SHAPE, "states have no backward");
   if (g == nullptr || !g->d_y || !g->dq || !g->dk || !g->dv) return fail(ACCT_ERR_NULL, "d_y, dq, dk, dv must be non-NULL");
   if (misaligned(g->d_y) || misaligned(g->dq) || misaligned(g->dk) || misaligned(g->dv)) return fail(ACCT_ERR_ALIGN, "d_y, dq, dk, dv must be 16-byte aligned");
-  const size_t need = acct_linear_bwd_workspace_bytes(a);
-  if (need > 0 && (g->workspace == nullptr || g->workspace_bytes < need))
-    return fail(ACCT_ERR_WORKSPACE, "workspace of %zu bytes is too small: %zu are needed", g->workspace_bytes, need);
-  if (need > 0 && misaligned(g->workspace)) return fail(ACCT_ERR_ALIGN, "workspace must be 16-byte aligned");
-  d = {g->d_y, {0, 0, 0}, 1};
-  if ((rc = strides_of("d_y", g->d_y_stride, a, a->N, d.stride))) return rc;
-  const int group = k.group, n_kv = a->N / group;
+  const size_t segment_bytes = segments_of(a, 3, &p);
+  if ((rc = check_workspace(segment_bytes + partial_bytes(a), g->workspace, g->workspace_bytes))) return rc;
+  p.seg_states = static_cast<float*>(g->workspace);
   const int64_t zero[3] = {0, 0, 0};
-  LinPass &dq = p.pass[0], &dk = p.pass[1], &dv = p.pass[2];
-  dq.a = d; dq.b = v; dq.c = k; dq.y = g->dq;
-  dk.a = v; dk.b = d; dk.c = q; dk.y = g->dk;
-  dv.a = k; dv.b = q; dv.c = d; dv.y = g->dv;
-  dk.reverse = dv.reverse = 1;
-  p.passes = 3;
-  LinReduce r;
-  memset(&r, 0, sizeof(r));
-  if ((rc = strides_of("dq", zero, a, a->N, dq.y_stride)) || (rc = strides_of("dk", zero, a, a->N, dk.y_stride)) ||
-      (rc = strides_of("dv", zero, a, a->N, dv.y_stride)))
+  Rows d = {"d_y", g->d_y, a->N, {0, 0, 0}}, dq = {"dq", g->dq, a->N, {0, 0, 0}};
+  Rows dk = {"dk", g->dk, k.heads, {0, 0, 0}}, dv = {"dv", g->dv, k.heads, {0, 0, 0}};
+  if ((rc = strides_of("d_y", g->d_y_stride, a, a->N, d.stride)) || (rc = strides_of("dq", zero, a, a->N, dq.stride)) ||
+      (rc = strides_of("dk", zero, a, k.heads, dk.stride)))
     return rc;
-  if (group > 1) {
-    float* parts = static_cast<float*>(g->workspace);
-    dk.y = parts;
-    dv.y = parts + static_cast<size_t>(a->B) * a->N * a->S * a->D;
-    dk.y_f32 = dv.y_f32 = 1;
-    r.parts[0] = static_cast<const float*>(dk.y); r.parts[1] = static_cast<const float*>(dv.y);
-    r.out[0] = g->dk; r.out[1] = g->dv;
-    if ((rc = strides_of("dk", zero, a, n_kv, r.out_stride[0])) || (rc = strides_of("dv", zero, a, n_kv, r.out_stride[1]))) return rc;
-    r.lens = a->seq_lens;
-    r.B = a->B; r.N_kv = n_kv; r.group = group; r.S = a->S; r.D = a->D;
-  }
+  std::copy(dk.stride, dk.stride + 3, dv.stride);
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
+  if ((rc = make_pass(a, d, v, k, &p.pass[0])) || (rc = make_pass(a, v, d, q, &p.pass[1])) || (rc = make_pass(a, k, q, d, &p.pass[2])) ||
+      (rc = make_output(a, dq, &p.pass[0])) || (rc = make_output(a, dk, &p.pass[1])) || (rc = make_output(a, dv, &p.pass[2])))
+    return rc;
+  p.pass[1].reverse = p.pass[2].reverse = 1;
+  const int group = a->N / k.heads;
+  LinReduce r;
+  memset(&r, 0, sizeof(r));
+  if (group > 1) {      // every query head's part in fp32, then their sums
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + segment_bytes);
+    for (int i = 0; i < 2; ++i) {
+      LinPass& pass = p.pass[1 + i];
+      pass.y = parts + i * (partial_bytes(a) / 8);
+      pass.y_f32 = 1;
+      std::copy(dq.stride, dq.stride + 3, pass.y_stride);
+      r.parts[i] = static_cast<const float*>(pass.y);
+    }
+    std::copy(dk.stride, dk.stride + 3, r.out_stride);
+    r.out[0] = g->dk; r.out[1] = g->dv;
+    r.lens = a->seq_lens;
+    r.B = a->B; r.N_kv = k.heads; r.group = group; r.S = a->S; r.D = a->D;
+  }
   cudaError_t e = launch_linear(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
   if (e == cudaSuccess && group > 1) e = launch_linear_reduce(r, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention backward");
