@@ -18,8 +18,8 @@
 // spare: the rows of P, the weighted C of a chunk and the state are scaled by powers of two that put their largest value near 2^15,
 // and what follows is scaled back in fp32.
 //
-// Warps: 0-3 weight P (thread = row), 4-7 have the state (thread = row of S), 8-11 split the weighted C and write y (thread = row), 12 loads,
-// 13 issues products, 14 stores.  The products of a chunk are issued as B^T C, the next chunk's A B^T, A S, P C: what each needs of the
+// Warps: 0-3 weight P (thread = row), 4-7 have the state (thread = row of S), 8-11 split the weighted C, both write half of y (thread = row), 12 loads,
+// 13 issues products.  The products of a chunk are issued as B^T C, A S, the next chunk's A B^T, P C: what each needs of the
 // other warps is made while the ones before it run.
 #include "fa_common.cuh"
 #include "fa_kernels.cuh"
@@ -33,7 +33,9 @@ constexpr int kThreads = 512;
 constexpr int kRegsWork = 152, kRegsControl = 56;      // of 128 a thread at launch: 3 x 128 x 152 + 128 x 56 = 512 x 128
 constexpr int kCols = 64;                              // columns of C, and of S, in a block
 constexpr uint32_t kTileBytes = kLinChunk * 128;       // 128 rows of 64 16-bit values
-constexpr uint32_t kColP = 0, kColIn = 256, kColOut = 320, kColState = 384;      // tensor memory: P (2 x 128), P C, A S, B^T C (2 x 64)
+// Tensor memory: P, twice 128 columns, of which P C takes the upper half once the scores there have been read; A S; B^T C, 64 columns for
+// each number that stands for a weighted C.
+constexpr uint32_t kColP = 0, kColIn = 64, kColOut = 256, kColState = 320;
 
 struct Item {
   int b, h, c0, pass;
@@ -45,13 +47,13 @@ struct Item {
 
 template <bool BF16>
 struct Shared {
-  uint64_t a_full[2], a_empty[2], b_full[2], b_empty[2], c_full[2], c_empty[2];
-  uint64_t p_full[2], p_ready[2], split_ready, inc_done[2], s_ready, s_read, o_done, o_free, o_staged[2];
+  uint64_t a_full[3], a_empty[3], b_full[3], b_empty[3], c_full[4], c_empty[4];
+  uint64_t p_full[2], p_ready[2], split_ready, inc_done, inc_free, s_ready, s_read, o_done, o_free;
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
   Item item;
   float power[kLinChunk + 1];                                   // l^j
-  float p_back[BF16 ? 1 : 4][BF16 ? 1 : kLinChunk], c_back[4], s_back[4];      // float16: 1 / the scales of a chunk
+  float p_back[BF16 ? 1 : 2][BF16 ? 1 : kLinChunk], c_back[4], s_back[4];      // float16: 1 / the scales of a chunk
   uint32_t most[2][2][4];
 };
 
@@ -75,6 +77,13 @@ __device__ __forceinline__ uint32_t narrow(uint64_t x) {
   float a, b;
   f2_unpack(x, a, b);
   return pack2<BF16>(a, b);
+}
+
+// 32 bytes at a multiple of 32: a whole sector of L2
+__device__ __forceinline__ void store32(void* to, const uint32_t (&u)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
+               "r"(u[6]), "r"(u[7])
+               : "memory");
 }
 
 // What the block works on; by one warp.
@@ -144,11 +153,15 @@ __device__ __forceinline__ Item find_item(const LinParams& p) {
 template <int DPAD, bool BF16, int SPLIT, bool STATES>
 __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_constant__ LinParams p) {
   constexpr int NB = DPAD / 64;                    // 64-column blocks of A and B
-  constexpr uint32_t kStage = (2 * NB + 1) * kTileBytes;
+  constexpr uint32_t kAB = NB * kTileBytes;
+  // Buffers.  A chunk of C is needed from its split to P C, longer than its A and B.
+  constexpr int kStAB = DPAD == 64 ? 3 : 2, kStC = DPAD == 64 ? 4 : SPLIT == 2 ? 3 : 2;
 
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));      // 2 x (A, B, C)
-  uint8_t* sSplit = stages + 2 * kStage;
+  uint8_t* sA = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sB = sA + kStAB * kAB;
+  uint8_t* sC = sB + kStAB * kAB;                  // (behind B: at head_dim up to 64 the product B^T C reads 128 columns of B, of which 64 are not)
+  uint8_t* sSplit = sC + kStC * kTileBytes;
   uint8_t* sS = sSplit + SPLIT * kTileBytes;       // DPAD rows of 64 values
   __shared__ Shared<BF16> sh;
 
@@ -159,15 +172,15 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     if (elect_one()) sh.item = x;
   }
   if (tid == 12 * 32) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kStAB; ++i) {
       mbar_init(&sh.a_full[i], 1); mbar_init(&sh.a_empty[i], 1);
       mbar_init(&sh.b_full[i], 1); mbar_init(&sh.b_empty[i], 1);
-      mbar_init(&sh.c_full[i], 1); mbar_init(&sh.c_empty[i], 1);
-      mbar_init(&sh.p_full[i], 1); mbar_init(&sh.p_ready[i], 128);
-      mbar_init(&sh.inc_done[i], 1); mbar_init(&sh.o_staged[i], 128);
     }
-    mbar_init(&sh.split_ready, 128); mbar_init(&sh.s_ready, 128); mbar_init(&sh.s_read, 1);
-    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128);
+    for (int i = 0; i < kStC; ++i) { mbar_init(&sh.c_full[i], 1); mbar_init(&sh.c_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sh.p_full[i], 1); mbar_init(&sh.p_ready[i], 128); }
+    mbar_init(&sh.split_ready, 128); mbar_init(&sh.inc_done, 1); mbar_init(&sh.inc_free, 128);
+    mbar_init(&sh.s_ready, 128); mbar_init(&sh.s_read, 1);
+    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 256);
     sh.abort_flag = 0;
     mbar_fence_init();
   }
@@ -193,25 +206,80 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   }
   __syncthreads();
 
+  // y of chunk c, 32 columns of it; thread = row
+  auto write_y = [&](int c, int half) {
+    const int rows = rows_of(c), row = tid & 127;
+    const uint32_t t_y = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 32;
+    float w = p.scale * sh.power[reverse ? max(rows - row, 0) : row + 1], in = p.scale;
+    mbar_wait(&sh.o_done, c & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+    tc_fence_after_sync();
+    uint32_t r[32], q[32];
+    tmem_ld32(t_y + kColP + (c & 1) * 128 + kColIn, r);
+    tmem_ld32(t_y + kColOut, q);
+    if constexpr (!BF16) {
+      w *= sh.s_back[c & 3];
+      in *= sh.p_back[c & 1][row];
+    }
+    const uint64_t w2 = f2_pack(w, w), in2 = f2_pack(in, in);
+    const int64_t at = batch * pass.y_stride[0] + x.h * pass.y_stride[1] + (x.row0 + first_row(c) + row) * pass.y_stride[2] + x.c0 + half * 32;
+    const int left = row < rows ? p.D - x.c0 - half * 32 : 0;      // values that exist
+    tmem_wait_ld();
+    tc_fence_before_sync();
+    mbar_arrive(&sh.o_free);
+    uint64_t v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      v[j] = f2_fma(f2_pack(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), w2,
+                    f2_mul(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), in2));
+    if (pass.y_f32) {
+      float* out = static_cast<float*>(pass.y) + at;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t u[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float a, b;
+          f2_unpack(v[4 * j + e], a, b);
+          u[2 * e] = __float_as_uint(a);
+          u[2 * e + 1] = __float_as_uint(b);
+        }
+        if (8 * j < left) store32(out + 8 * j, u);
+      }
+    } else {
+      uint16_t* out = static_cast<uint16_t*>(pass.y) + at;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = narrow<BF16>(v[8 * j + e]);
+        if (pass.y_wide && 16 * j + 8 < left) {
+          store32(out + 16 * j, u);
+        } else {
+          if (16 * j < left) *reinterpret_cast<uint4*>(out + 16 * j) = make_uint4(u[0], u[1], u[2], u[3]);
+          if (16 * j + 8 < left) *reinterpret_cast<uint4*>(out + 16 * j + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+        }
+      }
+    }
+  };
+
   if (warp == 12) {
     // ------------------------------------------------------------------ loads
     reg_dealloc<kRegsControl>();
     if (elect_one()) {
       const int ha = x.h / pass.a.group, hb = x.h / pass.b.group, hc = x.h / pass.c.group;
       for (int c = 0; c < n; ++c) {
-        const int s = c & 1, before = ((c >> 1) - 1) & 1, row = x.row0 + first_row(c);
-        uint8_t *sA = stages + s * kStage, *sB = sA + NB * kTileBytes, *sC = sB + NB * kTileBytes;
-        if (c >= 2) mbar_wait(&sh.b_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        mbar_expect_tx(&sh.b_full[s], NB * kTileBytes);
-        for (int nb = 0; nb < NB; ++nb) tma_load_4d(sB + nb * kTileBytes, &pass.b.map, &sh.b_full[s], nb * 64, row, hb, batch);
-        if (c >= 2) mbar_wait(&sh.c_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        mbar_expect_tx(&sh.c_full[s], kTileBytes);
-        tma_load_4d(sC, &pass.c.map, &sh.c_full[s], x.c0, row, hc, batch);
+        const int s = c % kStAB, sc = c % kStC, row = x.row0 + first_row(c);
+        if (c >= kStAB) mbar_wait(&sh.b_empty[s], (c / kStAB - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        mbar_expect_tx(&sh.b_full[s], kAB);
+        for (int nb = 0; nb < NB; ++nb) tma_load_4d(sB + s * kAB + nb * kTileBytes, &pass.b.map, &sh.b_full[s], nb * 64, row, hb, batch);
         if constexpr (!STATES) {
-          if (c >= 2) mbar_wait(&sh.a_empty[s], before, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-          mbar_expect_tx(&sh.a_full[s], NB * kTileBytes);
-          for (int nb = 0; nb < NB; ++nb) tma_load_4d(sA + nb * kTileBytes, &pass.a.map, &sh.a_full[s], nb * 64, row, ha, batch);
+          if (c >= kStAB) mbar_wait(&sh.a_empty[s], (c / kStAB - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+          mbar_expect_tx(&sh.a_full[s], kAB);
+          for (int nb = 0; nb < NB; ++nb) tma_load_4d(sA + s * kAB + nb * kTileBytes, &pass.a.map, &sh.a_full[s], nb * 64, row, ha, batch);
         }
+        if (c >= kStC) mbar_wait(&sh.c_empty[sc], (c / kStC - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        mbar_expect_tx(&sh.c_full[sc], kTileBytes);
+        tma_load_4d(sC + sc * kTileBytes, &pass.c.map, &sh.c_full[sc], x.c0, row, hc, batch);
       }
     }
     __syncwarp();
@@ -219,18 +287,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     // ------------------------------------------------------------------ products
     reg_dealloc<kRegsControl>();
     const uint32_t idesc_p = make_idesc(BF16, 128, 128, false, false), idesc_in = make_idesc(BF16, 128, kCols, false, true);
-    const uint32_t idesc_s = make_idesc(BF16, 128, kCols, true, true);
+    const uint32_t idesc_s = make_idesc(BF16, 128, SPLIT * kCols, true, true);
     const uint64_t kmajor = make_sdesc_base(16, 1024), mnmajor = make_sdesc_base(kTileBytes, 1024);
     const uint32_t k_hi = static_cast<uint32_t>(kmajor >> 32), mn_hi = static_cast<uint32_t>(mnmajor >> 32);
     auto at = [](uint64_t base, const uint8_t* t) { return static_cast<uint32_t>(base) | ((smem_u32(t) >> 4) & 0x3fffu); };
-    const uint32_t a_lo = at(kmajor, stages), b_lo = at(kmajor, stages + NB * kTileBytes);
-    const uint32_t bt_lo = at(mnmajor, stages + NB * kTileBytes), c_lo = at(mnmajor, stages + 2 * NB * kTileBytes);
+    const uint32_t a_lo = at(kmajor, sA), b_lo = at(kmajor, sB), bt_lo = at(mnmajor, sB), c_lo = at(mnmajor, sC);
     const uint32_t split_lo = at(mnmajor, sSplit), s_lo = at(mnmajor, sS);
     const int k_steps = (p.D + 15) / 16;
     auto issue_p = [&](int c) {
-      const uint32_t off = (c & 1) * (kStage >> 4);
-      mbar_wait(&sh.a_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-      mbar_wait(&sh.b_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      const int s = c % kStAB;
+      const uint32_t off = s * (kAB >> 4);
+      mbar_wait(&sh.a_full[s], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      mbar_wait(&sh.b_full[s], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
       if (elect_one()) {
         for (int kk = 0; kk < k_steps; ++kk) {
           const uint32_t o = off + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u;
@@ -242,27 +310,22 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     };
     if (!STATES && n > 0) issue_p(0);
     for (int c = 0; c < n; ++c) {
-      const uint32_t off = (c & 1) * (kStage >> 4);
-      if constexpr (STATES) {      // the warps of the state have read the product before
-        mbar_wait(&sh.s_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        mbar_wait(&sh.b_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-      }
+      const int s = c % kStAB, sc = c % kStC;
+      const uint32_t off = s * (kAB >> 4), t_p = tmem + kColP + (c & 1) * 128;
+      if constexpr (STATES) mbar_wait(&sh.b_full[s], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      if (c > 0) mbar_wait(&sh.inc_free, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
       mbar_wait(&sh.split_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
       tc_fence_after_sync();
       if (elect_one()) {
 #pragma unroll
-        for (int i = 0; i < SPLIT; ++i)
-#pragma unroll
-          for (int kk = 0; kk < kLinChunk / 16; ++kk)
-            umma_ss_lohi(tmem + kColState + (c & 1) * kCols, bt_lo + off + kk * 128u, mn_hi, split_lo + i * (kTileBytes >> 4) + kk * 128u, mn_hi,
-                         idesc_s, i > 0 || kk > 0);
-        umma_commit(&sh.inc_done[c & 1]);
-        umma_commit(&sh.b_empty[c & 1]);
-        if constexpr (STATES) umma_commit(&sh.c_empty[c & 1]);
+        for (int kk = 0; kk < kLinChunk / 16; ++kk)
+          umma_ss_lohi(tmem + kColState, bt_lo + off + kk * 128u, mn_hi, split_lo + kk * 128u, mn_hi, idesc_s, kk > 0);
+        umma_commit(&sh.inc_done);
+        umma_commit(&sh.b_empty[s]);
+        if constexpr (STATES) umma_commit(&sh.c_empty[sc]);
       }
       __syncwarp();
       if constexpr (!STATES) {
-        if (c + 1 < n) issue_p(c + 1);      // (the P that it goes over has been consumed: products run in the order of their issue)
         mbar_wait(&sh.s_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         if (c > 0) mbar_wait(&sh.o_free, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         tc_fence_after_sync();
@@ -270,33 +333,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           for (int kk = 0; kk < k_steps; ++kk)
             umma_ss_lohi(tmem + kColOut, a_lo + off + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u, k_hi, s_lo + kk * 128u, mn_hi, idesc_in, kk > 0);
           umma_commit(&sh.s_read);
+          umma_commit(&sh.a_empty[s]);
         }
         __syncwarp();
+        if (c + 1 < n) issue_p(c + 1);      // (the P that it goes over has been consumed, as products run in the order of their issue, and P C read)
         mbar_wait(&sh.p_ready[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         tc_fence_after_sync();
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kLinChunk / 16; ++kk)
-            umma_ts_lohi(tmem + kColIn, tmem + kColP + (c & 1) * 128 + kk * 8, c_lo + off + kk * 128u, mn_hi, idesc_in, kk > 0);
+            umma_ts_lohi(t_p + kColIn, t_p + kk * 8, c_lo + sc * (kTileBytes >> 4) + kk * 128u, mn_hi, idesc_in, kk > 0);
           umma_commit(&sh.o_done);
-          umma_commit(&sh.c_empty[c & 1]);
-        }
-        __syncwarp();
-      }
-    }
-  } else if (warp == 14) {
-    // ------------------------------------------------------------------ stores of whole chunks
-    reg_dealloc<kRegsControl>();
-    if constexpr (!STATES) {
-      for (int c = 0; c < n; ++c) {
-        mbar_wait(&sh.o_staged[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        if (elect_one()) {
-          if (rows_of(c) == kLinChunk && !pass.y_f32) {
-            tma_store_4d(&pass.map_y, stages + (c & 1) * kStage, x.c0, x.row0 + first_row(c), x.h, batch);
-            tma_store_commit();
-            tma_store_wait_read();
-          }
-          mbar_arrive(&sh.a_empty[c & 1]);
+          umma_commit(&sh.c_empty[sc]);
         }
         __syncwarp();
       }
@@ -371,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           float scale, back;
           near_top(most, scale, back);
           scale2 = f2_pack(scale, scale);
-          sh.p_back[c & 3][tid] = back;
+          sh.p_back[c & 1][tid] = back;
         }
 #pragma unroll 1
         for (int block = 0; block < 4; ++block) {
@@ -396,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     // ------------------------------------------------------------------ the state
     reg_alloc<kRegsWork>();
     const int d = tid - 128, lane = tid & 31;
-    const uint32_t t_s = tmem + kColState + (static_cast<uint32_t>((warp - 4) * 32) << 16);
+    const uint32_t t_s = tmem + kColState + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const LinPower step = idle ? LinPower{1.f, 0.f} : lin_power(p.log_decay[x.h], kLinChunk);
     const int width = min(kCols, p.D - x.c0);      // columns that exist
     const int64_t one = (static_cast<int64_t>(x.b) * p.N + x.h) * p.D * p.D, row = static_cast<int64_t>(d) * p.D + x.c0;
@@ -413,63 +461,70 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     }
     // the state before chunk c, to shared memory in 16 bits
     auto publish = [&](int c) {
-      if constexpr (!STATES) {
-        uint64_t scale2 = 0;
-        if constexpr (!BF16) {
-          float most = 0.f;
+      uint64_t scale2 = 0;
+      if constexpr (!BF16) {
+        float most = 0.f;
 #pragma unroll
-          for (int j = 0; j < kCols / 2; ++j) {
-            float a, b;
-            f2_unpack(s[j], a, b);
-            most = fmax3(most, fabsf(a), fabsf(b));
-          }
-          const uint32_t of_warp = __reduce_max_sync(0xffffffffu, DPAD == 128 || warp < 6 ? __float_as_uint(most) : 0u);
-          if (lane == 0) sh.most[0][c & 1][warp - 4] = of_warp;
-          named_barrier(1, 128);
-          const float of_all = __uint_as_float(max(max(sh.most[0][c & 1][0], sh.most[0][c & 1][1]), max(sh.most[0][c & 1][2], sh.most[0][c & 1][3])));
-          float scale, back;
-          near_top(of_all, scale, back);
-          scale2 = f2_pack(scale, scale);
-          if (d == 0) sh.s_back[c & 3] = back;
+        for (int j = 0; j < kCols / 2; ++j) {
+          float a, b;
+          f2_unpack(s[j], a, b);
+          most = fmax3(most, fabsf(a), fabsf(b));
         }
-        if (c > 0) mbar_wait(&sh.s_read, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
-        if (d < DPAD) {
-#pragma unroll
-          for (int j = 0; j < kCols / 8; ++j) {
-            uint32_t pk[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) pk[u] = narrow<BF16>(BF16 ? s[4 * j + u] : f2_mul(s[4 * j + u], scale2));
-            *reinterpret_cast<uint4*>(sS + swz128(d, j)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-          }
-        }
-        fence_proxy_async_smem();
+        const uint32_t of_warp = __reduce_max_sync(0xffffffffu, DPAD == 128 || warp < 6 ? __float_as_uint(most) : 0u);
+        if (lane == 0) sh.most[0][c & 1][warp - 4] = of_warp;
+        named_barrier(1, 128);
+        const float of_all = __uint_as_float(max(max(sh.most[0][c & 1][0], sh.most[0][c & 1][1]), max(sh.most[0][c & 1][2], sh.most[0][c & 1][3])));
+        float scale, back;
+        near_top(of_all, scale, back);
+        scale2 = f2_pack(scale, scale);
+        if (d == 0) sh.s_back[c & 3] = back;
       }
+      if (c > 0) mbar_wait(&sh.s_read, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      if (d < DPAD) {
+#pragma unroll
+        for (int j = 0; j < kCols / 8; ++j) {
+          uint32_t pk[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) pk[u] = narrow<BF16>(BF16 ? s[4 * j + u] : f2_mul(s[4 * j + u], scale2));
+          *reinterpret_cast<uint4*>(sS + swz128(d, j)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+        }
+      }
+      fence_proxy_async_smem();
       mbar_arrive(&sh.s_ready);
     };
-    if (n > 0) publish(0);
+    if (!STATES && n > 0) publish(0);
     for (int c = 0; c < n; ++c) {
       const int rows = rows_of(c);
       const LinPower w = rows == kLinChunk ? step : lin_power(p.log_decay[x.h], rows);
       const uint64_t hi2 = f2_pack(w.hi, w.hi), lo2 = f2_pack(w.lo, w.lo);
-      mbar_wait(&sh.inc_done[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      mbar_wait(&sh.inc_done, c & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
       tc_fence_after_sync();
       uint64_t back2 = 0;
       if constexpr (!BF16) back2 = f2_pack(sh.c_back[c & 3], sh.c_back[c & 3]);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t r[32];
-        tmem_ld32(t_s + (c & 1) * kCols + half * 32, r);
-        tmem_wait_ld();
+      for (int part = 0; part < kCols / 16; ++part) {
+        uint32_t r[SPLIT][16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          uint64_t inc = f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+        for (int i = 0; i < SPLIT; ++i) tmem_ld16(t_s + i * kCols + part * 16, r[i]);
+        tmem_wait_ld();
+        if (part + 1 == kCols / 16) {
+          tc_fence_before_sync();
+          mbar_arrive(&sh.inc_free);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint64_t inc = f2_pack(__uint_as_float(r[SPLIT - 1][2 * j]), __uint_as_float(r[SPLIT - 1][2 * j + 1]));
+#pragma unroll
+          for (int i = SPLIT - 2; i >= 0; --i) inc = f2_add(inc, f2_pack(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1])));
           if constexpr (!BF16) inc = f2_mul(inc, back2);
-          uint64_t& v = s[half * 16 + j];
+          uint64_t& v = s[part * 8 + j];
           v = f2_fma(v, hi2, f2_fma(v, lo2, inc));
         }
       }
-      tc_fence_before_sync();
-      if (c + 1 < n) publish(c + 1);
+      if constexpr (!STATES) {
+        if (c + 1 < n) publish(c + 1);
+        write_y(c, 1);
+      }
     }
     if (to != nullptr && d < p.D) {
 #pragma unroll
@@ -484,15 +539,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     // ------------------------------------------------------------------ weighted C, and y
     reg_alloc<kRegsWork>();
     const int row = tid - 256;
-    const uint32_t lanes = static_cast<uint32_t>((warp - 8) * 32) << 16;
     auto split = [&](int c) {
-      const int rows = rows_of(c), st = c & 1;
-      uint8_t *sB = stages + st * kStage + NB * kTileBytes, *sC = sB + NB * kTileBytes;
-      mbar_wait(&sh.c_full[st], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      const int rows = rows_of(c);
+      uint8_t *mine = sC + c % kStC * kTileBytes, *its_b = sB + c % kStAB * kAB;
+      mbar_wait(&sh.c_full[c % kStC], (c / kStC) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
       const bool there = row < rows;
       uint4 raw[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) raw[j] = there ? *reinterpret_cast<const uint4*>(sC + swz128(row, j)) : make_uint4(0u, 0u, 0u, 0u);
+      for (int j = 0; j < 8; ++j) raw[j] = there ? *reinterpret_cast<const uint4*>(mine + swz128(row, j)) : make_uint4(0u, 0u, 0u, 0u);
       float w = there ? sh.power[reverse ? row : rows - 1 - row] : 0.f;
       if constexpr (!BF16) {
         uint32_t most = 0;      // of the absolute values, as 16-bit patterns, which have their order
@@ -513,91 +567,41 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         if (row == 0) sh.c_back[c & 3] = back;
       }
       const uint64_t w2 = f2_pack(w, w);
-      if (c > 0) mbar_wait(&sh.inc_done[(c - 1) & 1], ((c - 1) >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      // all of it in registers before the product of the chunk before has left the buffers
+      uint32_t out[SPLIT][32];
+      const uint64_t minus = f2_pack(-1.f, -1.f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t in[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-        uint32_t out[SPLIT][4];
+      for (int j = 0; j < 32; ++j) {
+        const uint32_t in = j % 4 == 0 ? raw[j / 4].x : j % 4 == 1 ? raw[j / 4].y : j % 4 == 2 ? raw[j / 4].z : raw[j / 4].w;
+        uint64_t v = f2_mul(widen<BF16>(in), w2);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint64_t v = f2_mul(widen<BF16>(in[u]), w2);
-#pragma unroll
-          for (int i = 0; i < SPLIT; ++i) {
-            out[i][u] = narrow<BF16>(v);
-            if (i + 1 < SPLIT) {
-              const uint64_t part = widen<BF16>(out[i][u] ^ 0x80008000u);      // minus
-              v = f2_add(v, part);
-            }
-          }
+        for (int i = 0; i < SPLIT; ++i) {
+          out[i][j] = narrow<BF16>(v);
+          if (i + 1 < SPLIT) v = f2_fma(widen<BF16>(out[i][j]), minus, v);
         }
-#pragma unroll
-        for (int i = 0; i < SPLIT; ++i)
-          *reinterpret_cast<uint4*>(sSplit + i * kTileBytes + swz128(row, j)) = make_uint4(out[i][0], out[i][1], out[i][2], out[i][3]);
       }
+      if (c > 0) mbar_wait(&sh.inc_done, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+#pragma unroll
+      for (int i = 0; i < SPLIT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4*>(sSplit + i * kTileBytes + swz128(row, j)) = make_uint4(out[i][4 * j], out[i][4 * j + 1], out[i][4 * j + 2], out[i][4 * j + 3]);
       if (rows < kLinChunk) {      // rows that are not this sequence's: 0 times what they hold might be a NaN
-        mbar_wait(&sh.b_full[st], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+        mbar_wait(&sh.b_full[c % kStAB], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
         if (!there) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            for (int nb = 0; nb < NB; ++nb) *reinterpret_cast<uint4*>(sB + nb * kTileBytes + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(sC + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
+            for (int nb = 0; nb < NB; ++nb) *reinterpret_cast<uint4*>(its_b + nb * kTileBytes + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(mine + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
           }
         }
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.split_ready);
     };
-    auto write_y = [&](int c) {
-      const int rows = rows_of(c);
-      float w = p.scale * sh.power[reverse ? max(rows - row, 0) : row + 1], in = p.scale;
-      mbar_wait(&sh.o_done, c & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
-      tc_fence_after_sync();
-      if constexpr (!BF16) {
-        w *= sh.s_back[c & 3];
-        in *= sh.p_back[c & 3][row];
-      }
-      const uint64_t w2 = f2_pack(w, w), in2 = f2_pack(in, in);
-      const bool direct = rows < kLinChunk || pass.y_f32;
-      const int64_t at = batch * pass.y_stride[0] + x.h * pass.y_stride[1] + (x.row0 + first_row(c) + row) * pass.y_stride[2] + x.c0;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t r[32], q[32];
-        tmem_ld32(tmem + lanes + kColIn + half * 32, r);
-        tmem_ld32(tmem + lanes + kColOut + half * 32, q);
-        tmem_wait_ld();
-        if (half == 1) {
-          tc_fence_before_sync();
-          mbar_arrive(&sh.o_free);
-        }
-        uint64_t v[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          v[j] = f2_fma(f2_pack(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), w2,
-                        f2_mul(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), in2));
-        if (pass.y_f32) {
-          float* out = static_cast<float*>(pass.y) + at + half * 32;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float4 f;
-            f2_unpack(v[2 * j], f.x, f.y);
-            f2_unpack(v[2 * j + 1], f.z, f.w);
-            if (row < rows && x.c0 + half * 32 + 4 * j < p.D) *reinterpret_cast<float4*>(out + 4 * j) = f;
-          }
-          continue;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 u = make_uint4(narrow<BF16>(v[4 * j]), narrow<BF16>(v[4 * j + 1]), narrow<BF16>(v[4 * j + 2]), narrow<BF16>(v[4 * j + 3]));
-          if (!direct) *reinterpret_cast<uint4*>(stages + (c & 1) * kStage + swz128(row, half * 4 + j)) = u;      // (A is not needed any more)
-          else if (row < rows && x.c0 + half * 32 + 8 * j < p.D) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(pass.y) + at + half * 32 + 8 * j) = u;
-        }
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&sh.o_staged[c & 1]);
-    };
     for (int c = 0; c <= n; ++c) {
       if (c < n) split(c);
-      if (!STATES && c > 0) write_y(c - 1);
+      if (!STATES && c > 0) write_y(c - 1, 0);
     }
   } else {
     reg_dealloc<kRegsControl>();
@@ -666,7 +670,8 @@ __global__ void __launch_bounds__(256) linear_reduce_kernel(const LinReduce p) {
 
 template <int DPAD, bool BF16, int SPLIT, bool STATES>
 cudaError_t launch(const LinParams& p, unsigned int blocks, cudaStream_t stream) {
-  const size_t smem = (2 * (2 * DPAD / 64 + 1) + SPLIT) * static_cast<size_t>(kTileBytes) + DPAD * 128 + 1024;
+  const size_t tiles = DPAD == 64 ? 3 * 2 + 4 : 2 * 4 + (SPLIT == 2 ? 3 : 2);      // (A, B and C as in the kernel)
+  const size_t smem = (tiles + SPLIT) * kTileBytes + DPAD * 128 + 1024;
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(linear_kernel<DPAD, BF16, SPLIT, STATES>), smem);
   if (e != cudaSuccess) return e;
   linear_kernel<DPAD, BF16, SPLIT, STATES><<<blocks, kThreads, smem, stream>>>(p);

@@ -84,10 +84,13 @@ int make_pass(const acct_linear_args* a, const Rows& x, const Rows& y, const Row
   }
   return 0;
 }
-int make_output(const acct_linear_args* a, const Rows& y, LinPass* pass) {
+void set_output(const Rows& y, LinPass* pass) {
   pass->y = const_cast<void*>(y.ptr);
-  for (int i = 0; i < 3; ++i) pass->y_stride[i] = y.stride[i];
-  return make_map(a, y, &pass->map_y);
+  pass->y_wide = (reinterpret_cast<uintptr_t>(y.ptr) & 31u) == 0;
+  for (int i = 0; i < 3; ++i) {
+    pass->y_stride[i] = y.stride[i];
+    pass->y_wide = pass->y_wide && y.stride[i] % 16 == 0;
+  }
 }
 
 // fp32 parts of dk and dv by query head, where heads share their keys and values
@@ -106,12 +109,12 @@ size_t segments_of(const acct_linear_args* a, int passes, LinParams* p) {
   p->cu = a->cu_seqlens;
   p->passes = passes;
   linear_segments(*p, kSms);
-  return (linear_segment_bytes(*p) + 15) / 16 * 16;
+  return (linear_segment_bytes(*p) + 31) / 32 * 32;
 }
 
 int check_workspace(size_t need, const void* workspace, size_t bytes) {
   if (need > 0 && (workspace == nullptr || bytes < need)) return fail(ACCT_ERR_WORKSPACE, "workspace of %zu bytes is too small: %zu are needed", bytes, need);
-  if (need > 0 && misaligned(workspace)) return fail(ACCT_ERR_ALIGN, "workspace must be 16-byte aligned");
+  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 31u) != 0) return fail(ACCT_ERR_ALIGN, "workspace must be 32-byte aligned");
   return 0;
 }
 
@@ -151,7 +154,8 @@ int acct_linear_fwd(const acct_linear_args* a, void* stream) {
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
   if (a->S == 0) return copy_states(a, stream);
-  if ((rc = make_pass(a, q, k, v, &p.pass[0])) || (rc = make_output(a, y, &p.pass[0]))) return rc;
+  if ((rc = make_pass(a, q, k, v, &p.pass[0]))) return rc;
+  set_output(y, &p.pass[0]);
   const cudaError_t e = launch_linear(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention kernel");
   return ACCT_OK;
@@ -184,9 +188,10 @@ int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
-  if ((rc = make_pass(a, d, v, k, &p.pass[0])) || (rc = make_pass(a, v, d, q, &p.pass[1])) || (rc = make_pass(a, k, q, d, &p.pass[2])) ||
-      (rc = make_output(a, dq, &p.pass[0])) || (rc = make_output(a, dk, &p.pass[1])) || (rc = make_output(a, dv, &p.pass[2])))
-    return rc;
+  if ((rc = make_pass(a, d, v, k, &p.pass[0])) || (rc = make_pass(a, v, d, q, &p.pass[1])) || (rc = make_pass(a, k, q, d, &p.pass[2]))) return rc;
+  set_output(dq, &p.pass[0]);
+  set_output(dk, &p.pass[1]);
+  set_output(dv, &p.pass[2]);
   p.pass[1].reverse = p.pass[2].reverse = 1;
   const int group = a->N / k.heads;
   LinReduce r;
@@ -195,7 +200,7 @@ int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + segment_bytes);
     for (int i = 0; i < 2; ++i) {
       LinPass& pass = p.pass[1 + i];
-      pass.y = parts + i * (partial_bytes(a) / 8);
+      pass.y = parts + i * (partial_bytes(a) / 8);      // (rows of a multiple of 8 fp32 values)
       pass.y_f32 = 1;
       std::copy(dq.stride, dq.stride + 3, pass.y_stride);
       r.parts[i] = static_cast<const float*>(pass.y);
