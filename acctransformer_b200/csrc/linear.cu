@@ -79,6 +79,25 @@ __device__ __forceinline__ uint32_t narrow(uint64_t x) {
   return pack2<BF16>(a, b);
 }
 
+// The next 16-bit number of two values' sums, and what it leaves of them.  bfloat16: the leading 8 bits as they are, so that no conversion is
+// needed and the rest has the same sign; the last number of a sum is rounded.
+template <bool BF16, bool LAST>
+__device__ __forceinline__ uint32_t next_part(uint64_t& v) {
+  if constexpr (LAST) {
+    return narrow<BF16>(v);
+  } else if constexpr (BF16) {
+    float a, b;
+    f2_unpack(v, a, b);
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    v = f2_fma(f2_pack(__uint_as_float(ua & 0xffff0000u), __uint_as_float(ub & 0xffff0000u)), f2_pack(-1.f, -1.f), v);
+    return __byte_perm(ua, ub, 0x7632);
+  } else {
+    const uint32_t w = narrow<BF16>(v);
+    v = f2_fma(widen<BF16>(w), f2_pack(-1.f, -1.f), v);
+    return w;
+  }
+}
+
 // 32 bytes at a multiple of 32: a whole sector of L2
 __device__ __forceinline__ void store32(void* to, const uint32_t (&u)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
@@ -380,12 +399,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           uint32_t r[32];
           tmem_ld32(t + block * 32, r);
           tmem_wait_ld();
-          if (block == warp) {      // (by a choice, not by a weight of 0: what is not finite stays out)
+          if (block == warp) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const bool in0 = reverse ? 2 * j >= lane : 2 * j <= lane, in1 = reverse ? 2 * j + 1 >= lane : 2 * j + 1 <= lane;
-              v[j] = f2_mul(f2_pack(in0 ? __uint_as_float(r[2 * j]) : 0.f, in1 ? __uint_as_float(r[2 * j + 1]) : 0.f), diagonal[j]);
-            }
+            for (int j = 0; j < 16; ++j) v[j] = f2_mul(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), diagonal[j]);
           } else {
             const float w = sh.power[reverse ? 32 * (block - warp) - lane : 32 * (warp - block) + lane - 31];
             const uint64_t w2 = f2_pack(w, w);
@@ -440,14 +456,15 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         mbar_arrive(&sh.p_ready[c & 1]);
       }
     }
-  } else if (warp < 8) {
-    // ------------------------------------------------------------------ the state
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ warps 4-7: the state; 8-11: weighted C; both: y
     reg_alloc<kRegsWork>();
-    const int d = tid - 128, lane = tid & 31;
+    const int row = tid & 127, lane = tid & 31;      // of the state, or of C
+    const bool keeps_state = warp < 8;
     const uint32_t t_s = tmem + kColState + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const LinPower step = idle ? LinPower{1.f, 0.f} : lin_power(p.log_decay[x.h], kLinChunk);
     const int width = min(kCols, p.D - x.c0);      // columns that exist
-    const int64_t one = (static_cast<int64_t>(x.b) * p.N + x.h) * p.D * p.D, row = static_cast<int64_t>(d) * p.D + x.c0;
+    const int64_t one = (static_cast<int64_t>(x.b) * p.N + x.h) * p.D * p.D, mine = static_cast<int64_t>(row) * p.D + x.c0;
     const int64_t slot = ((static_cast<int64_t>(x.slot) * p.passes + x.pass) * p.N + x.h) * p.D * p.D;
     const float* from = STATES || idle ? nullptr : x.slot >= 0 ? p.seg_states + slot : p.state_in != nullptr ? p.state_in + one : nullptr;
     float* to = idle ? nullptr : STATES ? p.seg_states + slot : x.slot < 0 && p.state_out != nullptr ? p.state_out + one : nullptr;
@@ -455,12 +472,42 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
 #pragma unroll
     for (int j = 0; j < kCols / 4; ++j) {
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (from != nullptr && d < p.D && 4 * j < width) f = *reinterpret_cast<const float4*>(from + row + 4 * j);
+      if (keeps_state && from != nullptr && row < p.D && 4 * j < width) f = *reinterpret_cast<const float4*>(from + mine + 4 * j);
       s[2 * j] = f2_pack(f.x, f.y);
       s[2 * j + 1] = f2_pack(f.z, f.w);
     }
-    // the state before chunk c, to shared memory in 16 bits
-    auto publish = [&](int c) {
+    // The state before chunk c, to shared memory in 16 bits; from chunk 1 on it is made from the one before first.
+    auto advance = [&](int c) {
+      if (c > 0) {
+        const int rows = rows_of(c - 1);
+        const LinPower w = rows == kLinChunk ? step : lin_power(p.log_decay[x.h], rows);
+        const uint64_t hi2 = f2_pack(w.hi, w.hi), lo2 = f2_pack(w.lo, w.lo);
+        mbar_wait(&sh.inc_done, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+        tc_fence_after_sync();
+        uint64_t back2 = 0;
+        if constexpr (!BF16) back2 = f2_pack(sh.c_back[(c - 1) & 3], sh.c_back[(c - 1) & 3]);
+#pragma unroll
+        for (int part = 0; part < kCols / 16; ++part) {
+          uint32_t r[SPLIT][16];
+#pragma unroll
+          for (int i = 0; i < SPLIT; ++i) tmem_ld16(t_s + i * kCols + part * 16, r[i]);
+          tmem_wait_ld();
+          if (part + 1 == kCols / 16) {
+            tc_fence_before_sync();
+            mbar_arrive(&sh.inc_free);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint64_t inc = f2_pack(__uint_as_float(r[SPLIT - 1][2 * j]), __uint_as_float(r[SPLIT - 1][2 * j + 1]));
+#pragma unroll
+            for (int i = SPLIT - 2; i >= 0; --i) inc = f2_add(inc, f2_pack(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1])));
+            if constexpr (!BF16) inc = f2_mul(inc, back2);
+            uint64_t& v = s[part * 8 + j];
+            v = f2_fma(v, hi2, f2_fma(v, lo2, inc));
+          }
+        }
+      }
+      if (STATES || c == n) return;
       uint64_t scale2 = 0;
       if constexpr (!BF16) {
         float most = 0.f;
@@ -477,88 +524,48 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         float scale, back;
         near_top(of_all, scale, back);
         scale2 = f2_pack(scale, scale);
-        if (d == 0) sh.s_back[c & 3] = back;
+        if (row == 0) sh.s_back[c & 3] = back;
       }
       if (c > 0) mbar_wait(&sh.s_read, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
-      if (d < DPAD) {
+      if (row < DPAD) {
 #pragma unroll
         for (int j = 0; j < kCols / 8; ++j) {
           uint32_t pk[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) pk[u] = narrow<BF16>(BF16 ? s[4 * j + u] : f2_mul(s[4 * j + u], scale2));
-          *reinterpret_cast<uint4*>(sS + swz128(d, j)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          *reinterpret_cast<uint4*>(sS + swz128(row, j)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         }
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.s_ready);
     };
-    if (!STATES && n > 0) publish(0);
-    for (int c = 0; c < n; ++c) {
-      const int rows = rows_of(c);
-      const LinPower w = rows == kLinChunk ? step : lin_power(p.log_decay[x.h], rows);
-      const uint64_t hi2 = f2_pack(w.hi, w.hi), lo2 = f2_pack(w.lo, w.lo);
-      mbar_wait(&sh.inc_done, c & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
-      tc_fence_after_sync();
-      uint64_t back2 = 0;
-      if constexpr (!BF16) back2 = f2_pack(sh.c_back[c & 3], sh.c_back[c & 3]);
-#pragma unroll
-      for (int part = 0; part < kCols / 16; ++part) {
-        uint32_t r[SPLIT][16];
-#pragma unroll
-        for (int i = 0; i < SPLIT; ++i) tmem_ld16(t_s + i * kCols + part * 16, r[i]);
-        tmem_wait_ld();
-        if (part + 1 == kCols / 16) {
-          tc_fence_before_sync();
-          mbar_arrive(&sh.inc_free);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint64_t inc = f2_pack(__uint_as_float(r[SPLIT - 1][2 * j]), __uint_as_float(r[SPLIT - 1][2 * j + 1]));
-#pragma unroll
-          for (int i = SPLIT - 2; i >= 0; --i) inc = f2_add(inc, f2_pack(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1])));
-          if constexpr (!BF16) inc = f2_mul(inc, back2);
-          uint64_t& v = s[part * 8 + j];
-          v = f2_fma(v, hi2, f2_fma(v, lo2, inc));
-        }
-      }
-      if constexpr (!STATES) {
-        if (c + 1 < n) publish(c + 1);
-        write_y(c, 1);
-      }
-    }
-    if (to != nullptr && d < p.D) {
-#pragma unroll
-      for (int j = 0; j < kCols / 4; ++j) {
-        float4 f;
-        f2_unpack(s[2 * j], f.x, f.y);
-        f2_unpack(s[2 * j + 1], f.z, f.w);
-        if (4 * j < width) *reinterpret_cast<float4*>(to + row + 4 * j) = f;
-      }
-    }
-  } else if (warp < 12) {
-    // ------------------------------------------------------------------ weighted C, and y
-    reg_alloc<kRegsWork>();
-    const int row = tid - 256;
+    // C of chunk c, weighted, as sums of 16-bit numbers
     auto split = [&](int c) {
       const int rows = rows_of(c);
-      uint8_t *mine = sC + c % kStC * kTileBytes, *its_b = sB + c % kStAB * kAB;
-      mbar_wait(&sh.c_full[c % kStC], (c / kStC) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      uint8_t *its_c = sC + c % kStC * kTileBytes, *its_b = sB + c % kStAB * kAB;
       const bool there = row < rows;
-      uint4 raw[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) raw[j] = there ? *reinterpret_cast<const uint4*>(mine + swz128(row, j)) : make_uint4(0u, 0u, 0u, 0u);
       float w = there ? sh.power[reverse ? row : rows - 1 - row] : 0.f;
+      mbar_wait(&sh.c_full[c % kStC], (c / kStC) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      if (!there) {      // rows that are not this sequence's: 0 times what they hold might be a NaN
+        mbar_wait(&sh.b_full[c % kStAB], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+          for (int nb = 0; nb < NB; ++nb) *reinterpret_cast<uint4*>(its_b + nb * kTileBytes + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(its_c + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      __syncwarp();
       if constexpr (!BF16) {
         uint32_t most = 0;      // of the absolute values, as 16-bit patterns, which have their order
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint32_t v[4] = {raw[j].x & 0x7fff7fffu, raw[j].y & 0x7fff7fffu, raw[j].z & 0x7fff7fffu, raw[j].w & 0x7fff7fffu};
-          most = __vmaxu2(most, __vmaxu2(__vmaxu2(v[0], v[1]), __vmaxu2(v[2], v[3])));
+          const uint4 raw = *reinterpret_cast<const uint4*>(its_c + swz128(row, j));
+          most = __vmaxu2(most, __vmaxu2(__vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu), __vmaxu2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu)));
         }
         // times this row's weight
         const float of_row = __half2float(__ushort_as_half(static_cast<unsigned short>(max(most >> 16, most & 0xffffu)))) * w;
         const uint32_t of_warp = __reduce_max_sync(0xffffffffu, __float_as_uint(of_row));
-        if ((tid & 31) == 0) sh.most[1][c & 1][warp - 8] = of_warp;
+        if (lane == 0) sh.most[1][c & 1][warp - 8] = of_warp;
         named_barrier(2, 128);
         const float of_all = __uint_as_float(max(max(sh.most[1][c & 1][0], sh.most[1][c & 1][1]), max(sh.most[1][c & 1][2], sh.most[1][c & 1][3])));
         float scale, back;
@@ -567,41 +574,41 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         if (row == 0) sh.c_back[c & 3] = back;
       }
       const uint64_t w2 = f2_pack(w, w);
-      // all of it in registers before the product of the chunk before has left the buffers
-      uint32_t out[SPLIT][32];
-      const uint64_t minus = f2_pack(-1.f, -1.f);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const uint32_t in = j % 4 == 0 ? raw[j / 4].x : j % 4 == 1 ? raw[j / 4].y : j % 4 == 2 ? raw[j / 4].z : raw[j / 4].w;
-        uint64_t v = f2_mul(widen<BF16>(in), w2);
-#pragma unroll
-        for (int i = 0; i < SPLIT; ++i) {
-          out[i][j] = narrow<BF16>(v);
-          if (i + 1 < SPLIT) v = f2_fma(widen<BF16>(out[i][j]), minus, v);
-        }
-      }
       if (c > 0) mbar_wait(&sh.inc_done, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+#pragma unroll 2
+      for (int j = 0; j < 8; ++j) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(its_c + swz128(row, j));
+        const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t out[3][4];
 #pragma unroll
-      for (int i = 0; i < SPLIT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          *reinterpret_cast<uint4*>(sSplit + i * kTileBytes + swz128(row, j)) = make_uint4(out[i][4 * j], out[i][4 * j + 1], out[i][4 * j + 2], out[i][4 * j + 3]);
-      if (rows < kLinChunk) {      // rows that are not this sequence's: 0 times what they hold might be a NaN
-        mbar_wait(&sh.b_full[c % kStAB], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-        if (!there) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            for (int nb = 0; nb < NB; ++nb) *reinterpret_cast<uint4*>(its_b + nb * kTileBytes + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(mine + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
-          }
+        for (int u = 0; u < 4; ++u) {
+          uint64_t v = f2_mul(widen<BF16>(in[u]), w2);
+          out[0][u] = next_part<BF16, false>(v);
+          if constexpr (SPLIT == 3) out[1][u] = next_part<BF16, false>(v);
+          out[SPLIT - 1][u] = next_part<BF16, true>(v);
         }
+#pragma unroll
+        for (int i = 0; i < SPLIT; ++i)
+          *reinterpret_cast<uint4*>(sSplit + i * kTileBytes + swz128(row, j)) = make_uint4(out[i][0], out[i][1], out[i][2], out[i][3]);
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.split_ready);
     };
+    if (keeps_state) advance(0);
+#pragma unroll 1
     for (int c = 0; c <= n; ++c) {
-      if (c < n) split(c);
-      if (!STATES && c > 0) write_y(c - 1, 0);
+      if (!keeps_state && c < n) split(c);
+      if (!STATES && c > 0) write_y(c - 1, keeps_state ? 1 : 0);
+      if (keeps_state && c < n) advance(c + 1);
+    }
+    if (keeps_state && to != nullptr && row < p.D) {
+#pragma unroll
+      for (int j = 0; j < kCols / 4; ++j) {
+        float4 f;
+        f2_unpack(s[2 * j], f.x, f.y);
+        f2_unpack(s[2 * j + 1], f.z, f.w);
+        if (4 * j < width) *reinterpret_cast<float4*>(to + mine + 4 * j) = f;
+      }
     }
   } else {
     reg_dealloc<kRegsControl>();
