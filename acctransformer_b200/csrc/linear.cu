@@ -18,8 +18,8 @@
 // spare: the rows of P, the weighted C of a chunk and the state are scaled by powers of two that put their largest value near 2^15,
 // and what follows is scaled back in fp32.
 //
-// Warps: 0-3 weight P (thread = row), 4-7 have the state (thread = row of S), 8-11 split the weighted C, both write half of y (thread = row), 12 loads,
-// 13 issues products.  The products of a chunk are issued as B^T C, A S, the next chunk's A B^T, P C: what each needs of the
+// Warps: 0-3 weight P (thread = row), 4-7 have the state (thread = row of S) and make y (thread = row), 8-11 split the weighted C, 12 loads,
+// 13 issues products, 14 stores y.  The products of a chunk are issued as B^T C, A S, the next chunk's A B^T, P C: what each needs of the
 // other warps is made while the ones before it run.
 #include "fa_common.cuh"
 #include "fa_kernels.cuh"
@@ -48,7 +48,7 @@ struct Item {
 template <bool BF16>
 struct Shared {
   uint64_t a_full[3], a_empty[3], b_full[3], b_empty[3], c_full[4], c_empty[4];
-  uint64_t p_full[2], p_ready[2], split_ready, inc_done, inc_free, s_ready, s_read, o_done, o_free;
+  uint64_t p_full[2], p_ready[2], split_ready, inc_done, inc_free, s_ready, s_read, o_done, o_free, y_staged;
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
   Item item;
@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   constexpr uint32_t kAB = NB * kTileBytes;
   // Buffers.  A chunk of C is needed from its split to P C, longer than its A and B.
   constexpr int kStAB = DPAD == 64 ? 3 : 2, kStC = DPAD == 64 ? 4 : SPLIT == 2 ? 3 : 2;
+  constexpr bool kStaged = kStC > 2;               // whole chunks of y leave through the buffer of their C; with two it could not wait for that
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sA = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     for (int i = 0; i < 2; ++i) { mbar_init(&sh.p_full[i], 1); mbar_init(&sh.p_ready[i], 128); }
     mbar_init(&sh.split_ready, 128); mbar_init(&sh.inc_done, 1); mbar_init(&sh.inc_free, 128);
     mbar_init(&sh.s_ready, 128); mbar_init(&sh.s_read, 1);
-    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 256);
+    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128); mbar_init(&sh.y_staged, 128);
     sh.abort_flag = 0;
     mbar_fence_init();
   }
@@ -225,59 +226,78 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   }
   __syncthreads();
 
-  // y of chunk c, 32 columns of it; thread = row
-  auto write_y = [&](int c, int half) {
+  void* const y = pass.y;
+  const int64_t y_stride = pass.y_stride[2];
+  const int64_t y_first = batch * pass.y_stride[0] + x.h * pass.y_stride[1] + (x.row0 + (tid & 127)) * y_stride + x.c0;
+  const bool y_f32 = pass.y_f32 != 0, y_wide = pass.y_wide != 0;
+  // y of chunk c; thread = row.  Whole chunks leave through the buffer of their C (kStaged), which P C was the last to read, others straight.
+  auto write_y = [&](int c) {
     const int rows = rows_of(c), row = tid & 127;
-    const uint32_t t_y = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 32;
+    const uint32_t t_y = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    uint8_t* stage = sC + c % kStC * kTileBytes;
     float w = p.scale * sh.power[reverse ? max(rows - row, 0) : row + 1], in = p.scale;
     mbar_wait(&sh.o_done, c & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
     tc_fence_after_sync();
-    uint32_t r[32], q[32];
-    tmem_ld32(t_y + kColP + (c & 1) * 128 + kColIn, r);
-    tmem_ld32(t_y + kColOut, q);
     if constexpr (!BF16) {
       w *= sh.s_back[c & 3];
       in *= sh.p_back[c & 1][row];
     }
     const uint64_t w2 = f2_pack(w, w), in2 = f2_pack(in, in);
-    const int64_t at = batch * pass.y_stride[0] + x.h * pass.y_stride[1] + (x.row0 + first_row(c) + row) * pass.y_stride[2] + x.c0 + half * 32;
-    const int left = row < rows ? p.D - x.c0 - half * 32 : 0;      // values that exist
-    tmem_wait_ld();
-    tc_fence_before_sync();
-    mbar_arrive(&sh.o_free);
-    uint64_t v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      v[j] = f2_fma(f2_pack(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), w2,
-                    f2_mul(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), in2));
-    if (pass.y_f32) {
-      float* out = static_cast<float*>(pass.y) + at;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t u[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a, b;
-          f2_unpack(v[4 * j + e], a, b);
-          u[2 * e] = __float_as_uint(a);
-          u[2 * e + 1] = __float_as_uint(b);
-        }
-        if (8 * j < left) store32(out + 8 * j, u);
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      uint32_t r[32], q[32];
+      tmem_ld32(t_y + kColP + (c & 1) * 128 + kColIn + half * 32, r);
+      tmem_ld32(t_y + kColOut + half * 32, q);
+      tmem_wait_ld();
+      if (half == 1) {
+        tc_fence_before_sync();
+        mbar_arrive(&sh.o_free);
       }
-    } else {
-      uint16_t* out = static_cast<uint16_t*>(pass.y) + at;
+      uint64_t v[16];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t u[8];
+      for (int j = 0; j < 16; ++j)
+        v[j] = f2_fma(f2_pack(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), w2,
+                      f2_mul(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), in2));
+      const int64_t at = y_first + static_cast<int64_t>(first_row(c)) * y_stride + half * 32;
+      const int left = row < rows ? p.D - x.c0 - half * 32 : 0;      // values that exist
+      if (y_f32) {
+        float* out = static_cast<float*>(y) + at;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = narrow<BF16>(v[8 * j + e]);
-        if (pass.y_wide && 16 * j + 8 < left) {
-          store32(out + 16 * j, u);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t u[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a, b;
+            f2_unpack(v[4 * j + e], a, b);
+            u[2 * e] = __float_as_uint(a);
+            u[2 * e + 1] = __float_as_uint(b);
+          }
+          if (8 * j < left) store32(out + 8 * j, u);
+        }
+      } else {
+        uint16_t* out = static_cast<uint16_t*>(y) + at;
+        uint32_t u[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) u[j] = narrow<BF16>(v[j]);
+        if (kStaged && rows == kLinChunk) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + swz128(row, half * 4 + j)) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+        } else if (!kStaged && y_wide && left >= 32) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t x8[8] = {u[8 * j], u[8 * j + 1], u[8 * j + 2], u[8 * j + 3], u[8 * j + 4], u[8 * j + 5], u[8 * j + 6], u[8 * j + 7]};
+            store32(out + 16 * j, x8);
+          }
         } else {
-          if (16 * j < left) *reinterpret_cast<uint4*>(out + 16 * j) = make_uint4(u[0], u[1], u[2], u[3]);
-          if (16 * j + 8 < left) *reinterpret_cast<uint4*>(out + 16 * j + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (8 * j < left) *reinterpret_cast<uint4*>(out + 8 * j) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
         }
       }
+    }
+    if constexpr (kStaged) {
+      fence_proxy_async_smem();
+      mbar_arrive(&sh.y_staged);
     }
   };
 
@@ -288,6 +308,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       const int ha = x.h / pass.a.group, hb = x.h / pass.b.group, hc = x.h / pass.c.group;
       for (int c = 0; c < n; ++c) {
         const int s = c % kStAB, sc = c % kStC, row = x.row0 + first_row(c);
+        auto load_c = [&]() {
+          if (c >= kStC) mbar_wait(&sh.c_empty[sc], (c / kStC - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+          mbar_expect_tx(&sh.c_full[sc], kTileBytes);
+          tma_load_4d(sC + sc * kTileBytes, &pass.c.map, &sh.c_full[sc], x.c0, row, hc, batch);
+        };
+        if constexpr (kStC > 2) load_c();      // (in the order in which the buffers become free)
         if (c >= kStAB) mbar_wait(&sh.b_empty[s], (c / kStAB - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
         mbar_expect_tx(&sh.b_full[s], kAB);
         for (int nb = 0; nb < NB; ++nb) tma_load_4d(sB + s * kAB + nb * kTileBytes, &pass.b.map, &sh.b_full[s], nb * 64, row, hb, batch);
@@ -296,9 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           mbar_expect_tx(&sh.a_full[s], kAB);
           for (int nb = 0; nb < NB; ++nb) tma_load_4d(sA + s * kAB + nb * kTileBytes, &pass.a.map, &sh.a_full[s], nb * 64, row, ha, batch);
         }
-        if (c >= kStC) mbar_wait(&sh.c_empty[sc], (c / kStC - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        mbar_expect_tx(&sh.c_full[sc], kTileBytes);
-        tma_load_4d(sC + sc * kTileBytes, &pass.c.map, &sh.c_full[sc], x.c0, row, hc, batch);
+        if constexpr (kStC == 2) load_c();
       }
     }
     __syncwarp();
@@ -363,7 +387,24 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           for (int kk = 0; kk < kLinChunk / 16; ++kk)
             umma_ts_lohi(t_p + kColIn, t_p + kk * 8, c_lo + sc * (kTileBytes >> 4) + kk * 128u, mn_hi, idesc_in, kk > 0);
           umma_commit(&sh.o_done);
-          umma_commit(&sh.c_empty[sc]);
+          if constexpr (!kStaged) umma_commit(&sh.c_empty[sc]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 14) {
+    // ------------------------------------------------------------------ stores of whole chunks
+    reg_dealloc<kRegsControl>();
+    if constexpr (!STATES && kStaged) {
+      for (int c = 0; c < n; ++c) {
+        mbar_wait(&sh.y_staged, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        if (elect_one()) {
+          if (rows_of(c) == kLinChunk && !y_f32) {
+            tma_store_4d(&pass.map_y, sC + c % kStC * kTileBytes, x.c0, x.row0 + first_row(c), x.h, batch);
+            tma_store_commit();
+            tma_store_wait_read();
+          }
+          mbar_arrive(&sh.c_empty[c % kStC]);
         }
         __syncwarp();
       }
@@ -457,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       }
     }
   } else if (warp < 12) {
-    // ------------------------------------------------------------------ warps 4-7: the state; 8-11: weighted C; both: y
+    // ------------------------------------------------------------------ warps 4-7: the state, and y; 8-11: weighted C
     reg_alloc<kRegsWork>();
     const int row = tid & 127, lane = tid & 31;      // of the state, or of C
     const bool keeps_state = warp < 8;
@@ -598,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
 #pragma unroll 1
     for (int c = 0; c <= n; ++c) {
       if (!keeps_state && c < n) split(c);
-      if (!STATES && c > 0) write_y(c - 1, keeps_state ? 1 : 0);
+      if (!STATES && c > 0 && keeps_state) write_y(c - 1);
       if (keeps_state && c < n) advance(c + 1);
     }
     if (keeps_state && to != nullptr && row < p.D) {

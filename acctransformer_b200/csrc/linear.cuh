@@ -20,6 +20,7 @@ struct LinOperand {
 // (dy, v, k), dk (v, dy, q) reversed and dv (k, q, dy) reversed: one computation serves all four.
 struct LinPass {
   LinOperand a, b, c;
+  CUtensorMap map_y;                // (unused where y is fp32)
   void* y;
   int64_t y_stride[3];              // of batch entry, head and row
   int y_f32;                        // y is fp32 (partial gradients of shared heads), rows at multiples of 32 bytes

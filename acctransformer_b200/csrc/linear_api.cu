@@ -84,13 +84,14 @@ int make_pass(const acct_linear_args* a, const Rows& x, const Rows& y, const Row
   }
   return 0;
 }
-void set_output(const Rows& y, LinPass* pass) {
+int make_output(const acct_linear_args* a, const Rows& y, LinPass* pass) {
   pass->y = const_cast<void*>(y.ptr);
   pass->y_wide = (reinterpret_cast<uintptr_t>(y.ptr) & 31u) == 0;
   for (int i = 0; i < 3; ++i) {
     pass->y_stride[i] = y.stride[i];
     pass->y_wide = pass->y_wide && y.stride[i] % 16 == 0;
   }
+  return make_map(a, y, &pass->map_y);
 }
 
 // fp32 parts of dk and dv by query head, where heads share their keys and values
@@ -154,8 +155,7 @@ int acct_linear_fwd(const acct_linear_args* a, void* stream) {
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
   if (a->S == 0) return copy_states(a, stream);
-  if ((rc = make_pass(a, q, k, v, &p.pass[0]))) return rc;
-  set_output(y, &p.pass[0]);
+  if ((rc = make_pass(a, q, k, v, &p.pass[0])) || (rc = make_output(a, y, &p.pass[0]))) return rc;
   const cudaError_t e = launch_linear(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention kernel");
   return ACCT_OK;
@@ -188,10 +188,9 @@ int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
-  if ((rc = make_pass(a, d, v, k, &p.pass[0])) || (rc = make_pass(a, v, d, q, &p.pass[1])) || (rc = make_pass(a, k, q, d, &p.pass[2]))) return rc;
-  set_output(dq, &p.pass[0]);
-  set_output(dk, &p.pass[1]);
-  set_output(dv, &p.pass[2]);
+  if ((rc = make_pass(a, d, v, k, &p.pass[0])) || (rc = make_pass(a, v, d, q, &p.pass[1])) || (rc = make_pass(a, k, q, d, &p.pass[2])) ||
+      (rc = make_output(a, dq, &p.pass[0])) || (rc = make_output(a, dk, &p.pass[1])) || (rc = make_output(a, dv, &p.pass[2])))
+    return rc;
   p.pass[1].reverse = p.pass[2].reverse = 1;
   const int group = a->N / k.heads;
   LinReduce r;
