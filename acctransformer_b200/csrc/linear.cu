@@ -45,6 +45,11 @@ struct Item {
   int last;                 // nothing behind this segment (in the order of the pass)
 };
 
+struct LoadPlan {
+  const CUtensorMap *a, *b, *c;
+  int ha, hb, hc, row, step, batch, c0;
+};
+
 template <bool BF16>
 struct Shared {
   uint64_t a_full[3], a_empty[3], b_full[3], b_empty[3], c_full[4], c_empty[4];
@@ -53,9 +58,21 @@ struct Shared {
   volatile uint32_t abort_flag;
   Item item;
   float power[kLinChunk + 1];                                   // l^j
+  float chunk_power[4];                                         // that of a whole chunk, and of one that is not, as sums of two numbers
   float p_back[BF16 ? 1 : 2][BF16 ? 1 : kLinChunk], c_back[4], s_back[4];      // float16: 1 / the scales of a chunk
   uint32_t most[2][2][4];
 };
+
+// mbar_wait in fewer instructions, of which this kernel has many copies in one instruction cache: a wait that runs out leaves its code in the
+// block's abort flag, which ends all others, and the block records it before it retires.
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned int code) {
+  uint32_t polls = 0;
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (++polls >= kWaitPollLimit) *abort_flag = code;
+    if (*abort_flag != 0u) break;
+  }
+}
 
 // The power of two that brings `most` (>= 0) to [2^14, 2^15), and its inverse; 1 for 0 and what is not finite.
 __device__ __forceinline__ void near_top(float most, float& scale, float& back) {
@@ -105,14 +122,19 @@ __device__ __forceinline__ void store32(void* to, const uint32_t (&u)[8]) {
                : "memory");
 }
 
+// Blocks are numbered by columns of C, pass, head, and sequence or segment, fastest first: what reads the same rows runs at the same time.
+__device__ __forceinline__ int slices_of(const LinParams& p) { return (p.D + kCols - 1) / kCols; }
+__device__ __forceinline__ int pass_of_block(const LinParams& p) { return blockIdx.x / slices_of(p) % p.passes; }
+__device__ __forceinline__ int head_of_block(const LinParams& p) { return blockIdx.x / (slices_of(p) * p.passes) % p.N; }
+
 // What the block works on; by one warp.
 __device__ __forceinline__ Item find_item(const LinParams& p) {
-  const int lane = threadIdx.x & 31, slices = (p.D + kCols - 1) / kCols;
-  int at = blockIdx.x;
+  const int lane = threadIdx.x & 31;
   Item x;
-  x.c0 = at % slices * kCols; at /= slices;
-  x.pass = at % p.passes; at /= p.passes;
-  x.h = at % p.N; at /= p.N;
+  x.c0 = blockIdx.x % slices_of(p) * kCols;
+  x.pass = pass_of_block(p);
+  x.h = head_of_block(p);
+  const int at = blockIdx.x / (slices_of(p) * p.passes * p.N);
   x.chunks = 0; x.chunk0 = 0; x.slot = -1; x.last = 1;
   const bool reverse = p.pass[x.pass].reverse != 0;
   if (p.seg_chunks == 0) {
@@ -124,6 +146,7 @@ __device__ __forceinline__ Item find_item(const LinParams& p) {
         n[i] = -1;
         if (lane + 32 * i < p.B) lin_rows(p, lane + 32 * i, row, n[i]);
       }
+#pragma unroll 1
       for (int j = 0; j < p.B; ++j) {
         const int other = __shfl_sync(0xffffffffu, n[j >> 5], j & 31);
 #pragma unroll
@@ -140,6 +163,7 @@ __device__ __forceinline__ Item find_item(const LinParams& p) {
   x.b = -1;
   x.row0 = x.rows = 0;
   int left = at;
+#pragma unroll 1
   for (int b0 = 0; b0 < p.B && x.b < 0; b0 += 32) {      // the sequence that has the at-th segment
     int row = 0, n = 0;
     if (b0 + lane < p.B) lin_rows(p, b0 + lane, row, n);
@@ -187,45 +211,100 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
 
   const int tid = threadIdx.x;
   const int warp = static_cast<int>(warp_uniform(tid >> 5));
-  if (warp == 0) {
-    const Item x = find_item(p);
-    if (elect_one()) sh.item = x;
-  }
-  if (tid == 12 * 32) {
-    for (int i = 0; i < kStAB; ++i) {
-      mbar_init(&sh.a_full[i], 1); mbar_init(&sh.a_empty[i], 1);
-      mbar_init(&sh.b_full[i], 1); mbar_init(&sh.b_empty[i], 1);
+  volatile uint32_t* abort_flag = &sh.abort_flag;
+  // The loads of the c-th chunk, one by one as buffers become free.  The first ones are under way before the block has set itself up.
+  LoadPlan plan = {};
+  auto load = [&](int c) {
+    const int s = c % kStAB, sc = c % kStC, row = plan.row + c * plan.step;
+    if constexpr (kStC > 2) {      // (in the order in which the buffers become free)
+      if (c >= kStC) wait(&sh.c_empty[sc], (c / kStC - 1) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+      mbar_expect_tx(&sh.c_full[sc], kTileBytes);
+      tma_load_4d(sC + sc * kTileBytes, plan.c, &sh.c_full[sc], plan.c0, row, plan.hc, plan.batch);
     }
-    for (int i = 0; i < kStC; ++i) { mbar_init(&sh.c_full[i], 1); mbar_init(&sh.c_empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&sh.p_full[i], 1); mbar_init(&sh.p_ready[i], 128); }
-    mbar_init(&sh.split_ready, 128); mbar_init(&sh.inc_done, 1); mbar_init(&sh.inc_free, 128);
-    mbar_init(&sh.s_ready, 128); mbar_init(&sh.s_read, 1);
-    mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128); mbar_init(&sh.y_staged, 128);
-    sh.abort_flag = 0;
-    mbar_fence_init();
+    if (c >= kStAB) wait(&sh.b_empty[s], (c / kStAB - 1) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+    mbar_expect_tx(&sh.b_full[s], kAB);
+    for (int nb = 0; nb < NB; ++nb) tma_load_4d(sB + s * kAB + nb * kTileBytes, plan.b, &sh.b_full[s], nb * 64, row, plan.hb, plan.batch);
+    if constexpr (!STATES) {
+      if (c >= kStAB) wait(&sh.a_empty[s], (c / kStAB - 1) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+      mbar_expect_tx(&sh.a_full[s], kAB);
+      for (int nb = 0; nb < NB; ++nb) tma_load_4d(sA + s * kAB + nb * kTileBytes, plan.a, &sh.a_full[s], nb * 64, row, plan.ha, plan.batch);
+    }
+    if constexpr (kStC == 2) {
+      if (c >= kStC) wait(&sh.c_empty[sc], (c / kStC - 1) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+      mbar_expect_tx(&sh.c_full[sc], kTileBytes);
+      tma_load_4d(sC + sc * kTileBytes, plan.c, &sh.c_full[sc], plan.c0, row, plan.hc, plan.batch);
+    }
+  };
+  const int h = head_of_block(p);
+  if (warp == 12) {
+    if (elect_one()) {
+      const LinPass& pass = p.pass[pass_of_block(p)];
+      prefetch_tmap(&pass.b.map);
+      prefetch_tmap(&pass.c.map);
+      if (!STATES) prefetch_tmap(&pass.a.map);
+      for (int i = 0; i < kStAB; ++i) {
+        mbar_init(&sh.a_full[i], 1); mbar_init(&sh.a_empty[i], 1);
+        mbar_init(&sh.b_full[i], 1); mbar_init(&sh.b_empty[i], 1);
+      }
+      for (int i = 0; i < kStC; ++i) { mbar_init(&sh.c_full[i], 1); mbar_init(&sh.c_empty[i], 1); }
+      for (int i = 0; i < 2; ++i) { mbar_init(&sh.p_full[i], 1); mbar_init(&sh.p_ready[i], 128); }
+      mbar_init(&sh.split_ready, 128); mbar_init(&sh.inc_done, 1); mbar_init(&sh.inc_free, 128);
+      mbar_init(&sh.s_ready, 128); mbar_init(&sh.s_read, 1);
+      mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128); mbar_init(&sh.y_staged, 128);
+      sh.abort_flag = 0;
+      sh.s_back[0] = 1.f;
+      mbar_fence_init();
+    }
+    __syncwarp();
+    Item i = find_item(p);
+    // what leaves no trace: a block past the last segment; with STATES the last segment of a sequence whose state nobody asks for
+    if (i.b < 0 || (STATES && i.last && p.state_out == nullptr)) { i.b = -1; i.chunks = 0; }
+    const LinPass& pass = p.pass[i.pass];
+    const bool reverse = pass.reverse != 0;
+    plan.a = &pass.a.map; plan.b = &pass.b.map; plan.c = &pass.c.map;
+    plan.ha = i.h / pass.a.group; plan.hb = i.h / pass.b.group; plan.hc = i.h / pass.c.group;
+    plan.row = i.row0 + (i.chunk0 + (reverse ? i.chunks - 1 : 0)) * kLinChunk;
+    plan.step = reverse ? -kLinChunk : kLinChunk;
+    plan.batch = p.cu != nullptr ? 0 : i.b;
+    plan.c0 = i.c0;
+    if (elect_one()) {
+      sh.item = i;
+#pragma unroll 1
+      for (int c = 0; c < min(i.chunks, kStAB < kStC ? kStAB : kStC); ++c) load(c);
+    }
+    __syncwarp();
+    if ((tid & 31) < 2) {
+      const LinPower w = lin_power(p.log_decay[h], (tid & 31) == 0 ? kLinChunk : i.rows % kLinChunk);
+      sh.chunk_power[2 * (tid & 31)] = w.hi;
+      sh.chunk_power[2 * (tid & 31) + 1] = w.lo;
+      if ((tid & 31) == 0) sh.power[kLinChunk] = w.hi + w.lo;
+    }
+    __syncwarp();
+  } else if (warp == 13) {
+    tmem_alloc(&sh.tmem_base, 512);
+    tmem_relinquish();
   }
-  if (warp == 13) { tmem_alloc(&sh.tmem_base, 512); tmem_relinquish(); }
+  if (warp < 4) {
+    const LinPower w = lin_power(p.log_decay[h], tid);
+    sh.power[tid] = w.hi + w.lo;
+  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = warp_uniform(sh.tmem_base);
-  volatile uint32_t* abort_flag = &sh.abort_flag;
   const Item x = sh.item;
   const LinPass& pass = p.pass[x.pass];
   const bool reverse = pass.reverse != 0;
-  // what leaves no trace: a block past the last segment; with STATES the last segment of a sequence whose state nobody asks for
-  const bool idle = x.b < 0 || (STATES && x.last && p.state_out == nullptr);
-  const int n = idle ? 0 : x.chunks;
+  const bool idle = x.b < 0;
+  const int n = x.chunks;
   const int batch = p.cu != nullptr ? 0 : x.b;
+  // Nothing is before the first chunk, or nobody asks for what is behind the last one: the products that go with it are left out.
+  const bool has_first = x.slot >= 0 || p.state_in != nullptr;
+  const bool has_last = STATES || (x.slot < 0 && p.state_out != nullptr);
+  const int s0 = has_first ? 0 : 1;                // the first chunk that has a state before it
   // the c-th chunk in the order of the pass: its first row, and how many
   auto first_row = [&](int c) { return (x.chunk0 + (reverse ? n - 1 - c : c)) * kLinChunk; };
   auto rows_of = [&](int c) { return min(kLinChunk, x.rows - first_row(c)); };
-  if (tid < kLinChunk + 1 && !idle) {
-    const LinPower w = lin_power(p.log_decay[x.h], tid);
-    sh.power[tid] = w.hi + w.lo;
-  }
-  __syncthreads();
-
   void* const y = pass.y;
   const int64_t y_stride = pass.y_stride[2];
   const int64_t y_first = batch * pass.y_stride[0] + x.h * pass.y_stride[1] + (x.row0 + (tid & 127)) * y_stride + x.c0;
@@ -236,7 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     const uint32_t t_y = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     uint8_t* stage = sC + c % kStC * kTileBytes;
     float w = p.scale * sh.power[reverse ? max(rows - row, 0) : row + 1], in = p.scale;
-    mbar_wait(&sh.o_done, c & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+    wait(&sh.o_done, c & 1, abort_flag, DEV_TIMEOUT_MMA);
+    if (kStaged && c + 1 == n) wait(&sh.split_ready, c & 1, abort_flag, DEV_TIMEOUT_SYNC);      // (P C has not waited for it)
     tc_fence_after_sync();
     if constexpr (!BF16) {
       w *= sh.s_back[c & 3];
@@ -304,27 +384,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   if (warp == 12) {
     // ------------------------------------------------------------------ loads
     reg_dealloc<kRegsControl>();
-    if (elect_one()) {
-      const int ha = x.h / pass.a.group, hb = x.h / pass.b.group, hc = x.h / pass.c.group;
-      for (int c = 0; c < n; ++c) {
-        const int s = c % kStAB, sc = c % kStC, row = x.row0 + first_row(c);
-        auto load_c = [&]() {
-          if (c >= kStC) mbar_wait(&sh.c_empty[sc], (c / kStC - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-          mbar_expect_tx(&sh.c_full[sc], kTileBytes);
-          tma_load_4d(sC + sc * kTileBytes, &pass.c.map, &sh.c_full[sc], x.c0, row, hc, batch);
-        };
-        if constexpr (kStC > 2) load_c();      // (in the order in which the buffers become free)
-        if (c >= kStAB) mbar_wait(&sh.b_empty[s], (c / kStAB - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        mbar_expect_tx(&sh.b_full[s], kAB);
-        for (int nb = 0; nb < NB; ++nb) tma_load_4d(sB + s * kAB + nb * kTileBytes, &pass.b.map, &sh.b_full[s], nb * 64, row, hb, batch);
-        if constexpr (!STATES) {
-          if (c >= kStAB) mbar_wait(&sh.a_empty[s], (c / kStAB - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-          mbar_expect_tx(&sh.a_full[s], kAB);
-          for (int nb = 0; nb < NB; ++nb) tma_load_4d(sA + s * kAB + nb * kTileBytes, &pass.a.map, &sh.a_full[s], nb * 64, row, ha, batch);
-        }
-        if constexpr (kStC == 2) load_c();
-      }
-    }
+    if (elect_one())
+#pragma unroll 1
+      for (int c = kStAB < kStC ? kStAB : kStC; c < n; ++c) load(c);
     __syncwarp();
   } else if (warp == 13) {
     // ------------------------------------------------------------------ products
@@ -337,59 +399,76 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     const uint32_t a_lo = at(kmajor, sA), b_lo = at(kmajor, sB), bt_lo = at(mnmajor, sB), c_lo = at(mnmajor, sC);
     const uint32_t split_lo = at(mnmajor, sSplit), s_lo = at(mnmajor, sS);
     const int k_steps = (p.D + 15) / 16;
-    auto issue_p = [&](int c) {
-      const int s = c % kStAB;
-      const uint32_t off = s * (kAB >> 4);
-      mbar_wait(&sh.a_full[s], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-      mbar_wait(&sh.b_full[s], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-      if (elect_one()) {
-        for (int kk = 0; kk < k_steps; ++kk) {
-          const uint32_t o = off + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u;
-          umma_ss_lohi(tmem + kColP + (c & 1) * 128, a_lo + o, k_hi, b_lo + o, k_hi, idesc_p, kk > 0);
-        }
-        umma_commit(&sh.p_full[c & 1]);
-      }
-      __syncwarp();
-    };
-    if (!STATES && n > 0) issue_p(0);
-    for (int c = 0; c < n; ++c) {
-      const int s = c % kStAB, sc = c % kStC;
-      const uint32_t off = s * (kAB >> 4), t_p = tmem + kColP + (c & 1) * 128;
-      if constexpr (STATES) mbar_wait(&sh.b_full[s], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
-      if (c > 0) mbar_wait(&sh.inc_free, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-      mbar_wait(&sh.split_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-      tc_fence_after_sync();
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < kLinChunk / 16; ++kk)
-          umma_ss_lohi(tmem + kColState, bt_lo + off + kk * 128u, mn_hi, split_lo + kk * 128u, mn_hi, idesc_s, kk > 0);
-        umma_commit(&sh.inc_done);
-        umma_commit(&sh.b_empty[s]);
-        if constexpr (STATES) umma_commit(&sh.c_empty[sc]);
-      }
-      __syncwarp();
-      if constexpr (!STATES) {
-        mbar_wait(&sh.s_ready, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        if (c > 0) mbar_wait(&sh.o_free, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+    // (each product stands here once: the roles share an instruction cache)
+#pragma unroll 1
+    for (int j = STATES ? 0 : -1; j <= n; ++j) {
+      // B^T C of chunk j; of the last one behind what y needs, if at all
+      const int inc = STATES ? j : j < n - 1 ? j : j == n && has_last ? n - 1 : -1;
+      if (inc >= 0 && inc < n) {
+        const int s = inc % kStAB;
+        if constexpr (STATES) wait(&sh.b_full[s], (inc / kStAB) & 1, abort_flag, DEV_TIMEOUT_TMA);
+        if (inc > 0) wait(&sh.inc_free, (inc - 1) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+        wait(&sh.split_ready, inc & 1, abort_flag, DEV_TIMEOUT_SYNC);
         tc_fence_after_sync();
         if (elect_one()) {
-          for (int kk = 0; kk < k_steps; ++kk)
-            umma_ss_lohi(tmem + kColOut, a_lo + off + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u, k_hi, s_lo + kk * 128u, mn_hi, idesc_in, kk > 0);
-          umma_commit(&sh.s_read);
-          umma_commit(&sh.a_empty[s]);
-        }
-        __syncwarp();
-        if (c + 1 < n) issue_p(c + 1);      // (the P that it goes over has been consumed, as products run in the order of their issue, and P C read)
-        mbar_wait(&sh.p_ready[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
-        tc_fence_after_sync();
-        if (elect_one()) {
-#pragma unroll
+#pragma unroll 4
           for (int kk = 0; kk < kLinChunk / 16; ++kk)
-            umma_ts_lohi(t_p + kColIn, t_p + kk * 8, c_lo + sc * (kTileBytes >> 4) + kk * 128u, mn_hi, idesc_in, kk > 0);
-          umma_commit(&sh.o_done);
-          if constexpr (!kStaged) umma_commit(&sh.c_empty[sc]);
+            umma_ss_lohi(tmem + kColState, bt_lo + s * (kAB >> 4) + kk * 128u, mn_hi, split_lo + kk * 128u, mn_hi, idesc_s, kk > 0);
+          umma_commit(&sh.inc_done);
+          umma_commit(&sh.b_empty[s]);
+          if constexpr (STATES) umma_commit(&sh.c_empty[inc % kStC]);
         }
         __syncwarp();
+      }
+      if constexpr (!STATES) {
+        if (j >= 0 && j < n) {      // A S of chunk j
+          const int s = j % kStAB;
+          if (j >= s0) wait(&sh.s_ready, (j - s0) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+          if (j > 0) wait(&sh.o_free, (j - 1) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+          tc_fence_after_sync();
+          if (elect_one()) {
+            if (j >= s0) {
+#pragma unroll 2
+              for (int kk = 0; kk < k_steps; ++kk)
+                umma_ss_lohi(tmem + kColOut, a_lo + s * (kAB >> 4) + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u, k_hi, s_lo + kk * 128u, mn_hi, idesc_in, kk > 0);
+              umma_commit(&sh.s_read);
+            }
+            umma_commit(&sh.a_empty[s]);
+          }
+          __syncwarp();
+        }
+        if (j + 1 < n) {            // P of chunk j + 1 (what it goes over has been consumed, as products run in the order of their issue, and P C read)
+          const int c = j + 1, s = c % kStAB;
+          wait(&sh.a_full[s], (c / kStAB) & 1, abort_flag, DEV_TIMEOUT_TMA);
+          wait(&sh.b_full[s], (c / kStAB) & 1, abort_flag, DEV_TIMEOUT_TMA);
+          if (elect_one()) {
+#pragma unroll 2
+            for (int kk = 0; kk < k_steps; ++kk) {
+              const uint32_t o = s * (kAB >> 4) + (kk >> 2) * (kTileBytes >> 4) + (kk & 3) * 2u;
+              umma_ss_lohi(tmem + kColP + (c & 1) * 128, a_lo + o, k_hi, b_lo + o, k_hi, idesc_p, kk > 0);
+            }
+            umma_commit(&sh.p_full[c & 1]);
+          }
+          __syncwarp();
+        }
+        if (j >= 0 && j < n) {      // P C of chunk j
+          const int sc = j % kStC;
+          const uint32_t t_p = tmem + kColP + (j & 1) * 128;
+          if (j + 1 == n) {         // (its B^T C has not waited yet: for C, and for rows of C to be set to 0)
+            wait(&sh.c_full[sc], (j / kStC) & 1, abort_flag, DEV_TIMEOUT_TMA);
+            if (rows_of(j) < kLinChunk) wait(&sh.split_ready, j & 1, abort_flag, DEV_TIMEOUT_SYNC);
+          }
+          wait(&sh.p_ready[j & 1], (j >> 1) & 1, abort_flag, DEV_TIMEOUT_SYNC);
+          tc_fence_after_sync();
+          if (elect_one()) {
+#pragma unroll 4
+            for (int kk = 0; kk < kLinChunk / 16; ++kk)
+              umma_ts_lohi(t_p + kColIn, t_p + kk * 8, c_lo + sc * (kTileBytes >> 4) + kk * 128u, mn_hi, idesc_in, kk > 0);
+            umma_commit(&sh.o_done);
+            if constexpr (!kStaged) umma_commit(&sh.c_empty[sc]);
+          }
+          __syncwarp();
+        }
       }
     }
   } else if (warp == 14) {
@@ -397,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     reg_dealloc<kRegsControl>();
     if constexpr (!STATES && kStaged) {
       for (int c = 0; c < n; ++c) {
-        mbar_wait(&sh.y_staged, c & 1, abort_flag, p.status, DEV_TIMEOUT_SYNC);
+        wait(&sh.y_staged, c & 1, abort_flag, DEV_TIMEOUT_SYNC);
         if (elect_one()) {
           if (rows_of(c) == kLinChunk && !y_f32) {
             tma_store_4d(&pass.map_y, sC + c % kStC * kTileBytes, x.c0, x.row0 + first_row(c), x.h, batch);
@@ -433,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       for (int c = 0; c < n; ++c) {
         const int rows = rows_of(c);
         const uint32_t t = t_p + (c & 1) * 128;
-        mbar_wait(&sh.p_full[c & 1], (c >> 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+        wait(&sh.p_full[c & 1], (c >> 1) & 1, abort_flag, DEV_TIMEOUT_MMA);
         tc_fence_after_sync();
         // one block of 32 columns, weighted
         auto weighted = [&](int block, uint64_t (&v)[16]) {
@@ -459,38 +538,41 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
             }
           }
         };
+        // float16: the largest value of the row first
+        float most = 0.f;
         uint64_t scale2 = 0;
-        if constexpr (!BF16) {
-          float most = 0.f;
 #pragma unroll 1
-          for (int block = reverse ? warp : 0; block <= (reverse ? 3 : warp); ++block) {
-            uint64_t v[16];
+        for (int round = BF16 ? 4 : 0; round < 8; ++round) {
+          const int block = round & 3;
+          if constexpr (!BF16) {
+            if (round == 4) {
+              float scale, back;
+              near_top(most, scale, back);
+              scale2 = f2_pack(scale, scale);
+              sh.p_back[c & 1][tid] = back;
+            }
+          }
+          uint64_t v[16];
+          const bool seen = reverse ? block >= warp : block <= warp;
+          if (seen) {
             weighted(block, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0ull;
+          }
+          if (!BF16 && round < 4) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               float a, b;
               f2_unpack(v[j], a, b);
               most = fmax3(most, fabsf(a), fabsf(b));
             }
-          }
-          float scale, back;
-          near_top(most, scale, back);
-          scale2 = f2_pack(scale, scale);
-          sh.p_back[c & 1][tid] = back;
-        }
-#pragma unroll 1
-        for (int block = 0; block < 4; ++block) {
-          uint32_t pk[16];
-          if (reverse ? block >= warp : block <= warp) {
-            uint64_t v[16];
-            weighted(block, v);
+          } else {
+            uint32_t pk[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) pk[j] = narrow<BF16>(BF16 ? v[j] : f2_mul(v[j], scale2));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) pk[j] = 0u;
+            tmem_st16(t + block * 16, pk);      // (over scores that have been read, or that nobody needs)
           }
-          tmem_st16(t + block * 16, pk);      // (over scores that have been read, or that nobody needs)
         }
         tmem_wait_st();
         tc_fence_before_sync();
@@ -503,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     const int row = tid & 127, lane = tid & 31;      // of the state, or of C
     const bool keeps_state = warp < 8;
     const uint32_t t_s = tmem + kColState + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const LinPower step = idle ? LinPower{1.f, 0.f} : lin_power(p.log_decay[x.h], kLinChunk);
+    const LinPower step = {sh.chunk_power[0], sh.chunk_power[1]}, part = {sh.chunk_power[2], sh.chunk_power[3]};
     const int width = min(kCols, p.D - x.c0);      // columns that exist
     const int64_t one = (static_cast<int64_t>(x.b) * p.N + x.h) * p.D * p.D, mine = static_cast<int64_t>(row) * p.D + x.c0;
     const int64_t slot = ((static_cast<int64_t>(x.slot) * p.passes + x.pass) * p.N + x.h) * p.D * p.D;
@@ -521,9 +603,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     auto advance = [&](int c) {
       if (c > 0) {
         const int rows = rows_of(c - 1);
-        const LinPower w = rows == kLinChunk ? step : lin_power(p.log_decay[x.h], rows);
+        const LinPower w = rows == kLinChunk ? step : part;
         const uint64_t hi2 = f2_pack(w.hi, w.hi), lo2 = f2_pack(w.lo, w.lo);
-        mbar_wait(&sh.inc_done, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+        wait(&sh.inc_done, (c - 1) & 1, abort_flag, DEV_TIMEOUT_MMA);
         tc_fence_after_sync();
         uint64_t back2 = 0;
         if constexpr (!BF16) back2 = f2_pack(sh.c_back[(c - 1) & 3], sh.c_back[(c - 1) & 3]);
@@ -548,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           }
         }
       }
-      if (STATES || c == n) return;
+      if (STATES || c >= n) return;
       uint64_t scale2 = 0;
       if constexpr (!BF16) {
         float most = 0.f;
@@ -567,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         scale2 = f2_pack(scale, scale);
         if (row == 0) sh.s_back[c & 3] = back;
       }
-      if (c > 0) mbar_wait(&sh.s_read, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      if (c > s0) wait(&sh.s_read, (c - 1 - s0) & 1, abort_flag, DEV_TIMEOUT_MMA);
       if (row < DPAD) {
 #pragma unroll
         for (int j = 0; j < kCols / 8; ++j) {
@@ -586,9 +668,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       uint8_t *its_c = sC + c % kStC * kTileBytes, *its_b = sB + c % kStAB * kAB;
       const bool there = row < rows;
       float w = there ? sh.power[reverse ? row : rows - 1 - row] : 0.f;
-      mbar_wait(&sh.c_full[c % kStC], (c / kStC) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+      wait(&sh.c_full[c % kStC], (c / kStC) & 1, abort_flag, DEV_TIMEOUT_TMA);
       if (!there) {      // rows that are not this sequence's: 0 times what they hold might be a NaN
-        mbar_wait(&sh.b_full[c % kStAB], (c / kStAB) & 1, abort_flag, p.status, DEV_TIMEOUT_TMA);
+        wait(&sh.b_full[c % kStAB], (c / kStAB) & 1, abort_flag, DEV_TIMEOUT_TMA);
 #pragma unroll 1
         for (int j = 0; j < 8; ++j) {
           for (int nb = 0; nb < NB; ++nb) *reinterpret_cast<uint4*>(its_b + nb * kTileBytes + swz128(row, j)) = make_uint4(0u, 0u, 0u, 0u);
@@ -596,6 +678,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         }
       }
       __syncwarp();
+      if (c + 1 == n && !has_last) {      // into no state
+        if (c > 0) wait(&sh.inc_done, (c - 1) & 1, abort_flag, DEV_TIMEOUT_MMA);      // (the barrier's phase before has been seen)
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.split_ready);
+        return;
+      }
       if constexpr (!BF16) {
         uint32_t most = 0;      // of the absolute values, as 16-bit patterns, which have their order
 #pragma unroll
@@ -615,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         if (row == 0) sh.c_back[c & 3] = back;
       }
       const uint64_t w2 = f2_pack(w, w);
-      if (c > 0) mbar_wait(&sh.inc_done, (c - 1) & 1, abort_flag, p.status, DEV_TIMEOUT_MMA);
+      if (c > 0) wait(&sh.inc_done, (c - 1) & 1, abort_flag, DEV_TIMEOUT_MMA);
 #pragma unroll 2
       for (int j = 0; j < 8; ++j) {
         const uint4 raw = *reinterpret_cast<const uint4*>(its_c + swz128(row, j));
@@ -635,12 +723,24 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       fence_proxy_async_smem();
       mbar_arrive(&sh.split_ready);
     };
-    if (keeps_state) advance(0);
+    if (keeps_state && !has_first) {      // A S of the first chunk; these threads read it
+      uint32_t zero[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) zero[j] = 0u;
+      const uint32_t t_out = tmem + kColOut + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+      tmem_st32(t_out, zero);
+      tmem_st32(t_out + 32, zero);
+      tmem_wait_st();
+    }
+    if (keeps_state) {
 #pragma unroll 1
-    for (int c = 0; c <= n; ++c) {
-      if (!keeps_state && c < n) split(c);
-      if (!STATES && c > 0 && keeps_state) write_y(c - 1);
-      if (keeps_state && c < n) advance(c + 1);
+      for (int c = has_first && !STATES ? -1 : 0; c <= n; ++c) {      // (advance stands here once)
+        if (!STATES && c > 0) write_y(c - 1);
+        if (has_last ? c < n : c + 1 < n) advance(c + 1);
+      }
+    } else {
+#pragma unroll 1
+      for (int c = 0; c < n; ++c) split(c);
     }
     if (keeps_state && to != nullptr && row < p.D) {
 #pragma unroll
@@ -658,6 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   tc_fence_before_sync();
   linger_after_abort(abort_flag);
   __syncthreads();
+  if (tid == 0 && *abort_flag != 0u) atomicMax(p.status, *abort_flag);
   if (warp == 13) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, 512);

@@ -34,6 +34,7 @@ struct Rows {
   const void* ptr;
   int heads;
   int64_t stride[3];
+  CUtensorMap map;
 };
 
 int check_linear(const acct_linear_args* a, LinParams* p, Rows* q, Rows* k, Rows* v) {
@@ -51,9 +52,9 @@ int check_linear(const acct_linear_args* a, LinParams* p, Rows* q, Rows* k, Rows
   if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v)) return fail(ACCT_ERR_ALIGN, "q, k, v must be 16-byte aligned");
   if (!(a->scale > -1e30f) || !(a->scale < 1e30f)) return fail(ACCT_ERR_SHAPE, "scale must be a finite number");
   const int n_kv = a->N_kv > 0 ? a->N_kv : a->N;
-  *q = {"q", a->q, a->N, {0, 0, 0}};
-  *k = {"k", a->k, n_kv, {0, 0, 0}};
-  *v = {"v", a->v, n_kv, {0, 0, 0}};
+  *q = {"q", a->q, a->N, {0, 0, 0}, {}};
+  *k = {"k", a->k, n_kv, {0, 0, 0}, {}};
+  *v = {"v", a->v, n_kv, {0, 0, 0}, {}};
   if ((rc = strides_of("q", a->q_stride, a, a->N, q->stride)) || (rc = strides_of("k", a->k_stride, a, n_kv, k->stride)) ||
       (rc = strides_of("v", a->v_stride, a, n_kv, v->stride)))
     return rc;
@@ -66,25 +67,24 @@ int check_linear(const acct_linear_args* a, LinParams* p, Rows* q, Rows* k, Rows
   return 0;
 }
 
-int make_map(const acct_linear_args* a, const Rows& x, CUtensorMap* map) {
+int make_map(const acct_linear_args* a, Rows& x, CUtensorMap* map = nullptr) {
   TensorDesc4 t;
   t.ptr = x.ptr;
   t.dtype = a->dtype;
   t.dims[0] = a->D; t.dims[1] = a->S; t.dims[2] = x.heads; t.dims[3] = a->cu_seqlens != nullptr ? 1 : a->B;
   t.strides[0] = x.stride[2]; t.strides[1] = x.stride[1]; t.strides[2] = x.stride[0];
-  return make_tmap_4d(map, t, kLinChunk);
+  return make_tmap_4d(map != nullptr ? map : &x.map, t, kLinChunk);
 }
 
-int make_pass(const acct_linear_args* a, const Rows& x, const Rows& y, const Rows& z, LinPass* pass) {
+void set_pass(const acct_linear_args* a, const Rows& x, const Rows& y, const Rows& z, LinPass* pass) {
   const Rows* from[3] = {&x, &y, &z};
   LinOperand* to[3] = {&pass->a, &pass->b, &pass->c};
   for (int i = 0; i < 3; ++i) {
     to[i]->group = a->N / from[i]->heads;
-    if (const int rc = make_map(a, *from[i], &to[i]->map)) return rc;
+    to[i]->map = from[i]->map;
   }
-  return 0;
 }
-int make_output(const acct_linear_args* a, const Rows& y, LinPass* pass) {
+int make_output(const acct_linear_args* a, Rows& y, LinPass* pass) {
   pass->y = const_cast<void*>(y.ptr);
   pass->y_wide = (reinterpret_cast<uintptr_t>(y.ptr) & 31u) == 0;
   for (int i = 0; i < 3; ++i) {
@@ -145,7 +145,7 @@ int acct_linear_fwd(const acct_linear_args* a, void* stream) {
   if (rc) return rc;
   if (a->S > 0 && !a->y) return fail(ACCT_ERR_NULL, "y must be non-NULL");
   if (misaligned(a->y) || misaligned(a->state_in) || misaligned(a->state_out)) return fail(ACCT_ERR_ALIGN, "y and the states must be 16-byte aligned");
-  y = {"y", a->y, a->N, {0, 0, 0}};
+  y = {"y", a->y, a->N, {0, 0, 0}, {}};
   if ((rc = strides_of("y", a->y_stride, a, a->N, y.stride))) return rc;
   if ((rc = check_workspace(segments_of(a, 1, &p), a->workspace, a->workspace_bytes))) return rc;
   p.seg_states = static_cast<float*>(a->workspace);
@@ -155,7 +155,8 @@ int acct_linear_fwd(const acct_linear_args* a, void* stream) {
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
   if (a->S == 0) return copy_states(a, stream);
-  if ((rc = make_pass(a, q, k, v, &p.pass[0])) || (rc = make_output(a, y, &p.pass[0]))) return rc;
+  if ((rc = make_map(a, q)) || (rc = make_map(a, k)) || (rc = make_map(a, v)) || (rc = make_output(a, y, &p.pass[0]))) return rc;
+  set_pass(a, q, k, v, &p.pass[0]);
   const cudaError_t e = launch_linear(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "launching the linear attention kernel");
   return ACCT_OK;
@@ -179,8 +180,8 @@ int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void
   if ((rc = check_workspace(segment_bytes + partial_bytes(a), g->workspace, g->workspace_bytes))) return rc;
   p.seg_states = static_cast<float*>(g->workspace);
   const int64_t zero[3] = {0, 0, 0};
-  Rows d = {"d_y", g->d_y, a->N, {0, 0, 0}}, dq = {"dq", g->dq, a->N, {0, 0, 0}};
-  Rows dk = {"dk", g->dk, k.heads, {0, 0, 0}}, dv = {"dv", g->dv, k.heads, {0, 0, 0}};
+  Rows d = {"d_y", g->d_y, a->N, {0, 0, 0}, {}}, dq = {"dq", g->dq, a->N, {0, 0, 0}, {}};
+  Rows dk = {"dk", g->dk, k.heads, {0, 0, 0}, {}}, dv = {"dv", g->dv, k.heads, {0, 0, 0}, {}};
   if ((rc = strides_of("d_y", g->d_y_stride, a, a->N, d.stride)) || (rc = strides_of("dq", zero, a, a->N, dq.stride)) ||
       (rc = strides_of("dk", zero, a, k.heads, dk.stride)))
     return rc;
@@ -188,9 +189,11 @@ int acct_linear_bwd(const acct_linear_args* a, const acct_linear_bwd_io* g, void
   DeviceInfo info;
   if ((rc = device_info(&info))) return rc;
   p.status = device_status_ptr();
-  if ((rc = make_pass(a, d, v, k, &p.pass[0])) || (rc = make_pass(a, v, d, q, &p.pass[1])) || (rc = make_pass(a, k, q, d, &p.pass[2])) ||
-      (rc = make_output(a, dq, &p.pass[0])) || (rc = make_output(a, dk, &p.pass[1])) || (rc = make_output(a, dv, &p.pass[2])))
+  if ((rc = make_map(a, q)) || (rc = make_map(a, k)) || (rc = make_map(a, v)) || (rc = make_map(a, d)) || (rc = make_output(a, dq, &p.pass[0])) || (rc = make_output(a, dk, &p.pass[1])) || (rc = make_output(a, dv, &p.pass[2])))
     return rc;
+  set_pass(a, d, v, k, &p.pass[0]);
+  set_pass(a, v, d, q, &p.pass[1]);
+  set_pass(a, k, q, d, &p.pass[2]);
   p.pass[1].reverse = p.pass[2].reverse = 1;
   const int group = a->N / k.heads;
   LinReduce r;
@@ -278,7 +281,7 @@ int acct_rotary(const acct_rotary_args* a, void* stream) {
     p.t[w].x = t[w].x; p.t[w].y = t[w].y;
     p.t[w].heads = t[w].heads;
   }
-  if (rows > INT32_MAX || rows * (static_cast<int64_t>(a->N) + a->N_kv) * (a->D / 2) / 256 > INT32_MAX)
+  if (rows > INT32_MAX || static_cast<double>(rows) * (static_cast<double>(a->N) + a->N_kv) * a->D >= 0x1p34)      // (thread numbers have 32 bits)
     return fail(ACCT_ERR_SHAPE, "B*S = %lld rows are too many for one call", (long long)rows);
   p.positions = a->positions;
   for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->pos_stride[i];

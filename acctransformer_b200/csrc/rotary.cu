@@ -43,63 +43,86 @@ __device__ __forceinline__ typename Raw<VEC>::type repack(const float (&x)[VEC])
 }
 
 // A unit: VEC neighbouring values of a row (adjacent: VEC / 2 pairs), or VEC values and their VEC partners half of the turned part on;
-// behind those, VEC values that are copied.
-template <bool BF16, int VEC, bool ADJACENT>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, int units, int turned_units, int head_blocks) {
+// behind those, VEC values that are copied.  A thread has a unit of one row in HEADS heads, all of which it loads before it turns any.
+template <bool BF16, int VEC, bool ADJACENT, int HEADS>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p, unsigned int units, unsigned int turned_units,
+                                                          unsigned int q_blocks) {
   using R = typename Raw<VEC>::type;
   constexpr int kPairs = ADJACENT ? VEC / 2 : VEC;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int unit = static_cast<int>(i % units);
-  const int64_t rest = i / units;
-  const int hb = static_cast<int>(rest % head_blocks);
-  const int64_t row = rest / head_blocks;
-  if (row >= static_cast<int64_t>(p.B) * p.S) return;
-  const int b = static_cast<int>(row / p.S), s = static_cast<int>(row % p.S);
+  const bool is_k = blockIdx.x >= q_blocks;
+  const auto& t = is_k ? p.t[1] : p.t[0];
+  const unsigned int groups = (t.heads + HEADS - 1) / HEADS;
+  const unsigned int i = (blockIdx.x - (is_k ? q_blocks : 0u)) * kThreads + threadIdx.x;
+  const unsigned int unit = i % units, rest = i / units;
+  // (neighbouring rows lie beside each other where rows are packed by head, neighbouring heads where they are packed by row)
+  const bool by_head = t.x_stride[1] < t.x_stride[2];
+  const unsigned int rows = static_cast<unsigned int>(p.B) * p.S;
+  const unsigned int group = by_head ? rest % groups : rest / rows, row = by_head ? rest / groups : rest % rows;
+  if (group >= groups || row >= rows) return;
+  const unsigned int b = row / p.S, s = row % p.S;
   const bool copied = unit >= turned_units;
   const int pair0 = unit * kPairs, half = p.rotated / 2;
   const int d = copied ? p.rotated + (unit - turned_units) * VEC : ADJACENT ? unit * VEC : pair0;
-  float c[kPairs], sn[kPairs];
-  if (!copied) {
+  const int h0 = group * HEADS, heads = min(HEADS, t.heads - h0);
+  const uint16_t* x = static_cast<const uint16_t*>(t.x) + b * t.x_stride[0] + h0 * t.x_stride[1] + s * t.x_stride[2] + d;
+  uint16_t* y = static_cast<uint16_t*>(t.y) + b * t.y_stride[0] + h0 * t.y_stride[1] + s * t.y_stride[2] + d;
+  R r1[HEADS], r2[ADJACENT ? 1 : HEADS];
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      const long long pos = p.positions[p.axis[pair0 + j] * p.pos_stride[0] + b * p.pos_stride[1] + s * p.pos_stride[2]];
-      const long long turn = static_cast<long long>(static_cast<unsigned long long>(pos) * p.turns[pair0 + j]);      // of 2^64; as signed: in [-1/2, 1/2)
-      sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * (1.f / 2147483648.f), &sn[j], &c[j]);
-      if (p.inverse) sn[j] = -sn[j];
+  for (int h = 0; h < HEADS; ++h)
+    if (h < heads) {
+      r1[h] = *reinterpret_cast<const R*>(x + h * t.x_stride[1]);
+      if constexpr (!ADJACENT)
+        if (!copied) r2[h] = *reinterpret_cast<const R*>(x + h * t.x_stride[1] + half);
     }
+  if (copied) {
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+      if (h < heads) *reinterpret_cast<R*>(y + h * t.y_stride[1]) = r1[h];
+    return;
   }
-  const int heads = p.t[0].heads + p.t[1].heads;
-  for (int h = hb; h < heads; h += head_blocks) {
-    const int which = h >= p.t[0].heads;
-    const int hh = which ? h - p.t[0].heads : h;
-    const uint16_t* x = static_cast<const uint16_t*>(p.t[which].x) + b * p.t[which].x_stride[0] + hh * p.t[which].x_stride[1] + s * p.t[which].x_stride[2] + d;
-    uint16_t* y = static_cast<uint16_t*>(p.t[which].y) + b * p.t[which].y_stride[0] + hh * p.t[which].y_stride[1] + s * p.t[which].y_stride[2] + d;
-    const R r1 = *reinterpret_cast<const R*>(x);
-    if (copied) {
-      *reinterpret_cast<R*>(y) = r1;
-    } else if constexpr (ADJACENT) {
+  float c[kPairs], sn[kPairs];
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    const long long pos = p.positions[p.axis[pair0 + j] * p.pos_stride[0] + b * p.pos_stride[1] + s * p.pos_stride[2]];
+    const long long turn = static_cast<long long>(static_cast<unsigned long long>(pos) * p.turns[pair0 + j]);      // of 2^64; as signed: in [-1/2, 1/2)
+    sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * (1.f / 2147483648.f), &sn[j], &c[j]);
+    if (p.inverse) sn[j] = -sn[j];
+  }
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    if (h >= heads) break;
+    uint16_t* to = y + h * t.y_stride[1];
+    if constexpr (ADJACENT) {
       float v[VEC], o[VEC];
-      unpack<BF16, VEC>(r1, v);
+      unpack<BF16, VEC>(r1[h], v);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
         o[2 * j] = v[2 * j] * c[j] - v[2 * j + 1] * sn[j];
         o[2 * j + 1] = v[2 * j + 1] * c[j] + v[2 * j] * sn[j];
       }
-      *reinterpret_cast<R*>(y) = repack<BF16, VEC>(o);
+      *reinterpret_cast<R*>(to) = repack<BF16, VEC>(o);
     } else {
-      const R r2 = *reinterpret_cast<const R*>(x + half);
       float v1[VEC], v2[VEC], o1[VEC], o2[VEC];
-      unpack<BF16, VEC>(r1, v1);
-      unpack<BF16, VEC>(r2, v2);
+      unpack<BF16, VEC>(r1[h], v1);
+      unpack<BF16, VEC>(r2[h], v2);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         o1[j] = v1[j] * c[j] - v2[j] * sn[j];
         o2[j] = v2[j] * c[j] + v1[j] * sn[j];
       }
-      *reinterpret_cast<R*>(y) = repack<BF16, VEC>(o1);
-      *reinterpret_cast<R*>(y + half) = repack<BF16, VEC>(o2);
+      *reinterpret_cast<R*>(to) = repack<BF16, VEC>(o1);
+      *reinterpret_cast<R*>(to + half) = repack<BF16, VEC>(o2);
     }
   }
+}
+
+template <bool BF16, int VEC, bool ADJACENT, int HEADS>
+cudaError_t launch_heads(const RotaryParams& p, int units, int turned_units, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(p.B) * p.S * units;
+  unsigned int blocks[2];
+  for (int w = 0; w < 2; ++w) blocks[w] = static_cast<unsigned int>((rows * ((p.t[w].heads + HEADS - 1) / HEADS) + kThreads - 1) / kThreads);
+  rotary_kernel<BF16, VEC, ADJACENT, HEADS><<<blocks[0] + blocks[1], kThreads, 0, stream>>>(p, units, turned_units, blocks[0]);
+  return cudaGetLastError();
 }
 
 template <bool BF16, int VEC, bool ADJACENT>
@@ -107,12 +130,10 @@ cudaError_t launch(const RotaryParams& p, cudaStream_t stream) {
   const int turned_units = ADJACENT ? p.rotated / VEC : p.rotated / 2 / VEC;
   const bool in_place = p.t[0].x == p.t[0].y && p.t[1].x == p.t[1].y;      // (both null where there are no heads)
   const int units = turned_units + (in_place ? 0 : (p.D - p.rotated) / VEC);
-  const int heads = p.t[0].heads + p.t[1].heads;
-  const int64_t per_head = static_cast<int64_t>(p.B) * p.S * units;
-  const int head_blocks = per_head >= 148 * 2048 ? (heads + 7) / 8 : per_head * heads < 148 * 2048 ? heads : (heads + 1) / 2;
-  const int64_t blocks = (per_head * head_blocks + kThreads - 1) / kThreads;
-  rotary_kernel<BF16, VEC, ADJACENT><<<static_cast<unsigned int>(blocks), kThreads, 0, stream>>>(p, units, turned_units, head_blocks);
-  return cudaGetLastError();
+  // Sines and cosines for four heads at a time, unless there are so few rows that a head for each thread does not fill the SMs' 148 x 2 048.
+  const int64_t threads = static_cast<int64_t>(p.B) * p.S * units * (p.t[0].heads + p.t[1].heads);
+  return threads > 148 * 2048 ? launch_heads<BF16, VEC, ADJACENT, 4>(p, units, turned_units, stream)
+                              : launch_heads<BF16, VEC, ADJACENT, 1>(p, units, turned_units, stream);
 }
 
 template <bool BF16>

@@ -858,7 +858,7 @@ Tensor decays(const Tensor& g, int64_t N, const Tensor& q) {
              g.scalar_type(), " ", g.sizes());
   HOST_CHECK(!g.requires_grad() || !at::GradMode::is_enabled(), "log_decay has no gradient: give a detached tensor");
   TORCH_CHECK_NOT_IMPLEMENTED(!g._fw_grad(/*level=*/0).defined(), "linear attention does not support forward mode AD");
-  return g.to(at::kFloat).contiguous();
+  return g.scalar_type() == at::kFloat && g.is_contiguous() ? g : g.to(at::kFloat).contiguous();
 }
 
 void check_linear_inputs(const Tensor& q, const Tensor& k, const Tensor& v) {
