@@ -42,7 +42,7 @@ struct Item {
   int row0, rows;           // of the sequence
   int chunk0, chunks;       // of the segment
   int slot;                 // of the segment's state; -1: whole sequences
-  int last;                 // nothing behind this segment (in the order of the pass)
+  int first, last;          // nothing is before, or behind, this segment in the order of the pass
 };
 
 struct LoadPlan {
@@ -135,7 +135,7 @@ __device__ __forceinline__ Item find_item(const LinParams& p) {
   x.pass = pass_of_block(p);
   x.h = head_of_block(p);
   const int at = blockIdx.x / (slices_of(p) * p.passes * p.N);
-  x.chunks = 0; x.chunk0 = 0; x.slot = -1; x.last = 1;
+  x.chunks = 0; x.chunk0 = 0; x.slot = -1; x.first = x.last = 1;
   const bool reverse = p.pass[x.pass].reverse != 0;
   if (p.seg_chunks == 0) {
     x.b = at;
@@ -184,6 +184,7 @@ __device__ __forceinline__ Item find_item(const LinParams& p) {
       const int all = (x.rows + kLinChunk - 1) / kLinChunk;
       x.chunk0 = seg * p.seg_chunks;
       x.chunks = min(p.seg_chunks, all - x.chunk0);
+      x.first = reverse ? x.chunk0 + x.chunks == all : seg == 0;
       x.last = reverse ? seg == 0 : x.chunk0 + x.chunks == all;
     } else {
       left -= __shfl_sync(0xffffffffu, upto, 31);
@@ -257,8 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     }
     __syncwarp();
     Item i = find_item(p);
-    // what leaves no trace: a block past the last segment; with STATES the last segment of a sequence whose state nobody asks for
-    if (i.b < 0 || (STATES && i.last && p.state_out == nullptr)) { i.b = -1; i.chunks = 0; }
+    // what leaves no trace: a block past the last segment; with STATES the last segment of a sequence, which nothing comes behind
+    if (i.b < 0 || (STATES && i.last)) { i.b = -1; i.chunks = 0; }
     const LinPass& pass = p.pass[i.pass];
     const bool reverse = pass.reverse != 0;
     plan.a = &pass.a.map; plan.b = &pass.b.map; plan.c = &pass.c.map;
@@ -299,8 +300,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   const int n = x.chunks;
   const int batch = p.cu != nullptr ? 0 : x.b;
   // Nothing is before the first chunk, or nobody asks for what is behind the last one: the products that go with it are left out.
-  const bool has_first = x.slot >= 0 || p.state_in != nullptr;
-  const bool has_last = STATES || (x.slot < 0 && p.state_out != nullptr);
+  const bool has_first = !x.first || p.state_in != nullptr;
+  const bool has_last = STATES || (x.last && p.state_out != nullptr);
   const int s0 = has_first ? 0 : 1;                // the first chunk that has a state before it
   // the c-th chunk in the order of the pass: its first row, and how many
   auto first_row = [&](int c) { return (x.chunk0 + (reverse ? n - 1 - c : c)) * kLinChunk; };
@@ -589,8 +590,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     const int width = min(kCols, p.D - x.c0);      // columns that exist
     const int64_t one = (static_cast<int64_t>(x.b) * p.N + x.h) * p.D * p.D, mine = static_cast<int64_t>(row) * p.D + x.c0;
     const int64_t slot = ((static_cast<int64_t>(x.slot) * p.passes + x.pass) * p.N + x.h) * p.D * p.D;
-    const float* from = STATES || idle ? nullptr : x.slot >= 0 ? p.seg_states + slot : p.state_in != nullptr ? p.state_in + one : nullptr;
-    float* to = idle ? nullptr : STATES ? p.seg_states + slot : x.slot < 0 && p.state_out != nullptr ? p.state_out + one : nullptr;
+    const float* from = STATES || idle ? nullptr : !x.first ? p.seg_states + slot : p.state_in != nullptr ? p.state_in + one : nullptr;
+    float* to = idle ? nullptr : STATES ? p.seg_states + slot : has_last ? p.state_out + one : nullptr;
     uint64_t s[kCols / 2];
 #pragma unroll
     for (int j = 0; j < kCols / 4; ++j) {
@@ -765,7 +766,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   }
 }
 
-// What the segments leave, one by one, to the states before them, and the state behind the last; a thread has 4 neighbouring elements.
+// From what each segment alone leaves to the states before all but the first; a thread has 4 neighbouring elements.  (And sequences without
+// rows, which no block of the other kernel works on: their states stay as they are.)
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinParams p) {
   const int quads = p.D * p.D / 4, i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y % p.N, pass = blockIdx.y / p.N % p.passes, b = blockIdx.y / p.N / p.passes;
   int slot0 = 0, row0, rows;
@@ -778,24 +780,26 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   if (i >= quads) return;
   lin_rows(p, b, row0, rows);
   const int segs = (rows + per - 1) / per;
-  const bool reverse = p.pass[pass].reverse != 0;
-  const float g = p.log_decay[h];
   const int64_t one = (static_cast<int64_t>(b) * p.N + h) * quads + i, stride = static_cast<int64_t>(p.passes) * p.N * quads;
-  float4* slots = reinterpret_cast<float4*>(p.seg_states) + slot0 * stride + (static_cast<int64_t>(pass) * p.N + h) * quads + i;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (p.state_in != nullptr) s = reinterpret_cast<const float4*>(p.state_in)[one];
-  const LinPower whole = lin_power(g, per);
-  for (int at = 0; at < segs; ++at) {
-    const int seg = reverse ? segs - 1 - at : at;
-    const LinPower w = seg + 1 < segs ? whole : lin_power(g, rows - seg * per);
-    const bool last = at + 1 == segs;
-    float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!last || p.state_out != nullptr) add = slots[seg * stride];      // (the last one's is not there otherwise)
-    slots[seg * stride] = s;
+  if (segs == 0 && p.state_out != nullptr) reinterpret_cast<float4*>(p.state_out)[one] = s;
+  if (segs < 2) return;
+  const bool reverse = p.pass[pass].reverse != 0;
+  const float g = p.log_decay[h];
+  float4* slots = reinterpret_cast<float4*>(p.seg_states) + slot0 * stride + (static_cast<int64_t>(pass) * p.N + h) * quads + i;
+  auto slot = [&](int at) { return slots + (reverse ? segs - 1 - at : at) * stride; };
+  const LinPower whole = lin_power(g, per), first = reverse ? lin_power(g, rows - (segs - 1) * per) : whole;
+  float4 add = *slot(0);
+  for (int at = 0; at + 1 < segs; ++at) {
+    const LinPower w = at == 0 ? first : whole;      // (of a segment that is not whole, the last one, reversed the first)
+    float4 next = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at + 2 < segs) next = *slot(at + 1);         // (before its place is taken)
     s.x = fmaf(s.x, w.hi, fmaf(s.x, w.lo, add.x)); s.y = fmaf(s.y, w.hi, fmaf(s.y, w.lo, add.y));
     s.z = fmaf(s.z, w.hi, fmaf(s.z, w.lo, add.z)); s.w = fmaf(s.w, w.hi, fmaf(s.w, w.lo, add.w));
+    *slot(at + 1) = s;
+    add = next;
   }
-  if (p.state_out != nullptr) reinterpret_cast<float4*>(p.state_out)[one] = s;
 }
 
 // a thread: 4 neighbouring values
@@ -841,8 +845,25 @@ cudaError_t launch_all(const LinParams& p, cudaStream_t stream) {
 
 }  // namespace
 
+// In units of a chunk of the whole computation (1.6 us), of which a block has one SM to itself: a chunk of a segment's state alone takes half
+// of one, and the two launches more about 4.  (Packed sequences count as equally long, since the host does not know them.)
 void linear_segments(LinParams& p, int sm_count) {
+  const int64_t items = static_cast<int64_t>((p.D + kCols - 1) / kCols) * p.passes * p.N * p.B;
+  const int64_t rows = p.cu != nullptr ? (p.S + p.B - 1) / p.B : p.S, chunks = (rows + kLinChunk - 1) / kLinChunk;
+  auto waves = [&](int64_t blocks) { return (blocks + sm_count - 1) / sm_count; };
+  int64_t best = 2 * waves(items) * chunks, segs = 1;
+  for (int64_t n = 2; n <= chunks && items * (n - 1) < 2 * sm_count; ++n) {
+    const int64_t per = (chunks + n - 1) / n, cost = 2 * waves(items * n) * per + waves(items * (n - 1)) * per + 8;
+    if (cost < best) {
+      best = cost;
+      segs = n;
+    }
+  }
   p.seg_chunks = p.seg_slots = 0;
+  if (segs == 1) return;
+  const int64_t per = (chunks + segs - 1) / segs;
+  p.seg_chunks = static_cast<int>(per);
+  p.seg_slots = static_cast<int>(p.cu != nullptr ? p.S / (per * kLinChunk) + p.B : p.B * ((chunks + per - 1) / per));
 }
 
 cudaError_t launch_linear(const LinParams& p, bool bf16, cudaStream_t stream) {
