@@ -53,7 +53,7 @@ struct LoadPlan {
 template <bool BF16>
 struct Shared {
   uint64_t a_full[3], a_empty[3], b_full[3], b_empty[3], c_full[4], c_empty[4];
-  uint64_t p_full[2], p_ready[2], split_ready, inc_done, inc_free, s_ready, s_read, o_done, o_free, y_staged;
+  uint64_t p_full[2], p_ready[2], split_ready, inc_done, inc_free, s_ready, s_read, o_done, o_free, y_staged[4];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
   Item item;
@@ -247,11 +247,11 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         mbar_init(&sh.a_full[i], 1); mbar_init(&sh.a_empty[i], 1);
         mbar_init(&sh.b_full[i], 1); mbar_init(&sh.b_empty[i], 1);
       }
-      for (int i = 0; i < kStC; ++i) { mbar_init(&sh.c_full[i], 1); mbar_init(&sh.c_empty[i], 1); }
+      for (int i = 0; i < kStC; ++i) { mbar_init(&sh.c_full[i], 1); mbar_init(&sh.c_empty[i], 1); mbar_init(&sh.y_staged[i], 128); }
       for (int i = 0; i < 2; ++i) { mbar_init(&sh.p_full[i], 1); mbar_init(&sh.p_ready[i], 128); }
       mbar_init(&sh.split_ready, 128); mbar_init(&sh.inc_done, 1); mbar_init(&sh.inc_free, 128);
       mbar_init(&sh.s_ready, 128); mbar_init(&sh.s_read, 1);
-      mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128); mbar_init(&sh.y_staged, 128);
+      mbar_init(&sh.o_done, 1); mbar_init(&sh.o_free, 128);
       sh.abort_flag = 0;
       sh.s_back[0] = 1.f;
       mbar_fence_init();
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     }
     if constexpr (kStaged) {
       fence_proxy_async_smem();
-      mbar_arrive(&sh.y_staged);
+      mbar_arrive(&sh.y_staged[c % kStC]);
     }
   };
 
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     reg_dealloc<kRegsControl>();
     if constexpr (!STATES && kStaged) {
       for (int c = 0; c < n; ++c) {
-        wait(&sh.y_staged, c & 1, abort_flag, DEV_TIMEOUT_SYNC);
+        wait(&sh.y_staged[c % kStC], (c / kStC) & 1, abort_flag, DEV_TIMEOUT_SYNC);
         if (elect_one()) {
           if (rows_of(c) == kLinChunk && !y_f32) {
             tma_store_4d(&pass.map_y, sC + c % kStC * kTileBytes, x.c0, x.row0 + first_row(c), x.h, batch);

@@ -21,7 +21,7 @@ int strides_of(const char* name, const int64_t (&given)[3], const acct_linear_ar
   const bool packed = a->cu_seqlens != nullptr;
   const int64_t dense[3] = {D * S * heads, packed ? D : D * S, packed ? D * heads : D};
   for (int i = 0; i < 3; ++i) {
-    out[i] = packed_or(given[i], dense[i]);
+    out[i] = packed_or(given[i], std::max(dense[i], D));      // (no rows: nothing is read)
     if (out[i] < D) return fail(ACCT_ERR_SHAPE, "%s strides must not be smaller than head_dim", name);
     if (out[i] % 8 != 0) return fail(ACCT_ERR_ALIGN, "%s stride (%lld elements) is not a multiple of 8", name, (long long)out[i]);
   }

@@ -14,11 +14,13 @@
 #include <dlfcn.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
@@ -877,12 +879,18 @@ void check_linear_inputs(const Tensor& q, const Tensor& k, const Tensor& v) {
   for (int i = 0; i < 4; ++i) HOST_CHECK(q.size(i) >= 1 && q.size(i) <= INT32_MAX, "q must not be empty, got ", q.sizes());
 }
 
+// readable() of an operand that may also be packed from an address that is no multiple of 16 bytes
+Tensor readable_anywhere(const Tensor& t, int64_t (&strides)[3]) {
+  const Tensor x = readable(t, strides);
+  return at_16_bytes(x) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
 // The operands' part of the argument block; `q`, `k`, `v` become what the pointers point into.
 void fill_linear(acct_linear_args& a, Tensor& q, Tensor& k, Tensor& v, const Tensor& g, const LinearCall& call) {
   memset(&a, 0, sizeof(a));
   a.dtype = q.scalar_type() == at::kBFloat16 ? ACCT_BF16 : ACCT_F16;
   a.B = q.size(0); a.N = q.size(1); a.S = q.size(2); a.D = q.size(3); a.N_kv = k.size(1);
-  q = readable(q, a.q_stride); k = readable(k, a.k_stride); v = readable(v, a.v_stride);
+  q = readable_anywhere(q, a.q_stride); k = readable_anywhere(k, a.k_stride); v = readable_anywhere(v, a.v_stride);
   a.q = q.const_data_ptr(); a.k = k.const_data_ptr(); a.v = v.const_data_ptr();
   a.log_decay = static_cast<const float*>(g.const_data_ptr());
   if (call.lens.defined()) a.seq_lens = static_cast<const int32_t*>(call.lens.const_data_ptr());
@@ -931,7 +939,7 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
     fill_linear(a, q, k, v, log_decay, call);
     acct_linear_bwd_io io;
     memset(&io, 0, sizeof(io));
-    d_y = readable(d_y, io.d_y_stride);
+    d_y = readable_anywhere(d_y, io.d_y_stride);
     io.d_y = d_y.const_data_ptr();
     io.dq = dq.data_ptr(); io.dk = dk.data_ptr(); io.dv = dv.data_ptr();
     if ((io.workspace_bytes = g_lib.linear_bwd_workspace_bytes(&a)) > 0) {
@@ -939,7 +947,12 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
       io.workspace = ws.data_ptr();
     }
     check(g_lib.linear_bwd(&a, &io, stream_of(q)));
-    return {dq, dk, dv, Tensor(), Tensor()};
+    variable_list out = {dq, dk, dv};
+    if (at::GradMode::is_enabled()) {      // (create_graph: a gradient of these is an error, not nothing)
+      for (Tensor& t : out) t.set_requires_grad(true);
+      out = (*std::make_shared<torch::autograd::DelayedError>("linear attention has no second derivative", 3))(std::move(out));
+    }
+    return {out[0], out[1], out[2], Tensor(), Tensor()};
   }
 };
 
@@ -965,6 +978,16 @@ PyObject* py_linear_apply(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   return wrap(y);
   END_HANDLE_TH_ERRORS
+}
+
+// What a call writes is no memory that it reads as something else.  (Dense tensors; of others the caller knows.)
+void apart(const char* name, const Tensor& written, std::initializer_list<const Tensor*> read) {
+  for (const Tensor* t : read) {
+    if (!t->defined() || t->numel() == 0 || written.numel() == 0) continue;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(written.const_data_ptr()), b = reinterpret_cast<uintptr_t>(t->const_data_ptr());
+    const bool dense = written.is_non_overlapping_and_dense() && t->is_non_overlapping_and_dense();
+    HOST_CHECK(!(dense && a < b + t->nbytes() && b < a + written.nbytes()) && a != b, name, " must not share memory with the other operands");
+  }
 }
 
 // a state that a call moves on in place
@@ -1007,6 +1030,7 @@ PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
     memset(&a, 0, sizeof(a));
     if (state.defined()) {
       check_state(state, B, N, D, q);
+      apart("state", state, {&q, &k, &v, &cu, &g});
       a.state_in = static_cast<const float*>(state.const_data_ptr());
     } else {
       state = empty_like_shape({B, N, D, D}, at::kFloat, q);
@@ -1023,6 +1047,7 @@ PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (y.defined()) {
       require_on("out", y, q);
       HOST_CHECK(y.scalar_type() == dt && y.sizes() == q.sizes() && y.is_contiguous() && at_16_bytes(y), "out must be a contiguous tensor shaped and typed like q");
+      apart("out", y, {&q, &k, &v, &state});
     } else {
       y = empty_like_shape(q.sizes(), dt, q);
     }
@@ -1063,6 +1088,7 @@ PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     check_state(state, B, N, D, q);
     c10::cuda::OptionalCUDAGuard guard(q.device());
     g = decays(g, N, q);
+    apart("state", state, {&q, &k, &v, &g});
     acct_linear_step_args a;
     memset(&a, 0, sizeof(a));
     // (the stride of the one token may be anything)
@@ -1075,6 +1101,7 @@ PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
       require_on("out", y, q);
       HOST_CHECK(y.scalar_type() == q.scalar_type() && y.is_contiguous() && y.numel() == q.numel() && at_16_bytes(y),
                  "out must be a contiguous tensor with the dtype and the number of elements of q");
+      apart("out", y, {&q, &k, &v, &state});
     } else {
       y = empty_like_shape({B, N, 1, D}, q.scalar_type(), q);
     }
@@ -1115,7 +1142,7 @@ void rotary_launch(const RotaryCall& call, const Tensor (&x)[2], const Tensor (&
     if (!x[i].defined()) continue;
     int64_t(&xs)[3] = i == 0 ? a.q_stride : a.k_stride;
     int64_t(&ys)[3] = i == 0 ? a.q_out_stride : a.k_out_stride;
-    from[i] = readable(rotary_rows(x[i]), xs);
+    from[i] = readable_anywhere(rotary_rows(x[i]), xs);
     const Tensor to = rotary_rows(y[i]);
     for (int j = 0; j < 3; ++j) ys[j] = y[i].is_same(x[i]) ? xs[j] : to.stride(j);
     (i == 0 ? a.q : a.k) = from[i].const_data_ptr();
@@ -1136,12 +1163,12 @@ void rotary_launch(const RotaryCall& call, const Tensor (&x)[2], const Tensor (&
 Tensor rotary_result(const Tensor& t) { return t.defined() ? empty_like_shape(t.sizes(), t.scalar_type(), t) : Tensor(); }
 
 struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
-  static variable_list forward(AutogradContext* ctx, const std::optional<Tensor>& q, const std::optional<Tensor>& k, const RotaryCall& call) {
+  static variable_list forward(AutogradContext* ctx, const std::optional<Tensor>& q, const std::optional<Tensor>& k, const RotaryCall& call, bool inverse) {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x[2] = {q.value_or(Tensor()), k.value_or(Tensor())}, y[2] = {rotary_result(x[0]), rotary_result(x[1])};
-    rotary_launch(call, x, y, false);
+    rotary_launch(call, x, y, inverse);
     ctx->save_for_backward({call.positions, call.turns, call.axis});
-    ctx->saved_data["sizes"] = std::vector<int64_t>{call.head_dim, call.rotated, call.axes, call.adjacent, x[0].defined()};
+    ctx->saved_data["sizes"] = std::vector<int64_t>{call.head_dim, call.rotated, call.axes, call.adjacent, x[0].defined(), x[1].defined(), inverse};
     variable_list out;
     for (const Tensor& t : y)
       if (t.defined()) out.push_back(t);
@@ -1152,14 +1179,18 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     const std::vector<int64_t> sizes = ctx->saved_data.at("sizes").toIntVector();
     const variable_list saved = ctx->get_saved_variables();
     const RotaryCall call{saved[0], saved[1], saved[2], sizes[0], sizes[1], sizes[2], sizes[3]};
-    at::AutoDispatchBelowADInplaceOrView below;
-    Tensor x[2];
+    Tensor x[2], y[2];
     size_t at = 0;
-    if (sizes[4]) x[0] = grads[at++];
-    if (at < grads.size()) x[1] = grads[at];
-    const Tensor y[2] = {rotary_result(x[0]), rotary_result(x[1])};
-    if (x[0].defined() || x[1].defined()) rotary_launch(call, x, y, true);
-    return {y[0], y[1], Tensor()};
+    for (int i = 0; i < 2; ++i)
+      if (sizes[4 + i]) x[i] = grads[at++];
+    const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    if (x[0].defined() || x[1].defined()) {      // the turn back, differentiable itself
+      const variable_list out = RotaryFunction::apply(given(x[0]), given(x[1]), call, sizes[6] == 0);
+      at = 0;
+      for (int i = 0; i < 2; ++i)
+        if (x[i].defined()) y[i] = out[at++];
+    }
+    return {y[0], y[1], Tensor(), Tensor()};
   }
 };
 
@@ -1215,8 +1246,9 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (B * S > 0) {
         int64_t strides[3];
         for (const Tensor* t : both)
-          HOST_CHECK(!t->defined() || readable(rotary_rows(*t), strides).const_data_ptr() == t->const_data_ptr(),
+          HOST_CHECK(!t->defined() || readable_anywhere(rotary_rows(*t), strides).const_data_ptr() == t->const_data_ptr(),
                      "in place, rows must be contiguous, and addresses and strides whole 16 bytes");
+        if (q.defined()) apart("q", q, {&k});
         rotary_launch(call, {q, k}, {q, k}, false);
       }
       for (const Tensor* t : both)
@@ -1227,7 +1259,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     if (out.empty()) {
       const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-      out = RotaryFunction::apply(given(q), given(k), call);
+      out = RotaryFunction::apply(given(q), given(k), call, false);
     }
   }
   PyObject* r = PyTuple_New(2);
