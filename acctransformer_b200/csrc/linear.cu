@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           }
           __syncwarp();
         }
-        if (j + 1 < n) {            // P of chunk j + 1 (what it goes over has been consumed, as products run in the order of their issue, and P C read)
+        auto issue_p = [&]() {      // P of chunk j + 1 (what it goes over has been consumed, as products run in the order of their issue, and P C read)
           const int c = j + 1, s = c % kStAB;
           wait(&sh.a_full[s], (c / kStAB) & 1, abort_flag, DEV_TIMEOUT_TMA);
           wait(&sh.b_full[s], (c / kStAB) & 1, abort_flag, DEV_TIMEOUT_TMA);
@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
             umma_commit(&sh.p_full[c & 1]);
           }
           __syncwarp();
-        }
-        if (j >= 0 && j < n) {      // P C of chunk j
+        };
+        auto issue_pc = [&]() {     // P C of chunk j
           const int sc = j % kStC;
           const uint32_t t_p = tmem + kColP + (j & 1) * 128;
           if (j + 1 == n) {         // (its B^T C has not waited yet: for C, and for rows of C to be set to 0)
@@ -469,7 +469,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
             if constexpr (!kStaged) umma_commit(&sh.c_empty[sc]);
           }
           __syncwarp();
-        }
+        };
+        // P C first, which frees C early; float16, whose P takes the warps that weight it twice as long, gives them the time of P's product
+        // (2 x 32 heads, 8 192 tokens, with states: bfloat16 145 -> 137 us, float16 171 -> 146 us).
+        if (BF16 && j >= 0 && j < n) issue_pc();
+        if (j + 1 < n) issue_p();
+        if (!BF16 && j >= 0 && j < n) issue_pc();
       }
     }
   } else if (warp == 14) {
