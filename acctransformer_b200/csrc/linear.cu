@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (p.state_in != nullptr) s = reinterpret_cast<const float4*>(p.state_in)[one];
   if (segs == 0 && p.state_out != nullptr) reinterpret_cast<float4*>(p.state_out)[one] = s;
-  if (segs < 2) return;
+  if (segs < 2 || slot0 + segs > p.seg_slots) return;      // (sequences that share rows make more segments than there are slots)
   const bool reverse = p.pass[pass].reverse != 0;
   const float g = p.log_decay[h];
   float4* slots = reinterpret_cast<float4*>(p.seg_states) + slot0 * stride + (static_cast<int64_t>(pass) * p.N + h) * quads + i;

@@ -71,6 +71,12 @@ class LinearAttention(torch.nn.Module):
         self.head_num, self.head_dim, self.scale, self.rotary = head_num, head_dim, scale, rotary
         self.register_buffer("log_decay", log_decay.detach().clone())
 
+    def _apply(self, fn, recurse=True):
+        decays = self.log_decay
+        super()._apply(fn, recurse)
+        self.log_decay = decays.to(self.log_decay.device)      # in float32, whatever type the module is cast to
+        return self
+
     def forward(self, q, k, v, seq_lens=None, positions=None):
         if self.rotary is not None:
             if positions is None:

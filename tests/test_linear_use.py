@@ -235,6 +235,38 @@ def test_other_streams():
     assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
 
 
+@pytest.mark.parametrize("N,T", [(1, 4000), (16, 300)])
+def test_starts_that_are_no_starts(N, T):
+    """Rows that two sequences claim, starts that go back or leave the rows: nothing outside the outputs is touched."""
+    m, D = _ours(), 64
+    q, k, v = (_rand(T, N, D, dtype=torch.bfloat16, seed=s) for s in (1, 2, 3))
+    g = _decays(N, 6)
+    good = torch.tensor([0, T // 3, T], dtype=torch.int32, device="cuda")
+    want = m.linear_attention_packed(q, k, v, g, good)
+    for cu in ([0, T, 0, T, 0, T], [-5, T + 1000, 7, 3, 2 ** 31 - 1], [T, T - 1, 5, -2 ** 31], [0, 2 ** 31 - 1, -1, T]):
+        band = torch.full((3, T, N, D), 7.0, device="cuda", dtype=torch.bfloat16)
+        y, state = m.linear_attention_packed(q, k, v, g, torch.tensor(cu, dtype=torch.int32, device="cuda"), out=band[1])
+        torch.cuda.synchronize()
+        assert band[0].eq(7.0).all() and band[2].eq(7.0).all() and state.shape[0] == len(cu) - 1
+    assert all(torch.equal(a, b) for a, b in zip(m.linear_attention_packed(q, k, v, g, good), want))
+    from acctransformer_b200 import _lib
+    _lib.device_status()
+
+
+def test_inference_mode_and_casts():
+    m, N, D = _ours(), 4, 64
+    cell = m.LinearAttention(N, D, log_decay=[-0.1, -0.0123456, 0.0, -3.0], rotary=m.Rotary(D, (16, 16)))
+    assert cell.cuda().bfloat16().log_decay.dtype == torch.float32 and cell.log_decay.is_cuda
+    q, k, v = (_rand(2, N, 200, D, dtype=torch.bfloat16, seed=s) for s in (1, 2, 3))
+    want = cell(q, k, v)
+    with torch.inference_mode():
+        a, b, c = (t.clone() for t in (q, k, v))
+        assert torch.equal(cell(a, b, c), want)
+        state = torch.zeros(2, N, D, D, device="cuda")
+        cell.step(*(t[:, :, :1] for t in (a, b, c)), state, positions=torch.zeros(2, 2, 1, dtype=torch.int32, device="cuda"))
+        assert state.ne(0).any()
+
+
 def test_refusals():
     m = _ours()
     q, k, v, g, cu = _packed([64], 4, 2, 64, torch.bfloat16)
