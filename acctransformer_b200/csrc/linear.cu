@@ -856,15 +856,17 @@ cudaError_t launch_all(const LinParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// In units of a chunk of the whole computation (1.6 us), of which a block has one SM to itself: a chunk of a segment's state alone takes half
-// of one, and the two launches more about 4.  (Packed sequences count as equally long, since the host does not know them.)
+// In halves of a chunk of the whole computation (0.8 to 1.1 us), for which a block has one SM to itself: a chunk of a segment's state alone takes one, and
+// the two launches more, with what a block needs to begin and end, 20.  (Packed sequences count as equally long, since the host does not know
+// them.)  Cut or whole, us: 1 x 8 heads of 128, 2 048 tokens 33 and 39, 8 192 tokens 54 and 109, 1 x 16, 4 096 tokens 53 and 69; whole: 2 x 16, 4 096 tokens 72
+// (cut 80), 2 x 8, 2 048 tokens 39 (41), 1 x 1, 1 024 tokens 24 (25).
 void linear_segments(LinParams& p, int sm_count) {
   const int64_t items = static_cast<int64_t>((p.D + kCols - 1) / kCols) * p.passes * p.N * p.B;
   const int64_t rows = p.cu != nullptr ? (p.S + p.B - 1) / p.B : p.S, chunks = (rows + kLinChunk - 1) / kLinChunk;
   auto waves = [&](int64_t blocks) { return (blocks + sm_count - 1) / sm_count; };
   int64_t best = 2 * waves(items) * chunks, segs = 1;
   for (int64_t n = 2; n <= chunks && items * (n - 1) < 2 * sm_count; ++n) {
-    const int64_t per = (chunks + n - 1) / n, cost = 2 * waves(items * n) * per + waves(items * (n - 1)) * per + 8;
+    const int64_t per = (chunks + n - 1) / n, cost = 2 * waves(items * n) * per + waves(items * (n - 1)) * per + 20;
     if (cost < best) {
       best = cost;
       segs = n;
