@@ -601,7 +601,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     const int width = min(kCols, p.D - x.c0);      // columns that exist
     const int64_t one = (static_cast<int64_t>(x.b) * p.N + x.h) * p.D * p.D, mine = static_cast<int64_t>(row) * p.D + x.c0;
     const int64_t slot = ((static_cast<int64_t>(x.slot) * p.passes + x.pass) * p.N + x.h) * p.D * p.D;
-    const float* from = STATES || idle ? nullptr : !x.first ? p.seg_states + slot : p.state_in != nullptr ? p.state_in + one : nullptr;
+    // (of a sequence in several segments the first one reads a copy, too: the last one's block may be done before this one begins, and what it
+    // writes may be what the call was given)
+    const bool whole = x.first && x.last;
+    const float* from = STATES || idle || !has_first ? nullptr : whole ? p.state_in + one : p.seg_states + slot;
     float* to = idle ? nullptr : STATES ? p.seg_states + slot : has_last ? p.state_out + one : nullptr;
     uint64_t s[kCols / 2];
 #pragma unroll
@@ -777,8 +780,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   }
 }
 
-// From what each segment alone leaves to the states before all but the first; a thread has 4 neighbouring elements.  (And sequences without
-// rows, which no block of the other kernel works on: their states stay as they are.)
+// From what each segment alone leaves to the states before each of them, in its place; a thread has 4 neighbouring elements.  (And sequences
+// without rows, which no block of the other kernel works on: their states stay as they are.)
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinParams p) {
   const int quads = p.D * p.D / 4, i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y % p.N, pass = blockIdx.y / p.N % p.passes, b = blockIdx.y / p.N / p.passes;
   int slot0 = 0, row0, rows;
@@ -802,6 +805,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   auto slot = [&](int at) { return slots + (reverse ? segs - 1 - at : at) * stride; };
   const LinPower whole = lin_power(g, per), first = reverse ? lin_power(g, rows - (segs - 1) * per) : whole;
   float4 add = *slot(0);
+  if (p.state_in != nullptr) *slot(0) = s;             // (zeros otherwise, which nothing reads)
   for (int at = 0; at + 1 < segs; ++at) {
     const LinPower w = at == 0 ? first : whole;      // (of a segment that is not whole, the last one, reversed the first)
     float4 next = make_float4(0.f, 0.f, 0.f, 0.f);

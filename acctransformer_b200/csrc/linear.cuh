@@ -40,7 +40,7 @@ struct alignas(64) LinParams {
   float scale;
   unsigned int* status;
   // Sequences cut into segments of so many chunks; 0: whole.  The slots hold a state for each pass, segment and head, [slots, passes, N, D, D]:
-  // first what a segment alone leaves, then what is before it.
+  // first what a segment alone leaves, then what is before it (the first one's is a copy of state_in).
   int seg_chunks, seg_slots;
   float* seg_states;
 };
