@@ -13,7 +13,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, _traced
 
 __all__ = ["Rotary"]
 
@@ -65,8 +65,18 @@ class Rotary:
     def __call__(self, q, k, positions):
         """(q, k) turned, as new tensors; differentiable in both, either may be None.  ``positions``: integers [axes, T] for rows
         [T, heads, D], [axes, B, S] or [axes, S] for [B, heads, S, D]; with one axis that dimension may be missing."""
+        if torch.jit.is_tracing():
+            return self._recorded(q, k, positions)
         return _lib.host().rotary(q, k, positions, self.turns, self.axis, self._plan, False)
 
     def apply_(self, q, k, positions):
         """The same in place, without a gradient; rows must be contiguous, and addresses and strides whole 16 bytes."""
+        _traced.refuse("Rotary.apply_")
         return _lib.host().rotary(q, k, positions, self.turns, self.axis, self._plan, True)
+
+    def _recorded(self, q, k, positions):
+        out = list(_traced.call(self._defined, q, k, positions))
+        return tuple(None if x is None else out.pop(0) for x in (q, k))
+
+    def _defined(self, q, k, positions):
+        return tuple(x for x in _lib.host().rotary(q, k, positions, self.turns, self.axis, self._plan, False) if x is not None)
