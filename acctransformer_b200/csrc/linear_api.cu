@@ -281,7 +281,7 @@ int acct_rotary(const acct_rotary_args* a, void* stream) {
     p.t[w].x = t[w].x; p.t[w].y = t[w].y;
     p.t[w].heads = t[w].heads;
   }
-  if (rows > INT32_MAX || static_cast<double>(rows) * (static_cast<double>(a->N) + a->N_kv) * a->D >= 0x1p34)      // (thread numbers have 32 bits)
+  if (rows > INT32_MAX || static_cast<double>(rows) * (static_cast<double>(a->N) + a->N_kv) * a->D >= 0x1p34)      // (a few launches at most)
     return fail(ACCT_ERR_SHAPE, "B*S = %lld rows are too many for one call", (long long)rows);
   p.positions = a->positions;
   for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->pos_stride[i];

@@ -10,6 +10,8 @@
 // sines and cosines once; queries and keys go in one launch.
 // 2 x 8 192 rows of 32 + 8 heads of 128, there and back: 115 us, 89 % of the copy rate (a loop over eight heads, each loaded when the one before
 // was done: 192 us).
+#include <algorithm>
+
 #include "fa_common.cuh"
 #include "linear.cuh"
 
@@ -45,10 +47,11 @@ __device__ __forceinline__ typename Raw<VEC>::type repack(const float (&x)[VEC])
 }
 
 // A unit: VEC neighbouring values of a row (adjacent: VEC / 2 pairs), or VEC values and their VEC partners half of the turned part on;
-// behind those, VEC values that are copied.  A thread has a unit of one row in HEADS heads, all of which it loads before it turns any.
+// behind those, VEC values that are copied.  A thread has a unit of one row in HEADS heads, all of which it loads before it turns any.  A
+// launch has `rows` rows from row0 on, so few that threads can be counted in 32 bits (whose division is a fraction of that in 64).
 template <bool BF16, int VEC, bool ADJACENT, int HEADS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p, unsigned int units, unsigned int turned_units,
-                                                          unsigned int q_blocks) {
+                                                          unsigned int q_blocks, unsigned int row0, unsigned int rows) {
   using R = typename Raw<VEC>::type;
   constexpr int kPairs = ADJACENT ? VEC / 2 : VEC;
   const bool is_k = blockIdx.x >= q_blocks;
@@ -58,10 +61,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const unsigned int unit = i % units, rest = i / units;
   // (neighbouring rows lie beside each other where rows are packed by head, neighbouring heads where they are packed by row)
   const bool by_head = t.x_stride[1] < t.x_stride[2];
-  const unsigned int rows = static_cast<unsigned int>(p.B) * p.S;
-  const unsigned int group = by_head ? rest % groups : rest / rows, row = by_head ? rest / groups : rest % rows;
-  if (group >= groups || row >= rows) return;
-  const unsigned int b = row / p.S, s = row % p.S;
+  const unsigned int group = by_head ? rest % groups : rest / rows, at = by_head ? rest / groups : rest % rows;
+  if (group >= groups || at >= rows) return;
+  const unsigned int row = row0 + at, b = row / p.S, s = row % p.S;
   const bool copied = unit >= turned_units;
   const int pair0 = unit * kPairs, half = p.rotated / 2;
   const int d = copied ? p.rotated + (unit - turned_units) * VEC : ADJACENT ? unit * VEC : pair0;
@@ -120,11 +122,20 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 
 template <bool BF16, int VEC, bool ADJACENT, int HEADS>
 cudaError_t launch_heads(const RotaryParams& p, int units, int turned_units, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.B) * p.S * units;
-  unsigned int blocks[2];
-  for (int w = 0; w < 2; ++w) blocks[w] = static_cast<unsigned int>((rows * ((p.t[w].heads + HEADS - 1) / HEADS) + kThreads - 1) / kThreads);
-  rotary_kernel<BF16, VEC, ADJACENT, HEADS><<<blocks[0] + blocks[1], kThreads, 0, stream>>>(p, units, turned_units, blocks[0]);
-  return cudaGetLastError();
+  const int64_t rows = static_cast<int64_t>(p.B) * p.S;
+  int64_t threads[2];      // of a row
+  for (int w = 0; w < 2; ++w) threads[w] = static_cast<int64_t>(units) * ((p.t[w].heads + HEADS - 1) / HEADS);
+  const int64_t most = ((int64_t(1) << 32) - kThreads) / std::max(threads[0], threads[1]);      // rows of a launch
+  for (int64_t row0 = 0; row0 < rows; row0 += most) {
+    const int64_t n = std::min(rows - row0, most);
+    unsigned int blocks[2];
+    for (int w = 0; w < 2; ++w) blocks[w] = static_cast<unsigned int>((n * threads[w] + kThreads - 1) / kThreads);
+    rotary_kernel<BF16, VEC, ADJACENT, HEADS><<<blocks[0] + blocks[1], kThreads, 0, stream>>>(p, units, turned_units, blocks[0], static_cast<unsigned int>(row0),
+                                                                                              static_cast<unsigned int>(n));
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 template <bool BF16, int VEC, bool ADJACENT>
