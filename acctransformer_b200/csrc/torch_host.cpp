@@ -1127,6 +1127,39 @@ struct RotaryCall {
 // q or k as [B, heads, rows, D]
 Tensor rotary_rows(const Tensor& t) { return t.dim() == 3 ? t.transpose(0, 1).unsqueeze(0) : t; }
 
+// the operands that are there: rows of the plan's width, as many of one as of the other
+void check_rotary_rows(const Tensor& q, const Tensor& k, const RotaryCall& call) {
+  HOST_CHECK(q.defined() || k.defined(), "give q, k or both");
+  const Tensor& first = q.defined() ? q : k;
+  const Tensor* both[2] = {&q, &k};
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& t = *both[i];
+    const char* name = i == 0 ? "q" : "k";
+    if (!t.defined()) continue;
+    require_on(name, t, first);
+    HOST_CHECK((t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) && t.scalar_type() == first.scalar_type(),
+               "q and k must share dtype float16 or bfloat16");
+    HOST_CHECK((t.dim() == 3 || t.dim() == 4) && t.dim() == first.dim() && t.size(1) >= 1 && t.size(-1) == call.head_dim && t.size(0) == first.size(0) &&
+                   (t.dim() == 3 || t.size(2) == first.size(2)),
+               name, " must be [T, heads, ", call.head_dim, "] or [B, heads, S, ", call.head_dim, "], with as many rows as the other, got ", t.sizes());
+    for (int64_t size : t.sizes()) HOST_CHECK(size <= INT32_MAX, "too many rows");
+  }
+}
+
+// the table, and positions as the kernel reads them, [axes, batch entries or 1, rows] (`first`: an operand)
+void check_rotary_call(const RotaryCall& call, const Tensor& first) {
+  HOST_CHECK(call.turns.device() == first.device() && call.axis.device() == first.device(), "q and k must be on the device of the plan, ",
+             call.turns.device(), ", not on ", first.device());
+  for (const Tensor* t : {&call.turns, &call.axis})
+    HOST_CHECK(t->scalar_type() == (t == &call.turns ? at::kLong : at::kInt) && t->dim() == 1 && t->numel() == call.rotated / 2 && t->is_contiguous(),
+               "not a rotary plan");
+  require_on("positions", call.positions, first);
+  const Tensor& pos = call.positions;
+  const int64_t B = first.dim() == 4 ? first.size(0) : 1, S = first.dim() == 4 ? first.size(2) : first.size(0);
+  HOST_CHECK(pos.scalar_type() == at::kInt && pos.dim() == 3 && pos.size(0) == call.axes && (pos.size(1) == 1 || pos.size(1) == B) && pos.size(2) == S,
+             "positions do not go with the rows: ", pos.scalar_type(), " ", pos.sizes(), " for ", first.sizes());
+}
+
 // Turns `x` (undefined ones are left out) into `y`.
 void rotary_launch(const RotaryCall& call, const Tensor (&x)[2], const Tensor (&y)[2], bool inverse) {
   acct_rotary_args a;
@@ -1167,7 +1200,9 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x[2] = {q.value_or(Tensor()), k.value_or(Tensor())}, y[2] = {rotary_result(x[0]), rotary_result(x[1])};
     rotary_launch(call, x, y, inverse);
-    ctx->save_for_backward({call.positions, call.turns, call.axis});
+    ctx->save_for_backward({call.positions});
+    ctx->saved_data["turns"] = call.turns;      // (the plan's own: no hook of a user's sees them)
+    ctx->saved_data["axis"] = call.axis;
     ctx->saved_data["sizes"] = std::vector<int64_t>{call.head_dim, call.rotated, call.axes, call.adjacent, x[0].defined(), x[1].defined(), inverse};
     variable_list out;
     for (const Tensor& t : y)
@@ -1178,13 +1213,15 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const std::vector<int64_t> sizes = ctx->saved_data.at("sizes").toIntVector();
     const variable_list saved = ctx->get_saved_variables();
-    const RotaryCall call{saved[0], saved[1], saved[2], sizes[0], sizes[1], sizes[2], sizes[3]};
+    const RotaryCall call{saved[0], ctx->saved_data.at("turns").toTensor(), ctx->saved_data.at("axis").toTensor(), sizes[0], sizes[1], sizes[2], sizes[3]};
     Tensor x[2], y[2];
     size_t at = 0;
     for (int i = 0; i < 2; ++i)
       if (sizes[4 + i]) x[i] = grads[at++];
     const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     if (x[0].defined() || x[1].defined()) {      // the turn back, differentiable itself
+      check_rotary_rows(x[0], x[1], call);       // (hooks may have handed back others)
+      check_rotary_call(call, x[0].defined() ? x[0] : x[1]);
       const variable_list out = RotaryFunction::apply(given(x[0]), given(x[1]), call, sizes[6] == 0);
       at = 0;
       for (int i = 0; i < 2; ++i)
@@ -1210,23 +1247,11 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   variable_list out;
   {
     pybind11::gil_scoped_release no_gil;
-    HOST_CHECK(q.defined() || k.defined(), "give q, k or both");
+    check_rotary_rows(q, k, call);
     const Tensor& first = q.defined() ? q : k;
     const Tensor* both[2] = {&q, &k};
-    for (int i = 0; i < 2; ++i) {
-      const Tensor& t = *both[i];
-      const char* name = i == 0 ? "q" : "k";
-      if (!t.defined()) continue;
-      require_on(name, t, first);
-      HOST_CHECK((t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) && t.scalar_type() == first.scalar_type(),
-                 "q and k must share dtype float16 or bfloat16");
-      HOST_CHECK((t.dim() == 3 || t.dim() == 4) && t.dim() == first.dim() && t.size(1) >= 1 && t.size(-1) == call.head_dim && t.size(0) == first.size(0) &&
-                     (t.dim() == 3 || t.size(2) == first.size(2)),
-                 name, " must be [T, heads, ", call.head_dim, "] or [B, heads, S, ", call.head_dim, "], with as many rows as the other, got ", t.sizes());
-      for (int64_t size : t.sizes()) HOST_CHECK(size <= INT32_MAX, "too many rows");
-      TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), "rotary positions do not support forward mode AD");
-    }
-    HOST_CHECK(call.turns.device() == first.device(), "q and k must be on the device of the plan, ", call.turns.device(), ", not on ", first.device());
+    for (const Tensor* t : both)
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "rotary positions do not support forward mode AD");
     const int64_t B = first.dim() == 4 ? first.size(0) : 1, S = first.dim() == 4 ? first.size(2) : first.size(0);
     c10::cuda::OptionalCUDAGuard guard(first.device());
     Tensor pos = call.positions;      // (as a view that shares its version counter: a change before the backward is noticed)
@@ -1241,6 +1266,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
       HOST_CHECK(first.dim() == 4 && is({call.axes, B, S}), "positions must be [", call.axes, " axes, ", first.dim() == 4 ? "batch entries, " : "", S,
                  " rows]", call.axes == 1 ? " or [rows]" : "", ", got ", pos.sizes());
     call.positions = pos.scalar_type() == at::kInt ? pos : pos.to(at::kInt);
+    check_rotary_call(call, first);
     if (in_place || B * S == 0) {
       at::AutoDispatchBelowADInplaceOrView below;
       if (B * S > 0) {
