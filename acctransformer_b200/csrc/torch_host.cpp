@@ -1009,7 +1009,7 @@ PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), g = tensor_arg(args[3], "log_decay");
   Tensor cu = tensor_arg(args[4], "cu_seqlens"), state = tensor_or_undefined(args[5]), y = tensor_or_undefined(args[7]);
   const double scale = float_arg(args[6]);
-  no_gradient("linear_attention_packed", {&q, &k, &v, &state});
+  no_gradient("linear_attention_packed", {&q, &k, &v, &state, &y});
   {
     pybind11::gil_scoped_release no_gil;
     at::AutoDispatchBelowADInplaceOrView below;
@@ -1047,7 +1047,7 @@ PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (y.defined()) {
       require_on("out", y, q);
       HOST_CHECK(y.scalar_type() == dt && y.sizes() == q.sizes() && y.is_contiguous() && at_16_bytes(y), "out must be a contiguous tensor shaped and typed like q");
-      apart("out", y, {&q, &k, &v, &state});
+      apart("out", y, {&q, &k, &v, &state, &cu, &g});
     } else {
       y = empty_like_shape(q.sizes(), dt, q);
     }
@@ -1062,7 +1062,7 @@ PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
       a.workspace = ws.data_ptr();
     }
     check(g_lib.linear_fwd(&a, stream_of(q)));
-    written(state);
+    written(state); written(y);
   }
   PyObject* out = PyTuple_New(2);
   PyTuple_SET_ITEM(out, 0, wrap(y));
@@ -1078,7 +1078,7 @@ PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), g = tensor_arg(args[3], "log_decay");
   Tensor state = tensor_arg(args[4], "state"), y = tensor_or_undefined(args[6]);
   const double scale = float_arg(args[5]);
-  no_gradient("linear_attention_step", {&q, &k, &v, &state});
+  no_gradient("linear_attention_step", {&q, &k, &v, &state, &y});
   {
     pybind11::gil_scoped_release no_gil;
     at::AutoDispatchBelowADInplaceOrView below;
@@ -1101,7 +1101,7 @@ PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
       require_on("out", y, q);
       HOST_CHECK(y.scalar_type() == q.scalar_type() && y.is_contiguous() && y.numel() == q.numel() && at_16_bytes(y),
                  "out must be a contiguous tensor with the dtype and the number of elements of q");
-      apart("out", y, {&q, &k, &v, &state});
+      apart("out", y, {&q, &k, &v, &state, &g});
     } else {
       y = empty_like_shape({B, N, 1, D}, q.scalar_type(), q);
     }
@@ -1112,7 +1112,7 @@ PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.log_decay = static_cast<const float*>(g.const_data_ptr());
     a.scale = static_cast<float>(scale);
     check(g_lib.linear_step(&a, stream_of(q)));
-    written(state);
+    written(state); written(y);
   }
   return wrap(y);
   END_HANDLE_TH_ERRORS
