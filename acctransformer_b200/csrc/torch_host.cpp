@@ -14,7 +14,6 @@
 #include <dlfcn.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -980,13 +979,31 @@ PyObject* py_linear_apply(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// What a call writes is no memory that it reads as something else.  (Dense tensors; of others the caller knows.)
+// Does any element of a strided tensor from `dim` on, that begins at `at`, lie in [from, to)?  (strides are not negative)
+bool lies_in(const Tensor& t, int64_t dim, uintptr_t at, uintptr_t from, uintptr_t to) {
+  const int64_t size = static_cast<int64_t>(t.element_size());
+  int64_t span = size;      // from the first byte to behind the last one
+  for (int64_t d = dim; d < t.dim(); ++d) span += (t.size(d) - 1) * t.stride(d) * size;
+  if (at >= to || at + span <= from) return false;
+  if (at >= from || dim == t.dim()) return true;      // (an element, as large as its span, meets; a first element inside does, too)
+  const int64_t step = t.stride(dim) * size;
+  if (step == 0) return lies_in(t, dim + 1, at, from, to);
+  // of this dimension's entries those whose span may reach the interval
+  const int64_t rest = span - (t.size(dim) - 1) * step, before = static_cast<int64_t>(from - at) - rest;
+  for (int64_t i = before < 0 ? 0 : before / step; i < t.size(dim) && at + i * step < to; ++i)
+    if (lies_in(t, dim + 1, at + i * step, from, to)) return true;
+  return false;
+}
+
+// What a call writes is no memory that it reads as something else.  (Of two that both have gaps, as q and k behind one projection do, only the
+// same beginning is refused.)
 void apart(const char* name, const Tensor& written, std::initializer_list<const Tensor*> read) {
+  const auto begin = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
+  const auto in = [&](const Tensor& t, const Tensor& dense) { return lies_in(t, 0, begin(t), begin(dense), begin(dense) + dense.nbytes()); };
   for (const Tensor* t : read) {
     if (!t->defined() || t->numel() == 0 || written.numel() == 0) continue;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(written.const_data_ptr()), b = reinterpret_cast<uintptr_t>(t->const_data_ptr());
-    const bool dense = written.is_non_overlapping_and_dense() && t->is_non_overlapping_and_dense();
-    HOST_CHECK(!(dense && a < b + t->nbytes() && b < a + written.nbytes()) && a != b, name, " must not share memory with the other operands");
+    const bool shared = written.is_non_overlapping_and_dense() ? in(*t, written) : t->is_non_overlapping_and_dense() && in(written, *t);
+    HOST_CHECK(begin(*t) != begin(written) && !shared, name, " must not share memory with the other operands");
   }
 }
 
