@@ -2,7 +2,7 @@
 //
 //   y1 = x1 cos - x2 sin,   y2 = x2 cos + x1 sin;   the way back of a gradient is the turn by minus the angle
 //
-// The frequency is a fraction of a turn in units of 2^-64, so position * frequency modulo a turn is one 64-bit product, exact
+// The frequency is the nearest fraction of a turn in units of 2^-64, so position * frequency modulo a turn is one 64-bit product, exact
 // to position * 2^-65 turns whatever the position; the sine and cosine of its leading 24 bits are good to 2^-23, also where position *
 // frequency in fp32 would have lost the angle (from some 10^5 on).
 //

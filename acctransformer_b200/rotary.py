@@ -9,6 +9,7 @@ The reference has no counterpart (its cells know positions by ``alibi`` only).
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -18,6 +19,31 @@ from . import _lib, _traced
 __all__ = ["Rotary"]
 
 MAX_HEAD_DIM = 256
+
+
+@functools.lru_cache(maxsize=8)
+def _two_pi(bits):
+    """2 pi times 2^bits, off by less than one (Machin: pi / 4 = 4 atan(1/5) - atan(1/239))."""
+    guard = 32
+
+    def atan_inverse(n):      # atan(1 / n), its series, truncated term by term
+        power = (1 << (bits + guard)) // n
+        total, k = power, 1
+        while power:
+            power //= n * n
+            total += (-power if k % 2 else power) // (2 * k + 1)
+            k += 1
+        return total
+    return (8 * (4 * atan_inverse(5) - atan_inverse(239))) >> guard
+
+
+def turns_of(frequency):
+    """Turns per position modulo one, in units of 2^-64, nearest to frequency / 2 pi as it is, as a signed 64-bit number."""
+    numerator, denominator = float(frequency).as_integer_ratio()
+    bits = 96 + max(0, numerator.bit_length() - denominator.bit_length())      # (what a large frequency multiplies)
+    period = denominator * _two_pi(bits)
+    turns = ((numerator << (64 + bits)) + period // 2) // period % 2 ** 64
+    return turns - 2 ** 64 if turns >= 2 ** 63 else turns
 
 
 class Rotary:
@@ -52,9 +78,7 @@ class Rotary:
             if len(frequencies) != pairs or not all(math.isfinite(f) for f in frequencies):
                 raise ValueError(f"frequencies must be {pairs} finite numbers, one for each pair")
         self.head_dim, self.rotary_dim, self.sections, self.adjacent = head_dim, 2 * pairs, sections, bool(adjacent)
-        # turns per position modulo one, in units of 2^-64
-        turns = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % 2 ** 64 for f in frequencies]
-        turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
+        turns = [turns_of(f) for f in frequencies]
         axis = [a for a, n in enumerate(sections) for _ in range(n)]
         self.turns = torch.tensor(turns, dtype=torch.int64, device=device)
         self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
