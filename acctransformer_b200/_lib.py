@@ -36,6 +36,7 @@ EXPORTS = [
     "acct_infer_packed", "acct_kv4_record_bytes", "acct_kv4_append", "acct_kv4_read", "acct_kv4_decode_workspace_bytes", "acct_kv4_decode",
     "acct_kv4_evict",
     "acct_linear_fwd_workspace_bytes", "acct_linear_fwd", "acct_linear_bwd_workspace_bytes", "acct_linear_bwd", "acct_linear_step", "acct_rotary",
+    "acct_rotary_wide",
 ] + [f"acct_ms_fa_{kind}_s{k}" for k in range(32) for kind in ("fwd", "grad")]
 
 
@@ -262,6 +263,8 @@ def load():
     lib.acct_linear_step.restype = C.c_int
     lib.acct_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
     lib.acct_rotary.restype = C.c_int
+    lib.acct_rotary_wide.argtypes = [C.POINTER(RotaryArgs), C.c_void_p, C.c_void_p]
+    lib.acct_rotary_wide.restype = C.c_int
     lib.acct_abi_version.argtypes = []
     lib.acct_abi_version.restype = C.c_int
     if lib.acct_abi_version() != ABI_VERSION:

@@ -109,7 +109,8 @@ struct RotaryParams {
     int64_t x_stride[3], y_stride[3];      // of batch entry, head, row
     int heads;
   } t[2];
-  const int* positions;             // [axes] x rows, with element strides
+  const int* positions;             // [axes] x rows, with element strides; or null ...
+  const long long* wide_positions;  // ... of 64 bits
   int64_t pos_stride[3];            // of axis, batch entry, row
   const unsigned long long* turns;  // [rotated / 2]: turns per position, as a fraction of 2^64
   const int* axis;                  // [rotated / 2]

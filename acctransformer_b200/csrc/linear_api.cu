@@ -129,6 +129,53 @@ int copy_states(const acct_linear_args* a, void* stream) {
   return e == cudaSuccess ? ACCT_OK : fail_cuda(e, "copying the states");
 }
 
+// positions of 32 or of 64 bits
+int rotary(const acct_rotary_args* a, const int32_t* positions, const int64_t* wide, void* stream) {
+  if (a == nullptr) return fail(ACCT_ERR_NULL, "args is NULL");
+  if (a->dtype != ACCT_F16 && a->dtype != ACCT_BF16) return fail(ACCT_ERR_DTYPE, "dtype must be ACCT_F16 or ACCT_BF16");
+  if (a->B < 0 || a->S < 0 || a->N < 0 || a->N_kv < 0) return fail(ACCT_ERR_SHAPE, "sizes must not be negative");
+  if (a->D <= 0 || a->D % 8 != 0 || a->D > 256) return fail(ACCT_ERR_UNSUPPORTED_D, "head_dim %d must be a multiple of 8 in (0, 256]", a->D);
+  if (a->rotated <= 0 || a->rotated % 2 != 0 || a->rotated > a->D) return fail(ACCT_ERR_SHAPE, "rotated = %d must be even, in (0, head_dim = %d]", a->rotated, a->D);
+  if ((!positions && !wide) || !a->turns || !a->axis) return fail(ACCT_ERR_NULL, "positions, turns, axis must be non-NULL");
+  RotaryParams p;
+  memset(&p, 0, sizeof(p));
+  const int64_t rows = static_cast<int64_t>(a->B) * a->S;
+  const struct { const char* name; const void* x; void* y; const int64_t *xs, *ys; int heads; } t[2] = {
+      {"q", a->q, a->q_out, a->q_stride, a->q_out_stride, a->N}, {"k", a->k, a->k_out, a->k_stride, a->k_out_stride, a->N_kv}};
+  for (int w = 0; w < 2; ++w) {
+    if (t[w].heads == 0 || rows == 0) continue;
+    if (!t[w].x || !t[w].y) return fail(ACCT_ERR_NULL, "%s and its output must be non-NULL", t[w].name);
+    if (misaligned(t[w].x) || misaligned(t[w].y)) return fail(ACCT_ERR_ALIGN, "%s and its output must be 16-byte aligned", t[w].name);
+    const int64_t dense[3] = {static_cast<int64_t>(a->D) * a->S * t[w].heads, static_cast<int64_t>(a->D) * a->S, a->D};
+    for (int i = 0; i < 3; ++i) {
+      p.t[w].x_stride[i] = packed_or(t[w].xs[i], dense[i]);
+      p.t[w].y_stride[i] = packed_or(t[w].ys[i], dense[i]);
+      for (int64_t s : {p.t[w].x_stride[i], p.t[w].y_stride[i]}) {
+        if (s < a->D) return fail(ACCT_ERR_SHAPE, "%s strides must not be smaller than head_dim", t[w].name);
+        if (s % 8 != 0) return fail(ACCT_ERR_ALIGN, "%s stride (%lld elements) is not a multiple of 8", t[w].name, (long long)s);
+      }
+    }
+    p.t[w].x = t[w].x; p.t[w].y = t[w].y;
+    p.t[w].heads = t[w].heads;
+  }
+  if (rows > INT32_MAX || static_cast<double>(rows) * (static_cast<double>(a->N) + a->N_kv) * a->D >= 0x1p34)      // (a few launches at most)
+    return fail(ACCT_ERR_SHAPE, "B*S = %lld rows are too many for one call", (long long)rows);
+  p.positions = positions;
+  p.wide_positions = reinterpret_cast<const long long*>(wide);
+  for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->pos_stride[i];
+  p.turns = reinterpret_cast<const unsigned long long*>(a->turns);
+  p.axis = a->axis;
+  p.B = a->B; p.S = a->S; p.D = a->D; p.rotated = a->rotated;
+  p.adjacent = a->adjacent; p.inverse = a->inverse;
+  DeviceInfo info;
+  int rc = device_info(&info);
+  if (rc) return rc;
+  if (rows == 0 || a->N + a->N_kv == 0) return ACCT_OK;
+  const cudaError_t e = launch_rotary(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda(e, "launching the rotary kernel");
+  return ACCT_OK;
+}
+
 }  // namespace
 }  // namespace acct
 
@@ -253,49 +300,7 @@ int acct_linear_step(const acct_linear_step_args* a, void* stream) {
   return ACCT_OK;
 }
 
-int acct_rotary(const acct_rotary_args* a, void* stream) {
-  if (a == nullptr) return fail(ACCT_ERR_NULL, "args is NULL");
-  if (a->dtype != ACCT_F16 && a->dtype != ACCT_BF16) return fail(ACCT_ERR_DTYPE, "dtype must be ACCT_F16 or ACCT_BF16");
-  if (a->B < 0 || a->S < 0 || a->N < 0 || a->N_kv < 0) return fail(ACCT_ERR_SHAPE, "sizes must not be negative");
-  if (a->D <= 0 || a->D % 8 != 0 || a->D > 256) return fail(ACCT_ERR_UNSUPPORTED_D, "head_dim %d must be a multiple of 8 in (0, 256]", a->D);
-  if (a->rotated <= 0 || a->rotated % 2 != 0 || a->rotated > a->D) return fail(ACCT_ERR_SHAPE, "rotated = %d must be even, in (0, head_dim = %d]", a->rotated, a->D);
-  if (!a->positions || !a->turns || !a->axis) return fail(ACCT_ERR_NULL, "positions, turns, axis must be non-NULL");
-  RotaryParams p;
-  memset(&p, 0, sizeof(p));
-  const int64_t rows = static_cast<int64_t>(a->B) * a->S;
-  const struct { const char* name; const void* x; void* y; const int64_t *xs, *ys; int heads; } t[2] = {
-      {"q", a->q, a->q_out, a->q_stride, a->q_out_stride, a->N}, {"k", a->k, a->k_out, a->k_stride, a->k_out_stride, a->N_kv}};
-  for (int w = 0; w < 2; ++w) {
-    if (t[w].heads == 0 || rows == 0) continue;
-    if (!t[w].x || !t[w].y) return fail(ACCT_ERR_NULL, "%s and its output must be non-NULL", t[w].name);
-    if (misaligned(t[w].x) || misaligned(t[w].y)) return fail(ACCT_ERR_ALIGN, "%s and its output must be 16-byte aligned", t[w].name);
-    const int64_t dense[3] = {static_cast<int64_t>(a->D) * a->S * t[w].heads, static_cast<int64_t>(a->D) * a->S, a->D};
-    for (int i = 0; i < 3; ++i) {
-      p.t[w].x_stride[i] = packed_or(t[w].xs[i], dense[i]);
-      p.t[w].y_stride[i] = packed_or(t[w].ys[i], dense[i]);
-      for (int64_t s : {p.t[w].x_stride[i], p.t[w].y_stride[i]}) {
-        if (s < a->D) return fail(ACCT_ERR_SHAPE, "%s strides must not be smaller than head_dim", t[w].name);
-        if (s % 8 != 0) return fail(ACCT_ERR_ALIGN, "%s stride (%lld elements) is not a multiple of 8", t[w].name, (long long)s);
-      }
-    }
-    p.t[w].x = t[w].x; p.t[w].y = t[w].y;
-    p.t[w].heads = t[w].heads;
-  }
-  if (rows > INT32_MAX || static_cast<double>(rows) * (static_cast<double>(a->N) + a->N_kv) * a->D >= 0x1p34)      // (a few launches at most)
-    return fail(ACCT_ERR_SHAPE, "B*S = %lld rows are too many for one call", (long long)rows);
-  p.positions = a->positions;
-  for (int i = 0; i < 3; ++i) p.pos_stride[i] = a->pos_stride[i];
-  p.turns = reinterpret_cast<const unsigned long long*>(a->turns);
-  p.axis = a->axis;
-  p.B = a->B; p.S = a->S; p.D = a->D; p.rotated = a->rotated;
-  p.adjacent = a->adjacent; p.inverse = a->inverse;
-  DeviceInfo info;
-  int rc = device_info(&info);
-  if (rc) return rc;
-  if (rows == 0 || a->N + a->N_kv == 0) return ACCT_OK;
-  const cudaError_t e = launch_rotary(p, a->dtype == ACCT_BF16, static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return fail_cuda(e, "launching the rotary kernel");
-  return ACCT_OK;
-}
+int acct_rotary(const acct_rotary_args* a, void* stream) { return rotary(a, a != nullptr ? a->positions : nullptr, nullptr, stream); }
+int acct_rotary_wide(const acct_rotary_args* a, const int64_t* positions, void* stream) { return rotary(a, nullptr, positions, stream); }
 
 }  // extern "C"

@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   float c[kPairs], sn[kPairs];
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
-    const long long pos = p.positions[p.axis[pair0 + j] * p.pos_stride[0] + b * p.pos_stride[1] + s * p.pos_stride[2]];
+    const int64_t at = p.axis[pair0 + j] * p.pos_stride[0] + b * p.pos_stride[1] + s * p.pos_stride[2];
+    const long long pos = p.positions != nullptr ? p.positions[at] : p.wide_positions[at];
     const long long turn = static_cast<long long>(static_cast<unsigned long long>(pos) * p.turns[pair0 + j]);      // of 2^64; as signed: in [-1/2, 1/2)
     sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * (1.f / 2147483648.f), &sn[j], &c[j]);
     if (p.inverse) sn[j] = -sn[j];

@@ -50,6 +50,7 @@ struct Library {
   decltype(&acct_linear_bwd) linear_bwd;
   decltype(&acct_linear_step) linear_step;
   decltype(&acct_rotary) rotary;
+  decltype(&acct_rotary_wide) rotary_wide;
 } g_lib;
 
 #define HOST_CHECK TORCH_CHECK_VALUE
@@ -420,6 +421,7 @@ PyObject* py_init(PyObject*, PyObject* path) {
   g_lib.linear_bwd = reinterpret_cast<decltype(g_lib.linear_bwd)>(sym("acct_linear_bwd"));
   g_lib.linear_step = reinterpret_cast<decltype(g_lib.linear_step)>(sym("acct_linear_step"));
   g_lib.rotary = reinterpret_cast<decltype(g_lib.rotary)>(sym("acct_rotary"));
+  g_lib.rotary_wide = reinterpret_cast<decltype(g_lib.rotary_wide)>(sym("acct_rotary_wide"));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -1139,6 +1141,7 @@ PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
 struct RotaryCall {
   Tensor positions, turns, axis;
   int64_t head_dim, rotated, axes, adjacent;
+  int64_t wide;      // positions are int64, not int32
 };
 
 // q or k as [B, heads, rows, D]
@@ -1173,7 +1176,7 @@ void check_rotary_call(const RotaryCall& call, const Tensor& first) {
   require_on("positions", call.positions, first);
   const Tensor& pos = call.positions;
   const int64_t B = first.dim() == 4 ? first.size(0) : 1, S = first.dim() == 4 ? first.size(2) : first.size(0);
-  HOST_CHECK(pos.scalar_type() == at::kInt && pos.dim() == 3 && pos.size(0) == call.axes && (pos.size(1) == 1 || pos.size(1) == B) && pos.size(2) == S,
+  HOST_CHECK(pos.scalar_type() == (call.wide ? at::kLong : at::kInt) && pos.dim() == 3 && pos.size(0) == call.axes && (pos.size(1) == 1 || pos.size(1) == B) && pos.size(2) == S,
              "positions do not go with the rows: ", pos.scalar_type(), " ", pos.sizes(), " for ", first.sizes());
 }
 
@@ -1200,13 +1203,13 @@ void rotary_launch(const RotaryCall& call, const Tensor (&x)[2], const Tensor (&
     (i == 0 ? a.N : a.N_kv) = from[i].size(1);
   }
   const Tensor& pos = call.positions;
-  a.positions = static_cast<const int32_t*>(pos.const_data_ptr());
+  if (!call.wide) a.positions = static_cast<const int32_t*>(pos.const_data_ptr());
   for (int i = 0; i < 3; ++i) a.pos_stride[i] = pos.size(i) == 1 ? 0 : pos.stride(i);
   a.turns = static_cast<const uint64_t*>(call.turns.const_data_ptr());
   a.axis = static_cast<const int32_t*>(call.axis.const_data_ptr());
   a.adjacent = call.adjacent;
   a.inverse = inverse;
-  check(g_lib.rotary(&a, stream_of(first)));
+  check(call.wide ? g_lib.rotary_wide(&a, static_cast<const int64_t*>(pos.const_data_ptr()), stream_of(first)) : g_lib.rotary(&a, stream_of(first)));
 }
 
 // a new packed tensor of the shape of `t` whose strides are multiples of 8 whatever the sizes of its dimensions
@@ -1220,7 +1223,7 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     ctx->save_for_backward({call.positions});
     ctx->saved_data["turns"] = call.turns;      // (the plan's own: no hook of a user's sees them)
     ctx->saved_data["axis"] = call.axis;
-    ctx->saved_data["sizes"] = std::vector<int64_t>{call.head_dim, call.rotated, call.axes, call.adjacent, x[0].defined(), x[1].defined(), inverse};
+    ctx->saved_data["sizes"] = std::vector<int64_t>{call.head_dim, call.rotated, call.axes, call.adjacent, x[0].defined(), x[1].defined(), inverse, call.wide};
     variable_list out;
     for (const Tensor& t : y)
       if (t.defined()) out.push_back(t);
@@ -1230,7 +1233,8 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const std::vector<int64_t> sizes = ctx->saved_data.at("sizes").toIntVector();
     const variable_list saved = ctx->get_saved_variables();
-    const RotaryCall call{saved[0], ctx->saved_data.at("turns").toTensor(), ctx->saved_data.at("axis").toTensor(), sizes[0], sizes[1], sizes[2], sizes[3]};
+    const RotaryCall call{saved[0], ctx->saved_data.at("turns").toTensor(), ctx->saved_data.at("axis").toTensor(), sizes[0], sizes[1], sizes[2], sizes[3],
+                          sizes[7]};
     Tensor x[2], y[2];
     size_t at = 0;
     for (int i = 0; i < 2; ++i)
@@ -1253,7 +1257,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   HOST_CHECK(n == 7, "rotary takes 7 arguments, got ", n);
   const Tensor q = tensor_or_undefined(args[0]), k = tensor_or_undefined(args[1]);
-  RotaryCall call{tensor_arg(args[2], "positions"), tensor_arg(args[3], "turns"), tensor_arg(args[4], "axis"), 0, 0, 0, 0};
+  RotaryCall call{tensor_arg(args[2], "positions"), tensor_arg(args[3], "turns"), tensor_arg(args[4], "axis"), 0, 0, 0, 0, 0};
   HOST_CHECK(PyTuple_Check(args[5]) && PyTuple_GET_SIZE(args[5]) == 4, "not a rotary plan");
   call.head_dim = int_arg(PyTuple_GET_ITEM(args[5], 0));
   call.rotated = int_arg(PyTuple_GET_ITEM(args[5], 1));
@@ -1282,7 +1286,13 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     else
       HOST_CHECK(first.dim() == 4 && is({call.axes, B, S}), "positions must be [", call.axes, " axes, ", first.dim() == 4 ? "batch entries, " : "", S,
                  " rows]", call.axes == 1 ? " or [rows]" : "", ", got ", pos.sizes());
-    call.positions = pos.scalar_type() == at::kInt ? pos : pos.to(at::kInt);
+    // (of 32 bits where all of their type are, else of 64)
+    call.wide = c10::elementSize(pos.scalar_type()) > 4 || pos.scalar_type() == at::kUInt32;
+    const auto type = call.wide ? at::kLong : at::kInt;
+    call.positions = pos.scalar_type() == type ? pos : pos.to(type);
+    // (of 64 bits they may move on before the backward: it gets a copy, as it does of other types that are converted)
+    const auto graph = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    if (pos.scalar_type() == at::kLong && at::GradMode::is_enabled() && (graph(q) || graph(k))) call.positions = pos.clone();
     check_rotary_call(call, first);
     if (in_place || B * S == 0) {
       at::AutoDispatchBelowADInplaceOrView below;

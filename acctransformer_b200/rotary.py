@@ -87,7 +87,7 @@ class Rotary:
         self._plan = (head_dim, 2 * pairs, len(sections), int(self.adjacent))
 
     def __call__(self, q, k, positions):
-        """(q, k) turned, as new tensors; differentiable in both, either may be None.  ``positions``: integers [axes, T] for rows
+        """(q, k) turned, as new tensors; differentiable in both, either may be None.  ``positions``: integers of up to 64 bits, [axes, T] for rows
         [T, heads, D], [axes, B, S] or [axes, S] for [B, heads, S, D]; with one axis that dimension may be missing."""
         if torch.jit.is_tracing():
             return self._recorded(q, k, positions)

@@ -492,7 +492,7 @@ ACCT_API int acct_linear_step(const acct_linear_step_args* a, void* stream);
 /* Rotary positions with several axes; the reference has no counterpart.  Of every row's first `rotated` values each pair (x1, x2) becomes
  *   y1 = x1 cos(w) - x2 sin(w),   y2 = x2 cos(w) + x1 sin(w),   w = 2 pi turns[i] / 2^64 * position on axis[i]
  * for pair i: values i and i + rotated / 2, or with `adjacent` 2 i and 2 i + 1.  The values behind them are copied.  Sums are fp32,
- * angles exact for any position.  An output is its input (in place) or other memory. */
+ * angles those of the table whatever the position.  An output is its input (in place) or other memory. */
 typedef struct acct_rotary_args {
   int32_t dtype;               /* ACCT_F16 or ACCT_BF16 */
   int32_t B, S, D;             /* batch entries, rows, head_dim: a multiple of 8 up to 256 */
@@ -515,6 +515,9 @@ typedef struct acct_rotary_args {
 } acct_rotary_args;
 
 ACCT_API int acct_rotary(const acct_rotary_args* a, void* stream);
+
+/* The same with positions of 64 bits, in the place of a->positions, which is not read; a->pos_stride counts their elements. */
+ACCT_API int acct_rotary_wide(const acct_rotary_args* a, const int64_t* positions, void* stream);
 
 /* The same operators behind the calling convention MindSpore uses for ops.Custom(func_type="aot"):
  *   int f(int nparam, void** params, int* ndims, int64_t** shapes, const char** dtypes, void* stream, void* extra)

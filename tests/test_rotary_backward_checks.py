@@ -32,7 +32,7 @@ def test_copies_are_taken():
     x, y, pos, rotary = _turned(lambda t: t.clone() if t.dim() != 3 else t.transpose(0, 2).contiguous().transpose(0, 2))
     d = _rand(T, N, D, dtype=torch.float16, seed=2)
     (got,) = torch.autograd.grad(y, x, d)
-    assert torch.equal(got, rotary(d, None, -pos)[0])
+    assert torch.equal(got, torch.autograd.grad(rotary(x, None, pos)[0], x, d)[0])
 
 
 def test_other_gradients_are_refused():
