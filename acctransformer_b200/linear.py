@@ -73,7 +73,7 @@ class LinearAttention(torch.nn.Module):
         log_decay = default_log_decay(head_num) if log_decay is None else torch.as_tensor(log_decay, dtype=torch.float32)
         if tuple(log_decay.shape) != (head_num,):
             raise ValueError(f"log_decay must hold a number for each of {head_num} heads, got {tuple(log_decay.shape)}")
-        if bool((log_decay > 0).any()) or bool(log_decay.isnan().any()):
+        if not log_decay.is_meta and (bool((log_decay > 0).any()) or bool(log_decay.isnan().any())):
             raise ValueError("log_decay must be at most 0")
         if rotary is not None and rotary.head_dim != head_dim:
             raise ValueError(f"rotary is a plan for head_dim {rotary.head_dim}, not {head_dim}")
@@ -83,7 +83,9 @@ class LinearAttention(torch.nn.Module):
     def _apply(self, fn, recurse=True):
         decays = self.log_decay
         super()._apply(fn, recurse)
-        self.log_decay = decays.to(self.log_decay.device)      # in float32, whatever type the module is cast to
+        if self.log_decay.dtype != torch.float32:      # they stay float32, whatever type the module is cast to
+            device = self.log_decay.device
+            self.log_decay = torch.empty_like(decays, dtype=torch.float32, device=device) if decays.is_meta else decays.to(device, torch.float32)
         return self
 
     def forward(self, q, k, v, seq_lens=None, positions=None):
