@@ -1294,7 +1294,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const auto graph = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
     if (pos.scalar_type() == at::kLong && at::GradMode::is_enabled() && (graph(q) || graph(k))) call.positions = pos.clone();
     check_rotary_call(call, first);
-    if (in_place || B * S == 0) {
+    if (in_place) {
       at::AutoDispatchBelowADInplaceOrView below;
       if (B * S > 0) {
         int64_t strides[3];
@@ -1306,11 +1306,13 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
       }
       for (const Tensor* t : both)
         if (t->defined()) {
-          if (in_place) written(*t);
+          written(*t);
           out.push_back(*t);
         }
-    }
-    if (out.empty()) {
+    } else if (B * S == 0) {
+      for (const Tensor* t : both)
+        if (t->defined()) out.push_back(t->clone());
+    } else {
       const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
       out = RotaryFunction::apply(given(q), given(k), call, false);
     }
