@@ -109,13 +109,13 @@ struct RotaryParams {
     int64_t x_stride[3], y_stride[3];      // of batch entry, head, row
     int heads;
   } t[2];
-  const int* positions;             // [axes] x rows, with element strides; or null ...
-  const long long* wide_positions;  // ... of 64 bits
+  const int* positions;             // [axes] x rows, with element strides
   int64_t pos_stride[3];            // of axis, batch entry, row
   const unsigned long long* turns;  // [rotated / 2]: turns per position, as a fraction of 2^64
   const int* axis;                  // [rotated / 2]
   int B, S, D, rotated;
   int adjacent, inverse;
+  const long long* wide_positions;  // in the place of positions: of 64 bits
 };
 cudaError_t launch_rotary(const RotaryParams& p, bool bf16, cudaStream_t stream);
 

@@ -47,11 +47,12 @@ __device__ __forceinline__ typename Raw<VEC>::type repack(const float (&x)[VEC])
 }
 
 // A unit: VEC neighbouring values of a row (adjacent: VEC / 2 pairs), or VEC values and their VEC partners half of the turned part on;
-// behind those, VEC values that are copied.  A thread has a unit of one row in HEADS heads, all of which it loads before it turns any.  A
-// launch has `rows` rows from row0 on, so few that threads can be counted in 32 bits (whose division is a fraction of that in 64).
-template <bool BF16, int VEC, bool ADJACENT, int HEADS>
+// behind those, VEC values that are copied.  A thread has a unit of one row in HEADS heads, all of which it loads before it turns any.
+// Threads are counted in 32 bits, whose division is a fraction of that in 64: see launch_heads.  WIDE: positions of 64 bits (chosen for each pair at
+// run time they cost 4 %).
+template <bool BF16, int VEC, bool ADJACENT, int HEADS, bool WIDE>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p, unsigned int units, unsigned int turned_units,
-                                                          unsigned int q_blocks, unsigned int row0, unsigned int rows) {
+                                                          unsigned int q_blocks) {
   using R = typename Raw<VEC>::type;
   constexpr int kPairs = ADJACENT ? VEC / 2 : VEC;
   const bool is_k = blockIdx.x >= q_blocks;
@@ -61,9 +62,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const unsigned int unit = i % units, rest = i / units;
   // (neighbouring rows lie beside each other where rows are packed by head, neighbouring heads where they are packed by row)
   const bool by_head = t.x_stride[1] < t.x_stride[2];
-  const unsigned int group = by_head ? rest % groups : rest / rows, at = by_head ? rest / groups : rest % rows;
-  if (group >= groups || at >= rows) return;
-  const unsigned int row = row0 + at, b = row / p.S, s = row % p.S;
+  const unsigned int rows = static_cast<unsigned int>(p.B) * p.S;
+  const unsigned int group = by_head ? rest % groups : rest / rows, row = by_head ? rest / groups : rest % rows;
+  if (group >= groups || row >= rows) return;
+  const unsigned int b = row / p.S, s = row % p.S;
   const bool copied = unit >= turned_units;
   const int pair0 = unit * kPairs, half = p.rotated / 2;
   const int d = copied ? p.rotated + (unit - turned_units) * VEC : ADJACENT ? unit * VEC : pair0;
@@ -88,7 +90,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
     const int64_t at = p.axis[pair0 + j] * p.pos_stride[0] + b * p.pos_stride[1] + s * p.pos_stride[2];
-    const long long pos = p.positions != nullptr ? p.positions[at] : p.wide_positions[at];
+    const long long pos = WIDE ? p.wide_positions[at] : p.positions[at];
     const long long turn = static_cast<long long>(static_cast<unsigned long long>(pos) * p.turns[pair0 + j]);      // of 2^64; as signed: in [-1/2, 1/2)
     sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * (1.f / 2147483648.f), &sn[j], &c[j]);
     if (p.inverse) sn[j] = -sn[j];
@@ -121,21 +123,41 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   }
 }
 
+// Batch entries b0 .. b0 + B - 1, rows s0 .. s0 + S - 1 of each.
+RotaryParams part_of(const RotaryParams& p, int b0, int B, int s0, int S) {
+  RotaryParams part = p;
+  part.B = B;
+  part.S = S;
+  for (auto& t : part.t) {
+    if (t.x == nullptr) continue;
+    t.x = static_cast<const uint16_t*>(t.x) + b0 * t.x_stride[0] + s0 * t.x_stride[2];
+    t.y = static_cast<uint16_t*>(t.y) + b0 * t.y_stride[0] + s0 * t.y_stride[2];
+  }
+  const int64_t at = b0 * p.pos_stride[1] + s0 * p.pos_stride[2];
+  if (p.positions != nullptr) part.positions += at;
+  if (p.wide_positions != nullptr) part.wide_positions += at;
+  return part;
+}
+
 template <bool BF16, int VEC, bool ADJACENT, int HEADS>
 cudaError_t launch_heads(const RotaryParams& p, int units, int turned_units, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.B) * p.S;
   int64_t threads[2];      // of a row
   for (int w = 0; w < 2; ++w) threads[w] = static_cast<int64_t>(units) * ((p.t[w].heads + HEADS - 1) / HEADS);
-  const int64_t most = ((int64_t(1) << 32) - kThreads) / std::max(threads[0], threads[1]);      // rows of a launch
-  for (int64_t row0 = 0; row0 < rows; row0 += most) {
-    const int64_t n = std::min(rows - row0, most);
-    unsigned int blocks[2];
-    for (int w = 0; w < 2; ++w) blocks[w] = static_cast<unsigned int>((n * threads[w] + kThreads - 1) / kThreads);
-    rotary_kernel<BF16, VEC, ADJACENT, HEADS><<<blocks[0] + blocks[1], kThreads, 0, stream>>>(p, units, turned_units, blocks[0], static_cast<unsigned int>(row0),
-                                                                                              static_cast<unsigned int>(n));
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
+  // A launch has as many rows as 32 bits count the threads of (small units of few heads pass that): whole batch entries, or part of one.
+  const int64_t most = ((int64_t(1) << 32) - kThreads) / std::max(threads[0], threads[1]);
+  const int S = static_cast<int>(std::min<int64_t>(p.S, most)), B = static_cast<int>(std::min<int64_t>(p.B, S < p.S ? 1 : most / S));
+  const auto kernel = p.wide_positions != nullptr ? rotary_kernel<BF16, VEC, ADJACENT, HEADS, true> : rotary_kernel<BF16, VEC, ADJACENT, HEADS, false>;
+  for (int64_t b0 = 0; b0 < p.B; b0 += B)
+    for (int64_t s0 = 0; s0 < p.S; s0 += S) {
+      const RotaryParams part = part_of(p, static_cast<int>(b0), static_cast<int>(std::min<int64_t>(B, p.B - b0)), static_cast<int>(s0),
+                                        static_cast<int>(std::min<int64_t>(S, p.S - s0)));
+      const int64_t rows = static_cast<int64_t>(part.B) * part.S;
+      unsigned int blocks[2];
+      for (int w = 0; w < 2; ++w) blocks[w] = static_cast<unsigned int>((rows * threads[w] + kThreads - 1) / kThreads);
+      kernel<<<blocks[0] + blocks[1], kThreads, 0, stream>>>(part, units, turned_units, blocks[0]);
+      const cudaError_t e = cudaGetLastError();
+      if (e != cudaSuccess) return e;
+    }
   return cudaSuccess;
 }
 

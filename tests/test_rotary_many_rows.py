@@ -23,3 +23,19 @@ def test_all_rows_are_turned(sections, adjacent, N, rows):
     for at in range(0, rows, 1 << 20):      # (a row's values do not depend on how many there are: calls of few threads)
         part = slice(at, min(rows, at + (1 << 20)))
         assert torch.equal(y[part], rotary(x[part], None, pos[part])[0])
+
+
+@pytest.mark.parametrize("B,S,wide,shared", [(3, 23_000_001, False, False), (5, 7_000_003, True, False), (2, 34_000_000, True, True), (34_000, 1000, False, True)])
+def test_batches(B, S, wide, shared):
+    """[B, 1, S, D], a launch each of some batch entries, or of a part of one."""
+    from acctransformer_b200 import Rotary
+    D, T = 128, B * S
+    assert T * 127 > 2 ** 32
+    rotary = Rotary(D, (1,), base=100.0)
+    x = torch.empty(B, 1, S, D, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    pos = torch.randint(0, 1000, (S,) if shared else (B, S), dtype=torch.int64 if wide else torch.int32, device="cuda")
+    y = rotary(x, None, pos)[0].view(T, D)
+    rows, at = x.view(T, 1, D), pos.expand(B, S).reshape(T)
+    for i in range(0, T, 1 << 20):
+        part = slice(i, min(T, i + (1 << 20)))
+        assert torch.equal(y[part], rotary(rows[part], None, at[part])[0].view(-1, D))
