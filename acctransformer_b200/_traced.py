@@ -8,7 +8,7 @@ import contextlib
 
 import torch
 
-__all__ = ["call", "refuse"]
+__all__ = ["call"]
 
 
 @contextlib.contextmanager
@@ -56,8 +56,3 @@ def call(operator, *operands):
     """operator(*operands), a tuple of tensors, as a trace can record it; operands are tensors or None.  `operator` prints alike each time it is
     recorded (a trace is checked against a second one by what it prints)."""
     return _Traced.apply(operator, *operands)
-
-
-def refuse(name):
-    if torch.jit.is_tracing():
-        raise RuntimeError(f"{name} cannot be traced: a trace would hold its results as constants")

@@ -14,6 +14,7 @@
 #include <dlfcn.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -957,10 +958,16 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
   }
 };
 
-// linear_apply(q, k, v, log_decay, seq_lens | None, scale) -> y, differentiable in q, k, v
+// A trace would hold what comes out of here as constants.  (Asked here, since the question costs 0.4 us in Python.)
+bool is_tracing() { return at::tracer::impl::is_dispatch_enabled(); }
+void not_traced(const char* op) { TORCH_CHECK(!is_tracing(), op, " cannot be traced: a trace would hold its results as constants"); }
+
+// linear_apply(q, k, v, log_decay, seq_lens | None, scale) -> y, differentiable in q, k, v; None under torch.jit.trace: to be called in a form
+// that can be traced
 PyObject* py_linear_apply(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   HOST_CHECK(n == 6, "linear_apply takes 6 arguments, got ", n);
+  if (is_tracing()) Py_RETURN_NONE;
   const Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v");
   Tensor g = tensor_arg(args[3], "log_decay"), y;
   LinearCall call{tensor_or_undefined(args[4]), float_arg(args[5])};
@@ -1025,6 +1032,7 @@ void written(const Tensor& t) {
 PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   HOST_CHECK(n == 8, "linear_packed takes 8 arguments, got ", n);
+  not_traced("linear_attention_packed");
   Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), g = tensor_arg(args[3], "log_decay");
   Tensor cu = tensor_arg(args[4], "cu_seqlens"), state = tensor_or_undefined(args[5]), y = tensor_or_undefined(args[7]);
   const double scale = float_arg(args[6]);
@@ -1094,6 +1102,7 @@ PyObject* py_linear_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_linear_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   HOST_CHECK(n == 7, "linear_step takes 7 arguments, got ", n);
+  not_traced("linear_attention_step");
   Tensor q = tensor_arg(args[0], "q"), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v"), g = tensor_arg(args[3], "log_decay");
   Tensor state = tensor_arg(args[4], "state"), y = tensor_or_undefined(args[6]);
   const double scale = float_arg(args[5]);
@@ -1252,7 +1261,7 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
   }
 };
 
-// rotary(q | None, k | None, positions, turns, axis, (head_dim, rotated, axes, adjacent), in_place) -> (q | None, k | None)
+// rotary(q | None, k | None, positions, turns, axis, (head_dim, rotated, axes, adjacent), in_place) -> (q | None, k | None); None under torch.jit.trace, in place an error
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   HOST_CHECK(n == 7, "rotary takes 7 arguments, got ", n);
@@ -1264,6 +1273,8 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   call.axes = int_arg(PyTuple_GET_ITEM(args[5], 2));
   call.adjacent = int_arg(PyTuple_GET_ITEM(args[5], 3));
   const bool in_place = bool_arg(args[6]);
+  if (in_place) not_traced("Rotary.apply_");
+  if (is_tracing()) Py_RETURN_NONE;
   if (in_place) no_gradient("Rotary.apply_", {&q, &k});
   variable_list out;
   {

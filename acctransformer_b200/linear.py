@@ -31,9 +31,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, seq_lens=None):
     """y [B, N, S, D] of q [B, N, S, D], k and v [B, N_kv, S, D] with N_kv dividing N, float16 or bfloat16, D a multiple of 8 up to 128;
     differentiable in q, k and v.  ``log_decay``: [N], without a gradient.  ``seq_lens`` ([B] integers): rows from there on are
     padding, which nothing reads and whose outputs and gradients are 0.  scale defaults to D^-1/2."""
-    if torch.jit.is_tracing():
-        return _traced.call(functools.partial(_recorded, scale), q, k, v, log_decay, seq_lens)[0]
-    return _lib.host().linear_apply(q, k, v, log_decay, seq_lens, _scale(q, scale))
+    y = _lib.host().linear_apply(q, k, v, log_decay, seq_lens, _scale(q, scale))
+    return _traced.call(functools.partial(_recorded, scale), q, k, v, log_decay, seq_lens)[0] if y is None else y
 
 
 def _recorded(scale, q, *operands):
@@ -46,14 +45,12 @@ def linear_attention_packed(q, k, v, log_decay, cu_seqlens, *, state=None, scale
 
     ``state`` (float32 [B, N, D, D]): the states before the first rows; it is moved on in place.  Without it they are zeros, and
     the states behind the last rows come as a new tensor.  Rows that belong to no sequence are not written.  For serving: no gradient."""
-    _traced.refuse("linear_attention_packed")
     return _lib.host().linear_packed(q, k, v, log_decay, cu_seqlens, state, _scale(q, scale), out)
 
 
 def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
     """y [B, N, 1, D] of one token per sequence, q [B, N, 1, D], k and v [B, N_kv, 1, D], after it has gone into ``state`` (float32
     [B, N, D, D], moved on in place).  For serving: no gradient."""
-    _traced.refuse("linear_attention_step")
     return _lib.host().linear_step(q, k, v, log_decay, state, _scale(q, scale), out)
 
 

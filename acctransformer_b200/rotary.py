@@ -89,13 +89,11 @@ class Rotary:
     def __call__(self, q, k, positions):
         """(q, k) turned, as new tensors; differentiable in both, either may be None.  ``positions``: integers of up to 64 bits, [axes, T] for rows
         [T, heads, D], [axes, B, S] or [axes, S] for [B, heads, S, D]; with one axis that dimension may be missing."""
-        if torch.jit.is_tracing():
-            return self._recorded(q, k, positions)
-        return _lib.host().rotary(q, k, positions, self.turns, self.axis, self._plan, False)
+        out = _lib.host().rotary(q, k, positions, self.turns, self.axis, self._plan, False)
+        return self._recorded(q, k, positions) if out is None else out
 
     def apply_(self, q, k, positions):
         """The same in place, without a gradient; rows must be contiguous, and addresses and strides whole 16 bytes."""
-        _traced.refuse("Rotary.apply_")
         return _lib.host().rotary(q, k, positions, self.turns, self.axis, self._plan, True)
 
     def _recorded(self, q, k, positions):
