@@ -1312,7 +1312,8 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
         for (const Tensor* t : both)
           HOST_CHECK(!t->defined() || readable_anywhere(rotary_rows(*t), strides).const_data_ptr() == t->const_data_ptr(),
                      "in place, rows must be contiguous, and addresses and strides whole 16 bytes");
-        if (q.defined()) apart("q", q, {&k});
+        if (q.defined()) apart("q", q, {&k, &call.positions, &call.turns, &call.axis});
+        if (k.defined()) apart("k", k, {&call.positions, &call.turns, &call.axis});
         rotary_launch(call, {q, k}, {q, k}, false);
       }
       for (const Tensor* t : both)

@@ -68,4 +68,9 @@ def test_rotary_in_place():
     _refused(rotary.apply_, dense, k, pos)
     _refused(rotary.apply_, k, dense, pos)
     _refused(rotary.apply_, q, q[:, :1], pos)
+    for mine in (dense, q):
+        at = mine[1].reshape(-1)[:2 * T].view(torch.int32) if mine is dense else buf[N * D - 2 * T:N * D].view(torch.int32)
+        assert at.numel() == T and at.data_ptr() < dense.data_ptr() + dense.nbytes
+        _refused(rotary.apply_, mine, None, at.copy_(pos))
+        _refused(rotary.apply_, None, mine, at)
     rotary.apply_(q, buf[3 * T * N * D:][:T * N * D].view(T, N, D), pos)
